@@ -139,6 +139,47 @@ def edges_workspace_ints(num_nodes: int) -> int:
     return (num_nodes + 15) // 16 + (num_nodes + 255) // 256 + 1
 
 
+# ---- libomq_net_ops.so (include/omq_net_ops.h) ----------------------------------------------
+NET_LIB_PATH = os.path.join(_HERE, "libomq_net_ops.so")
+NET_ABI_VERSION = 1
+OMQ_NET_F32, OMQ_NET_BF16, OMQ_NET_F16 = 0, 1, 2
+_i64, _u64, _f32, _f64, _int = (ctypes.c_int64, ctypes.c_uint64, ctypes.c_float, ctypes.c_double,
+                                ctypes.c_int)
+
+
+class OmqPolicyRows(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("actions", _i64), ("logits", _p), ("logits_stride", _i64),
+        ("legal", _p), ("legal_stride", _i64), ("target", _p), ("target_stride", _i64),
+        ("taken", _p), ("advantages", _p), ("old_logp", _p), ("ref_logp", _p), ("dtype", _i32),
+        ("taken_are_64", _i32), ("clip_low", _f32), ("clip_high", _f32), ("kl_coef", _f32),
+        ("reserved", _f32),
+    ]
+
+
+_RP = ctypes.POINTER(OmqPolicyRows)
+NET_SIGNATURES = {
+    "omq_net_abi_version": (_int, []),
+    "omq_net_last_error": (ctypes.c_char_p, []),
+    "omq_token_embedding": (_int, [_p, _int, _i64, _p, _i64, _i64, _i64, _int, _f32, _p, _p]),
+    "omq_token_embedding_grad_workspace": (_i64, [_i64, _i64, _i64]),
+    "omq_token_embedding_grad": (_int, [_p, _i64, _int, _p, _int, _i64, _i64, _i64, _f32, _p, _int,
+                                        _p, _i64, _p]),
+    "omq_dropout": (_int, [_p, _i64, _i64, _int, _f64, _u64, _u64, _p, _p]),
+    "omq_add_rms_norm": (_int, [_p, _i64, _p, _i64, _p, _int, _i64, _i64, _int, _f32, _f64, _u64,
+                                _u64, _p, _p, _p]),
+    "omq_add_rms_norm_fp8": (_int, [_p, _i64, _p, _i64, _p, _int, _i64, _i64, _int, _f32, _int, _p,
+                                    _p, _p, _p]),
+    "omq_add_rms_norm_grad_workspace": (_i64, [_i64, _i64]),
+    "omq_add_rms_norm_grad": (_int, [_p, _i64, _p, _i64, _p, _i64, _p, _int, _i64, _i64, _int,
+                                     _f32, _f64, _u64, _u64, _p, _p, _p, _p, _i64, _p]),
+    "omq_clipped_policy_loss_workspace": (_i64, [_i64, _i64]),
+    "omq_clipped_policy_loss": (_int, [_RP, _p, _p, _p, _p, _p, _i64, _p]),
+    "omq_clipped_policy_loss_grad": (_int, [_RP, _p, _p, _p, _p]),
+    "omq_clipped_policy_loss_with_grad": (_int, [_RP, _p, _p, _p, _p, _p, _p, _i64, _p]),
+}
+
+
 class LibraryNotBuilt(RuntimeError):
     pass
 
@@ -191,6 +232,31 @@ def load(path: str | None = None) -> ctypes.CDLL:
         if path is None:
             _lib = lib
         return lib
+
+
+_net = None
+
+
+def load_net() -> ctypes.CDLL:
+    """Load libomq_net_ops.so once, as load() does the tree library."""
+    global _net
+    import torch  # noqa: F401  (the HIP runtime the library shares)
+
+    with _lock:
+        if _net is None:
+            if not os.path.exists(NET_LIB_PATH):
+                raise LibraryNotBuilt(f"{NET_LIB_PATH} is missing: build it with `python -c "
+                                      "'import __graft_entry__ as g; g.build()'`")
+            lib = ctypes.CDLL(NET_LIB_PATH)
+            if lib.omq_net_abi_version() != NET_ABI_VERSION:
+                raise LibraryNotBuilt(f"{NET_LIB_PATH} has ABI {lib.omq_net_abi_version()}, "
+                                      f"expected {NET_ABI_VERSION}")
+            for name, (res, args) in NET_SIGNATURES.items():
+                fn = getattr(lib, name)
+                fn.restype = res
+                fn.argtypes = args
+            _net = lib
+        return _net
 
 
 def check(rc: int, what: str) -> None:

@@ -1,0 +1,59 @@
+// Dropout from a counter-based generator (gfx950): the mask is a function of the element's
+// position, formed where it is needed and never stored.  Bound by memory: each element is read
+// and written once.  A lane takes eight elements of a row, two words of the generator.
+#include "net_common.h"
+
+namespace omq_net {
+
+int check_dropout(const char* name, double p);
+
+namespace {
+
+template <class T>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t rows, int dim,
+                                                      int blocks, Dropout d, T* out) {
+  const int64_t first = (int64_t)blockIdx.x * 256;
+  const int64_t row0 = first / blocks;
+  const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
+  const int64_t row = row0 + in / (uint32_t)blocks;
+  const uint32_t block = in % (uint32_t)blocks;
+  if (row >= rows) return;
+  const int n = dim - 8 * (int)block;
+  const int64_t at = row * dim + 8 * block;
+  const F8 v = drop8(load8<T>(x + at, n), d, (uint64_t)row * (uint32_t)((dim + 3) / 4), block);
+  store8<T>(out + at, v, n);
+}
+
+}  // namespace
+}  // namespace omq_net
+
+using namespace omq_net;
+
+extern "C" int omq_dropout(const void* x, int64_t rows, int64_t dim, int dtype, double p,
+                           uint64_t seed, uint64_t offset, void* out, void* stream) {
+  const char* name = "omq_dropout";
+  if (!dtype_known(dtype)) return net_fail(OMQ_NET_E_ARG, "%s: unknown type %d", name, dtype);
+  if (int rc = check_dropout(name, p)) return rc;
+  if (rows < 0 || dim < 1)
+    return net_fail(OMQ_NET_E_ARG, "%s: rows %lld, dim %lld", name, (long long)rows,
+                    (long long)dim);
+  if (rows > OMQ_NET_MAX_COUNT || dim > OMQ_NET_MAX_DIM ||
+      ceil_div(rows * ceil_div(dim, 8), 256) > OMQ_NET_MAX_COUNT)
+    return net_fail(OMQ_NET_E_LIMIT, "%s: rows %lld, dim %lld too large", name, (long long)rows,
+                    (long long)dim);
+  if (rows == 0) return OMQ_NET_OK;
+  if (!x || !out) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  const Dropout d = make_dropout(p, seed, offset);
+  const int blocks = (int)ceil_div(dim, 8);
+  const uint32_t grid = (uint32_t)ceil_div(rows * blocks, 256);
+  hipStream_t st = (hipStream_t)stream;
+  const auto go = [&](auto t) {
+    using T = decltype(t);
+    dropout_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(x), rows, (int)dim, blocks, d,
+                                            static_cast<T*>(out));
+  };
+  if (dtype == OMQ_NET_F32) go(float{});
+  else if (dtype == OMQ_NET_BF16) go(bf16{});
+  else go(f16{});
+  return net_status(name);
+}
