@@ -2,10 +2,10 @@
 // torch.ops.load_library): each checks its tensors, allocates its outputs and its workspace from
 // torch's allocator and calls the C ABI (omq_net_ops.h) on the caller's current HIP stream.
 //
-//   omq::token_embedding, omq::token_embedding_grad
-//   omq::add_rms_norm, omq::add_rms_norm_fp8, omq::add_rms_norm_grad
-//   omq::net_dropout
-//   omq::clipped_policy_loss, omq::clipped_policy_loss_grad, omq::clipped_policy_loss_with_grad
+//   omq_net::token_embedding, omq_net::token_embedding_grad
+//   omq_net::add_rms_norm, omq_net::add_rms_norm_fp8, omq_net::add_rms_norm_grad
+//   omq_net::dropout
+//   omq_net::clipped_policy_loss, omq_net::clipped_policy_loss_grad, omq_net::clipped_policy_loss_with_grad
 //
 // Tensors must be on one HIP device; host tensors are refused (there is no CPU implementation).
 // On meta tensors the operators give the shapes only.
@@ -37,10 +37,10 @@ void check_rc(int rc, const char* what) {
 // The tensors' common device: a HIP device, or meta.
 c10::Device common_device(const char* name, std::initializer_list<const at::Tensor*> ts) {
   const c10::Device dev = (*ts.begin())->device();
-  TORCH_CHECK(dev.is_cuda() || dev.is_meta(), "omq::", name,
+  TORCH_CHECK(dev.is_cuda() || dev.is_meta(), "omq_net::", name,
               ": tensors must be on a HIP device (got ", dev, ")");
   for (const at::Tensor* t : ts)
-    if (t) TORCH_CHECK(t->device() == dev, "omq::", name, ": all tensors must be on ", dev);
+    if (t) TORCH_CHECK(t->device() == dev, "omq_net::", name, ": all tensors must be on ", dev);
   return dev;
 }
 
@@ -51,14 +51,14 @@ int type_of(const char* name, const char* arg, const at::Tensor& t) {
     case at::kHalf: return OMQ_NET_F16;
     default: break;
   }
-  TORCH_CHECK(false, "omq::", name, ": ", arg, " must be float32, bfloat16 or float16, not ",
+  TORCH_CHECK(false, "omq_net::", name, ": ", arg, " must be float32, bfloat16 or float16, not ",
               t.scalar_type());
 }
 
 bool ids_are_64(const char* name, const char* arg, const at::Tensor& t) {
-  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "omq::", name, ": ",
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "omq_net::", name, ": ",
               arg, " must be int32 or int64, not ", t.scalar_type());
-  TORCH_CHECK(t.is_contiguous(), "omq::", name, ": ", arg, " must be contiguous");
+  TORCH_CHECK(t.is_contiguous(), "omq_net::", name, ": ", arg, " must be contiguous");
   return t.scalar_type() == at::kLong;
 }
 
@@ -76,7 +76,7 @@ int64_t row_stride(const char* name, const char* arg, const at::Tensor& t) {
       ok = ok && t.stride(i) == expected;
     expected = t.stride(i) * t.size(i);
   }
-  TORCH_CHECK(ok, "omq::", name, ": the rows of ", arg,
+  TORCH_CHECK(ok, "omq_net::", name, ": the rows of ", arg,
               " must have adjacent elements and equal distances (use .contiguous())");
   return stride < 0 ? t.size(-1) : stride;
 }
@@ -84,31 +84,31 @@ int64_t row_stride(const char* name, const char* arg, const at::Tensor& t) {
 void* stream_of(c10::Device dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
 
 at::Tensor workspace(const char* name, int64_t bytes, const at::Tensor& like) {
-  TORCH_CHECK(bytes >= 0, "omq::", name, ": sizes beyond the library's limits");
+  TORCH_CHECK(bytes >= 0, "omq_net::", name, ": sizes beyond the library's limits");
   return at::empty({bytes}, like.options().dtype(at::kByte));
 }
 
 bool drops(const char* name, double p) {
-  TORCH_CHECK(p >= 0.0 && p <= 1.0, "omq::", name, ": p ", p, " outside [0, 1]");
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, "omq_net::", name, ": p ", p, " outside [0, 1]");
   return (uint32_t)(p * 65536.0 + 0.5) != 0;
 }
 
 void check_same(const char* name, const char* arg, const at::Tensor& t, const at::Tensor& x) {
-  TORCH_CHECK(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type(), "omq::", name, ": ",
+  TORCH_CHECK(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type(), "omq_net::", name, ": ",
               arg, " must have the rows' shape and type (", x.sizes(), ", ", x.scalar_type(),
               "), not ", t.sizes(), ", ", t.scalar_type());
 }
 
 int check_weight(const char* name, const at::Tensor& w, const at::Tensor& x) {
-  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous(), "omq::", name,
+  TORCH_CHECK(w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous(), "omq_net::", name,
               ": weight must be contiguous [", x.size(-1), "]");
-  TORCH_CHECK(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "omq::", name,
+  TORCH_CHECK(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "omq_net::", name,
               ": weight must be ", x.scalar_type(), " or float32, not ", w.scalar_type());
   return type_of(name, "weight", w);
 }
 
 void check_rows_of(const char* name, const char* arg, const at::Tensor& x) {
-  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "omq::", name, ": ", arg,
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "omq_net::", name, ": ", arg,
               " must have a last dimension of at least 1");
 }
 
@@ -118,7 +118,7 @@ at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, doub
   const c10::Device dev = common_device(name, {&weight, &ids});
   const bool wide = ids_are_64(name, "ids", ids);
   const int type = type_of(name, "weight", weight);
-  TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "omq::", name,
+  TORCH_CHECK(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1, "omq_net::", name,
               ": weight must be [vocabulary, dim]");
   const int64_t stride = row_stride(name, "weight", weight);
   auto shape = ids.sizes().vec();
@@ -141,11 +141,11 @@ at::Tensor token_embedding_grad(const at::Tensor& grad, const at::Tensor& ids,
   const bool wide = ids_are_64(name, "ids", ids);
   const int type = type_of(name, "grad", grad);
   check_rows_of(name, "grad", grad);
-  TORCH_CHECK(grad.sizes().slice(0, grad.dim() - 1) == ids.sizes(), "omq::", name,
+  TORCH_CHECK(grad.sizes().slice(0, grad.dim() - 1) == ids.sizes(), "omq_net::", name,
               ": grad must be ids' shape and a last dimension");
-  TORCH_CHECK(num_embeddings >= 1, "omq::", name, ": num_embeddings ", num_embeddings, " < 1");
+  TORCH_CHECK(num_embeddings >= 1, "omq_net::", name, ": num_embeddings ", num_embeddings, " < 1");
   const at::ScalarType to = dtype.value_or(grad.scalar_type());
-  TORCH_CHECK(to == grad.scalar_type() || to == at::kFloat, "omq::", name, ": dtype must be ",
+  TORCH_CHECK(to == grad.scalar_type() || to == at::kFloat, "omq_net::", name, ": dtype must be ",
               grad.scalar_type(), " or float32, not ", to);
   const int64_t dim = grad.size(-1), stride = row_stride(name, "grad", grad);
   at::Tensor out = at::empty({num_embeddings, dim}, grad.options().dtype(to));
@@ -162,13 +162,13 @@ at::Tensor token_embedding_grad(const at::Tensor& grad, const at::Tensor& ids,
 }
 
 // ---- dropout --------------------------------------------------------------------------------
-at::Tensor net_dropout(const at::Tensor& x, double p, int64_t seed, int64_t offset) {
-  const char* name = "net_dropout";
+at::Tensor dropout(const at::Tensor& x, double p, int64_t seed, int64_t offset) {
+  const char* name = "dropout";
   const c10::Device dev = common_device(name, {&x});
   const int type = type_of(name, "x", x);
   check_rows_of(name, "x", x);
   drops(name, p);
-  TORCH_CHECK(x.is_contiguous(), "omq::", name, ": tensors must be contiguous");
+  TORCH_CHECK(x.is_contiguous(), "omq_net::", name, ": tensors must be contiguous");
   at::Tensor out = at::empty(x.sizes(), x.options());
   if (dev.is_meta()) return out;
   const c10::hip::HIPGuard guard(dev.index());
@@ -216,7 +216,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_fp8(const at::Tensor
   check_rows_of(name, "x", x);
   const int type = type_of(name, "x", x), w_type = check_weight(name, weight, x);
   if (res) check_same(name, "residual", *res, x);
-  TORCH_CHECK(group == 0 || group == 128, "omq::", name, ": group must be 0 (a row) or 128, not ",
+  TORCH_CHECK(group == 0 || group == 128, "omq_net::", name, ": group must be 0 (a row) or 128, not ",
               group);
   const int64_t dim = x.size(-1), stride = row_stride(name, "x", x);
   const int64_t r_stride = res ? row_stride(name, "residual", *res) : 0;
@@ -273,7 +273,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_grad(
 const float* row_floats(const char* name, const char* arg, const at::Tensor& t, int64_t rows) {
   TORCH_CHECK(t.dim() == 1 && t.size(0) == rows && t.scalar_type() == at::kFloat &&
                   t.is_contiguous(),
-              "omq::", name, ": ", arg, " must be contiguous float32 [", rows, "]");
+              "omq_net::", name, ": ", arg, " must be contiguous float32 [", rows, "]");
   return t.is_meta() ? nullptr : t.data_ptr<float>();
 }
 
@@ -285,31 +285,31 @@ omq_policy_rows policy_rows(const char* name, const at::Tensor& logits, const at
   const at::Tensor *ref = get(ref_logp), *pi = get(target), *ok = get(legal);
   const c10::Device dev =
       common_device(name, {&logits, &actions, &advantages, &old_logp, ref, pi, ok});
-  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1, "omq::", name,
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1, "omq_net::", name,
               ": logits must be [rows, actions]");
-  TORCH_CHECK(!(ref && pi), "omq::", name, ": ref_logp and target exclude each other");
+  TORCH_CHECK(!(ref && pi), "omq_net::", name, ": ref_logp and target exclude each other");
   omq_policy_rows r{};
   r.rows = logits.size(0);
   r.actions = logits.size(1);
   r.dtype = type_of(name, "logits", logits);
   r.logits_stride = row_stride(name, "logits", logits);
   r.taken_are_64 = ids_are_64(name, "actions", actions);
-  TORCH_CHECK(actions.dim() == 1 && actions.size(0) == r.rows, "omq::", name,
+  TORCH_CHECK(actions.dim() == 1 && actions.size(0) == r.rows, "omq_net::", name,
               ": actions must be [", r.rows, "]");
   r.advantages = row_floats(name, "advantages", advantages, r.rows);
   r.old_logp = row_floats(name, "old_logp", old_logp, r.rows);
   if (ref) r.ref_logp = row_floats(name, "ref_logp", *ref, r.rows);
   if (pi) {
-    TORCH_CHECK(pi->sizes() == logits.sizes() && pi->scalar_type() == at::kFloat, "omq::", name,
+    TORCH_CHECK(pi->sizes() == logits.sizes() && pi->scalar_type() == at::kFloat, "omq_net::", name,
                 ": target must be float32 ", logits.sizes());
     r.target_stride = row_stride(name, "target", *pi);
   }
   if (ok) {
-    TORCH_CHECK(ok->sizes() == logits.sizes() && ok->scalar_type() == at::kBool, "omq::", name,
+    TORCH_CHECK(ok->sizes() == logits.sizes() && ok->scalar_type() == at::kBool, "omq_net::", name,
                 ": legal must be bool ", logits.sizes());
     r.legal_stride = row_stride(name, "legal", *ok);
   }
-  TORCH_CHECK(clip_low >= 0.0 && clip_high >= 0.0, "omq::", name, ": clip_low ", clip_low,
+  TORCH_CHECK(clip_low >= 0.0 && clip_high >= 0.0, "omq_net::", name, ": clip_low ", clip_low,
               " and clip_high ", clip_high, " must not be negative");
   r.clip_low = (float)clip_low;
   r.clip_high = (float)clip_high;
@@ -361,7 +361,7 @@ at::Tensor clipped_policy_loss_grad(const at::Tensor& logits, const at::Tensor& 
   common_device(name, {&logits, &stats, w});
   TORCH_CHECK(stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == 4 &&
                   stats.scalar_type() == at::kFloat && stats.is_contiguous(),
-              "omq::", name, ": stats must be those of clipped_policy_loss, [", r.rows, ", 4]");
+              "omq_net::", name, ": stats must be those of clipped_policy_loss, [", r.rows, ", 4]");
   const float* wp = w ? row_floats(name, "row_weight", *w, r.rows) : nullptr;
   at::Tensor grad =
       at::empty({r.rows, r.actions}, logits.options().memory_format(at::MemoryFormat::Contiguous));
@@ -419,13 +419,13 @@ const std::string kLossArgs =
 
 }  // namespace
 
-TORCH_LIBRARY_FRAGMENT(omq, m) {
+TORCH_LIBRARY(omq_net, m) {
   define(m, "token_embedding", "(Tensor ids, Tensor weight, float scale) -> Tensor",
          token_embedding);
   define(m, "token_embedding_grad",
          "(Tensor grad, Tensor ids, int num_embeddings, float scale, ScalarType? dtype) -> Tensor",
          token_embedding_grad);
-  define(m, "net_dropout", "(Tensor x, float p, int seed, int offset) -> Tensor", net_dropout);
+  define(m, "dropout", "(Tensor x, float p, int seed, int offset) -> Tensor", dropout);
   define(m, "add_rms_norm",
          "(Tensor x, Tensor? residual, Tensor weight, float eps, float p, int seed, int offset) "
          "-> (Tensor, Tensor)",

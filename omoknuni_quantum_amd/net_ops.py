@@ -33,7 +33,7 @@ NET_TORCH_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libom
 
 def _load_net_torch() -> None:
     """Loads libomq_net_torch.so, after the library it links."""
-    if hasattr(torch.ops.omq, "token_embedding"):
+    if hasattr(torch.ops.omq_net, "token_embedding"):
         return
     if not os.path.exists(NET_TORCH_PATH):
         raise _lib.LibraryNotBuilt(
@@ -46,15 +46,15 @@ def _load_net_torch() -> None:
 _load_net_torch()
 
 # (the overloads themselves: the packets look theirs up at every call)
-_EMBEDDING = torch.ops.omq.token_embedding.default
-_EMBEDDING_GRAD = torch.ops.omq.token_embedding_grad.default
-_DROPOUT = torch.ops.omq.net_dropout.default
-_NORM = torch.ops.omq.add_rms_norm.default
-_NORM_FP8 = torch.ops.omq.add_rms_norm_fp8.default
-_NORM_GRAD = torch.ops.omq.add_rms_norm_grad.default
-_LOSS = torch.ops.omq.clipped_policy_loss.default
-_LOSS_GRAD = torch.ops.omq.clipped_policy_loss_grad.default
-_LOSS_WITH_GRAD = torch.ops.omq.clipped_policy_loss_with_grad.default
+_EMBEDDING = torch.ops.omq_net.token_embedding.default
+_EMBEDDING_GRAD = torch.ops.omq_net.token_embedding_grad.default
+_DROPOUT = torch.ops.omq_net.dropout.default
+_NORM = torch.ops.omq_net.add_rms_norm.default
+_NORM_FP8 = torch.ops.omq_net.add_rms_norm_fp8.default
+_NORM_GRAD = torch.ops.omq_net.add_rms_norm_grad.default
+_LOSS = torch.ops.omq_net.clipped_policy_loss.default
+_LOSS_GRAD = torch.ops.omq_net.clipped_policy_loss_grad.default
+_LOSS_WITH_GRAD = torch.ops.omq_net.clipped_policy_loss_with_grad.default
 
 
 def _word(x: int) -> int:
