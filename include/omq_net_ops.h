@@ -39,7 +39,8 @@ extern "C" {
 /* limits of this build */
 #define OMQ_NET_MAX_NORM_DIM 16384    /* columns of a normed row (a row is held in registers) */
 #define OMQ_NET_MAX_DIM (1 << 20)     /* columns of an embedding row, of a dropout row */
-#define OMQ_NET_MAX_COUNT 2147483647  /* rows, tokens, vocabulary, actions */
+#define OMQ_NET_MAX_ACTIONS (1 << 30) /* columns of a policy loss's row */
+#define OMQ_NET_MAX_COUNT 2147483647  /* rows, tokens, vocabulary */
 
 int omq_net_abi_version(void);
 const char* omq_net_last_error(void);

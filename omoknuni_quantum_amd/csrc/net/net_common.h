@@ -14,52 +14,142 @@ constexpr int kWave = 64;
 using bf16 = __bf16;
 using f16 = _Float16;
 
-// Eight elements are the unit of work of a lane: 16 bytes of a 16-bit type.  The types carry the
-// alignment of one element: gfx950 loads and stores 16 bytes at any address that an element may
-// have, so odd row lengths and sliced tensors take the same instructions as aligned ones.
+// Eight elements (a block) are the unit of work of a lane: 16 bytes of a 16-bit type.  The types
+// carry the alignment of one element: gfx950 loads and stores 16 bytes at any address that an
+// element may have, so odd row lengths and sliced tensors take the same instructions as aligned
+// ones.
+//
+// Loading is in two steps, so that a lane has all its loads in flight before it waits for one:
+// load_raw is free of branches (a block that is not whole, or beyond the row, is read from the
+// row's last eight elements), and to_front and block_of_raw, where the values are used, move a
+// part block's elements to the front (and fill up with zeros).  A branch at the load would make the compiler
+// wait for each load before the next: the sums of the embedding's gradient ran at 2.5 TB/s so.
+//
+// kWhole: rows are whole blocks (the columns a multiple of 8), and all this is left out.
 template <class T>
 using Vec8 __attribute__((aligned(sizeof(T)))) = T __attribute__((ext_vector_type(8)));
+template <class T>
+using Reg8 = T __attribute__((ext_vector_type(8)));
 using F8 = float __attribute__((ext_vector_type(8)));
 
-template <class T>
-__device__ inline F8 to_f8(Vec8<T> v) {
-  return __builtin_convertvector(v, F8);
-}
-
-// Eight elements from p, of which n are there (n >= 8: all); the others are `fill`.
-template <class T>
-__device__ inline Vec8<T> load_raw(const T* p, int n, T fill = T(0)) {
-  if (n >= 8) return *reinterpret_cast<const Vec8<T>*>(p);
-  Vec8<T> v;
+// The block at column col (a multiple of 8) of a row of `dim` elements, as described above.
+template <class T, bool kWhole>
+__device__ inline Reg8<T> load_raw(const T* row, int col, int dim) {
+  const int last = dim - 8;
+  if (kWhole || dim >= 8) return *reinterpret_cast<const Vec8<T>*>(row + (col < last ? col : last));
+  Reg8<T> v = {};  // (a row shorter than a block: uniform over the launch)
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : fill;
+  for (int j = 0; j < 7; ++j)
+    if (j < dim) v[j] = row[j];
   return v;
 }
 
-template <class T>
-__device__ inline F8 load8(const T* p, int n) {
-  return to_f8<T>(load_raw<T>(p, n));
+// The block moved to the front; what follows the row's end is whatever was there.
+template <class T, bool kWhole>
+__device__ inline Reg8<T> to_front(Reg8<T> v, int col, int dim) {
+  if (!kWhole && dim >= 8) {
+    const int s = dim - col < 8 ? (col - dim) & 7 : 0;  // the places to move by
+    if constexpr (sizeof(T) == 2) {
+      using U4 = uint32_t __attribute__((ext_vector_type(4)));
+      U4 d = __builtin_bit_cast(U4, v);
+      const bool four = s & 4, two = s & 2;
+      const uint32_t one = (s & 1) * 16;
+      d[0] = four ? d[2] : d[0], d[1] = four ? d[3] : d[1];
+      d[0] = two ? d[1] : d[0], d[1] = two ? d[2] : d[1], d[2] = two ? d[3] : d[2];
+      d[0] = __builtin_amdgcn_alignbit(d[1], d[0], one);
+      d[1] = __builtin_amdgcn_alignbit(d[2], d[1], one);
+      d[2] = __builtin_amdgcn_alignbit(d[3], d[2], one);
+      d[3] >>= one;
+      v = __builtin_bit_cast(Reg8<T>, d);
+    } else {
+      const bool four = s & 4, two = s & 2, one = s & 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = four ? v[j + 4] : v[j];
+#pragma unroll
+      for (int j = 0; j < 6; ++j) v[j] = two ? v[j + 2] : v[j];
+#pragma unroll
+      for (int j = 0; j < 7; ++j) v[j] = one ? v[j + 1] : v[j];
+    }
+  }
+  return v;
 }
 
-// Rounds to T (to nearest even) and stores the first n of eight.
-template <class T>
-__device__ inline void store8(T* p, F8 v, int n) {
-  using V = T __attribute__((ext_vector_type(8)));
-  const V t = __builtin_convertvector(v, V);
-  if (n >= 8) {
-    *reinterpret_cast<Vec8<T>*>(p) = t;
-  } else {
+// The same with zeros from column dim on.
+template <class T, bool kWhole>
+__device__ inline Reg8<T> block_of_raw(Reg8<T> v, int col, int dim) {
+  v = to_front<T, kWhole>(v, col, dim);
+  const int n = dim - col;
+  if constexpr (kWhole) {
+    if (n <= 0) v = Reg8<T>{};
+  } else if (n < 8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = t[j];
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] : T(0);
+  }
+  return v;
+}
+
+template <class T, bool kWhole>
+__device__ inline F8 widen(Reg8<T> v, int col, int dim) {
+  return __builtin_convertvector((block_of_raw<T, kWhole>(v, col, dim)), F8);
+}
+
+// Rounds to T (to nearest even) and stores the block at column col of the row.  kStream: past the
+// caches, for what this kernel does not read again while it still needs what they hold.
+template <class T, bool kWhole, bool kStream = false>
+__device__ inline void store8(T* row, int col, int dim, F8 v) {
+  Reg8<T> t = __builtin_convertvector(v, Reg8<T>);
+  T* p = row + col;
+  const int n = dim - col;
+  if (kWhole ? n > 0 : n >= 8) {
+    if constexpr (kStream)
+      __builtin_nontemporal_store(t, reinterpret_cast<Vec8<T>*>(p));
+    else
+      *reinterpret_cast<Vec8<T>*>(p) = t;
+  } else if (!kWhole && n > 0) {
+    using V4 __attribute__((aligned(sizeof(T)))) = T __attribute__((ext_vector_type(4)));
+    using V2 __attribute__((aligned(sizeof(T)))) = T __attribute__((ext_vector_type(2)));
+    if (n & 4) {
+      *reinterpret_cast<V4*>(p) = V4{t[0], t[1], t[2], t[3]};
+      p += 4;
+      t = Reg8<T>{t[4], t[5], t[6], t[7], T(0), T(0), T(0), T(0)};
+    }
+    if (n & 2) {
+      *reinterpret_cast<V2*>(p) = V2{t[0], t[1]};
+      p += 2;
+      t[0] = t[2];
+    }
+    if (n & 1) *p = t[0];
   }
 }
 
-// A weight of the rows' type or of float32.
+// A weight of the rows' type or of float32 (uniform over the launch).
 template <class T>
-__device__ inline F8 load_weight(const void* w, bool w_f32, int64_t at, int n) {
-  return w_f32 ? load8<float>(static_cast<const float*>(w) + at, n)
-               : load8<T>(static_cast<const T*>(w) + at, n);
+struct Weight8 {
+  Reg8<T> t;
+  F8 f;
+};
+
+template <class T, bool kWhole>
+__device__ inline Weight8<T> load_weight(const void* w, bool w_f32, int col, int dim) {
+  Weight8<T> r = {};
+  if (w_f32)
+    r.f = load_raw<float, kWhole>(static_cast<const float*>(w), col, dim);
+  else
+    r.t = load_raw<T, kWhole>(static_cast<const T*>(w), col, dim);
+  return r;
+}
+
+template <class T, bool kWhole>
+__device__ inline F8 widen(const Weight8<T>& w, bool w_f32, int col, int dim) {
+  return w_f32 ? widen<float, kWhole>(w.f, col, dim) : widen<T, kWhole>(w.t, col, dim);
+}
+
+// Which of the rows of its workgroup a thread belongs to, kThreads threads a row: a scalar where
+// a row has whole waves.
+template <int kThreads>
+__device__ inline int row_slot() {
+  const int slot = threadIdx.x / kThreads;
+  return kThreads >= kWave ? __builtin_amdgcn_readfirstlane(slot) : slot;
 }
 
 // ---- reductions ---------------------------------------------------------------------------
@@ -146,9 +236,14 @@ inline Dropout make_dropout(double p, uint64_t seed, uint64_t offset) {
   return d;
 }
 
-// Eight elements from column 8*block of a row whose quads begin at `quad0`.
-__device__ inline F8 drop8(F8 v, const Dropout& d, uint64_t quad0, uint32_t block) {
-  const uint64_t at = d.base + kGolden * (quad0 + 2ull * block);
+// What the words of a row start from.
+__device__ inline uint64_t drop_row(const Dropout& d, int64_t row, int dim) {
+  return d.base + kGolden * ((uint64_t)row * (uint32_t)((dim + 3) / 4));
+}
+
+// The block at column col of the row.
+__device__ inline F8 drop8(F8 v, const Dropout& d, uint64_t row_base, int col) {
+  const uint64_t at = row_base + kGolden * (uint32_t)(col / 4);
   const uint64_t w0 = mix64(at), w1 = mix64(at + kGolden);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

@@ -9,19 +9,17 @@ int check_dropout(const char* name, double p);
 
 namespace {
 
-template <class T>
+template <class T, bool kWhole>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t rows, int dim,
                                                       int blocks, Dropout d, T* out) {
   const int64_t first = (int64_t)blockIdx.x * 256;
   const int64_t row0 = first / blocks;
   const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
   const int64_t row = row0 + in / (uint32_t)blocks;
-  const uint32_t block = in % (uint32_t)blocks;
+  const int col = 8 * (int)(in % (uint32_t)blocks);
   if (row >= rows) return;
-  const int n = dim - 8 * (int)block;
-  const int64_t at = row * dim + 8 * block;
-  const F8 v = drop8(load8<T>(x + at, n), d, (uint64_t)row * (uint32_t)((dim + 3) / 4), block);
-  store8<T>(out + at, v, n);
+  const F8 v = widen<T, kWhole>(load_raw<T, kWhole>(x + row * dim, col, dim), col, dim);
+  store8<T, kWhole>(out + row * dim, col, dim, drop8(v, d, drop_row(d, row, dim), col));
 }
 
 }  // namespace
@@ -49,8 +47,9 @@ extern "C" int omq_dropout(const void* x, int64_t rows, int64_t dim, int dtype, 
   hipStream_t st = (hipStream_t)stream;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    dropout_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(x), rows, (int)dim, blocks, d,
-                                            static_cast<T*>(out));
+    const auto kernel = dim % 8 == 0 ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+    kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(x), rows, (int)dim, blocks, d,
+                                 static_cast<T*>(out));
   };
   if (dtype == OMQ_NET_F32) go(float{});
   else if (dtype == OMQ_NET_BF16) go(bf16{});

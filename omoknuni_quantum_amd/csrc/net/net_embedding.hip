@@ -16,7 +16,7 @@ namespace omq_net {
 namespace {
 
 // ---- forward --------------------------------------------------------------------------------
-template <class T, class Id>
+template <class T, class Id, bool kWhole>
 __global__ __launch_bounds__(256) void embed_kernel(const Id* __restrict__ ids, int64_t tokens,
                                                     const T* __restrict__ weight,
                                                     int64_t weight_stride, int64_t vocab,
@@ -29,16 +29,16 @@ __global__ __launch_bounds__(256) void embed_kernel(const Id* __restrict__ ids, 
   const int col = 8 * (int)(in % (uint32_t)blocks);
   if (t >= tokens) return;
   const int64_t id = (int64_t)ids[t];
-  F8 v = {};
-  if (id >= 0 && id < vocab) v = load8<T>(weight + id * weight_stride + col, dim - col) * scale;
-  store8<T>(out + t * dim + col, v, dim - col);
+  const bool in_table = id >= 0 && id < vocab;
+  const Reg8<T> raw = load_raw<T, kWhole>(weight + (in_table ? id : 0) * weight_stride, col, dim);
+  store8<T, kWhole>(out + t * dim, col, dim, in_table ? widen<T, kWhole>(raw, col, dim) * scale : F8{});
 }
 
 // ---- sort -----------------------------------------------------------------------------------
 // A pair is (key, token).  Keys lie in [0, vocab]; `vocab` stands for an id outside the
 // vocabulary, so those tokens sort behind all others.
 constexpr int kMaxDigitBits = 11;
-constexpr int kTile = 2048;       // tokens of a workgroup of the radix passes
+constexpr int kTile = 1024;       // tokens of a workgroup of the radix passes
 constexpr int kSmallSort = 4096;  // tokens that one workgroup sorts in LDS
 
 template <class Id>
@@ -103,13 +103,13 @@ __device__ inline uint32_t take_places(uint32_t digit, int bits, bool here, uint
   return place;
 }
 
-// All passes of up to kSmallSort tokens in one workgroup.  8-bit digits.
-template <class Id>
-__global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__ ids, int tokens,
+// All passes of up to kThreads * kRounds tokens in one workgroup.  8-bit digits.
+template <class Id, int kThreads, int kRounds>
+__global__ __launch_bounds__(kThreads) void sort_small_kernel(const Id* __restrict__ ids, int tokens,
                                                           int64_t vocab, int bits,
                                                           uint2* __restrict__ pairs) {
-  constexpr int kWaves = 16, kRounds = kSmallSort / 1024;
-  __shared__ uint2 kept[kSmallSort];
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ uint2 kept[kThreads * kRounds];
   __shared__ uint32_t next[kWaves][256];
   __shared__ uint32_t base[256];
   __shared__ uint32_t wave_sums[kWaves];
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__
     if (i < tokens) mine[r] = make_uint2(key_of(ids, i, vocab), (uint32_t)i);
   }
   for (int shift = 0; shift < bits; shift += 8) {
-    for (int j = threadIdx.x; j < kWaves * 256; j += 1024) (&next[0][0])[j] = 0;
+    for (int j = threadIdx.x; j < kWaves * 256; j += kThreads) (&next[0][0])[j] = 0;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
@@ -139,8 +139,8 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__
       base[threadIdx.x] = sum;
     }
     __syncthreads();
-    block_scan<1024>(base, 256, wave_sums);
-    for (int j = threadIdx.x; j < kWaves * 256; j += 1024) (&next[0][0])[j] += base[j & 255];
+    block_scan<kThreads>(base, 256, wave_sums);
+    for (int j = threadIdx.x; j < kWaves * 256; j += kThreads) (&next[0][0])[j] += base[j & 255];
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__
   }
 }
 
-// Radix pass, step 1: counts[digit * tiles + tile].
+// Radix pass, step 1: counts[tile * bins + digit].
 template <class Id>
 __global__ __launch_bounds__(256) void digit_counts_kernel(const Id* __restrict__ ids,
                                                            const uint2* __restrict__ in,
@@ -174,42 +174,61 @@ __global__ __launch_bounds__(256) void digit_counts_kernel(const Id* __restrict_
                                                            uint32_t* __restrict__ counts) {
   __shared__ uint32_t hist[1 << kMaxDigitBits];
   const int bins = 1 << bits;
-  for (int j = threadIdx.x; j < bins; j += 256) hist[j] = 0;
-  __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * kTile;
+  uint32_t key[kTile / 256];
 #pragma unroll
   for (int r = 0; r < kTile / 256; ++r) {
     const int64_t t = first + r * 256 + threadIdx.x;
-    if (t < tokens) {
-      const uint32_t key = in ? in[t].x : key_of(ids, t, vocab);
-      atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
-    }
+    if (t < tokens) key[r] = in ? in[t].x : key_of(ids, t, vocab);
   }
+  for (int j = threadIdx.x; j < bins; j += 256) hist[j] = 0;
   __syncthreads();
-  for (int j = threadIdx.x; j < bins; j += 256)
-    counts[(int64_t)j * gridDim.x + blockIdx.x] = hist[j];
+#pragma unroll
+  for (int r = 0; r < kTile / 256; ++r)
+    if (first + r * 256 + threadIdx.x < tokens)
+      atomicAdd(&hist[(key[r] >> shift) & (bins - 1)], 1u);
+  __syncthreads();
+  for (int j = threadIdx.x; j < bins; j += 256) counts[(int64_t)blockIdx.x * bins + j] = hist[j];
 }
 
-// Step 2: per digit (one wave), the exclusive prefix sums over the tiles, and the total.
-__global__ __launch_bounds__(256) void digit_scan_kernel(uint32_t* __restrict__ counts, int tiles,
-                                                         int bins, uint32_t* __restrict__ totals) {
-  const int digit = blockIdx.x * 4 + threadIdx.x / kWave;
-  const int lane = threadIdx.x & (kWave - 1);
-  if (digit >= bins) return;
-  uint32_t* row = counts + (int64_t)digit * tiles;
-  uint32_t carry = 0;
-  for (int t0 = 0; t0 < tiles; t0 += kWave) {
-    const int t = t0 + lane;
-    const uint32_t mine = t < tiles ? row[t] : 0u;
-    uint32_t incl = mine;
-    for (int d = 1; d < kWave; d <<= 1) {
-      const uint32_t up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
-    if (t < tiles) row[t] = carry + incl - mine;
-    carry += __shfl(incl, kWave - 1);
+// Step 2: per digit, the exclusive prefix sums over the tiles, and the total.  A workgroup takes
+// 64 digits; its 16 waves take a sixteenth of the tiles each.
+__global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__ counts, int tiles,
+                                                          int bins, uint32_t* __restrict__ totals) {
+  __shared__ uint32_t sums[16][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int digit = blockIdx.x * kWave + lane;
+  const int per = (tiles + 15) / 16;
+  const int from = wave * per, to = from + per < tiles ? from + per : tiles;
+  // (eight loads in flight, the last ones too)
+  const uint32_t* column = counts + (digit < bins ? digit : bins - 1);
+  const auto eight = [&](int t, uint32_t (&c)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) c[u] = column[(int64_t)(t + u < to ? t + u : t) * bins];
+  };
+  uint32_t sum = 0;
+  for (int t = from; t < to; t += 8) {
+    uint32_t c[8];
+    eight(t, c);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += t + u < to ? c[u] : 0u;
   }
-  if (lane == 0) totals[digit] = carry;
+  sums[wave][lane] = sum;
+  __syncthreads();
+  uint32_t base = 0;
+  for (int w = 0; w < wave; ++w) base += sums[w][lane];
+  if (digit >= bins) return;
+  if (wave == 15) totals[digit] = base + sum;
+  for (int t = from; t < to; t += 8) {
+    uint32_t c[8];
+    eight(t, c);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (t + u < to) {
+        counts[(int64_t)(t + u) * bins + digit] = base;
+        base += c[u];
+      }
+  }
 }
 
 // Step 3: every pair to its place.
@@ -218,22 +237,28 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(
     const Id* __restrict__ ids, const uint2* __restrict__ in, int64_t tokens, int64_t vocab,
     int shift, int bits, const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
     uint2* __restrict__ out) {
-  constexpr int kWaves = 4, kRounds = kTile / 256;
-  __shared__ uint32_t next[kWaves][1 << kMaxDigitBits];
-  __shared__ uint32_t base[1 << kMaxDigitBits];
+  constexpr int kWaves = 4, kRounds = kTile / 256, kBins = 1 << kMaxDigitBits;
+  __shared__ uint32_t next[kWaves][kBins];
+  __shared__ uint32_t base[kBins];
   __shared__ uint32_t wave_sums[kWaves];
   const int bins = 1 << bits;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int64_t first = (int64_t)blockIdx.x * kTile + wave * (kTile / kWaves);
   uint2 mine[kRounds];
+  uint32_t before[kBins / 256];  // of this thread's digits, in the tiles before
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int64_t t = first + r * kWave + lane;
     if (t < tokens) mine[r] = in ? in[t] : make_uint2(key_of(ids, t, vocab), (uint32_t)t);
   }
-  for (int j = threadIdx.x; j < bins; j += 256) {
-    base[j] = totals[j];
-    for (int w = 0; w < kWaves; ++w) next[w][j] = 0;
+#pragma unroll
+  for (int k = 0; k < kBins / 256; ++k) {
+    const int j = k * 256 + threadIdx.x;
+    if (j < bins) {
+      before[k] = counts[(int64_t)blockIdx.x * bins + j];
+      base[j] = totals[j];
+      for (int w = 0; w < kWaves; ++w) next[w][j] = 0;
+    }
   }
   __syncthreads();
   block_scan<256>(base, bins, wave_sums);
@@ -242,12 +267,16 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(
     if (first + r * kWave + lane < tokens)
       atomicAdd(&next[wave][(mine[r].x >> shift) & (bins - 1)], 1u);
   __syncthreads();
-  for (int j = threadIdx.x; j < bins; j += 256) {
-    uint32_t at = base[j] + counts[(int64_t)j * gridDim.x + blockIdx.x];
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t c = next[w][j];
-      next[w][j] = at;
-      at += c;
+#pragma unroll
+  for (int k = 0; k < kBins / 256; ++k) {
+    const int j = k * 256 + threadIdx.x;
+    if (j < bins) {
+      uint32_t at = base[j] + before[k];
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t c = next[w][j];
+        next[w][j] = at;
+        at += c;
+      }
     }
   }
   __syncthreads();
@@ -269,129 +298,220 @@ struct Piece {
   int32_t unused;
 };
 
-// The number of tokens among the first `at` items of the merged list, by a search in which the
-// kLanes lanes of a piece probe together: each step leaves 1/(kLanes+1) of the range.
+// The numbers of tokens among the first at[0] and at[1] items of the merged list: two searches
+// side by side, in each of which the kLanes lanes of a piece probe together, so that a step
+// leaves 1/(kLanes+1) of the range.
 template <int kLanes>
-__device__ inline int64_t tokens_before(const uint2* pairs, int64_t tokens, int64_t vocab,
-                                        int64_t at) {
-  int64_t lo = at > vocab ? at - vocab : 0, hi = at < tokens ? at : tokens;
+__device__ inline void tokens_before(const uint2* pairs, int64_t tokens, int64_t vocab,
+                                     const int64_t (&at)[2], int64_t (&found)[2]) {
+  int64_t lo[2], hi[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    lo[k] = at[k] > vocab ? at[k] - vocab : 0;
+    hi[k] = at[k] < tokens ? at[k] : tokens;
+  }
   const int lane = threadIdx.x & (kLanes - 1);
   const int shift = (threadIdx.x & (kWave - 1)) & ~(kLanes - 1);
-  while (__any(lo < hi)) {  // (the pieces of a wave go on until the last is done)
-    const int64_t n = hi - lo;
-    // probes lo + n*(lane+1)/(kLanes+1), in [lo, hi)
-    const int64_t i = lo + n * (lane + 1) / (kLanes + 1);
-    const bool before = n > 0 && (int64_t)pairs[i < hi ? i : hi - 1].x <= at - i - 1;
-    // token i is among the first `at` items; true for a prefix of the probes
-    const uint64_t all = __ballot(before) >> shift;
-    const int count = __popcll(kLanes == 64 ? all : all & ((1ull << (kLanes & 63)) - 1));
-    if (n > 0) {
-      const int64_t new_lo = count > 0 ? lo + n * count / (kLanes + 1) + 1 : lo;
-      const int64_t new_hi = count < kLanes ? lo + n * (count + 1) / (kLanes + 1) : hi;
-      lo = new_lo;
-      hi = new_hi;
+  while (__any(lo[0] < hi[0] || lo[1] < hi[1])) {  // (until the last piece of the wave is done)
+    bool before[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      // probe lo + n*(lane+1)/(kLanes+1), in [lo, hi): is that token among the first `at` items?
+      const int64_t n = hi[k] - lo[k], i = lo[k] + n * (lane + 1) / (kLanes + 1);
+      before[k] = n > 0 && (int64_t)pairs[i].x <= at[k] - i - 1;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // true for a prefix of the probes
+      const int64_t n = hi[k] - lo[k];
+      const uint64_t all = __ballot(before[k]) >> shift;
+      const int count = __popcll(kLanes == 64 ? all : all & ((1ull << (kLanes & 63)) - 1));
+      if (n > 0) {
+        const int64_t from = lo[k];
+        if (count > 0) lo[k] = from + n * count / (kLanes + 1) + 1;
+        if (count < kLanes) hi[k] = from + n * (count + 1) / (kLanes + 1);
+      }
     }
   }
-  return lo;
+  found[0] = lo[0];
+  found[1] = lo[1];
 }
 
-template <class T, class O, int kLanes>
+// The value that lane `from` of this lane's group of kLanes holds; uniform over a whole wave
+// where the group is one (the loops over it are scalar then).
+template <int kLanes>
+__device__ inline uint32_t group_read(uint32_t v, int from) {
+  if constexpr (kLanes == kWave) return (uint32_t)__builtin_amdgcn_readlane((int)v, from);
+  return (uint32_t)__shfl((int)v, from, kLanes);
+}
+
+template <int kLanes>
+__device__ inline int64_t group_uniform(int64_t v) {
+  if constexpr (kLanes == kWave) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+  }
+  return v;
+}
+
+template <class T, class O, int kLanes, bool kWhole>
 __global__ __launch_bounds__(256) void sum_pieces_kernel(
     const T* __restrict__ grad, int64_t grad_stride, const uint2* __restrict__ pairs,
     int64_t tokens, int64_t vocab, int dim, float scale, int64_t piece, int64_t pieces,
     O* __restrict__ out, Piece* __restrict__ info, float* __restrict__ heads,
     float* __restrict__ tails) {
-  constexpr int kBatch = 4;  // rows of `grad` in flight
-  const int64_t c = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  const int col = 8 * (int)(blockIdx.y * kLanes + (threadIdx.x & (kLanes - 1)));
-  const int n = dim - col;
+  constexpr int kBatch = 8;  // rows of `grad` in flight
+  int64_t c = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if constexpr (kLanes == kWave)
+    c = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kLanes - 1);
+  const int col = 8 * (int)(blockIdx.y * kLanes + lane);
   const int64_t items = tokens + vocab;
   const int64_t d0 = c * piece < items ? c * piece : items;
   const int64_t d1 = d0 + piece < items ? d0 + piece : items;
-  int64_t i = tokens_before<kLanes>(pairs, tokens, vocab, d0);
-  const int64_t i1 = tokens_before<kLanes>(pairs, tokens, vocab, d1);
+  const int64_t ends[2] = {d0, d1};
+  int64_t at[2];
+  tokens_before<kLanes>(pairs, tokens, vocab, ends, at);
+  const int64_t i0 = group_uniform<kLanes>(at[0]), i1 = group_uniform<kLanes>(at[1]);
   if (c >= pieces) return;
-  int64_t row = d0 - i;
-  const int64_t row0 = row, row1 = d1 - i1;
-  const bool shared = row0 < vocab && i > 0 && (int64_t)pairs[i - 1].x == row0;
+  const int64_t row0 = d0 - i0, row1 = d1 - i1;
+  const bool shared = row0 < vocab && i0 > 0 && (int64_t)pairs[i0 - 1].x == row0;
+  int64_t row = row0;
   F8 acc = {};
   bool open = false;
   const auto end_row = [&]() {
-    if (n > 0) {
-      if (shared && row == row0)
-        store8<float>(heads + c * dim + col, acc, n);
-      else
-        store8<O>(out + row * dim + col, acc * scale, n);
-    }
+    if (shared && row == row0)
+      store8<float, kWhole>(heads + c * dim, col, dim, acc);
+    else
+      store8<O, kWhole>(out + row * dim, col, dim, acc * scale);
     acc = F8{};
     open = false;
     ++row;
   };
-  while (i < i1) {
-    uint2 p[kBatch];
-    F8 v[kBatch];
+  for (int64_t i = i0; i < i1; i += kLanes) {
+    const uint2 mine = i + lane < i1 ? pairs[i + lane] : make_uint2(0u, 0u);
+    const int here = i1 - i < kLanes ? (int)(i1 - i) : kLanes;
+    for (int k = 0; k < here; k += kBatch) {
+      Reg8<T> v[kBatch];
+      uint32_t key[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      p[u] = i + u < i1 ? pairs[i + u] : make_uint2(0xFFFFFFFFu, 0u);
-      if ((int64_t)p[u].x >= vocab) p[u].x = 0xFFFFFFFFu;
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (p[u].x != 0xFFFFFFFFu && n > 0)
-        v[u] = load8<T>(grad + (int64_t)p[u].y * grad_stride + col, n);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (p[u].x != 0xFFFFFFFFu) {
-        while (row < (int64_t)p[u].x) end_row();
-        if (n > 0) acc += v[u];
-        open = true;
+      for (int e = 0; e < kBatch; ++e) {
+        const int at = k + e < here ? k + e : here - 1;
+        key[e] = group_read<kLanes>(mine.x, at);
+        const uint32_t token = group_read<kLanes>(mine.y, at);
+        v[e] = load_raw<T, kWhole>(grad + (int64_t)token * grad_stride, col, dim);
       }
-    i += kBatch;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        if (k + e < here && (int64_t)key[e] < vocab) {
+          while (row < (int64_t)key[e]) end_row();
+          acc += widen<T, kWhole>(v[e], col, dim);
+          open = true;
+        }
+    }
   }
   while (row < row1) end_row();
-  if (open && n > 0) store8<float>(tails + c * dim + col, acc, n);
-  if (blockIdx.y == 0 && (threadIdx.x & (kLanes - 1)) == 0)
+  if (open) store8<float, kWhole>(tails + c * dim, col, dim, acc);
+  if (blockIdx.y == 0 && lane == 0)
     info[c] = Piece{shared && row1 > row0 ? (int32_t)row0 : -1, (int32_t)row1, open ? 1 : 0, 0};
 }
 
-// The row that piece c ends and did not begin: the sums that the pieces before it left open, in
-// their order, then its own.  64 columns a workgroup: 16 lanes of four columns, 16 slots of
-// pieces, the slots' sums added in order.
+// The rows that a piece ends and did not begin: the sums that the pieces before it left open (its
+// run), in their order, then its own.  A wave takes a piece and 256 columns, four a lane; a run of
+// more than kOwnRun pieces is taken by all 16 waves of the workgroup, every 16th piece each, and
+// their sums are added in order.
+constexpr int kJoinWaves = 16, kOwnRun = 32;
+
 template <class O>
-__global__ __launch_bounds__(256) void join_pieces_kernel(const Piece* __restrict__ info, int dim,
-                                                          float scale,
-                                                          const float* __restrict__ heads,
-                                                          const float* __restrict__ tails,
-                                                          O* __restrict__ out) {
-  __shared__ float part[16][64];
-  const int64_t c = blockIdx.x;
-  const int32_t row = info[c].first_row;
-  if (row < 0) return;
-  int64_t lo = 0, hi = c;  // the first piece at whose end `row` is open (or a later row)
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (info[mid].last_row >= row)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  const int slot = threadIdx.x / 16, col = blockIdx.y * 64 + 4 * (threadIdx.x & 15);
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t k = lo + slot; k < c; k += 16)
-    if (info[k].open) {
+__global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restrict__ info,
+                                                           int64_t pieces, int dim, float scale,
+                                                           const float* __restrict__ heads,
+                                                           const float* __restrict__ tails,
+                                                           O* __restrict__ out) {
+  using F4 = float __attribute__((ext_vector_type(4)));
+  __shared__ F4 part[kJoinWaves][kWave];
+  __shared__ int64_t run_from[kJoinWaves];  // of the long runs, else -1
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t c0 = (int64_t)blockIdx.x * kJoinWaves;
+  const int col = 4 * ((int)blockIdx.y * kWave + lane);
+  const auto four = [&](const float* p) {
+    F4 v = {};
+    if (col + 3 < dim) {
+      using F4u __attribute__((aligned(4))) = F4;
+      v = *reinterpret_cast<const F4u*>(p + col);
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col + j < dim) acc[j] += tails[k * dim + col + j];
+        if (col + j < dim) v[j] = p[col + j];
     }
+    return v;
+  };
+  const auto sum = [&](int64_t from, int64_t to, int step) {
+    F4 acc = {};
+    for (int64_t k = from; k < to; k += 8 * step) {  // eight loads in flight, the last ones too
+      F4 v[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) part[slot][4 * (threadIdx.x & 15) + j] = acc[j];
+      for (int u = 0; u < 8; ++u) v[u] = four(tails + (k + u * step < to ? k + u * step : k) * dim);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k + u * step < to) acc += v[u];
+    }
+    return acc;
+  };
+  const auto write = [&](int64_t c, F4 acc) {
+    acc += four(heads + c * dim);
+    const int64_t row = info[c].first_row;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < dim) out[row * dim + col + j] = (O)(acc[j] * scale);
+  };
+  const int64_t c = c0 + wave;
+  // lane 0: piece c - 1, lane 1: the one before, ...
+  const Piece own = c < pieces ? info[c] : Piece{-1, 0, 0, 0};
+  const Piece near = c < pieces && c - 1 - lane >= 0 ? info[c - 1 - lane] : Piece{-1, -1, 0, 0};
+  const int32_t row = own.first_row;
+  int64_t long_from = -1;
+  if (row >= 0) {
+    // the run: the pieces just before c at whose end `row` is open
+    const uint64_t all = __ballot(near.last_row == row);
+    int64_t from;
+    bool open;  // the first may end with the end of the row before; the others left something
+    if (~all != 0) {
+      const int n = __builtin_ctzll(~all);
+      from = c - n;
+      open = (__ballot(near.open != 0) >> (n - 1)) & 1;
+    } else {  // the first of all pieces whose last row is `row` or a later one
+      int64_t lo = 0, hi = c - kWave;
+      while (lo < hi) {
+        const int64_t n = hi - lo, i = lo + n * (lane + 1) / (kWave + 1);
+        const int below = __popcll(__ballot(info[i].last_row < row));
+        const int64_t was = lo;
+        if (below > 0) lo = was + n * below / (kWave + 1) + 1;
+        if (below < kWave) hi = was + n * (below + 1) / (kWave + 1);
+      }
+      from = lo;
+      open = info[from].open;
+    }
+    if (!open) ++from;
+    if (c - from <= kOwnRun)
+      write(c, sum(from, c, 1));
+    else
+      long_from = from;
+  }
+  if (lane == 0) run_from[wave] = long_from;
   __syncthreads();
-  const int at = blockIdx.y * 64 + threadIdx.x;
-  if (threadIdx.x < 64 && at < dim) {
-    float s = part[0][threadIdx.x];
-    for (int k = 1; k < 16; ++k) s += part[k][threadIdx.x];
-    s += heads[c * dim + at];
-    out[(int64_t)row * dim + at] = (O)(s * scale);
+  for (int w = 0; w < kJoinWaves; ++w) {
+    const int64_t from = run_from[w];
+    if (from < 0) continue;
+    F4 acc = sum(from + wave, c0 + w, kJoinWaves);
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+      for (int k = 1; k < kJoinWaves; ++k) acc += part[k][lane];
+      write(c0 + w, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -424,9 +544,13 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   p.col_tiles = (int)ceil_div(dim, 8 * p.lanes);
   // pieces for about 4096 waves, of 16 to 1024 items
   const int64_t items = tokens + vocab;
-  const int64_t wanted = ceil_div(4096ll * (kWave / p.lanes), p.col_tiles);
+#ifndef PW
+#define PW 4096ll
+#define PMIN 16
+#endif
+  const int64_t wanted = ceil_div(PW * (kWave / p.lanes), p.col_tiles);
   p.piece = ceil_div(items, wanted);
-  p.piece = p.piece < 16 ? 16 : p.piece > 1024 ? 1024 : p.piece;
+  p.piece = p.piece < PMIN ? PMIN : p.piece > 1024 ? 1024 : p.piece;
   p.pieces = ceil_div(items, p.piece);
   int64_t at = 0;
   p.at_pairs[0] = take(&at, 8 * tokens);
@@ -449,7 +573,15 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
                    reinterpret_cast<uint2*>(ws + p.at_pairs[1])};
   if (tokens == 0) return buf[0];
   if (tokens <= kSmallSort) {
-    sort_small_kernel<Id><<<1, 1024, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
+    const auto sort = [&](auto kernel, int threads) {
+      kernel<<<1, threads, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
+    };
+    if (tokens <= 256)
+      sort(sort_small_kernel<Id, 256, 1>, 256);
+    else if (tokens <= 1024)
+      sort(sort_small_kernel<Id, 1024, 1>, 1024);
+    else
+      sort(sort_small_kernel<Id, 1024, kSmallSort / 1024>, 1024);
     return buf[0];
   }
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.at_counts);
@@ -460,8 +592,8 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
     const int shift = pass * p.digit_bits, bins = 1 << p.digit_bits;
     digit_counts_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(ids, in, tokens, vocab, shift,
                                                               p.digit_bits, counts);
-    digit_scan_kernel<<<(uint32_t)ceil_div(bins, 4), 256, 0, st>>>(counts, (int)p.tiles, bins,
-                                                                 totals);
+    digit_scan_kernel<<<(uint32_t)ceil_div(bins, kWave), 1024, 0, st>>>(counts, (int)p.tiles, bins,
+                                                                      totals);
     digit_scatter_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(
         ids, in, tokens, vocab, shift, p.digit_bits, counts, totals, to);
     in = to;
@@ -477,12 +609,16 @@ void launch_sums(const GradPlan& p, const void* grad, int64_t grad_stride, const
   float* heads = reinterpret_cast<float*>(ws + p.at_heads);
   float* tails = reinterpret_cast<float*>(ws + p.at_tails);
   const dim3 grid((uint32_t)ceil_div(p.pieces, 256 / kLanes), (uint32_t)p.col_tiles);
-  sum_pieces_kernel<T, O, kLanes><<<grid, 256, 0, st>>>(
+  const auto kernel = dim % 8 == 0 ? sum_pieces_kernel<T, O, kLanes, true>
+                                   : sum_pieces_kernel<T, O, kLanes, false>;
+  kernel<<<grid, 256, 0, st>>>(
       static_cast<const T*>(grad), grad_stride, pairs, tokens, vocab, dim, scale, p.piece,
       p.pieces, static_cast<O*>(out), info, heads, tails);
   if (p.pieces > 1)
-    join_pieces_kernel<O><<<dim3((uint32_t)p.pieces, (uint32_t)ceil_div(dim, 64)), 256, 0, st>>>(
-        info, dim, scale, heads, tails, static_cast<O*>(out));
+    join_pieces_kernel<O><<<dim3((uint32_t)ceil_div(p.pieces, kJoinWaves),
+                                 (uint32_t)ceil_div(dim, 4 * kWave)),
+                            1024, 0, st>>>(info, p.pieces, dim, scale, heads, tails,
+                                           static_cast<O*>(out));
 }
 
 template <class T, class O, class... A>
@@ -500,7 +636,8 @@ void launch_embed(const void* ids, int64_t tokens, const void* weight, int64_t w
                   int64_t vocab, int dim, float scale, void* out, hipStream_t st) {
   const int blocks = (int)ceil_div(dim, 8);
   const int64_t groups = ceil_div(tokens * blocks, 256);
-  embed_kernel<T, Id><<<(uint32_t)groups, 256, 0, st>>>(
+  const auto kernel = dim % 8 == 0 ? embed_kernel<T, Id, true> : embed_kernel<T, Id, false>;
+  kernel<<<(uint32_t)groups, 256, 0, st>>>(
       static_cast<const Id*>(ids), tokens, static_cast<const T*>(weight), weight_stride, vocab,
       dim, blocks, scale, static_cast<T*>(out));
 }

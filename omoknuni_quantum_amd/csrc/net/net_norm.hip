@@ -7,6 +7,8 @@
 // registers between the reduction and their use.  A row belongs to kThreads threads with kVecs
 // times eight elements each: 16 to 64 lanes of a wave for short rows (no barrier), a workgroup
 // of 256 threads for rows over 2048 columns.
+#include <type_traits>
+
 #include "net_common.h"
 
 namespace omq_net {
@@ -29,7 +31,7 @@ enum Mode { kPlain, kDrop, kFp8Row, kFp8Group };
 
 template <int kThreads>
 constexpr int block_of() {
-  return kThreads < 256 ? 256 : kThreads;
+  return kThreads <= kWave ? 256 : kThreads;
 }
 
 __device__ inline uint2 to_fp8(F8 v, float inv) {
@@ -60,29 +62,35 @@ __device__ inline float largest(F8 v) {
 constexpr float kFp8Max = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;
 
-template <class T, int kThreads, int kVecs, int kMode>
+template <class T, int kThreads, int kVecs, int kMode, bool kWhole>
 __global__ __launch_bounds__(block_of<kThreads>()) void norm_kernel(NormArgs a) {
   constexpr int kRows = block_of<kThreads>() / kThreads;
   __shared__ float smem[2][16];
   const int lane = threadIdx.x % kThreads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads;
+  const int64_t row = (int64_t)blockIdx.x * kRows + row_slot<kThreads>();
   if (row >= a.rows) return;  // (whole rows leave: no barrier or reduction spans two rows)
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
-  T* hout = a.h ? static_cast<T*>(a.h) + row * a.dim : nullptr;
-  const uint64_t quad0 = (uint64_t)row * (uint32_t)((a.dim + 3) / 4);
+  const T* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
+  T* hout = static_cast<T*>(a.h) + row * a.dim;
+  const uint64_t drop = drop_row(a.drop, row, a.dim);
+  Reg8<T> x_raw[kVecs], res_raw[kVecs];
+  Weight8<T> w_raw[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (lane + i * kThreads);
+    x_raw[i] = load_raw<T, kWhole>(x, col, a.dim);
+    res_raw[i] = a.residual ? load_raw<T, kWhole>(res, col, a.dim) : Reg8<T>{};
+    w_raw[i] = load_weight<T, kWhole>(a.weight, a.w_f32, col, a.dim);
+  }
   F8 h[kVecs];
   float sq = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int col = 8 * (lane + i * kThreads), n = a.dim - col;
-    h[i] = F8{};
-    if (n > 0) {
-      h[i] = load8<T>(x + col, n);
-      if constexpr (kMode == kDrop) h[i] = drop8(h[i], a.drop, quad0, (uint32_t)col / 8);
-      if (res) h[i] += load8<T>(res + col, n);
-      if (hout) store8<T>(hout + col, h[i], n);
-    }
+    const int col = 8 * (lane + i * kThreads);
+    h[i] = widen<T, kWhole>(x_raw[i], col, a.dim);
+    if constexpr (kMode == kDrop) h[i] = drop8(h[i], a.drop, drop, col);
+    if (a.residual) h[i] += widen<T, kWhole>(res_raw[i], col, a.dim);
+    if (a.h) store8<T, kWhole>(hout, col, a.dim, h[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sq = fmaf(h[i][j], h[i][j], sq);
   }
@@ -92,9 +100,9 @@ __global__ __launch_bounds__(block_of<kThreads>()) void norm_kernel(NormArgs a) 
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int col = 8 * (lane + i * kThreads), n = a.dim - col;
-    if (n > 0) h[i] = h[i] * r * load_weight<T>(a.weight, a.w_f32, col, n);
+    h[i] = h[i] * r * widen<T, kWhole>(w_raw[i], a.w_f32, col, a.dim);
     if constexpr (kMode == kPlain || kMode == kDrop) {
-      if (n > 0) store8<T>(static_cast<T*>(a.y) + row * a.dim + col, h[i], n);
+      store8<T, kWhole>(static_cast<T*>(a.y) + row * a.dim, col, a.dim, h[i]);
     } else if constexpr (kMode == kFp8Row) {
       top = fmaxf(top, largest(h[i]));
     } else {
@@ -134,53 +142,59 @@ struct NormGradArgs {
 
 // A workgroup takes the rows blockIdx.x*kRows + slot, and every gridDim.x*kRows-th after them,
 // and keeps the sum of grad_y * n over them in registers.
-template <class T, int kThreads, int kVecs, bool kDropped>
+template <class T, int kThreads, int kVecs, bool kDropped, bool kWhole>
 __global__ __launch_bounds__(block_of<kThreads>()) void norm_grad_kernel(NormGradArgs a) {
   constexpr int kBlock = block_of<kThreads>(), kRows = kBlock / kThreads;
   __shared__ float smem[2][2][16];
   __shared__ float joined[kRows > 1 ? 8 * kThreads * kVecs : 1];
-  const int lane = threadIdx.x % kThreads, slot = threadIdx.x / kThreads;
+  const int lane = threadIdx.x % kThreads, slot = row_slot<kThreads>();
   F8 dw[kVecs] = {};
+  Weight8<T> w_raw[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+    w_raw[i] = load_weight<T, kWhole>(a.weight, a.w_f32, 8 * (lane + i * kThreads), a.dim);
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kRows + slot; row < a.rows;
        row += (int64_t)gridDim.x * kRows, turn ^= 1) {
     const T* gy = static_cast<const T*>(a.gy) + row * a.gy_stride;
     const T* hp = static_cast<const T*>(a.h) + row * a.h_stride;
-    F8 h[kVecs], g[kVecs];
+    const T* gh = static_cast<const T*>(a.gh) + row * a.gh_stride;
+    Reg8<T> h_raw[kVecs], g_raw[kVecs], gh_raw[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (lane + i * kThreads);
+      h_raw[i] = load_raw<T, kWhole>(hp, col, a.dim);
+      g_raw[i] = load_raw<T, kWhole>(gy, col, a.dim);
+      gh_raw[i] = a.gh ? load_raw<T, kWhole>(gh, col, a.dim) : Reg8<T>{};
+    }
     float sq = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (lane + i * kThreads), n = a.dim - col;
-      h[i] = F8{};
-      g[i] = F8{};
-      if (n > 0) {
-        h[i] = load8<T>(hp + col, n);
-        g[i] = load8<T>(gy + col, n);
-        const F8 gw = g[i] * load_weight<T>(a.weight, a.w_f32, col, n);
+      const int col = 8 * (lane + i * kThreads);
+      const F8 h = widen<T, kWhole>(h_raw[i], col, a.dim);
+      const F8 gw = widen<T, kWhole>(g_raw[i], col, a.dim) * widen<T, kWhole>(w_raw[i], a.w_f32, col, a.dim);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sq = fmaf(h[i][j], h[i][j], sq);
-          dot = fmaf(gw[j], h[i][j], dot);
-        }
+      for (int j = 0; j < 8; ++j) {
+        sq = fmaf(h[j], h[j], sq);
+        dot = fmaf(gw[j], h[j], dot);
       }
     }
     sq = row_reduce<Sum, kThreads>(sq, smem[turn][0]);
     dot = row_reduce<Sum, kThreads>(dot, smem[turn][1]);
     const float r = 1.0f / sqrtf(fmaf(sq, a.inv_dim, a.eps));
     const float k = dot * a.inv_dim * r * r;  // grad = r * (g*w - h*k) + grad_h
-    const uint64_t quad0 = (uint64_t)row * (uint32_t)((a.dim + 3) / 4);
+    const uint64_t drop = drop_row(a.drop, row, a.dim);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (lane + i * kThreads), n = a.dim - col;
-      if (n > 0) {
-        dw[i] += g[i] * h[i] * r;
-        F8 d = (g[i] * load_weight<T>(a.weight, a.w_f32, col, n) - h[i] * k) * r;
-        if (a.gh) d += load8<T>(static_cast<const T*>(a.gh) + row * a.gh_stride + col, n);
-        if (a.gr) store8<T>(static_cast<T*>(a.gr) + row * a.dim + col, d, n);
-        if constexpr (kDropped)
-          store8<T>(static_cast<T*>(a.gx) + row * a.dim + col,
-                    drop8(d, a.drop, quad0, (uint32_t)col / 8), n);
-      }
+      const int col = 8 * (lane + i * kThreads);
+      const F8 h = widen<T, kWhole>(h_raw[i], col, a.dim), g = widen<T, kWhole>(g_raw[i], col, a.dim);
+      dw[i] += g * h * r;
+      F8 d = (g * widen<T, kWhole>(w_raw[i], a.w_f32, col, a.dim) - h * k) * r;
+      if (a.gh) d += widen<T, kWhole>(gh_raw[i], col, a.dim);
+      if (a.gr) store8<T, kWhole>(static_cast<T*>(a.gr) + row * a.dim, col, a.dim, d);
+      if constexpr (kDropped)
+        store8<T, kWhole>(static_cast<T*>(a.gx) + row * a.dim, col, a.dim,
+                  drop8(d, a.drop, drop, col));
     }
   }
   if (!a.partial) return;
@@ -202,28 +216,37 @@ __global__ __launch_bounds__(block_of<kThreads>()) void norm_grad_kernel(NormGra
   if (slot == kRows - 1) {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (lane + i * kThreads), n = a.dim - col;
-      if (n > 0) store8<float>(a.partial + (int64_t)blockIdx.x * a.dim + col, dw[i], n);
+      const int col = 8 * (lane + i * kThreads);
+      store8<float, kWhole>(a.partial + (int64_t)blockIdx.x * a.dim, col, a.dim, dw[i]);
     }
   }
 }
 
-// grad_weight from the workgroups' sums: 16 columns and 16 slices of the sums a workgroup.
+// grad_weight from the workgroups' sums: a workgroup takes 32 columns (a line of memory), 32
+// slices of the sums side by side, the slices added in order.
 template <class O>
-__global__ __launch_bounds__(256) void join_weight_kernel(const float* __restrict__ partial,
-                                                          int groups, int dim,
-                                                          O* __restrict__ out) {
-  __shared__ float part[16][16];
-  const int c = threadIdx.x % 16, slice = threadIdx.x / 16;
-  const int col = blockIdx.x * 16 + c;
+__global__ __launch_bounds__(1024) void join_weight_kernel(const float* __restrict__ partial,
+                                                           int groups, int dim,
+                                                           O* __restrict__ out) {
+  __shared__ float part[32][33];
+  const int c = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const int col = blockIdx.x * 32 + c;
   float s = 0.0f;
-  if (col < dim)
-    for (int g = slice; g < groups; g += 16) s += partial[(int64_t)g * dim + col];
+  if (col < dim) {
+    for (int g = slice; g < groups; g += 32 * 8) {  // eight loads in flight, the last ones too
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = partial[(int64_t)(g + 32 * u < groups ? g + 32 * u : g) * dim + col];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += g + 32 * u < groups ? v[u] : 0.0f;
+    }
+  }
   part[slice][c] = s;
   __syncthreads();
-  if (threadIdx.x < 16 && col < dim) {
+  if (threadIdx.x < 32 && col < dim) {
     s = part[0][c];
-    for (int k = 1; k < 16; ++k) s += part[k][c];
+    for (int k = 1; k < 32; ++k) s += part[k][c];
     out[col] = (O)s;
   }
 }
@@ -240,11 +263,11 @@ void with_layout(int64_t dim, F&& f) {
   if (dim <= 128) return f(Layout<16, 1>{});
   if (dim <= 256) return f(Layout<32, 1>{});
   if (dim <= 512) return f(Layout<64, 1>{});
-  if (dim <= 1024) return f(Layout<64, 2>{});
-  if (dim <= 2048) return f(Layout<64, 4>{});
-  if (dim <= 4096) return f(Layout<256, 2>{});
-  if (dim <= 8192) return f(Layout<256, 4>{});
-  return f(Layout<256, 8>{});
+  if (dim <= 1024) return f(Layout<128, 1>{});
+  if (dim <= 2048) return f(Layout<256, 1>{});
+  if (dim <= 4096) return f(Layout<512, 1>{});
+  if (dim <= 8192) return f(Layout<1024, 1>{});
+  return f(Layout<1024, 2>{});
 }
 
 template <class F>
@@ -262,21 +285,26 @@ void launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
       using L = decltype(l);
       constexpr int kBlock = block_of<L::kThreads>();
       const int64_t grid = ceil_div(a.rows, kBlock / L::kThreads);
-      norm_kernel<T, L::kThreads, L::kVecs, kMode><<<(uint32_t)grid, kBlock, 0, st>>>(a);
+      const auto kernel = a.dim % 8 == 0 ? norm_kernel<T, L::kThreads, L::kVecs, kMode, true>
+                                         : norm_kernel<T, L::kThreads, L::kVecs, kMode, false>;
+      kernel<<<(uint32_t)grid, kBlock, 0, st>>>(a);
     });
   });
 }
 
-// Workgroups of the gradient: as many as run at once (four of 256 threads a compute unit).
-constexpr int64_t kGradGroups = 1024;
+// Workgroups of the gradient: as many as run at once.
+constexpr int64_t kGradWaves = 256 * 16;
 
 int64_t grad_groups(int64_t rows, int64_t dim) {
   int64_t groups = 0;
   with_layout(dim, [&](auto l) {
     using L = decltype(l);
-    groups = ceil_div(rows, block_of<L::kThreads>() / L::kThreads);
+    constexpr int kBlock = block_of<L::kThreads>();
+    const int64_t all = ceil_div(rows, kBlock / L::kThreads);
+    const int64_t most = kGradWaves * kWave / kBlock;
+    groups = all < most ? all : most;
   });
-  return groups < kGradGroups ? groups : kGradGroups;
+  return groups;
 }
 
 int check_norm(const char* name, int64_t rows, int64_t dim, int dtype, int weight_dtype) {
@@ -396,19 +424,23 @@ int omq_add_rms_norm_grad(const void* grad_y, int64_t grad_y_stride, const void*
       with_layout(dim, [&](auto l) {
         using L = decltype(l);
         constexpr int kBlock = block_of<L::kThreads>();
+        const auto go = [&](auto dropped, auto whole) {
+          norm_grad_kernel<T, L::kThreads, L::kVecs, dropped.value, whole.value>
+              <<<(uint32_t)groups, kBlock, 0, st>>>(a);
+        };
+        using Yes = std::true_type;
+        using No = std::false_type;
         if (a.drop.threshold)
-          norm_grad_kernel<T, L::kThreads, L::kVecs, true>
-              <<<(uint32_t)groups, kBlock, 0, st>>>(a);
+          dim % 8 == 0 ? go(Yes{}, Yes{}) : go(Yes{}, No{});
         else
-          norm_grad_kernel<T, L::kThreads, L::kVecs, false>
-              <<<(uint32_t)groups, kBlock, 0, st>>>(a);
+          dim % 8 == 0 ? go(No{}, Yes{}) : go(No{}, No{});
       });
     });
   if (grad_weight) {
-    const uint32_t grid = (uint32_t)ceil_div(dim, 16);
+    const uint32_t grid = (uint32_t)ceil_div(dim, 32);
     with_type(weight_dtype, [&](auto t) {
       using O = decltype(t);
-      join_weight_kernel<O><<<grid, 256, 0, st>>>(static_cast<const float*>(workspace),
+      join_weight_kernel<O><<<grid, 1024, 0, st>>>(static_cast<const float*>(workspace),
                                                   (int)groups, (int)dim,
                                                   static_cast<O*>(grad_weight));
     });

@@ -1,16 +1,18 @@
 // The clipped policy loss over legal actions with a KL term, and its gradient (gfx950).
 //
-// Per row, with m the largest legal logit, s = sum e^(z-m), tp = sum pi, tz = sum pi (z - m) and
-// tl = sum pi log pi over the legal actions (pi the target):
+// Per row, about a base m near the largest legal logit, with s = sum e^(z-m), tp = sum pi and
+// tk = sum pi (log pi - (z - m)) over the legal actions (pi the target):
 //   logq_a = z_a - m - log s
-//   kl     = tl - tz + tp log s
+//   kl     = tk + tp log s
 //   dz_a   = push p_a + slope [a taken] - kl_coef pi_a,   p_a = e^(z_a - m) / s,
 // where slope is the loss's derivative by logp and push = kl_coef tp - slope.
 //
-// One pass over the logits where the row fits the registers of the threads that share it (the
-// maximum, the sums and the gradient all come from the same loads); longer rows, and rows so
-// few that they would leave most of the chip idle, are cut into spans whose running (m, s, tp,
-// tz, tl) are joined, and the gradient is a second, element-wise pass.  Bound by memory.
+// Bound by memory.  Three ways through a row:
+//   - short rows are held in registers: the base, the sums and the gradient come from one load;
+//   - a long row is read twice by its workgroup, for the sums and for the gradient, the second
+//     time from the last-level cache (256 MB; the rows under way are 64 KB to 1 MB each);
+//   - where the long rows are too few to occupy the chip they are cut into spans, a workgroup
+//     each; their statistics are joined, and the gradient is an element-wise launch.
 #include "net_common.h"
 
 namespace omq_net {
@@ -18,34 +20,53 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-// Running statistics of a part of a row.
+// Statistics of a part of a row; m is -inf while nothing in it has weight.
 struct Stats {
-  float m, s, tp, tz, tl;
+  float m, s, tp, tk;
 };
 
-__device__ inline Stats no_stats() { return Stats{-kInf, 0.0f, 0.0f, 0.0f, 0.0f}; }
+__device__ inline Stats no_stats() { return Stats{-kInf, 0.0f, 0.0f, 0.0f}; }
 
 __device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// m for exponents: -inf (nothing legal yet) and +-inf logits must not give inf - inf where the
-// true weight is 0.
+// The base that the sums of a part with base m were formed about.
 __device__ inline float base_of(float m) { return m == -kInf ? 0.0f : m; }
 
-__device__ inline Stats join(const Stats& a, const Stats& b) {
-  Stats r;
-  r.m = fmaxf(a.m, b.m);
-  const float base = base_of(r.m);
-  const float ea = a.m == r.m ? 1.0f : exp_fast(a.m - base);
-  const float eb = b.m == r.m ? 1.0f : exp_fast(b.m - base);
-  r.s = a.s * ea + b.s * eb;
-  r.tp = a.tp + b.tp;
-  r.tl = a.tl + b.tl;
-  // sum pi (z - m) about another m; a part whose m is -inf was formed about 0
-  r.tz = a.tz + b.tz;
-  if (a.tp != 0.0f) r.tz += a.tp * (base_of(a.m) - base);
-  if (b.tp != 0.0f) r.tz += b.tp * (base_of(b.m) - base);
-  return r;
+// The statistics about another base, which is finite or that of a part without weight.
+__device__ inline void rebase(Stats& t, float m) {
+  if (t.m != m) {
+    t.s *= exp_fast(t.m - base_of(m));
+    if (t.tp != 0.0f) t.tk -= t.tp * (base_of(t.m) - base_of(m));
+    t.m = m;
+  }
+}
+
+// Over the kLanes lanes of a group: all get the joined statistics.
+template <int kLanes, bool kTarget>
+__device__ inline void lanes_join(Stats& t) {
+  rebase(t, lanes_reduce<Max, kLanes>(t.m));
+  t.s = lanes_reduce<Sum, kLanes>(t.s);
+  if constexpr (kTarget) {
+    t.tp = lanes_reduce<Sum, kLanes>(t.tp);
+    t.tk = lanes_reduce<Sum, kLanes>(t.tk);
+  }
+}
+
+// Over the kThreads threads of a row (as row_reduce), with one barrier.
+template <int kThreads, bool kTarget>
+__device__ inline void row_join(Stats& t, Stats* smem) {
+  lanes_join<(kThreads < kWave ? kThreads : kWave), kTarget>(t);
+  if constexpr (kThreads > kWave) {
+    static_assert(kThreads <= 16 * kWave);
+    const int lane = threadIdx.x & (kWave - 1);
+    if (lane == 0) smem[threadIdx.x / kWave] = t;
+    __syncthreads();
+    const int w = lane & 15;
+    t = w < kThreads / kWave ? smem[w] : no_stats();
+    lanes_join<16, kTarget>(t);
+  }
 }
 
 // What the gradient of a row needs.
@@ -82,7 +103,7 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
       slope -= r.kl_coef * e;
     }
   }
-  if (r.target) o.kl = t.tl - t.tz + (t.tp != 0.0f ? t.tp * log_s : 0.0f);
+  if (r.target) o.kl = t.tk + (t.tp != 0.0f ? t.tp * log_s : 0.0f);
   o.loss += r.kl_coef != 0.0f ? r.kl_coef * o.kl : 0.0f;
   o.g.m = base;
   o.g.inv_s = 1.0f / t.s;
@@ -93,185 +114,350 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
   return o;
 }
 
-// The taken action of a row, -1 when it is out of range.
-__device__ inline int64_t taken_of(const omq_policy_rows& r, int64_t row) {
-  const int64_t a = r.taken_are_64 ? static_cast<const int64_t*>(r.taken)[row]
-                                   : (int64_t) static_cast<const int32_t*>(r.taken)[row];
-  return a >= 0 && a < r.actions ? a : -1;
+__device__ inline void write_row(const RowOut& o, int64_t row, float* loss, float* logp, float* kl,
+                                 float4* stats) {
+  loss[row] = o.loss;
+  logp[row] = o.logp;
+  kl[row] = o.kl;
+  if (stats) stats[row] = make_float4(o.g.m, o.g.inv_s, o.g.push, o.g.slope);
 }
 
-// Bit j: action 8*block + j of the row is there and legal.
-__device__ inline uint32_t legal_bits(const uint8_t* legal, int64_t col, int64_t n) {
-  uint32_t bits = n >= 8 ? 0xFFu : (1u << n) - 1u;
-  if (!legal) return bits;
-  uint64_t b = 0;
-  if (n >= 8) {
-    __builtin_memcpy(&b, legal + col, 8);
-  } else {
-    for (int j = 0; j < (int)n; ++j) b |= (uint64_t)legal[col + j] << (8 * j);
+// A row's action as it is given.  (Loaded before the row's blocks: loads are waited for in their
+// order.)
+__device__ inline int64_t action_of(const omq_policy_rows& r, int64_t row) {
+  return r.taken_are_64 ? static_cast<const int64_t*>(r.taken)[row]
+                        : (int64_t) static_cast<const int32_t*>(r.taken)[row];
+}
+
+// The taken action of a row, -1 when it is out of range or not legal, and its logit.
+template <class T>
+__device__ inline int taken_of(const omq_policy_rows& r, int64_t row, int64_t a, float* z) {
+  *z = 0.0f;
+  if (a < 0 || a >= r.actions || (r.legal && !r.legal[row * r.legal_stride + a])) return -1;
+  *z = (float)static_cast<const T*>(r.logits)[row * r.logits_stride + a];
+  return (int)a;
+}
+
+// A row's arrays.
+template <class T>
+struct RowIn {
+  const T* logits;
+  const uint8_t* legal;
+  const float* target;
+  int cols;
+};
+
+template <class T>
+__device__ inline RowIn<T> row_in(const omq_policy_rows& r, int64_t row) {
+  return {static_cast<const T*>(r.logits) + row * r.logits_stride,
+          r.legal + (r.legal ? row * r.legal_stride : 0),
+          r.target + (r.target ? row * r.target_stride : 0), (int)r.actions};
+}
+
+// Eight actions of a row as they are loaded (every load is in flight before the first use).
+template <class T, bool kTarget>
+struct Block {
+  Reg8<T> z;
+  uint64_t legal;
+  F8 pi;
+};
+
+template <class T, bool kTarget, bool kWhole>
+__device__ inline Block<T, kTarget> load_block(const RowIn<T>& in, int col) {
+  Block<T, kTarget> b;
+  b.z = load_raw<T, kWhole>(in.logits, col, in.cols);
+  b.legal = 0;
+  if (in.legal) {
+    const int last = in.cols - 8;
+    if (kWhole || in.cols >= 8)
+      __builtin_memcpy(&b.legal, in.legal + (col < last ? col : last), 8);
+    else
+      for (int j = 0; j < in.cols; ++j) b.legal |= (uint64_t)in.legal[j] << (8 * j);
   }
-  uint32_t some = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) some |= ((b >> (8 * j)) & 0xFFu) ? 1u << j : 0u;
-  return bits & some;
+  if constexpr (kTarget) b.pi = load_raw<float, kWhole>(in.target, col, in.cols);
+  return b;
 }
 
-__device__ inline float gradient(const RowGrad& g, float z, bool is_taken, float pi, float coef) {
-  const float p = exp_fast(z - g.m) * g.inv_s;
-  float d = g.push * p;
-  if (is_taken) d += g.slope;
-  if (pi > 0.0f) d -= coef * pi;
+// Which of a block's actions are there and legal: the highest bit of byte j of eight.
+template <class T, bool kTarget, bool kWhole>
+__device__ inline uint64_t ok_bytes(const Block<T, kTarget>& b, const RowIn<T>& in, int col) {
+  constexpr uint64_t kHigh = 0x8080808080808080ull;
+  const int left = in.cols - col;
+  uint64_t ok = kHigh;
+  if (in.legal) {
+    uint64_t f = b.legal;
+    if (!kWhole && in.cols >= 8 && left < 8) f >>= 8 * ((col - in.cols) & 7);
+    ok = (((f & ~kHigh) + ~kHigh) | f) & kHigh;  // (a byte that is not 0)
+  }
+  if (kWhole ? left <= 0 : left < 8) ok &= left > 0 ? kHigh >> (8 * (8 - left)) : 0;
+  return ok;
+}
+
+// All ones where action j of the block is there and legal, else 0.
+__device__ inline uint32_t ok_mask(uint64_t ok, int j) {
+  const int32_t half = (int32_t)(j < 4 ? ok : ok >> 32);
+  return (uint32_t)((half << (8 * (3 - (j & 3)))) >> 31);
+}
+
+__device__ inline float masked(float x, uint32_t mask, float other) {
+  return __uint_as_float((__float_as_uint(x) & mask) | (__float_as_uint(other) & ~mask));
+}
+
+// The logits, -inf where there is no legal action.
+template <class T, bool kTarget, bool kWhole>
+__device__ inline F8 legal_logits(const Block<T, kTarget>& b, const RowIn<T>& in, int col,
+                                  uint64_t ok) {
+  F8 z = __builtin_convertvector((to_front<T, kWhole>(b.z, col, in.cols)), F8);
+  if (kWhole && !in.legal) {
+    if (!ok) z = F8{-kInf, -kInf, -kInf, -kInf, -kInf, -kInf, -kInf, -kInf};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = masked(z[j], ok_mask(ok, j), -kInf);
+  }
+  return z;
+}
+
+// The target, 0 where it is not legal.
+template <class T, bool kWhole>
+__device__ inline F8 legal_target(const Block<T, true>& b, const RowIn<T>& in, int col,
+                                  uint64_t ok) {
+  F8 pi = to_front<float, kWhole>(b.pi, col, in.cols);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) pi[j] = masked(pi[j], ok_mask(ok, j), 0.0f);
+  return pi;
+}
+
+// The larger of two and of three; the other ones where one is NaN.  (The instruction itself:
+// fmaxf costs a second one, which quiets signalling NaN first.)
+__device__ inline float larger(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
+__device__ inline float larger(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+__device__ inline float largest(F8 z) {
+  return larger(larger(larger(larger(z[0], z[1]), z[2], z[3]), z[4], z[5]), z[6], z[7]);
+}
+
+// Adds a block's exponentials, which take the place of its logits.
+__device__ inline void add_logits(Stats& t, F8& z, float base) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    z[j] = exp_fast(z[j] - base);
+    t.s += z[j];
+  }
+}
+
+// Adds a block's targets, about the same base, and leaves 0 in place of those that are not
+// positive.  (The logarithm takes subnormals for 0: what they add is nothing beside the rest.)
+__device__ inline void add_target(Stats& t, F8& pi, F8 z, float base) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool some = pi[j] > 0.0f;
+    const float log_pi = __builtin_amdgcn_logf(larger(pi[j], 0x1p-126f));  // (base 2)
+    const float term = pi[j] * fmaf(log_pi, kLn2, base - z[j]);
+    t.tk += some ? term : 0.0f;
+    pi[j] = some ? pi[j] : 0.0f;
+    t.tp += pi[j];
+  }
+}
+
+// The gradient of eight actions, times the row's weight w: e holds e^(z - m), scale is
+// w * push / s (or that about the base of e).
+template <bool kTarget>
+__device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, int taken, float scale, float w_slope,
+                              float w_coef) {
+  F8 d = e * scale;
+  if constexpr (kTarget) d -= pi * w_coef;
+  if (taken >= 0 && taken < 8) {  // (the place of the taken action in the block)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] += j == taken ? w_slope : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] = masked(d[j], ok_mask(ok, j), 0.0f);
   return d;
 }
 
 // ---- rows in registers ----------------------------------------------------------------------
 template <int kThreads>
 constexpr int block_of() {
-  return kThreads < 256 ? 256 : kThreads;
+  return kThreads <= kWave ? 256 : kThreads;
 }
 
-template <class T, int kThreads, int kVecs, bool kGrad>
+template <class T, int kThreads, int kVecs, bool kTarget, bool kWhole>
 __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
     omq_policy_rows r, const float* __restrict__ row_weight, float* __restrict__ loss,
     float* __restrict__ logp, float* __restrict__ kl, float4* __restrict__ stats,
     T* __restrict__ grad) {
   constexpr int kRows = block_of<kThreads>() / kThreads;
-  __shared__ float smem[5][16];
+  __shared__ Stats smem[16];
   const int lane = threadIdx.x % kThreads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads;
+  const int64_t row = (int64_t)blockIdx.x * kRows + row_slot<kThreads>();
   if (row >= r.rows) return;
-  const int cols = (int)r.actions;
-  const T* logits = static_cast<const T*>(r.logits) + row * r.logits_stride;
-  const uint8_t* legal = r.legal ? r.legal + row * r.legal_stride : nullptr;
-  const float* target = r.target ? r.target + row * r.target_stride : nullptr;
-  const int64_t act = taken_of(r, row);
-  const bool taken = act >= 0 && (!legal || legal[act]);
-  const float z_taken = taken ? (float)logits[act] : 0.0f;
-  Vec8<T> z[kVecs];
-  uint32_t ok[kVecs];
+  const RowIn<T> in = row_in<T>(r, row);
+  const int64_t action = action_of(r, row);
+  Block<T, kTarget> b[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+    b[i] = load_block<T, kTarget, kWhole>(in, 8 * (lane + i * kThreads));
+  float z_taken;
+  const int taken = taken_of<T>(r, row, action, &z_taken);
+  F8 z[kVecs], pi[kTarget ? kVecs : 1];
+  uint64_t ok[kVecs];
   Stats t = no_stats();
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int col = 8 * (lane + i * kThreads), n = cols - col;
-    ok[i] = 0;
-    if (n > 0) {
-      z[i] = load_raw<T>(logits + col, n);
-      ok[i] = legal_bits(legal, col, n);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (ok[i] >> j & 1) t.m = fmaxf(t.m, (float)z[i][j]);
-    }
+    const int col = 8 * (lane + i * kThreads);
+    ok[i] = ok_bytes<T, kTarget, kWhole>(b[i], in, col);
+    z[i] = legal_logits<T, kTarget, kWhole>(b[i], in, col, ok[i]);
+    t.m = larger(t.m, largest(z[i]));
   }
-  t.m = row_reduce<Max, kThreads>(t.m, smem[0]);
+  t.m = lanes_reduce<Max, (kThreads < kWave ? kThreads : kWave)>(t.m);
   const float base = base_of(t.m);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int col = 8 * (lane + i * kThreads), n = cols - col;
-    if (n > 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (ok[i] >> j & 1) t.s += exp_fast((float)z[i][j] - base);
-      if (target) {
-        const F8 pi = load8<float>(target + col, n);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((ok[i] >> j & 1) && pi[j] > 0.0f) {
-            t.tp += pi[j];
-            t.tz += pi[j] * ((float)z[i][j] - base);
-            t.tl += pi[j] * logf(pi[j]);
-          }
-      }
+    if constexpr (kTarget) {
+      pi[i] = legal_target<T, kWhole>(b[i], in, 8 * (lane + i * kThreads), ok[i]);
+      add_target(t, pi[i], z[i], base);
     }
+    add_logits(t, z[i], base);
   }
-  t.s = row_reduce<Sum, kThreads>(t.s, smem[1]);
-  if (target) {
-    t.tp = row_reduce<Sum, kThreads>(t.tp, smem[2]);
-    t.tz = row_reduce<Sum, kThreads>(t.tz, smem[3]);
-    t.tl = row_reduce<Sum, kThreads>(t.tl, smem[4]);
-  }
-  const RowOut o = finish_row(r, row, t, z_taken, taken);
-  if (lane == 0) {
-    loss[row] = o.loss;
-    logp[row] = o.logp;
-    kl[row] = o.kl;
-    if (stats) stats[row] = make_float4(o.g.m, o.g.inv_s, o.g.push, o.g.slope);
-  }
-  if constexpr (kGrad) {
-    const float w = row_weight ? row_weight[row] : 1.0f;
-    T* g = grad + row * cols;
+  row_join<kThreads, kTarget>(t, smem);
+  const RowOut o = finish_row(r, row, t, z_taken, taken >= 0);
+  if (lane == 0) write_row(o, row, loss, logp, kl, stats);
+  if (!grad) return;
+  const float w = row_weight ? row_weight[row] : 1.0f;
+  const float scale = w * o.g.push * o.g.inv_s * exp_fast(base - o.g.m);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (lane + i * kThreads), n = cols - col;
-      if (n > 0) {
-        F8 pi = {}, d = {};
-        if (target) pi = load8<float>(target + col, n);
-        if (o.g.inv_s != 0.0f) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (ok[i] >> j & 1)
-              d[j] = w * gradient(o.g, (float)z[i][j], taken && col + j == act, pi[j], r.kl_coef);
-        }
-        store8<T>(g + col, d, n);
-      }
-    }
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (lane + i * kThreads);
+    F8 d = {};
+    if (o.g.inv_s != 0.0f)
+      d = gradient<kTarget>(z[i], pi[kTarget ? i : 0], ok[i], taken - col, scale, w * o.g.slope,
+                            w * r.kl_coef);
+    store8<T, kWhole>(grad + row * in.cols, col, in.cols, d);
   }
 }
 
-// ---- spans of rows --------------------------------------------------------------------------
-// Statistics of span blockIdx.x of row blockIdx.y.
-template <class T>
-__global__ __launch_bounds__(256) void loss_span_kernel(omq_policy_rows r, int64_t row0,
-                                                        int64_t span, Stats* __restrict__ parts) {
-  __shared__ Stats waves[4];
-  const int64_t row = row0 + blockIdx.y;
-  const T* logits = static_cast<const T*>(r.logits) + row * r.logits_stride;
-  const uint8_t* legal = r.legal ? r.legal + row * r.legal_stride : nullptr;
-  const float* target = r.target ? r.target + row * r.target_stride : nullptr;
-  const int64_t from = blockIdx.x * span;
-  const int64_t to = from + span < r.actions ? from + span : r.actions;
+// ---- long rows ------------------------------------------------------------------------------
+// Adds kCount blocks, kStep columns apart, the first at column `col`, to a thread's statistics.
+// The base follows the logits only when one passes it by more than kSlack: e^kSlack is far from
+// any limit, and after a few blocks no thread changes its base again.
+template <class T, bool kTarget, bool kWhole, int kCount, int kStep>
+__device__ inline void add_blocks(Stats& t, const Block<T, kTarget>* b, const RowIn<T>& in, int col,
+                                  int to) {
+  constexpr float kSlack = 8.0f;
+  F8 z[kCount];
+  uint64_t ok[kCount];
+  float m = -kInf;
+#pragma unroll
+  for (int u = 0; u < kCount; ++u) {
+    const int c = col + kStep * u;
+    ok[u] = c < to ? ok_bytes<T, kTarget, kWhole>(b[u], in, c) : 0;
+    z[u] = legal_logits<T, kTarget, kWhole>(b[u], in, c, ok[u]);
+    m = larger(m, largest(z[u]));
+  }
+  if (m > t.m + kSlack) rebase(t, m);  // (from -inf: at the first weight)
+  const float base = base_of(t.m);
+#pragma unroll
+  for (int u = 0; u < kCount; ++u) {
+    if constexpr (kTarget) {
+      F8 pi = legal_target<T, kWhole>(b[u], in, col + kStep * u, ok[u]);
+      add_target(t, pi, z[u], base);
+    }
+    add_logits(t, z[u], base);
+  }
+}
+
+// Statistics of the blocks from column `from` on, up to column `to`, that fall to this thread.
+template <class T, bool kTarget, bool kWhole, int kThreads>
+__device__ inline void stream(Stats& t, const RowIn<T>& in, int from, int to) {
+  constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
+  for (int col = from + 8 * threadIdx.x; col < to; col += kStep * kCount) {
+    Block<T, kTarget> b[kCount];
+#pragma unroll
+    for (int u = 0; u < kCount; ++u)
+      b[u] = load_block<T, kTarget, kWhole>(in, col + kStep * u);
+    add_blocks<T, kTarget, kWhole, kCount, kStep>(t, b, in, col, to);
+  }
+}
+
+// The gradient of the block at column col.
+template <class T, bool kTarget, bool kWhole, bool kStream>
+__device__ inline void put_gradient(T* grad, const Block<T, kTarget>& b, const RowIn<T>& in,
+                                    int col, const RowGrad& g, int taken, float coef, float w) {
+  F8 d = {}, pi = {};
+  if (g.inv_s != 0.0f) {
+    const uint64_t ok = ok_bytes<T, kTarget, kWhole>(b, in, col);
+    F8 z = legal_logits<T, kTarget, kWhole>(b, in, col, ok);
+    if constexpr (kTarget) {
+      pi = legal_target<T, kWhole>(b, in, col, ok);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pi[j] = pi[j] > 0.0f ? pi[j] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = exp_fast(z[j] - g.m);
+    d = gradient<kTarget>(z, pi, ok, taken - col, w * g.push * g.inv_s, w * g.slope, w * coef);
+  }
+  store8<T, kWhole, kStream>(grad, col, in.cols, d);
+}
+
+// A workgroup a row: the sums, then the gradient, for which the blocks are read again, the last
+// read first.
+template <class T, int kThreads, bool kTarget, bool kWhole>
+__global__ __launch_bounds__(kThreads) void loss_long_kernel(
+    omq_policy_rows r, const float* __restrict__ row_weight, float* __restrict__ loss,
+    float* __restrict__ logp, float* __restrict__ kl, float4* __restrict__ stats,
+    T* __restrict__ grad) {
+  constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
+  __shared__ Stats smem[16];
+  const int64_t row = blockIdx.x;
+  const RowIn<T> in = row_in<T>(r, row);
+  float z_taken;
+  const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
   Stats t = no_stats();
-  for (int64_t col = from + 8 * threadIdx.x; col < to; col += 8 * 256) {
-    const int64_t n = to - col;
-    const F8 z = load8<T>(logits + col, n < 8 ? (int)n : 8);
-    const uint32_t ok = legal_bits(legal, col, n);
-    Stats u = no_stats();
+  stream<T, kTarget, kWhole, kThreads>(t, in, 0, in.cols);
+  row_join<kThreads, kTarget>(t, smem);
+  const RowOut o = finish_row(r, row, t, z_taken, taken >= 0);
+  if (threadIdx.x == 0) write_row(o, row, loss, logp, kl, stats);
+  if (!grad) return;
+  const float w = row_weight ? row_weight[row] : 1.0f;
+  T* g = grad + row * in.cols;
+  for (int at = (in.cols - 1) / (kStep * kCount) * (kStep * kCount); at >= 0;
+       at -= kStep * kCount) {
+    Block<T, kTarget> b[kCount];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (ok >> j & 1) u.m = fmaxf(u.m, z[j]);
-    const float base = base_of(u.m);
+    for (int u = 0; u < kCount; ++u)
+      b[u] = load_block<T, kTarget, kWhole>(in, at + 8 * (int)threadIdx.x + kStep * u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (ok >> j & 1) u.s += exp_fast(z[j] - base);
-    if (target) {
-      const F8 pi = load8<float>(target + col, n < 8 ? (int)n : 8);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((ok >> j & 1) && pi[j] > 0.0f) {
-          u.tp += pi[j];
-          u.tz += pi[j] * (z[j] - base);
-          u.tl += pi[j] * logf(pi[j]);
-        }
-    }
-    t = join(t, u);
-  }
-  for (int d = 1; d < kWave; d <<= 1) {
-    Stats u;
-    u.m = __shfl_xor(t.m, d);
-    u.s = __shfl_xor(t.s, d);
-    u.tp = __shfl_xor(t.tp, d);
-    u.tz = __shfl_xor(t.tz, d);
-    u.tl = __shfl_xor(t.tl, d);
-    t = join(t, u);
-  }
-  if ((threadIdx.x & (kWave - 1)) == 0) waves[threadIdx.x / kWave] = t;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; ++w) t = join(t, waves[w]);
-    parts[row * gridDim.x + blockIdx.x] = t;
+    for (int u = 0; u < kCount; ++u)
+      put_gradient<T, kTarget, kWhole, true>(g, b[u], in, at + 8 * (int)threadIdx.x + kStep * u,
+                                         o.g, taken, r.kl_coef, w);
   }
 }
 
-// A thread a row: its spans joined in order.
+// Statistics of span blockIdx.x of row blockIdx.y.
+template <class T, bool kTarget, bool kWhole>
+__global__ __launch_bounds__(256) void loss_span_kernel(omq_policy_rows r, int span,
+                                                        Stats* __restrict__ parts) {
+  __shared__ Stats smem[16];
+  const int64_t row = blockIdx.y;
+  const RowIn<T> in = row_in<T>(r, row);
+  const int64_t from = (int64_t)blockIdx.x * span;
+  const int to = from + span < in.cols ? (int)(from + span) : in.cols;
+  Stats t = no_stats();
+  stream<T, kTarget, kWhole, 256>(t, in, (int)from, to);
+  row_join<256, kTarget>(t, smem);
+  if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = t;
+}
+
+// A wave a row: its spans joined.
 template <class T>
 __global__ __launch_bounds__(64) void loss_join_kernel(omq_policy_rows r,
                                                        const Stats* __restrict__ parts, int spans,
@@ -279,50 +465,41 @@ __global__ __launch_bounds__(64) void loss_join_kernel(omq_policy_rows r,
                                                        float* __restrict__ logp,
                                                        float* __restrict__ kl,
                                                        float4* __restrict__ stats) {
-  const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (row >= r.rows) return;
+  const int64_t row = blockIdx.x;
+  float z;
+  const int taken = taken_of<T>(r, row, action_of(r, row), &z);
   Stats t = no_stats();
-  for (int k = 0; k < spans; ++k) t = join(t, parts[row * spans + k]);
-  const int64_t act = taken_of(r, row);
-  const bool taken = act >= 0 && (!r.legal || r.legal[row * r.legal_stride + act]);
-  const float z =
-      taken ? (float)static_cast<const T*>(r.logits)[row * r.logits_stride + act] : 0.0f;
-  const RowOut o = finish_row(r, row, t, z, taken);
-  loss[row] = o.loss;
-  logp[row] = o.logp;
-  kl[row] = o.kl;
-  if (stats) stats[row] = make_float4(o.g.m, o.g.inv_s, o.g.push, o.g.slope);
+  for (int k = threadIdx.x; k < spans; k += kWave) {
+    Stats u = parts[row * spans + k];
+    const float m = fmaxf(t.m, u.m);
+    rebase(t, m);
+    rebase(u, m);
+    t = Stats{m, t.s + u.s, t.tp + u.tp, t.tk + u.tk};
+  }
+  lanes_join<kWave, true>(t);
+  if (threadIdx.x == 0) write_row(finish_row(r, row, t, z, taken >= 0), row, loss, logp, kl, stats);
 }
 
-// The gradient from a row's statistics: 2048 columns of a row a workgroup.
-template <class T>
+// The gradient from the rows' statistics, a block of eight actions a thread.
+template <class T, bool kTarget, bool kWhole>
 __global__ __launch_bounds__(256) void loss_grad_kernel(omq_policy_rows r, int blocks,
                                                         const float4* __restrict__ stats,
                                                         const float* __restrict__ row_weight,
                                                         T* __restrict__ grad) {
   const int64_t first = (int64_t)blockIdx.x * 256;
   const int64_t row0 = first / blocks;
-  const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
-  const int64_t row = row0 + in / (uint32_t)blocks;
-  const int64_t col = 8ll * (in % (uint32_t)blocks);
+  const uint32_t at = (uint32_t)(first - row0 * blocks) + threadIdx.x;
+  const int64_t row = row0 + at / (uint32_t)blocks;
+  const int col = 8 * (int)(at % (uint32_t)blocks);
   if (row >= r.rows) return;
-  const int64_t left = r.actions - col;
-  const int n = left < 8 ? (int)left : 8;
+  const RowIn<T> in = row_in<T>(r, row);
+  const Block<T, kTarget> b = load_block<T, kTarget, kWhole>(in, col);
   const float4 st = stats[row];
   const RowGrad g{st.x, st.y, st.z, st.w};
   const float w = row_weight ? row_weight[row] : 1.0f;
-  const int64_t act = taken_of(r, row);
-  F8 d = {};
-  if (g.inv_s != 0.0f) {
-    const F8 z = load8<T>(static_cast<const T*>(r.logits) + row * r.logits_stride + col, n);
-    const uint32_t ok = legal_bits(r.legal ? r.legal + row * r.legal_stride : nullptr, col, n);
-    F8 pi = {};
-    if (r.target) pi = load8<float>(r.target + row * r.target_stride + col, n);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (ok >> j & 1) d[j] = w * gradient(g, z[j], col + j == act, pi[j], r.kl_coef);
-  }
-  store8<T>(grad + row * r.actions + col, d, n);
+  float z_taken;
+  const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
+  put_gradient<T, kTarget, kWhole, false>(grad + row * in.cols, b, in, col, g, taken, r.kl_coef, w);
 }
 
 // ---- launches -------------------------------------------------------------------------------
@@ -331,18 +508,28 @@ struct Layout {
   static constexpr int kThreads = kThreads_, kVecs = kVecs_;
 };
 
-constexpr int64_t kRowActions = 16384;  // the longest row that is held in registers
+// The longest rows that are held in registers, without and with a target.
+constexpr int64_t kRowActions = 16384, kRowActionsTarget = 8192;
+// Long rows from this many on are a workgroup each, fewer are cut into spans.
+constexpr int64_t kLongRows = 128;
+// The workgroup of a long row: wide enough that the rows under way stay in the last-level cache.
+constexpr int64_t kWideActions = 65536;
 
-template <class F>
+template <bool kTarget, class F>
 void with_layout(int64_t cols, F&& f) {
   if (cols <= 128) return f(Layout<16, 1>{});
   if (cols <= 256) return f(Layout<32, 1>{});
   if (cols <= 512) return f(Layout<64, 1>{});
-  if (cols <= 1024) return f(Layout<64, 2>{});
-  if (cols <= 2048) return f(Layout<64, 4>{});
+  if (cols <= 1024) return f(Layout<128, 1>{});
+  if (cols <= 2048) return f(Layout<256, 1>{});
   if (cols <= 4096) return f(Layout<256, 2>{});
-  if (cols <= 8192) return f(Layout<256, 4>{});
-  return f(Layout<256, 8>{});
+  if (cols <= 6144) return f(Layout<256, 3>{});
+  if constexpr (kTarget) {
+    return f(Layout<256, 4>{});
+  } else {
+    if (cols <= 8192) return f(Layout<256, 4>{});
+    return f(Layout<256, 8>{});
+  }
 }
 
 template <class F>
@@ -352,29 +539,48 @@ void with_type(int dtype, F&& f) {
   return f(f16{});
 }
 
-struct LossPlan {
-  bool in_rows;
-  int64_t span, spans, at_parts, at_stats, bytes;
+template <bool kTarget, bool kWhole>
+struct Kind {
+  static constexpr bool target = kTarget, whole = kWhole;
 };
 
-LossPlan loss_plan(int64_t rows, int64_t actions) {
-  LossPlan p{};
-  p.in_rows = actions <= kRowActions;
-  if (p.in_rows) return p;
-  // spans for about 2048 workgroups, of at least 8192 columns
-  int64_t spans = ceil_div(2048, rows > 0 ? rows : 1);
-  const int64_t most = ceil_div(actions, 8192);
-  spans = spans < 1 ? 1 : spans > most ? most : spans;
+template <class F>
+void with_kind(const omq_policy_rows& r, F&& f) {
+  if (r.target)
+    r.actions % 8 == 0 ? f(Kind<true, true>{}) : f(Kind<true, false>{});
+  else
+    r.actions % 8 == 0 ? f(Kind<false, true>{}) : f(Kind<false, false>{});
+}
+
+// How rows of these sizes are cut, whatever the target; used where they are not in registers.
+struct SpanPlan {
+  int64_t span, spans, at_parts, bytes;
+};
+
+SpanPlan span_plan(int64_t rows, int64_t actions) {
+  SpanPlan p{};
+  if (actions <= kRowActionsTarget || rows >= kLongRows) return p;
+  // spans for about 1024 workgroups, of at least 4096 columns
+  int64_t spans = ceil_div(1024, rows > 0 ? rows : 1);
+  const int64_t most = ceil_div(actions, 4096);
+  spans = spans > most ? most : spans;
   p.span = ceil_div(ceil_div(actions, spans), 8) * 8;
   p.spans = ceil_div(actions, p.span);
-  p.at_stats = 0;
-  p.at_parts = 16 * rows;
+  p.at_parts = 16 * rows;  // (the rows' statistics for the gradient come first)
   p.bytes = p.at_parts + (int64_t)sizeof(Stats) * rows * p.spans;
   return p;
 }
 
+enum Way { kInRows, kLong, kSpans };
+
+Way way_of(const omq_policy_rows& r) {
+  if (r.actions <= (r.target ? kRowActionsTarget : kRowActions)) return kInRows;
+  return r.rows >= kLongRows ? kLong : kSpans;
+}
+
 bool loss_sizes_ok(int64_t rows, int64_t actions) {
-  return rows >= 0 && actions >= 1 && rows <= OMQ_NET_MAX_COUNT && actions <= OMQ_NET_MAX_COUNT &&
+  return rows >= 0 && actions >= 1 && rows <= OMQ_NET_MAX_COUNT &&
+         actions <= OMQ_NET_MAX_ACTIONS &&
          ceil_div(rows * ceil_div(actions, 8), 256) <= OMQ_NET_MAX_COUNT;
 }
 
@@ -395,34 +601,56 @@ int check_rows(const char* name, const omq_policy_rows* r) {
   return OMQ_NET_OK;
 }
 
-template <bool kGrad>
-void launch_rows(const omq_policy_rows& r, const float* row_weight, float* loss, float* logp,
-                 float* kl, float* stats, void* grad, hipStream_t st) {
+struct LossOut {
+  float *loss, *logp, *kl, *stats;
+};
+
+void launch_rows(const omq_policy_rows& r, const float* row_weight, const LossOut& o, void* grad,
+                 hipStream_t st) {
   with_type(r.dtype, [&](auto t) {
     using T = decltype(t);
-    with_layout(r.actions, [&](auto l) {
-      using L = decltype(l);
-      constexpr int kBlock = block_of<L::kThreads>();
-      const uint32_t grid = (uint32_t)ceil_div(r.rows, kBlock / L::kThreads);
-      loss_rows_kernel<T, L::kThreads, L::kVecs, kGrad><<<grid, kBlock, 0, st>>>(
-          r, row_weight, loss, logp, kl, reinterpret_cast<float4*>(stats),
+    with_kind(r, [&](auto kind) {
+      using K = decltype(kind);
+      with_layout<K::target>(r.actions, [&](auto l) {
+        using L = decltype(l);
+        constexpr int kBlock = block_of<L::kThreads>();
+        const uint32_t grid = (uint32_t)ceil_div(r.rows, kBlock / L::kThreads);
+        loss_rows_kernel<T, L::kThreads, L::kVecs, K::target, K::whole><<<grid, kBlock, 0, st>>>(
+            r, row_weight, o.loss, o.logp, o.kl, reinterpret_cast<float4*>(o.stats),
+            static_cast<T*>(grad));
+      });
+    });
+  });
+}
+
+void launch_long(const omq_policy_rows& r, const float* row_weight, const LossOut& o, void* grad,
+                 hipStream_t st) {
+  with_type(r.dtype, [&](auto t) {
+    using T = decltype(t);
+    with_kind(r, [&](auto kind) {
+      using K = decltype(kind);
+      const bool wide = r.actions > kWideActions;
+      const auto kernel = wide ? loss_long_kernel<T, 1024, K::target, K::whole>
+                               : loss_long_kernel<T, 512, K::target, K::whole>;
+      kernel<<<(uint32_t)r.rows, wide ? 1024 : 512, 0, st>>>(
+          r, row_weight, o.loss, o.logp, o.kl, reinterpret_cast<float4*>(o.stats),
           static_cast<T*>(grad));
     });
   });
 }
 
-void launch_spans(const omq_policy_rows& r, const LossPlan& p, float* loss, float* logp, float* kl,
-                  float* stats, char* ws, hipStream_t st) {
+void launch_spans(const omq_policy_rows& r, const SpanPlan& p, const LossOut& o, char* ws,
+                  hipStream_t st) {
   Stats* parts = reinterpret_cast<Stats*>(ws + p.at_parts);
   with_type(r.dtype, [&](auto t) {
     using T = decltype(t);
-    for (int64_t row0 = 0; row0 < r.rows; row0 += 65535) {
-      const int64_t n = r.rows - row0 < 65535 ? r.rows - row0 : 65535;
-      loss_span_kernel<T><<<dim3((uint32_t)p.spans, (uint32_t)n), 256, 0, st>>>(r, row0, p.span,
-                                                                               parts);
-    }
-    loss_join_kernel<T><<<(uint32_t)ceil_div(r.rows, 64), 64, 0, st>>>(
-        r, parts, (int)p.spans, loss, logp, kl, reinterpret_cast<float4*>(stats));
+    with_kind(r, [&](auto kind) {
+      using K = decltype(kind);
+      loss_span_kernel<T, K::target, K::whole>
+          <<<dim3((uint32_t)p.spans, (uint32_t)r.rows), 256, 0, st>>>(r, (int)p.span, parts);
+    });
+    loss_join_kernel<T><<<(uint32_t)r.rows, kWave, 0, st>>>(
+        r, parts, (int)p.spans, o.loss, o.logp, o.kl, reinterpret_cast<float4*>(o.stats));
   });
 }
 
@@ -430,14 +658,17 @@ void launch_grad(const omq_policy_rows& r, const float* stats, const float* row_
                  hipStream_t st) {
   with_type(r.dtype, [&](auto t) {
     using T = decltype(t);
-    const int blocks = (int)ceil_div(r.actions, 8);
-    const uint32_t grid = (uint32_t)ceil_div(r.rows * blocks, 256);
-    loss_grad_kernel<T><<<grid, 256, 0, st>>>(r, blocks, reinterpret_cast<const float4*>(stats),
-                                              row_weight, static_cast<T*>(grad));
+    with_kind(r, [&](auto kind) {
+      using K = decltype(kind);
+      const int blocks = (int)ceil_div(r.actions, 8);
+      const uint32_t grid = (uint32_t)ceil_div(r.rows * blocks, 256);
+      loss_grad_kernel<T, K::target, K::whole><<<grid, 256, 0, st>>>(
+          r, blocks, reinterpret_cast<const float4*>(stats), row_weight, static_cast<T*>(grad));
+    });
   });
 }
 
-int check_workspace(const char* name, const LossPlan& p, const void* ws, int64_t bytes) {
+int check_workspace(const char* name, const SpanPlan& p, const void* ws, int64_t bytes) {
   if (p.bytes > 0 && (!ws || bytes < p.bytes))
     return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes, %lld needed", name,
                     (long long)bytes, (long long)p.bytes);
@@ -453,7 +684,7 @@ extern "C" {
 
 int64_t omq_clipped_policy_loss_workspace(int64_t rows, int64_t actions) {
   if (!loss_sizes_ok(rows, actions)) return OMQ_NET_E_ARG;
-  return loss_plan(rows, actions).bytes;
+  return span_plan(rows, actions).bytes;
 }
 
 int omq_clipped_policy_loss(const omq_policy_rows* r, float* loss, float* logp, float* kl,
@@ -462,14 +693,16 @@ int omq_clipped_policy_loss(const omq_policy_rows* r, float* loss, float* logp, 
   const char* name = "omq_clipped_policy_loss";
   if (int rc = check_rows(name, r)) return rc;
   if (r->rows == 0) return OMQ_NET_OK;
-  const LossPlan p = loss_plan(r->rows, r->actions);
+  const SpanPlan p = span_plan(r->rows, r->actions);
   if (int rc = check_workspace(name, p, workspace, workspace_bytes)) return rc;
   if (!loss || !logp || !kl) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   hipStream_t st = (hipStream_t)stream;
-  if (p.in_rows)
-    launch_rows<false>(*r, nullptr, loss, logp, kl, stats, nullptr, st);
-  else
-    launch_spans(*r, p, loss, logp, kl, stats, static_cast<char*>(workspace), st);
+  const LossOut o{loss, logp, kl, stats};
+  switch (way_of(*r)) {
+    case kInRows: launch_rows(*r, nullptr, o, nullptr, st); break;
+    case kLong: launch_long(*r, nullptr, o, nullptr, st); break;
+    case kSpans: launch_spans(*r, p, o, static_cast<char*>(workspace), st); break;
+  }
   return net_status(name);
 }
 
@@ -489,16 +722,19 @@ int omq_clipped_policy_loss_with_grad(const omq_policy_rows* r, const float* row
   const char* name = "omq_clipped_policy_loss_with_grad";
   if (int rc = check_rows(name, r)) return rc;
   if (r->rows == 0) return OMQ_NET_OK;
-  const LossPlan p = loss_plan(r->rows, r->actions);
+  const SpanPlan p = span_plan(r->rows, r->actions);
   if (int rc = check_workspace(name, p, workspace, workspace_bytes)) return rc;
   if (!loss || !logp || !kl || !grad) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   hipStream_t st = (hipStream_t)stream;
-  if (p.in_rows) {
-    launch_rows<true>(*r, row_weight, loss, logp, kl, nullptr, grad, st);
-  } else {
-    float* stats = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.at_stats);
-    launch_spans(*r, p, loss, logp, kl, stats, static_cast<char*>(workspace), st);
-    launch_grad(*r, stats, row_weight, grad, st);
+  LossOut o{loss, logp, kl, nullptr};
+  switch (way_of(*r)) {
+    case kInRows: launch_rows(*r, row_weight, o, grad, st); break;
+    case kLong: launch_long(*r, row_weight, o, grad, st); break;
+    case kSpans:
+      o.stats = static_cast<float*>(workspace);
+      launch_spans(*r, p, o, static_cast<char*>(workspace), st);
+      launch_grad(*r, o.stats, row_weight, grad, st);
+      break;
   }
   return net_status(name);
 }
