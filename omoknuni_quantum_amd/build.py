@@ -95,14 +95,15 @@ def build_net_library(out: str | None = None, verbose: bool = False) -> str:
 def build_net_torch(out: str | None = None, verbose: bool = False) -> str:
     """libomq_net_torch.so: the torch operators over libomq_net_ops.so (csrc/net_torch.cpp)."""
     return build_torch_ops(out or os.path.join(_HERE, "libomq_net_torch.so"), verbose,
-                           "net_torch.cpp", "omq_net_ops")
+                           "net_torch.cpp", "omq_net_ops", ("torch_hip",))
 
 
 def build_torch_ops(out: str | None = None, verbose: bool = False,
-                    source: str = "torch_ops.cpp", library: str = "omq_tree_ops") -> str:
+                    source: str = "torch_ops.cpp", library: str = "omq_tree_ops",
+                    more: tuple = ()) -> str:
     """libomq_torch_ops.so: the torch operators (csrc/torch_ops.cpp), host C++ over the C ABI,
     linked against libomq_tree_ops.so beside it (build that first).  `source` and `library`:
-    another file of operators and the library it calls."""
+    another file of operators and the library it calls; `more`: libraries of torch's to link."""
     import torch
     from torch.utils import cpp_extension
 
@@ -117,7 +118,7 @@ def build_torch_ops(out: str | None = None, verbose: bool = False,
            f"-L{_HERE}", f"-l{library}", "-Wl,-rpath,$ORIGIN",
            *(f"-L{p}" for p in cpp_extension.library_paths()),
            *(f"-Wl,-rpath,{p}" for p in cpp_extension.library_paths()),
-           "-lc10", "-lc10_hip", "-ltorch_cpu"]
+           "-lc10", "-lc10_hip", "-ltorch_cpu", *(f"-l{m}" for m in more)]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -16,22 +16,39 @@ namespace omq_net {
 namespace {
 
 // ---- forward --------------------------------------------------------------------------------
-template <class T, class Id, bool kWhole>
+// A thread takes kBlocks blocks of eight columns, 256 blocks apart: their ids, then their rows are
+// in flight together.
+template <class T, class Id, bool kWhole, int kBlocks>
 __global__ __launch_bounds__(256) void embed_kernel(const Id* __restrict__ ids, int64_t tokens,
                                                     const T* __restrict__ weight,
                                                     int64_t weight_stride, int64_t vocab,
                                                     int dim, int blocks, float scale,
                                                     T* __restrict__ out) {
-  const int64_t first = (int64_t)blockIdx.x * 256;
+  const int64_t first = (int64_t)blockIdx.x * (256 * kBlocks);
   const int64_t row0 = first / blocks;
   const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
-  const int64_t t = row0 + in / (uint32_t)blocks;
-  const int col = 8 * (int)(in % (uint32_t)blocks);
-  if (t >= tokens) return;
-  const int64_t id = (int64_t)ids[t];
-  const bool in_table = id >= 0 && id < vocab;
-  const Reg8<T> raw = load_raw<T, kWhole>(weight + (in_table ? id : 0) * weight_stride, col, dim);
-  store8<T, kWhole>(out + t * dim, col, dim, in_table ? widen<T, kWhole>(raw, col, dim) * scale : F8{});
+  int64_t t[kBlocks], id[kBlocks];
+  int col[kBlocks];
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) {
+    const uint32_t down = (in + 256 * k) / (uint32_t)blocks;
+    t[k] = row0 + down;
+    col[k] = 8 * (int)(in + 256 * k - down * (uint32_t)blocks);
+    id[k] = (int64_t)ids[t[k] < tokens ? t[k] : tokens - 1];
+  }
+  Reg8<T> raw[kBlocks];
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) {
+    const bool in_table = id[k] >= 0 && id[k] < vocab;
+    raw[k] = load_raw<T, kWhole>(weight + (in_table ? id[k] : 0) * weight_stride, col[k], dim);
+  }
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) {
+    const bool in_table = id[k] >= 0 && id[k] < vocab;
+    if (t[k] < tokens)
+      store8<T, kWhole>(out + t[k] * dim, col[k], dim,
+                        in_table ? widen<T, kWhole>(raw[k], col[k], dim) * scale : F8{});
+  }
 }
 
 // ---- sort -----------------------------------------------------------------------------------
@@ -170,10 +187,10 @@ template <class Id>
 __global__ __launch_bounds__(256) void digit_counts_kernel(const Id* __restrict__ ids,
                                                            const uint2* __restrict__ in,
                                                            int64_t tokens, int64_t vocab,
-                                                           int shift, int bits,
+                                                           int shift, int bits, int bins,
                                                            uint32_t* __restrict__ counts) {
   __shared__ uint32_t hist[1 << kMaxDigitBits];
-  const int bins = 1 << bits;
+  const uint32_t mask = (1u << bits) - 1;
   const int64_t first = (int64_t)blockIdx.x * kTile;
   uint32_t key[kTile / 256];
 #pragma unroll
@@ -186,7 +203,7 @@ __global__ __launch_bounds__(256) void digit_counts_kernel(const Id* __restrict_
 #pragma unroll
   for (int r = 0; r < kTile / 256; ++r)
     if (first + r * 256 + threadIdx.x < tokens)
-      atomicAdd(&hist[(key[r] >> shift) & (bins - 1)], 1u);
+      atomicAdd(&hist[(key[r] >> shift) & mask], 1u);
   __syncthreads();
   for (int j = threadIdx.x; j < bins; j += 256) counts[(int64_t)blockIdx.x * bins + j] = hist[j];
 }
@@ -235,13 +252,13 @@ __global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__
 template <class Id>
 __global__ __launch_bounds__(256) void digit_scatter_kernel(
     const Id* __restrict__ ids, const uint2* __restrict__ in, int64_t tokens, int64_t vocab,
-    int shift, int bits, const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
-    uint2* __restrict__ out) {
+    int shift, int bits, int bins, const uint32_t* __restrict__ counts,
+    const uint32_t* __restrict__ totals, uint2* __restrict__ out) {
   constexpr int kWaves = 4, kRounds = kTile / 256, kBins = 1 << kMaxDigitBits;
   __shared__ uint32_t next[kWaves][kBins];
   __shared__ uint32_t base[kBins];
   __shared__ uint32_t wave_sums[kWaves];
-  const int bins = 1 << bits;
+  const uint32_t mask = (1u << bits) - 1;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int64_t first = (int64_t)blockIdx.x * kTile + wave * (kTile / kWaves);
   uint2 mine[kRounds];
@@ -265,17 +282,19 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
     if (first + r * kWave + lane < tokens)
-      atomicAdd(&next[wave][(mine[r].x >> shift) & (bins - 1)], 1u);
+      atomicAdd(&next[wave][(mine[r].x >> shift) & mask], 1u);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kBins / 256; ++k) {
     const int j = k * 256 + threadIdx.x;
     if (j < bins) {
-      uint32_t at = base[j] + before[k];
+      uint32_t at = base[j] + before[k], c[kWaves];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) c[w] = next[w][j];
+#pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const uint32_t c = next[w][j];
         next[w][j] = at;
-        at += c;
+        at += c[w];
       }
     }
   }
@@ -283,7 +302,7 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const bool here = first + r * kWave + lane < tokens;
-    const uint32_t digit = here ? (mine[r].x >> shift) & (bins - 1) : 0u;
+    const uint32_t digit = here ? (mine[r].x >> shift) & mask : 0u;
     const uint32_t at = take_places(digit, bits, here, next[wave]);
     if (here) out[at] = mine[r];
   }
@@ -447,8 +466,7 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
     }
     return v;
   };
-  const auto sum = [&](int64_t from, int64_t to, int step) {
-    F4 acc = {};
+  const auto sum = [&](F4 acc, int64_t from, int64_t to, int step) {
     for (int64_t k = from; k < to; k += 8 * step) {  // eight loads in flight, the last ones too
       F4 v[8];
 #pragma unroll
@@ -459,9 +477,7 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
     }
     return acc;
   };
-  const auto write = [&](int64_t c, F4 acc) {
-    acc += four(heads + c * dim);
-    const int64_t row = info[c].first_row;
+  const auto write = [&](int64_t row, F4 acc) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (col + j < dim) out[row * dim + col + j] = (O)(acc[j] * scale);
@@ -494,8 +510,9 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
       open = info[from].open;
     }
     if (!open) ++from;
+    const F4 head = four(heads + c * dim);
     if (c - from <= kOwnRun)
-      write(c, sum(from, c, 1));
+      write(row, sum(F4{}, from, c, 1) + head);
     else
       long_from = from;
   }
@@ -504,12 +521,12 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
   for (int w = 0; w < kJoinWaves; ++w) {
     const int64_t from = run_from[w];
     if (from < 0) continue;
-    F4 acc = sum(from + wave, c0 + w, kJoinWaves);
+    F4 acc = sum(F4{}, from + wave, c0 + w, kJoinWaves);
     part[wave][lane] = acc;
     __syncthreads();
     if (wave == 0) {
       for (int k = 1; k < kJoinWaves; ++k) acc += part[k][lane];
-      write(c0 + w, acc);
+      write(info[c0 + w].first_row, acc + four(heads + (c0 + w) * dim));
     }
     __syncthreads();
   }
@@ -542,15 +559,13 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   p.tiles = ceil_div(tokens, kTile);
   p.lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : dim <= 256 ? 32 : 64;
   p.col_tiles = (int)ceil_div(dim, 8 * p.lanes);
-  // pieces for about 4096 waves, of 16 to 1024 items
+  // Pieces for 2048 waves, of 16 to 1024 items.  Fewer leave memory idle, more are more partial
+  // sums: 115200 tokens of 675 rows and 256 columns take 34 us, 38 with 1024 waves and 40 with
+  // 4096; 131071 of 65536 rows and 1024 columns 125, 135 and 129.
   const int64_t items = tokens + vocab;
-#ifndef PW
-#define PW 4096ll
-#define PMIN 16
-#endif
-  const int64_t wanted = ceil_div(PW * (kWave / p.lanes), p.col_tiles);
+  const int64_t wanted = ceil_div(2048ll * (kWave / p.lanes), p.col_tiles);
   p.piece = ceil_div(items, wanted);
-  p.piece = p.piece < PMIN ? PMIN : p.piece > 1024 ? 1024 : p.piece;
+  p.piece = p.piece < 16 ? 16 : p.piece > 1024 ? 1024 : p.piece;
   p.pieces = ceil_div(items, p.piece);
   int64_t at = 0;
   p.at_pairs[0] = take(&at, 8 * tokens);
@@ -589,13 +604,16 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
   const uint2* in = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {
     uint2* to = buf[pass & 1];
-    const int shift = pass * p.digit_bits, bins = 1 << p.digit_bits;
+    // the digits that occur: the largest key is `vocab`
+    const int shift = pass * p.digit_bits;
+    const int64_t top = (vocab >> shift) + 1, all = 1 << p.digit_bits;
+    const int bins = (int)(top < all ? top : all);
     digit_counts_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(ids, in, tokens, vocab, shift,
-                                                              p.digit_bits, counts);
+                                                              p.digit_bits, bins, counts);
     digit_scan_kernel<<<(uint32_t)ceil_div(bins, kWave), 1024, 0, st>>>(counts, (int)p.tiles, bins,
                                                                       totals);
     digit_scatter_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(
-        ids, in, tokens, vocab, shift, p.digit_bits, counts, totals, to);
+        ids, in, tokens, vocab, shift, p.digit_bits, bins, counts, totals, to);
     in = to;
   }
   return in;
@@ -635,8 +653,12 @@ template <class T, class Id>
 void launch_embed(const void* ids, int64_t tokens, const void* weight, int64_t weight_stride,
                   int64_t vocab, int dim, float scale, void* out, hipStream_t st) {
   const int blocks = (int)ceil_div(dim, 8);
-  const int64_t groups = ceil_div(tokens * blocks, 256);
-  const auto kernel = dim % 8 == 0 ? embed_kernel<T, Id, true> : embed_kernel<T, Id, false>;
+  // Four blocks a thread once there are enough for four workgroups a compute unit all the same:
+  // 184832 rows of 512 bfloat16 take 41 us so and 56 us with one each.
+  const bool many = tokens * blocks >= 256 * 4 * 1024;
+  const int64_t groups = ceil_div(tokens * blocks, many ? 1024 : 256);
+  const auto kernel = dim % 8 == 0 ? (many ? embed_kernel<T, Id, true, 4> : embed_kernel<T, Id, true, 1>)
+                                   : (many ? embed_kernel<T, Id, false, 4> : embed_kernel<T, Id, false, 1>);
   kernel<<<(uint32_t)groups, 256, 0, st>>>(
       static_cast<const Id*>(ids), tokens, static_cast<const T*>(weight), weight_stride, vocab,
       dim, blocks, scale, static_cast<T*>(out));

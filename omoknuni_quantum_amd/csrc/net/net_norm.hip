@@ -292,7 +292,9 @@ void launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
   });
 }
 
-// Workgroups of the gradient: as many as run at once.
+// Workgroups of the gradient: 16 waves a compute unit (with 32, 16384 rows of 4096 take 135 us
+// instead of 128: more partial sums of the weight's gradient), and where the rows are few, four
+// rows or more each for the same reason, as long as the compute units have one.
 constexpr int64_t kGradWaves = 256 * 16;
 
 int64_t grad_groups(int64_t rows, int64_t dim) {
@@ -301,7 +303,8 @@ int64_t grad_groups(int64_t rows, int64_t dim) {
     using L = decltype(l);
     constexpr int kBlock = block_of<L::kThreads>();
     const int64_t all = ceil_div(rows, kBlock / L::kThreads);
-    const int64_t most = kGradWaves * kWave / kBlock;
+    const int64_t few = ceil_div(all, 4) < 256 ? 256 : ceil_div(all, 4);
+    const int64_t most = kGradWaves * kWave / kBlock < few ? kGradWaves * kWave / kBlock : few;
     groups = all < most ? all : most;
   });
   return groups;

@@ -43,10 +43,9 @@ __device__ inline void rebase(Stats& t, float m) {
   }
 }
 
-// Over the kLanes lanes of a group: all get the joined statistics.
+// Over the kLanes lanes of a group, of one base or of any: all get the joined statistics.
 template <int kLanes, bool kTarget>
-__device__ inline void lanes_join(Stats& t) {
-  rebase(t, lanes_reduce<Max, kLanes>(t.m));
+__device__ inline void lanes_sum(Stats& t) {
   t.s = lanes_reduce<Sum, kLanes>(t.s);
   if constexpr (kTarget) {
     t.tp = lanes_reduce<Sum, kLanes>(t.tp);
@@ -54,10 +53,20 @@ __device__ inline void lanes_join(Stats& t) {
   }
 }
 
-// Over the kThreads threads of a row (as row_reduce), with one barrier.
-template <int kThreads, bool kTarget>
+template <int kLanes, bool kTarget>
+__device__ inline void lanes_join(Stats& t) {
+  rebase(t, lanes_reduce<Max, kLanes>(t.m));
+  lanes_sum<kLanes, kTarget>(t);
+}
+
+// Over the kThreads threads of a row (as row_reduce), with one barrier.  kSame: the lanes of a
+// wave have one base.
+template <int kThreads, bool kTarget, bool kSame>
 __device__ inline void row_join(Stats& t, Stats* smem) {
-  lanes_join<(kThreads < kWave ? kThreads : kWave), kTarget>(t);
+  if constexpr (!kSame)
+    lanes_join<(kThreads < kWave ? kThreads : kWave), kTarget>(t);
+  else
+    lanes_sum<(kThreads < kWave ? kThreads : kWave), kTarget>(t);
   if constexpr (kThreads > kWave) {
     static_assert(kThreads <= 16 * kWave);
     const int lane = threadIdx.x & (kWave - 1);
@@ -87,12 +96,14 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
   const bool live = !(t.m == -kInf && t.s == 0.0f);
   if (!live) return o;
   const float base = base_of(t.m);
-  const float log_s = logf(t.s);
+  // (the instructions themselves, within a unit in the last place: s is at least e^-8 and an
+  // ordinary number)
+  const float log_s = __builtin_amdgcn_logf(t.s) * kLn2;
   float slope = 0.0f;
   if (taken) {
     o.logp = z_taken - base - log_s;
     const float adv = r.advantages[row];
-    const float ratio = expf(o.logp - r.old_logp[row]);
+    const float ratio = exp_fast(o.logp - r.old_logp[row]);
     const float one = ratio * adv;
     const float two = fminf(fmaxf(ratio, 1.0f - r.clip_low), 1.0f + r.clip_high) * adv;
     o.loss = -(one <= two || one != one ? one : two);
@@ -106,7 +117,7 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
   if (r.target) o.kl = t.tk + (t.tp != 0.0f ? t.tp * log_s : 0.0f);
   o.loss += r.kl_coef != 0.0f ? r.kl_coef * o.kl : 0.0f;
   o.g.m = base;
-  o.g.inv_s = 1.0f / t.s;
+  o.g.inv_s = __builtin_amdgcn_rcpf(t.s);
   o.g.slope = slope;
   o.g.push = (r.kl_coef != 0.0f ? r.kl_coef * t.tp : 0.0f) - slope;
   // a row that adds nothing to the loss has no gradient, whatever its logits hold (padding)
@@ -255,33 +266,40 @@ __device__ inline void add_logits(Stats& t, F8& z, float base) {
 }
 
 // Adds a block's targets, about the same base, and leaves 0 in place of those that are not
-// positive.  (The logarithm takes subnormals for 0: what they add is nothing beside the rest.)
+// positive.  (The logarithm takes subnormals for 0: what they add is nothing beside the rest.  The
+// legacy product is 0 where a factor is 0: the logit of a target of 0 may be -inf.)
 __device__ inline void add_target(Stats& t, F8& pi, F8 z, float base) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const bool some = pi[j] > 0.0f;
+    pi[j] = larger(pi[j], 0.0f);
     const float log_pi = __builtin_amdgcn_logf(larger(pi[j], 0x1p-126f));  // (base 2)
-    const float term = pi[j] * fmaf(log_pi, kLn2, base - z[j]);
-    t.tk += some ? term : 0.0f;
-    pi[j] = some ? pi[j] : 0.0f;
+    float term;
+    asm("v_mul_legacy_f32 %0, %1, %2"
+        : "=v"(term)
+        : "v"(pi[j]), "v"(fmaf(log_pi, kLn2, base - z[j])));
+    t.tk += term;
     t.tp += pi[j];
   }
 }
 
-// The gradient of eight actions, times the row's weight w: e holds e^(z - m), scale is
-// w * push / s (or that about the base of e).
+// The gradient of eight actions but for the slope of the taken one, times the row's weight w: e
+// holds e^(z - m), scale is w * push / s (or that about the base of e).
 template <bool kTarget>
-__device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, int taken, float scale, float w_slope,
-                              float w_coef) {
+__device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coef) {
   F8 d = e * scale;
   if constexpr (kTarget) d -= pi * w_coef;
-  if (taken >= 0 && taken < 8) {  // (the place of the taken action in the block)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] += j == taken ? w_slope : 0.0f;
-  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) d[j] = masked(d[j], ok_mask(ok, j), 0.0f);
   return d;
+}
+
+// The element of the taken action, in full; written by the thread that wrote its block, after it.
+template <class T>
+__device__ inline void put_taken(T* grad, const RowIn<T>& in, const RowGrad& g, float z_taken,
+                                 int taken, float coef, float w) {
+  float d = exp_fast(z_taken - g.m) * (w * g.push * g.inv_s);
+  if (in.target) d -= larger(in.target[taken], 0.0f) * (w * coef);
+  grad[taken] = (T)(d + w * g.slope);
 }
 
 // ---- rows in registers ----------------------------------------------------------------------
@@ -328,7 +346,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
     }
     add_logits(t, z[i], base);
   }
-  row_join<kThreads, kTarget>(t, smem);
+  row_join<kThreads, kTarget, true>(t, smem);
   const RowOut o = finish_row(r, row, t, z_taken, taken >= 0);
   if (lane == 0) write_row(o, row, loss, logp, kl, stats);
   if (!grad) return;
@@ -339,10 +357,11 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
     const int col = 8 * (lane + i * kThreads);
     F8 d = {};
     if (o.g.inv_s != 0.0f)
-      d = gradient<kTarget>(z[i], pi[kTarget ? i : 0], ok[i], taken - col, scale, w * o.g.slope,
-                            w * r.kl_coef);
+      d = gradient<kTarget>(z[i], pi[kTarget ? i : 0], ok[i], scale, w * r.kl_coef);
     store8<T, kWhole>(grad + row * in.cols, col, in.cols, d);
   }
+  if (taken >= 0 && o.g.inv_s != 0.0f && lane == (taken / 8) % kThreads)
+    put_taken(grad + row * in.cols, in, o.g, z_taken, taken, r.kl_coef, w);
 }
 
 // ---- long rows ------------------------------------------------------------------------------
@@ -391,7 +410,7 @@ __device__ inline void stream(Stats& t, const RowIn<T>& in, int from, int to) {
 // The gradient of the block at column col.
 template <class T, bool kTarget, bool kWhole, bool kStream>
 __device__ inline void put_gradient(T* grad, const Block<T, kTarget>& b, const RowIn<T>& in,
-                                    int col, const RowGrad& g, int taken, float coef, float w) {
+                                    int col, const RowGrad& g, float coef, float w) {
   F8 d = {}, pi = {};
   if (g.inv_s != 0.0f) {
     const uint64_t ok = ok_bytes<T, kTarget, kWhole>(b, in, col);
@@ -399,11 +418,11 @@ __device__ inline void put_gradient(T* grad, const Block<T, kTarget>& b, const R
     if constexpr (kTarget) {
       pi = legal_target<T, kWhole>(b, in, col, ok);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pi[j] = pi[j] > 0.0f ? pi[j] : 0.0f;
+      for (int j = 0; j < 8; ++j) pi[j] = larger(pi[j], 0.0f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) z[j] = exp_fast(z[j] - g.m);
-    d = gradient<kTarget>(z, pi, ok, taken - col, w * g.push * g.inv_s, w * g.slope, w * coef);
+    d = gradient<kTarget>(z, pi, ok, w * g.push * g.inv_s, w * coef);
   }
   store8<T, kWhole, kStream>(grad, col, in.cols, d);
 }
@@ -423,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
   Stats t = no_stats();
   stream<T, kTarget, kWhole, kThreads>(t, in, 0, in.cols);
-  row_join<kThreads, kTarget>(t, smem);
+  row_join<kThreads, kTarget, false>(t, smem);
   const RowOut o = finish_row(r, row, t, z_taken, taken >= 0);
   if (threadIdx.x == 0) write_row(o, row, loss, logp, kl, stats);
   if (!grad) return;
@@ -438,8 +457,10 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
 #pragma unroll
     for (int u = 0; u < kCount; ++u)
       put_gradient<T, kTarget, kWhole, true>(g, b[u], in, at + 8 * (int)threadIdx.x + kStep * u,
-                                         o.g, taken, r.kl_coef, w);
+                                         o.g, r.kl_coef, w);
   }
+  if (taken >= 0 && o.g.inv_s != 0.0f && (int)threadIdx.x == (taken / 8) % kThreads)
+    put_taken(g, in, o.g, z_taken, taken, r.kl_coef, w);
 }
 
 // Statistics of span blockIdx.x of row blockIdx.y.
@@ -453,7 +474,7 @@ __global__ __launch_bounds__(256) void loss_span_kernel(omq_policy_rows r, int s
   const int to = from + span < in.cols ? (int)(from + span) : in.cols;
   Stats t = no_stats();
   stream<T, kTarget, kWhole, 256>(t, in, (int)from, to);
-  row_join<256, kTarget>(t, smem);
+  row_join<256, kTarget, false>(t, smem);
   if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = t;
 }
 
@@ -499,7 +520,10 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(omq_policy_rows r, int b
   const float w = row_weight ? row_weight[row] : 1.0f;
   float z_taken;
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
-  put_gradient<T, kTarget, kWhole, false>(grad + row * in.cols, b, in, col, g, taken, r.kl_coef, w);
+  T* to = grad + row * in.cols;
+  put_gradient<T, kTarget, kWhole, false>(to, b, in, col, g, r.kl_coef, w);
+  if (taken >= 0 && g.inv_s != 0.0f && taken / 8 == col / 8)
+    put_taken(to, in, g, z_taken, taken, r.kl_coef, w);
 }
 
 // ---- launches -------------------------------------------------------------------------------
