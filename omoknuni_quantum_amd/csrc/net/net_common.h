@@ -255,6 +255,18 @@ __device__ inline F8 drop8(F8 v, const Dropout& d, uint64_t row_base, int col) {
   return v;
 }
 
+// ---- grids --------------------------------------------------------------------------------
+// A launch has fewer than 2^32 threads along x: grids of more workgroups go on along y.
+__device__ inline int64_t block_index() {
+  return (int64_t)blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+}
+
+inline dim3 grid_of(int64_t blocks, int threads) {
+  const int64_t most = 0xFFFFFFFFll / threads;
+  if (blocks <= most) return dim3((uint32_t)blocks);
+  return dim3((uint32_t)most, (uint32_t)((blocks + most - 1) / most));
+}
+
 // ---- host side ----------------------------------------------------------------------------
 int net_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int net_status(const char* what);  // of the launches made since the last call

@@ -12,7 +12,7 @@ namespace {
 template <class T, bool kWhole>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t rows, int dim,
                                                       int blocks, Dropout d, T* out) {
-  const int64_t first = (int64_t)blockIdx.x * 256;
+  const int64_t first = block_index() * 256;
   const int64_t row0 = first / blocks;
   const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
   const int64_t row = row0 + in / (uint32_t)blocks;
@@ -43,7 +43,7 @@ extern "C" int omq_dropout(const void* x, int64_t rows, int64_t dim, int dtype, 
   if (!x || !out) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   const Dropout d = make_dropout(p, seed, offset);
   const int blocks = (int)ceil_div(dim, 8);
-  const uint32_t grid = (uint32_t)ceil_div(rows * blocks, 256);
+  const dim3 grid = grid_of(ceil_div(rows * blocks, 256), 256);
   hipStream_t st = (hipStream_t)stream;
   const auto go = [&](auto t) {
     using T = decltype(t);

@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const Id* __restrict__ ids, 
                                                     int64_t weight_stride, int64_t vocab,
                                                     int dim, int blocks, float scale,
                                                     T* __restrict__ out) {
-  const int64_t first = (int64_t)blockIdx.x * (256 * kBlocks);
+  const int64_t first = block_index() * (256 * kBlocks);
   const int64_t row0 = first / blocks;
   const uint32_t in = (uint32_t)(first - row0 * blocks) + threadIdx.x;
   int64_t t[kBlocks], id[kBlocks];
@@ -532,6 +532,79 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
   }
 }
 
+// ---- few tokens -----------------------------------------------------------------------------
+// Up to 256 tokens take one launch: a workgroup has some rows of the vocabulary (and 512 columns),
+// picks the tokens of those rows out of all, in their order, and its waves take a row each in
+// turn.  225 tokens of 675 rows and 128 columns take 5 us a
+// call, and 15 by the sorted way; 256 of the same row 17 either way.
+constexpr int kFewTokens = 256;
+
+template <class T, class O, class Id, bool kWhole>
+__global__ __launch_bounds__(256) void sum_few_kernel(const T* __restrict__ grad,
+                                                      int64_t grad_stride,
+                                                      const Id* __restrict__ ids, int tokens,
+                                                      int64_t vocab, int dim, float scale,
+                                                      int rows, O* __restrict__ out) {
+  constexpr int kBatch = 8;  // rows of `grad` in flight
+  __shared__ uint32_t token_of[kFewTokens], row_of[kFewTokens];
+  __shared__ int counts[4];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t row0 = (int64_t)blockIdx.x * rows;
+  int64_t at = -1;
+  if ((int)threadIdx.x < tokens) {
+    const int64_t id = (int64_t)ids[threadIdx.x];
+    if (id >= row0 && id < row0 + rows && id < vocab) at = id - row0;
+  }
+  const uint64_t here = __ballot(at >= 0);
+  if (lane == 0) counts[wave] = __popcll(here);
+  __syncthreads();
+  int total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w == wave) before = total;
+    total += counts[w];
+  }
+  if (at >= 0) {
+    const int place = before + lanes_below(here);
+    token_of[place] = threadIdx.x;
+    row_of[place] = (uint32_t)at;
+  }
+  __syncthreads();
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int col = 8 * ((int)blockIdx.y * kWave + lane);
+  for (int r = wave; r < rows && row0 + r < vocab; r += 4) {
+    F8 acc = {};
+    for (int base = 0; base < total; base += kWave) {
+      const bool listed = base + lane < total;
+      const uint32_t token = listed ? token_of[base + lane] : 0u;
+      uint64_t mine = __ballot(listed && row_of[base + lane] == (uint32_t)r);
+      while (mine) {
+        Reg8<T> v[kBatch];
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {  // (the last token again where there are no more)
+          const int from = __builtin_ctzll(mine);
+          const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)token, from);
+          v[e] = load_raw<T, kWhole>(grad + (int64_t)t * grad_stride, col, dim);
+          if (n == e) {
+            n = e + 1;
+            if (mine & (mine - 1))
+              mine &= mine - 1;
+            else
+              n |= 0x100;  // the last one
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+          if (e < (n & 0xFF)) acc += widen<T, kWhole>(v[e], col, dim);
+        if (n & 0x100) mine = 0;
+      }
+    }
+    store8<O, kWhole>(out + (row0 + r) * dim, col, dim, acc * scale);
+  }
+}
+
 // ---- plan -----------------------------------------------------------------------------------
 struct GradPlan {
   int bits, passes, digit_bits;
@@ -553,6 +626,7 @@ bool grad_sizes_ok(int64_t tokens, int64_t vocab, int64_t dim) {
 
 GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   GradPlan p{};
+  if (tokens <= kFewTokens) return p;  // (no workspace)
   while (p.bits < 32 && (vocab >> p.bits) != 0) ++p.bits;
   p.passes = (int)ceil_div(p.bits, kMaxDigitBits);
   p.digit_bits = (int)ceil_div(p.bits, p.passes);
@@ -586,14 +660,11 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
                          hipStream_t st) {
   uint2* buf[2] = {reinterpret_cast<uint2*>(ws + p.at_pairs[0]),
                    reinterpret_cast<uint2*>(ws + p.at_pairs[1])};
-  if (tokens == 0) return buf[0];
   if (tokens <= kSmallSort) {
     const auto sort = [&](auto kernel, int threads) {
       kernel<<<1, threads, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
     };
-    if (tokens <= 256)
-      sort(sort_small_kernel<Id, 256, 1>, 256);
-    else if (tokens <= 1024)
+    if (tokens <= 1024)
       sort(sort_small_kernel<Id, 1024, 1>, 1024);
     else
       sort(sort_small_kernel<Id, 1024, kSmallSort / 1024>, 1024);
@@ -639,6 +710,26 @@ void launch_sums(const GradPlan& p, const void* grad, int64_t grad_stride, const
                                            static_cast<O*>(out));
 }
 
+template <class T, class O>
+void launch_few(const void* grad, int64_t grad_stride, const void* ids, int ids_are_64, int tokens,
+                int64_t vocab, int dim, float scale, void* out, hipStream_t st) {
+  const int64_t col_tiles = ceil_div(dim, 8 * kWave);
+  // rows for about 2048 workgroups, four or more (a wave's)
+  const int64_t rows = ceil_div(ceil_div(vocab * col_tiles, 2048), 4) * 4;
+  const dim3 grid((uint32_t)ceil_div(vocab, rows), (uint32_t)col_tiles);
+  const auto go = [&](auto id, auto kernel) {
+    using Id = decltype(id);
+    kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(grad), grad_stride,
+                                 static_cast<const Id*>(ids), tokens, vocab, dim, scale, (int)rows,
+                                 static_cast<O*>(out));
+  };
+  const bool whole = dim % 8 == 0;
+  if (ids_are_64)
+    go(int64_t{}, whole ? sum_few_kernel<T, O, int64_t, true> : sum_few_kernel<T, O, int64_t, false>);
+  else
+    go(int32_t{}, whole ? sum_few_kernel<T, O, int32_t, true> : sum_few_kernel<T, O, int32_t, false>);
+}
+
 template <class T, class O, class... A>
 void launch_sums_lanes(const GradPlan& p, A... a) {
   switch (p.lanes) {
@@ -659,7 +750,7 @@ void launch_embed(const void* ids, int64_t tokens, const void* weight, int64_t w
   const int64_t groups = ceil_div(tokens * blocks, many ? 1024 : 256);
   const auto kernel = dim % 8 == 0 ? (many ? embed_kernel<T, Id, true, 4> : embed_kernel<T, Id, true, 1>)
                                    : (many ? embed_kernel<T, Id, false, 4> : embed_kernel<T, Id, false, 1>);
-  kernel<<<(uint32_t)groups, 256, 0, st>>>(
+  kernel<<<grid_of(groups, 256), 256, 0, st>>>(
       static_cast<const Id*>(ids), tokens, static_cast<const T*>(weight), weight_stride, vocab,
       dim, blocks, scale, static_cast<T*>(out));
 }
@@ -717,25 +808,29 @@ int omq_token_embedding_grad(const void* grad, int64_t grad_stride, int dtype, c
     return net_fail(OMQ_NET_E_ARG, "%s: tokens %lld, vocab %lld, dim %lld, grad_stride %lld", name,
                     (long long)tokens, (long long)vocab, (long long)dim, (long long)grad_stride);
   const GradPlan p = grad_plan(tokens, vocab, dim);
-  if (workspace_bytes < p.bytes || !workspace)
+  if (p.bytes > 0 && (workspace_bytes < p.bytes || !workspace))
     return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes, %lld needed", name,
                     (long long)workspace_bytes, (long long)p.bytes);
   if (!out || (tokens > 0 && (!grad || !ids)))
     return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   hipStream_t st = (hipStream_t)stream;
   char* ws = static_cast<char*>(workspace);
-  const uint2* pairs =
-      ids_are_64 ? sort_tokens(p, static_cast<const int64_t*>(ids), tokens, vocab, ws, st)
-                 : sort_tokens(p, static_cast<const int32_t*>(ids), tokens, vocab, ws, st);
-  const auto go = [&](auto t) {
+  const bool few = tokens <= kFewTokens;
+  const uint2* pairs = nullptr;
+  if (!few)
+    pairs = ids_are_64 ? sort_tokens(p, static_cast<const int64_t*>(ids), tokens, vocab, ws, st)
+                       : sort_tokens(p, static_cast<const int32_t*>(ids), tokens, vocab, ws, st);
+  const auto sums = [&](auto t, auto o) {
     using T = decltype(t);
-    if (out_dtype == OMQ_NET_F32)
-      launch_sums_lanes<T, float>(p, grad, grad_stride, pairs, tokens, vocab, (int)dim, scale, out,
-                                  ws, st);
+    using O = decltype(o);
+    if (few)
+      launch_few<T, O>(grad, grad_stride, ids, ids_are_64, (int)tokens, vocab, (int)dim, scale, out,
+                       st);
     else
-      launch_sums_lanes<T, T>(p, grad, grad_stride, pairs, tokens, vocab, (int)dim, scale, out, ws,
+      launch_sums_lanes<T, O>(p, grad, grad_stride, pairs, tokens, vocab, (int)dim, scale, out, ws,
                               st);
   };
+  const auto go = [&](auto t) { out_dtype == OMQ_NET_F32 ? sums(t, float{}) : sums(t, t); };
   if (dtype == OMQ_NET_F32) go(float{});
   else if (dtype == OMQ_NET_BF16) go(bf16{});
   else go(f16{});

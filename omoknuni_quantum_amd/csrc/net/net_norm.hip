@@ -67,7 +67,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void norm_kernel(NormArgs a) 
   constexpr int kRows = block_of<kThreads>() / kThreads;
   __shared__ float smem[2][16];
   const int lane = threadIdx.x % kThreads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + row_slot<kThreads>();
+  const int64_t row = block_index() * kRows + row_slot<kThreads>();
   if (row >= a.rows) return;  // (whole rows leave: no barrier or reduction spans two rows)
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
@@ -284,10 +284,10 @@ void launch_norm(const NormArgs& a, int dtype, hipStream_t st) {
     with_layout(a.dim, [&](auto l) {
       using L = decltype(l);
       constexpr int kBlock = block_of<L::kThreads>();
-      const int64_t grid = ceil_div(a.rows, kBlock / L::kThreads);
+      const dim3 grid = grid_of(ceil_div(a.rows, kBlock / L::kThreads), kBlock);
       const auto kernel = a.dim % 8 == 0 ? norm_kernel<T, L::kThreads, L::kVecs, kMode, true>
                                          : norm_kernel<T, L::kThreads, L::kVecs, kMode, false>;
-      kernel<<<(uint32_t)grid, kBlock, 0, st>>>(a);
+      kernel<<<grid, kBlock, 0, st>>>(a);
     });
   });
 }

@@ -316,7 +316,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
   constexpr int kRows = block_of<kThreads>() / kThreads;
   __shared__ Stats smem[16];
   const int lane = threadIdx.x % kThreads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + row_slot<kThreads>();
+  const int64_t row = block_index() * kRows + row_slot<kThreads>();
   if (row >= r.rows) return;
   const RowIn<T> in = row_in<T>(r, row);
   const int64_t action = action_of(r, row);
@@ -436,7 +436,8 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
     T* __restrict__ grad) {
   constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
   __shared__ Stats smem[16];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= r.rows) return;
   const RowIn<T> in = row_in<T>(r, row);
   float z_taken;
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
@@ -507,7 +508,7 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(omq_policy_rows r, int b
                                                         const float4* __restrict__ stats,
                                                         const float* __restrict__ row_weight,
                                                         T* __restrict__ grad) {
-  const int64_t first = (int64_t)blockIdx.x * 256;
+  const int64_t first = block_index() * 256;
   const int64_t row0 = first / blocks;
   const uint32_t at = (uint32_t)(first - row0 * blocks) + threadIdx.x;
   const int64_t row = row0 + at / (uint32_t)blocks;
@@ -638,7 +639,7 @@ void launch_rows(const omq_policy_rows& r, const float* row_weight, const LossOu
       with_layout<K::target>(r.actions, [&](auto l) {
         using L = decltype(l);
         constexpr int kBlock = block_of<L::kThreads>();
-        const uint32_t grid = (uint32_t)ceil_div(r.rows, kBlock / L::kThreads);
+        const dim3 grid = grid_of(ceil_div(r.rows, kBlock / L::kThreads), kBlock);
         loss_rows_kernel<T, L::kThreads, L::kVecs, K::target, K::whole><<<grid, kBlock, 0, st>>>(
             r, row_weight, o.loss, o.logp, o.kl, reinterpret_cast<float4*>(o.stats),
             static_cast<T*>(grad));
@@ -656,7 +657,8 @@ void launch_long(const omq_policy_rows& r, const float* row_weight, const LossOu
       const bool wide = r.actions > kWideActions;
       const auto kernel = wide ? loss_long_kernel<T, 1024, K::target, K::whole>
                                : loss_long_kernel<T, 512, K::target, K::whole>;
-      kernel<<<(uint32_t)r.rows, wide ? 1024 : 512, 0, st>>>(
+      const int threads = wide ? 1024 : 512;
+      kernel<<<grid_of(r.rows, threads), threads, 0, st>>>(
           r, row_weight, o.loss, o.logp, o.kl, reinterpret_cast<float4*>(o.stats),
           static_cast<T*>(grad));
     });
@@ -685,7 +687,7 @@ void launch_grad(const omq_policy_rows& r, const float* stats, const float* row_
     with_kind(r, [&](auto kind) {
       using K = decltype(kind);
       const int blocks = (int)ceil_div(r.actions, 8);
-      const uint32_t grid = (uint32_t)ceil_div(r.rows * blocks, 256);
+      const dim3 grid = grid_of(ceil_div(r.rows * blocks, 256), 256);
       loss_grad_kernel<T, K::target, K::whole><<<grid, 256, 0, st>>>(
           r, blocks, reinterpret_cast<const float4*>(stats), row_weight, static_cast<T*>(grad));
     });

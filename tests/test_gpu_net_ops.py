@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from omoknuni_quantum_amd import net_ops
+from omoknuni_quantum_amd import _lib, net_ops
 from oracle import net_ref
 
 pytestmark = pytest.mark.gpu
@@ -21,6 +21,10 @@ u = 2.0**-24
 U = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
 TINY = {torch.float32: 2.0**-149, torch.bfloat16: 2.0**-133, torch.float16: 2.0**-25}
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _lib_check(rc):
+    assert rc == _lib.OMQ_OK, _lib.load_net().omq_net_last_error()
 
 
 def gen(seed):
@@ -76,9 +80,11 @@ def test_embedding_shapes_and_far_ids(device):
 
 
 GRAD_CASES = [
-    # tokens, vocab, dim, skew: no tokens; one; one vocabulary row; one workgroup's sort; radix
-    # sorts of one, two and three passes; tokens of few rows and rows of few tokens
-    (0, 5, 16, 1), (1, 1, 1, 1), (1, 3000, 40, 1), (225, 675, 128, 1), (4096, 1, 64, 1),
+    # tokens, vocab, dim, skew: no tokens; one; few; one vocabulary row; one workgroup's sorts;
+    # radix sorts of one, two and three passes; tokens of few rows and rows of few tokens
+    (0, 5, 16, 1), (1, 1, 1, 1), (1, 3000, 40, 1), (225, 675, 128, 1), (256, 2, 600, 1),
+    (256, 20_000, 7, 2), (257, 2, 600, 1), (1024, 40, 24, 1), (1025, 300, 129, 1),
+    (4096, 1, 64, 1),
     (4096, 300, 33, 3), (4097, 3, 64, 1), (5000, 2047, 130, 1), (9000, 2048, 257, 4),
     (20_000, 70_000, 65, 3), (6000, 5_000_000, 8, 1), (50_000, 2, 513, 1), (30_001, 900, 1031, 2),
 ]
@@ -448,6 +454,24 @@ def test_offsets_past_32_bits(device):
     tokens[-1] = 2
     grad = net_ops.token_embedding_grad(x, tokens, 7)
     assert torch.equal(grad[2], x[-1]) and not bool(grad[5].any())
+
+
+def test_more_threads_than_a_grid_dimension_holds(device):
+    """2^32 lanes of eight elements and more: the grid goes on along y."""
+    lib = _lib.load_net()
+    rows, dim = 2**29 + 5, 64
+    x = torch.empty(rows * dim, dtype=torch.bfloat16, device=device)
+    x[:64 * dim] = 1.0
+    x[-64 * dim:] = 1.0
+    _lib_check(lib.omq_dropout(x.data_ptr(), rows, dim, _lib.OMQ_NET_BF16, 0.5, 11, 3,
+                               x.data_ptr(), _lib.raw_stream(x.device)))
+    key = net_ref.splitmix64(net_ref.splitmix64(11) ^ 3)
+    for first in (0, rows - 64):
+        got = x[first * dim:(first + 64) * dim].float().cpu().view(64, dim)
+        for r, c in ((0, 0), (63, 63), (40, 17)):
+            word = net_ref.splitmix64(
+                (key + net_ref.GOLDEN * ((first + r) * 16 + c // 4)) & net_ref.M64)
+            assert float(got[r, c]) == (2.0 if word >> (16 * (c % 4)) & 0xFFFF >= 32768 else 0.0)
 
 
 def test_another_stream(device):
