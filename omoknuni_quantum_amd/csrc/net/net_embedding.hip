@@ -216,19 +216,25 @@ __global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int digit = blockIdx.x * kWave + lane;
   const int per = (tiles + 15) / 16;
-  const int from = wave * per, to = from + per < tiles ? from + per : tiles;
+  const int from = wave * per < tiles ? wave * per : tiles;
+  const int to = from + per < tiles ? from + per : tiles;
   // (eight loads in flight, the last ones too)
   const uint32_t* column = counts + (digit < bins ? digit : bins - 1);
   const auto eight = [&](int t, uint32_t (&c)[8]) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) c[u] = column[(int64_t)(t + u < to ? t + u : t) * bins];
+    for (int u = 0; u < 8; ++u) c[u] = column[(int64_t)(t + u < to ? t + u : to - 1) * bins];
   };
-  uint32_t sum = 0;
-  for (int t = from; t < to; t += 8) {
-    uint32_t c[8];
-    eight(t, c);
+  uint32_t held[8], sum = 0;  // the first eight, for the second time too
+  eight(from, held);
+  const auto add = [&](int t, const uint32_t (&c)[8]) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) sum += t + u < to ? c[u] : 0u;
+  };
+  add(from, held);
+  for (int t = from + 8; t < to; t += 8) {
+    uint32_t c[8];
+    eight(t, c);
+    add(t, c);
   }
   sums[wave][lane] = sum;
   __syncthreads();
@@ -236,15 +242,19 @@ __global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__
   for (int w = 0; w < wave; ++w) base += sums[w][lane];
   if (digit >= bins) return;
   if (wave == 15) totals[digit] = base + sum;
-  for (int t = from; t < to; t += 8) {
-    uint32_t c[8];
-    eight(t, c);
+  const auto put = [&](int t, const uint32_t (&c)[8]) {
 #pragma unroll
     for (int u = 0; u < 8; ++u)
       if (t + u < to) {
         counts[(int64_t)(t + u) * bins + digit] = base;
         base += c[u];
       }
+  };
+  put(from, held);
+  for (int t = from + 8; t < to; t += 8) {
+    uint32_t c[8];
+    eight(t, c);
+    put(t, c);
   }
 }
 
@@ -535,8 +545,8 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
 // ---- few tokens -----------------------------------------------------------------------------
 // Up to 256 tokens take one launch: a workgroup has some rows of the vocabulary (and 512 columns),
 // picks the tokens of those rows out of all, in their order, and its waves take a row each in
-// turn.  225 tokens of 675 rows and 128 columns take 5 us a
-// call, and 15 by the sorted way; 256 of the same row 17 either way.
+// turn.  225 tokens of 675 rows and 128 columns take 5 us a call, and 15 by the sorted way; 256
+// tokens of two rows 17 us either way.
 constexpr int kFewTokens = 256;
 
 template <class T, class O, class Id, bool kWhole>

@@ -287,7 +287,12 @@ __device__ inline void add_target(Stats& t, F8& pi, F8 z, float base) {
 template <bool kTarget>
 __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coef) {
   F8 d = e * scale;
-  if constexpr (kTarget) d -= pi * w_coef;
+  if constexpr (kTarget) {
+    // (fmaf where a product and a sum could be contracted one way here and another there: the
+    // gradient has the same bits whichever kernel forms it from the same statistics)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = fmaf(-pi[j], w_coef, d[j]);
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) d[j] = masked(d[j], ok_mask(ok, j), 0.0f);
   return d;
@@ -298,8 +303,8 @@ template <class T>
 __device__ inline void put_taken(T* grad, const RowIn<T>& in, const RowGrad& g, float z_taken,
                                  int taken, float coef, float w) {
   float d = exp_fast(z_taken - g.m) * (w * g.push * g.inv_s);
-  if (in.target) d -= larger(in.target[taken], 0.0f) * (w * coef);
-  grad[taken] = (T)(d + w * g.slope);
+  if (in.target) d = fmaf(-larger(in.target[taken], 0.0f), w * coef, d);
+  grad[taken] = (T)fmaf(w, g.slope, d);
 }
 
 // ---- rows in registers ----------------------------------------------------------------------
@@ -535,10 +540,15 @@ struct Layout {
 
 // The longest rows that are held in registers, without and with a target.
 constexpr int64_t kRowActions = 16384, kRowActionsTarget = 8192;
-// Long rows from this many on are a workgroup each, fewer are cut into spans.
-constexpr int64_t kLongRows = 128;
-// The workgroup of a long row: wide enough that the rows under way stay in the last-level cache.
-constexpr int64_t kWideActions = 65536;
+// Longer rows are a workgroup each, unless they are fewer than kLongRows and longer than
+// kWideActions: those are cut into spans (with their gradients, in bfloat16: 8 rows of 131072 take
+// 12 us so and 21 us with a workgroup each; 16 rows of 20000 take 7 us with a workgroup each and
+// 13 us cut; 128 rows of 131072 the same).
+constexpr int64_t kLongRows = 128, kWideActions = 65536;
+// A workgroup of 1024 threads for rows over kWideActions, so that the rows under way stay in the
+// last-level cache (4096 rows of 131072 bfloat16: 449 us, 484 with 512 threads), and where there
+// are fewer rows than compute units; else 512 (4096 rows of 32768: 113 us, 117 with 1024).
+bool wide_row(int64_t rows, int64_t actions) { return actions > kWideActions || rows < 256; }
 
 template <bool kTarget, class F>
 void with_layout(int64_t cols, F&& f) {
@@ -577,14 +587,14 @@ void with_kind(const omq_policy_rows& r, F&& f) {
     r.actions % 8 == 0 ? f(Kind<false, true>{}) : f(Kind<false, false>{});
 }
 
-// How rows of these sizes are cut, whatever the target; used where they are not in registers.
+// How rows are cut into spans, where they are.
 struct SpanPlan {
   int64_t span, spans, at_parts, bytes;
 };
 
 SpanPlan span_plan(int64_t rows, int64_t actions) {
   SpanPlan p{};
-  if (actions <= kRowActionsTarget || rows >= kLongRows) return p;
+  if (rows >= kLongRows || actions <= kWideActions) return p;
   // spans for about 1024 workgroups, of at least 4096 columns
   int64_t spans = ceil_div(1024, rows > 0 ? rows : 1);
   const int64_t most = ceil_div(actions, 4096);
@@ -600,7 +610,7 @@ enum Way { kInRows, kLong, kSpans };
 
 Way way_of(const omq_policy_rows& r) {
   if (r.actions <= (r.target ? kRowActionsTarget : kRowActions)) return kInRows;
-  return r.rows >= kLongRows ? kLong : kSpans;
+  return r.rows >= kLongRows || r.actions <= kWideActions ? kLong : kSpans;
 }
 
 bool loss_sizes_ok(int64_t rows, int64_t actions) {
@@ -654,7 +664,7 @@ void launch_long(const omq_policy_rows& r, const float* row_weight, const LossOu
     using T = decltype(t);
     with_kind(r, [&](auto kind) {
       using K = decltype(kind);
-      const bool wide = r.actions > kWideActions;
+      const bool wide = wide_row(r.rows, r.actions);
       const auto kernel = wide ? loss_long_kernel<T, 1024, K::target, K::whole>
                                : loss_long_kernel<T, 512, K::target, K::whole>;
       const int threads = wide ? 1024 : 512;

@@ -357,7 +357,7 @@ def check_loss(device, d, coef, low=0.2, high=0.3, with_grad=True):
 @pytest.mark.parametrize("rows,actions", [(1, 1), (3, 2), (20, 9), (33, 128), (31, 225), (30, 362),
                                           (17, 513), (14, 1025), (15, 2049), (16, 4672),
                                           (14, 8193), (8, 16384), (8, 16385), (15, 50_001),
-                                          (3, 131_072)])
+                                          (5, 70_001), (3, 131_072), (130, 65_537)])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kl", ["none", "sampled", "target"])
 def test_policy_loss(device, rows, actions, dtype, kl):
@@ -386,8 +386,7 @@ def test_policy_loss_of_rows_without_anything(device):
     assert logp[4] == -math.inf and kl[4] == math.inf and loss[4] == math.inf
     assert grad[4].tolist() == [0.5, -0.5]
     # padding: the logits are NaN, the row has no action
-    n = torch.full((3, 300), float("nan"))
-    for cols in (300, 20_000):
+    for cols in (300, 20_000, 80_000):
         n = torch.full((3, cols), float("nan"))
         out = net_ops.clipped_policy_loss_with_grad(
             n.to(device), torch.full((3,), -1).to(device), f[:3].to(device), f[:3].to(device))
@@ -395,7 +394,7 @@ def test_policy_loss_of_rows_without_anything(device):
 
 
 def test_policy_loss_nan_reaches_the_result(device):
-    for cols in (100, 3000, 20_000):
+    for cols in (100, 3000, 20_000, 80_000):
         z = torch.zeros(2, cols)
         z[1, 7] = float("nan")
         f, act = torch.ones(2, device=device), torch.zeros(2, dtype=torch.int32, device=device)
@@ -406,7 +405,7 @@ def test_policy_loss_nan_reaches_the_result(device):
 
 def test_policy_loss_far_logits(device):
     """Logits about a large common value: the statistics are formed about the largest one."""
-    for cols in (225, 20_000):
+    for cols in (225, 20_000, 80_000):
         d = loss_inputs(12, cols, torch.float32, "target", False, cols)
         d["z"] = (d["z"] + 1000.0).float()
         ref = net_ref.policy_loss(d["z"], d["act"], d["adv"], d["old"], 0.2, 0.3, 1.0,
@@ -494,7 +493,8 @@ def test_graph_replays(device):
     ids = torch.randint(0, 500, (6000,), generator=g).int().to(device)
     table = randn(g, 500, 200).to(device)
     w = torch.rand(200, generator=g).to(device)
-    z, act = randn(g, 64, 20_000).to(device), torch.randint(0, 20_000, (64,), generator=g).to(device)
+    # (spans, joined, and an element-wise gradient)
+    z, act = randn(g, 64, 70_000).to(device), torch.randint(0, 70_000, (64,), generator=g).to(device)
     f = torch.ones(64, device=device)
 
     def step():
@@ -511,7 +511,7 @@ def test_graph_replays(device):
         out = step()
     for turn in range(4):
         table.copy_(randn(g, 500, 200).to(device))
-        z.copy_(randn(g, 64, 20_000).to(device))
+        z.copy_(randn(g, 64, 70_000).to(device))
         want = [t.clone() for t in step()]
         torch.cuda.synchronize()
         for t in out:
@@ -544,7 +544,7 @@ def test_autograd_is_the_gradient_operators(device):
     assert torch.equal(gx, net_ops.add_rms_norm_grad(up_y[0, :7], None, x.detach(), w.detach())[0])
 
 
-@pytest.mark.parametrize("cols", [225, 20_000])
+@pytest.mark.parametrize("cols", [225, 20_000, 80_000])
 def test_policy_loss_autograd(device, cols):
     d = loss_inputs(40, cols, torch.float32, "target", True, 12)
     dev = {k: v.to(device) for k, v in d.items()}
