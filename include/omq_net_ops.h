@@ -36,6 +36,8 @@ extern "C" {
 #define OMQ_NET_BF16 1
 #define OMQ_NET_F16 2
 
+#define OMQ_NET_STATS 8 /* floats that a policy loss's row leaves for its gradient */
+
 /* limits of this build */
 #define OMQ_NET_MAX_NORM_DIM 16384    /* columns of a normed row (a row is held in registers) */
 #define OMQ_NET_MAX_DIM (1 << 20)     /* columns of an embedding row, of a dropout row */
@@ -153,8 +155,8 @@ typedef struct omq_policy_rows {
 /* Bytes of workspace of the two loss entry points; negative for sizes they refuse. */
 int64_t omq_clipped_policy_loss_workspace(int64_t rows, int64_t actions);
 
-/* loss, logp, kl: float32 [rows].  stats: float32 [rows, 4] for omq_clipped_policy_loss_grad,
- * or NULL. */
+/* loss, logp, kl: float32 [rows].  stats: float32 [rows, OMQ_NET_STATS] on a 16-byte boundary for
+ * omq_clipped_policy_loss_grad, or NULL. */
 int omq_clipped_policy_loss(const omq_policy_rows* r, float* loss, float* logp, float* kl,
                             float* stats, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -5,7 +5,9 @@
 //   logq_a = z_a - m - log s
 //   kl     = tk + tp log s
 //   dz_a   = push p_a + slope [a taken] - kl_coef pi_a,   p_a = e^(z_a - m) / s,
-// where slope is the loss's derivative by logp and push = kl_coef tp - slope.
+// where slope is the loss's derivative by logp and push = kl_coef tp - slope.  The taken action is
+// left out of s while it is formed (`rest`): 1 - p of the taken action, by which its slope is
+// multiplied, is rest / s, and keeps its bits where p is near 1.
 //
 // Bound by memory.  Three ways through a row:
 //   - short rows are held in registers: the base, the sums and the gradient come from one load;
@@ -22,9 +24,10 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Statistics of a part of a row; m is -inf while nothing in it has weight.
+// Statistics of a part of a row; m is -inf while nothing in it has weight; rest is s without the
+// taken action.
 struct Stats {
-  float m, s, tp, tk;
+  float m, rest, tp, tk;
 };
 
 __device__ inline Stats no_stats() { return Stats{-kInf, 0.0f, 0.0f, 0.0f}; }
@@ -37,7 +40,7 @@ __device__ inline float base_of(float m) { return m == -kInf ? 0.0f : m; }
 // The statistics about another base, which is finite or that of a part without weight.
 __device__ inline void rebase(Stats& t, float m) {
   if (t.m != m) {
-    t.s *= exp_fast(t.m - base_of(m));
+    t.rest *= exp_fast(t.m - base_of(m));
     if (t.tp != 0.0f) t.tk -= t.tp * (base_of(t.m) - base_of(m));
     t.m = m;
   }
@@ -46,7 +49,7 @@ __device__ inline void rebase(Stats& t, float m) {
 // Over the kLanes lanes of a group, of one base or of any: all get the joined statistics.
 template <int kLanes, bool kTarget>
 __device__ inline void lanes_sum(Stats& t) {
-  t.s = lanes_reduce<Sum, kLanes>(t.s);
+  t.rest = lanes_reduce<Sum, kLanes>(t.rest);
   if constexpr (kTarget) {
     t.tp = lanes_reduce<Sum, kLanes>(t.tp);
     t.tk = lanes_reduce<Sum, kLanes>(t.tk);
@@ -82,42 +85,81 @@ __device__ inline void row_join(Stats& t, Stats* smem) {
 struct RowGrad {
   float m, inv_s;  // p = e^(z - m) * inv_s; inv_s = 0: the row has no gradient
   float push, slope;
+  float others;  // 1 - p of the taken action
 };
+
+// Its place in the statistics that the loss leaves for its gradient: eight floats a row.
+__device__ inline void write_stats(float4* stats, int64_t row, const RowGrad& g) {
+  stats[2 * row] = make_float4(g.m, g.inv_s, g.push, g.slope);
+  stats[2 * row + 1] = make_float4(g.others, 0.0f, 0.0f, 0.0f);
+}
+
+__device__ inline RowGrad read_stats(const float4* stats, int64_t row) {
+  const float4 a = stats[2 * row];
+  return RowGrad{a.x, a.y, a.z, a.w, stats[2 * row + 1].x};
+}
 
 struct RowOut {
   float loss, logp, kl;
   RowGrad g;
 };
 
-// z_taken: the logit of the taken action, `taken`: it is legal and in range.
+// log s to about 2^-25 absolute, whatever its size: the exponent's part in 64 bits, the rest, below
+// 1/2 in magnitude, from the float32 instruction.
+__device__ inline double log_of_sum(float s) {
+  float f = __builtin_amdgcn_frexp_mantf(s);
+  int k = __builtin_amdgcn_frexp_expf(s);
+  const bool low = f < 0.70710678f;
+  f = low ? 2.0f * f : f;
+  k = low ? k - 1 : k;
+  return (double)k * 0.6931471805599453 + (double)(__builtin_amdgcn_logf(f) * kLn2);
+}
+
+// e^d - 1 - d without its cancellation about 0.
+__device__ inline float exp_above_line(float d) {
+  if (fabsf(d) > 0.5f) return expm1f(d) - d;
+  float p = 1.0f / 40320.0f;  // Taylor; the next term is below 2^-24 of the sum
+  p = fmaf(p, d, 1.0f / 5040.0f);
+  p = fmaf(p, d, 1.0f / 720.0f);
+  p = fmaf(p, d, 1.0f / 120.0f);
+  p = fmaf(p, d, 1.0f / 24.0f);
+  p = fmaf(p, d, 1.0f / 6.0f);
+  return d * d * fmaf(p, d, 0.5f);
+}
+
+// z_taken: the logit of the taken action, `taken`: it is legal and in range.  The differences of
+// log-probabilities are formed in 64 bits: a few operations a row, and the ratio and the kl do not
+// lose the bits that a log-probability of about -10 rounds away in float32.
 __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const Stats& t,
                                     float z_taken, bool taken) {
   RowOut o{};
-  const bool live = !(t.m == -kInf && t.s == 0.0f);
-  if (!live) return o;
   const float base = base_of(t.m);
-  // (the instructions themselves, within a unit in the last place: s is at least e^-8 and an
-  // ordinary number)
-  const float log_s = __builtin_amdgcn_logf(t.s) * kLn2;
+  const float s = taken ? t.rest + exp_fast(z_taken - base) : t.rest;
+  const bool live = !(t.m == -kInf && s == 0.0f);
+  if (!live) return o;
+  const double log_s = log_of_sum(s);
   float slope = 0.0f;
   if (taken) {
-    o.logp = z_taken - base - log_s;
+    const double logp = (double)z_taken - (double)base - log_s;
+    o.logp = (float)logp;
     const float adv = r.advantages[row];
-    const float ratio = exp_fast(o.logp - r.old_logp[row]);
+    const float ratio =
+        __builtin_amdgcn_exp2f((float)((logp - (double)r.old_logp[row]) * 1.4426950408889634));
     const float one = ratio * adv;
     const float two = fminf(fmaxf(ratio, 1.0f - r.clip_low), 1.0f + r.clip_high) * adv;
     o.loss = -(one <= two || one != one ? one : two);
     if (one <= two || one != one) slope = -one;
     if (r.ref_logp) {
-      const float d = r.ref_logp[row] - o.logp, e = expm1f(d);
-      o.kl = e - d;
-      slope -= r.kl_coef * e;
+      const float d = (float)((double)r.ref_logp[row] - logp);
+      o.kl = exp_above_line(d);
+      slope -= r.kl_coef * (o.kl + d);
     }
   }
-  if (r.target) o.kl = t.tk + (t.tp != 0.0f ? t.tp * log_s : 0.0f);
+  if (r.target) o.kl = (float)((double)t.tk + (t.tp != 0.0f ? (double)t.tp * log_s : 0.0));
   o.loss += r.kl_coef != 0.0f ? r.kl_coef * o.kl : 0.0f;
   o.g.m = base;
-  o.g.inv_s = __builtin_amdgcn_rcpf(t.s);
+  o.g.inv_s = 1.0f / s;
+  o.g.others = t.rest * o.g.inv_s;
   o.g.slope = slope;
   o.g.push = (r.kl_coef != 0.0f ? r.kl_coef * t.tp : 0.0f) - slope;
   // a row that adds nothing to the loss has no gradient, whatever its logits hold (padding)
@@ -130,7 +172,7 @@ __device__ inline void write_row(const RowOut& o, int64_t row, float* loss, floa
   loss[row] = o.loss;
   logp[row] = o.logp;
   kl[row] = o.kl;
-  if (stats) stats[row] = make_float4(o.g.m, o.g.inv_s, o.g.push, o.g.slope);
+  if (stats) write_stats(stats, row, o.g);
 }
 
 // A row's action as it is given.  (Loaded before the row's blocks: loads are waited for in their
@@ -256,12 +298,20 @@ __device__ inline float largest(F8 z) {
   return larger(larger(larger(larger(z[0], z[1]), z[2], z[3]), z[4], z[5]), z[6], z[7]);
 }
 
+// Takes the taken action, where it is in the block (at its place `at`), out of the block's sum.
+__device__ inline void leave_out(F8& z, int at) {
+  if ((uint32_t)at < 8u) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = j == at ? -kInf : z[j];
+  }
+}
+
 // Adds a block's exponentials, which take the place of its logits.
 __device__ inline void add_logits(Stats& t, F8& z, float base) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     z[j] = exp_fast(z[j] - base);
-    t.s += z[j];
+    t.rest += z[j];
   }
 }
 
@@ -299,12 +349,13 @@ __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coe
 }
 
 // The element of the taken action, in full; written by the thread that wrote its block, after it.
+// (push + slope) p + slope (1 - p), not push p + slope: the second cancels where p is near 1.
 template <class T>
 __device__ inline void put_taken(T* grad, const RowIn<T>& in, const RowGrad& g, float z_taken,
                                  int taken, float coef, float w) {
-  float d = exp_fast(z_taken - g.m) * (w * g.push * g.inv_s);
-  if (in.target) d = fmaf(-larger(in.target[taken], 0.0f), w * coef, d);
-  grad[taken] = (T)fmaf(w, g.slope, d);
+  float d = fmaf(g.push + g.slope, exp_fast(z_taken - g.m) * g.inv_s, g.slope * g.others);
+  if (in.target) d = fmaf(-larger(in.target[taken], 0.0f), coef, d);
+  grad[taken] = (T)(w * d);
 }
 
 // ---- rows in registers ----------------------------------------------------------------------
@@ -349,6 +400,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
       pi[i] = legal_target<T, kWhole>(b[i], in, 8 * (lane + i * kThreads), ok[i]);
       add_target(t, pi[i], z[i], base);
     }
+    leave_out(z[i], taken - 8 * (lane + i * kThreads));
     add_logits(t, z[i], base);
   }
   row_join<kThreads, kTarget, true>(t, smem);
@@ -375,7 +427,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
 // any limit, and after a few blocks no thread changes its base again.
 template <class T, bool kTarget, bool kWhole, int kCount, int kStep>
 __device__ inline void add_blocks(Stats& t, const Block<T, kTarget>* b, const RowIn<T>& in, int col,
-                                  int to) {
+                                  int to, int taken) {
   constexpr float kSlack = 8.0f;
   F8 z[kCount];
   uint64_t ok[kCount];
@@ -395,20 +447,21 @@ __device__ inline void add_blocks(Stats& t, const Block<T, kTarget>* b, const Ro
       F8 pi = legal_target<T, kWhole>(b[u], in, col + kStep * u, ok[u]);
       add_target(t, pi, z[u], base);
     }
+    leave_out(z[u], taken - (col + kStep * u));
     add_logits(t, z[u], base);
   }
 }
 
 // Statistics of the blocks from column `from` on, up to column `to`, that fall to this thread.
 template <class T, bool kTarget, bool kWhole, int kThreads>
-__device__ inline void stream(Stats& t, const RowIn<T>& in, int from, int to) {
+__device__ inline void stream(Stats& t, const RowIn<T>& in, int from, int to, int taken) {
   constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
   for (int col = from + 8 * threadIdx.x; col < to; col += kStep * kCount) {
     Block<T, kTarget> b[kCount];
 #pragma unroll
     for (int u = 0; u < kCount; ++u)
       b[u] = load_block<T, kTarget, kWhole>(in, col + kStep * u);
-    add_blocks<T, kTarget, kWhole, kCount, kStep>(t, b, in, col, to);
+    add_blocks<T, kTarget, kWhole, kCount, kStep>(t, b, in, col, to, taken);
   }
 }
 
@@ -447,7 +500,7 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
   float z_taken;
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
   Stats t = no_stats();
-  stream<T, kTarget, kWhole, kThreads>(t, in, 0, in.cols);
+  stream<T, kTarget, kWhole, kThreads>(t, in, 0, in.cols, taken);
   row_join<kThreads, kTarget, false>(t, smem);
   const RowOut o = finish_row(r, row, t, z_taken, taken >= 0);
   if (threadIdx.x == 0) write_row(o, row, loss, logp, kl, stats);
@@ -478,8 +531,10 @@ __global__ __launch_bounds__(256) void loss_span_kernel(omq_policy_rows r, int s
   const RowIn<T> in = row_in<T>(r, row);
   const int64_t from = (int64_t)blockIdx.x * span;
   const int to = from + span < in.cols ? (int)(from + span) : in.cols;
+  float z_taken;
+  const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
   Stats t = no_stats();
-  stream<T, kTarget, kWhole, 256>(t, in, (int)from, to);
+  stream<T, kTarget, kWhole, 256>(t, in, (int)from, to, taken);
   row_join<256, kTarget, false>(t, smem);
   if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = t;
 }
@@ -501,7 +556,7 @@ __global__ __launch_bounds__(64) void loss_join_kernel(omq_policy_rows r,
     const float m = fmaxf(t.m, u.m);
     rebase(t, m);
     rebase(u, m);
-    t = Stats{m, t.s + u.s, t.tp + u.tp, t.tk + u.tk};
+    t = Stats{m, t.rest + u.rest, t.tp + u.tp, t.tk + u.tk};
   }
   lanes_join<kWave, true>(t);
   if (threadIdx.x == 0) write_row(finish_row(r, row, t, z, taken >= 0), row, loss, logp, kl, stats);
@@ -521,8 +576,7 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(omq_policy_rows r, int b
   if (row >= r.rows) return;
   const RowIn<T> in = row_in<T>(r, row);
   const Block<T, kTarget> b = load_block<T, kTarget, kWhole>(in, col);
-  const float4 st = stats[row];
-  const RowGrad g{st.x, st.y, st.z, st.w};
+  const RowGrad g = read_stats(stats, row);
   const float w = row_weight ? row_weight[row] : 1.0f;
   float z_taken;
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
@@ -601,7 +655,7 @@ SpanPlan span_plan(int64_t rows, int64_t actions) {
   spans = spans > most ? most : spans;
   p.span = ceil_div(ceil_div(actions, spans), 8) * 8;
   p.spans = ceil_div(actions, p.span);
-  p.at_parts = 16 * rows;  // (the rows' statistics for the gradient come first)
+  p.at_parts = 32 * rows;  // (the rows' statistics for the gradient come first)
   p.bytes = p.at_parts + (int64_t)sizeof(Stats) * rows * p.spans;
   return p;
 }

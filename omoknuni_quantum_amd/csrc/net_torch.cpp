@@ -372,7 +372,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> clipped_policy_loss(
   const c10::Device dev = logits.device();
   const Guard guard(dev);
   auto [loss, logp, kl] = fresh_rows(r.rows, dev);
-  at::Tensor stats = fresh({want_stats ? r.rows : 0, 4}, at::kFloat, dev);
+  at::Tensor stats = fresh({want_stats ? r.rows : 0, OMQ_NET_STATS}, at::kFloat, dev);
   if (dev.is_meta()) return {loss, logp, kl, stats};
   const Workspace ws(name, omq_clipped_policy_loss_workspace(r.rows, r.actions), dev);
   check_rc(omq_clipped_policy_loss(&r, loss.data_ptr<float>(), logp.data_ptr<float>(),
@@ -394,9 +394,9 @@ at::Tensor clipped_policy_loss_grad(const at::Tensor& logits, const at::Tensor& 
                                         clip_high, kl_coef, ref_logp, target, legal);
   const at::Tensor* w = get(row_weight);
   common_device(name, {&logits, &stats, w});
-  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == 4 &&
+  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == OMQ_NET_STATS &&
                   stats.scalar_type() == at::kFloat && stats.is_contiguous(),
-              "omq_net::", name, ": stats must be those of clipped_policy_loss, [", r.rows, ", 4]");
+              "omq_net::", name, ": stats must be those of clipped_policy_loss");
   const float* wp = w ? row_floats(name, "row_weight", *w, r.rows) : nullptr;
   const c10::Device dev = logits.device();
   const Guard guard(dev);
