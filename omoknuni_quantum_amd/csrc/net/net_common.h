@@ -132,7 +132,7 @@ struct Weight8 {
 template <class T, bool kWhole>
 __device__ inline Weight8<T> load_weight(const void* w, bool w_f32, int col, int dim) {
   Weight8<T> r = {};
-  if (w_f32)
+  if (w_f32 || sizeof(T) == 4)
     r.f = load_raw<float, kWhole>(static_cast<const float*>(w), col, dim);
   else
     r.t = load_raw<T, kWhole>(static_cast<const T*>(w), col, dim);
@@ -141,7 +141,8 @@ __device__ inline Weight8<T> load_weight(const void* w, bool w_f32, int col, int
 
 template <class T, bool kWhole>
 __device__ inline F8 widen(const Weight8<T>& w, bool w_f32, int col, int dim) {
-  return w_f32 ? widen<float, kWhole>(w.f, col, dim) : widen<T, kWhole>(w.t, col, dim);
+  return w_f32 || sizeof(T) == 4 ? widen<float, kWhole>(w.f, col, dim)
+                                 : widen<T, kWhole>(w.t, col, dim);
 }
 
 // Which of the rows of its workgroup a thread belongs to, kThreads threads a row: a scalar where

