@@ -337,7 +337,7 @@ __device__ inline void add_target(Stats& t, F8& pi, F8 z, float base) {
 
 // The gradient of eight actions but for the slope of the taken one, times the row's weight w: e
 // holds e^(z - m), scale is w * push / s (or that about the base of e).
-template <bool kTarget>
+template <bool kTarget, bool kAll>
 __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coef) {
   F8 d = e * scale;
   if constexpr (kTarget) {
@@ -346,8 +346,10 @@ __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coe
 #pragma unroll
     for (int j = 0; j < 8; ++j) d[j] = fmaf(-pi[j], w_coef, d[j]);
   }
+  if constexpr (!kAll) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) d[j] = masked(d[j], ok_mask(ok, j), 0.0f);
+    for (int j = 0; j < 8; ++j) d[j] = masked(d[j], ok_mask(ok, j), 0.0f);
+  }
   return d;
 }
 
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
     const int col = 8 * (lane + i * kThreads);
     F8 d = {};
     if (o.g.inv_s != 0.0f)
-      d = gradient<kTarget>(z[i], pi[kTarget ? i : 0], ok[i], scale, w * r.kl_coef);
+      d = gradient<kTarget, false>(z[i], pi[kTarget ? i : 0], ok[i], scale, w * r.kl_coef);
     store8<T, kWhole>(grad + row * in.cols, col, in.cols, d);
   }
   if (taken >= 0 && o.g.inv_s != 0.0f && lane == (taken / 8) % kThreads)
@@ -425,67 +427,108 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
 }
 
 // ---- long rows ------------------------------------------------------------------------------
-// Adds kCount blocks, kStep columns apart, the first at column `col`, to a thread's statistics.
-// The base follows the logits only when one passes it by more than kSlack: e^kSlack is far from
-// any limit, and after a few blocks no thread changes its base again.
-template <class T, bool kTarget, bool kWhole, int kCount, int kStep>
-__device__ inline void add_blocks(Stats& t, const Block<T, kTarget>* b, const RowIn<T>& in, int col,
-                                  int to, int taken) {
+// Blocks that a thread has in flight: four of rows that are whole blocks (4096 rows of 131072
+// bfloat16 with gradient: 431 us, 442 with one), else one (4096 of 100003: 409 us, 479 with four;
+// 2018 of 87390 float32: 304 and 345 us: blocks at odd addresses take two lines each).
+template <bool kTarget, bool kWhole>
+constexpr int kInFlight = kWhole && !kTarget ? 4 : 1;
+
+// kAll: the blocks are whole and every action is legal, so that nothing is masked.  Long rows
+// without a mask are made of such blocks but for their end.  (4096 rows of 131072 bfloat16 with
+// gradient: the masks are a third of the instructions and 8 of 439 us.)
+template <class T, bool kTarget, bool kWhole, bool kAll>
+__device__ inline F8 logits_of(const Block<T, kTarget>& b, const RowIn<T>& in, int col,
+                               uint64_t ok) {
+  if constexpr (kAll) return __builtin_convertvector(b.z, F8);
+  return legal_logits<T, kTarget, kWhole>(b, in, col, ok);
+}
+
+template <class T, bool kWhole, bool kAll>
+__device__ inline F8 target_of(const Block<T, true>& b, const RowIn<T>& in, int col, uint64_t ok) {
+  if constexpr (kAll) return b.pi;
+  return legal_target<T, kWhole>(b, in, col, ok);
+}
+
+// Adds a thread's kCount blocks, kStep columns apart, of the columns from `at` on to its
+// statistics.  The base follows the logits only when one passes it by more than kSlack: e^kSlack
+// is far from any limit, and after a few blocks no thread changes its base again.
+template <class T, bool kTarget, bool kWhole, bool kAll, int kCount, int kStep>
+__device__ inline void add_blocks(Stats& t, const RowIn<T>& in, int at, int to, int taken) {
   constexpr float kSlack = 8.0f;
+  const int col = at + 8 * (int)threadIdx.x;
+  Block<T, kTarget> b[kCount];
+#pragma unroll
+  for (int u = 0; u < kCount; ++u)
+    b[u] = load_block<T, kTarget, kWhole || kAll>(in, col + kStep * u);
   F8 z[kCount];
   uint64_t ok[kCount];
   float m = -kInf;
 #pragma unroll
   for (int u = 0; u < kCount; ++u) {
     const int c = col + kStep * u;
-    ok[u] = c < to ? ok_bytes<T, kTarget, kWhole>(b[u], in, c) : 0;
-    z[u] = legal_logits<T, kTarget, kWhole>(b[u], in, c, ok[u]);
+    ok[u] = kAll ? 0 : c < to ? ok_bytes<T, kTarget, kWhole>(b[u], in, c) : 0;
+    z[u] = logits_of<T, kTarget, kWhole, kAll>(b[u], in, c, ok[u]);
     m = larger(m, largest(z[u]));
   }
   if (m > t.m + kSlack) rebase(t, m);  // (from -inf: at the first weight)
   const float base = base_of(t.m);
+  const bool takes = taken >= at && taken < at + kStep * kCount;  // (uniform)
 #pragma unroll
   for (int u = 0; u < kCount; ++u) {
     if constexpr (kTarget) {
-      F8 pi = legal_target<T, kWhole>(b[u], in, col + kStep * u, ok[u]);
+      F8 pi = target_of<T, kWhole, kAll>(b[u], in, col + kStep * u, ok[u]);
       add_target(t, pi, z[u], base);
     }
-    leave_out(z[u], taken - (col + kStep * u));
+    if (takes) leave_out(z[u], taken - (col + kStep * u));
     add_logits(t, z[u], base);
   }
 }
 
-// Statistics of the blocks from column `from` on, up to column `to`, that fall to this thread.
+// Statistics of the columns from `from` on, up to `to`, that fall to this thread.
 template <class T, bool kTarget, bool kWhole, int kThreads>
 __device__ inline void stream(Stats& t, const RowIn<T>& in, int from, int to, int taken) {
-  constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
-  for (int col = from + 8 * threadIdx.x; col < to; col += kStep * kCount) {
-    Block<T, kTarget> b[kCount];
-#pragma unroll
-    for (int u = 0; u < kCount; ++u)
-      b[u] = load_block<T, kTarget, kWhole>(in, col + kStep * u);
-    add_blocks<T, kTarget, kWhole, kCount, kStep>(t, b, in, col, to, taken);
-  }
+  constexpr int kCount = kInFlight<kTarget, kWhole>, kStep = 8 * kThreads;
+  constexpr int kChunk = kStep * kCount;
+  int at = from;
+  if (!in.legal)
+    for (; at + kChunk <= to; at += kChunk)
+      add_blocks<T, kTarget, kWhole, true, kCount, kStep>(t, in, at, to, taken);
+  for (; at < to; at += kChunk)
+    add_blocks<T, kTarget, kWhole, false, kCount, kStep>(t, in, at, to, taken);
 }
 
 // The gradient of the block at column col.
-template <class T, bool kTarget, bool kWhole, bool kStream>
+template <class T, bool kTarget, bool kWhole, bool kAll, bool kStream>
 __device__ inline void put_gradient(T* grad, const Block<T, kTarget>& b, const RowIn<T>& in,
                                     int col, const RowGrad& g, float coef, float w) {
   F8 d = {}, pi = {};
   if (g.inv_s != 0.0f) {
-    const uint64_t ok = ok_bytes<T, kTarget, kWhole>(b, in, col);
-    F8 z = legal_logits<T, kTarget, kWhole>(b, in, col, ok);
+    const uint64_t ok = kAll ? 0 : ok_bytes<T, kTarget, kWhole>(b, in, col);
+    F8 z = logits_of<T, kTarget, kWhole, kAll>(b, in, col, ok);
     if constexpr (kTarget) {
-      pi = legal_target<T, kWhole>(b, in, col, ok);
+      pi = target_of<T, kWhole, kAll>(b, in, col, ok);
 #pragma unroll
       for (int j = 0; j < 8; ++j) pi[j] = larger(pi[j], 0.0f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) z[j] = exp_fast(z[j] - g.m);
-    d = gradient<kTarget>(z, pi, ok, w * g.push * g.inv_s, w * coef);
+    d = gradient<kTarget, kAll>(z, pi, ok, w * g.push * g.inv_s, w * coef);
   }
-  store8<T, kWhole, kStream>(grad, col, in.cols, d);
+  store8<T, kWhole || kAll, kStream>(grad, col, in.cols, d);
+}
+
+// The gradients of a thread's kCount blocks of the columns from `at` on.
+template <class T, bool kTarget, bool kWhole, bool kAll, int kCount, int kStep>
+__device__ inline void put_blocks(T* grad, const RowIn<T>& in, int at, const RowGrad& g, float coef,
+                                  float w) {
+  const int col = at + 8 * (int)threadIdx.x;
+  Block<T, kTarget> b[kCount];
+#pragma unroll
+  for (int u = 0; u < kCount; ++u)
+    b[u] = load_block<T, kTarget, kWhole || kAll>(in, col + kStep * u);
+#pragma unroll
+  for (int u = 0; u < kCount; ++u)
+    put_gradient<T, kTarget, kWhole, kAll, true>(grad, b[u], in, col + kStep * u, g, coef, w);
 }
 
 // A workgroup a row: the sums, then the gradient, for which the blocks are read again, the last
@@ -495,7 +538,8 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
     omq_policy_rows r, const float* __restrict__ row_weight, float* __restrict__ loss,
     float* __restrict__ logp, float* __restrict__ kl, float4* __restrict__ stats,
     T* __restrict__ grad) {
-  constexpr int kCount = kTarget ? 2 : 4, kStep = 8 * kThreads;
+  constexpr int kCount = kInFlight<kTarget, kWhole>, kStep = 8 * kThreads;
+  constexpr int kChunk = kStep * kCount;
   __shared__ Stats smem[16];
   const int64_t row = block_index();
   if (row >= r.rows) return;
@@ -510,17 +554,12 @@ __global__ __launch_bounds__(kThreads) void loss_long_kernel(
   if (!grad) return;
   const float w = row_weight ? row_weight[row] : 1.0f;
   T* g = grad + row * in.cols;
-  for (int at = (in.cols - 1) / (kStep * kCount) * (kStep * kCount); at >= 0;
-       at -= kStep * kCount) {
-    Block<T, kTarget> b[kCount];
-#pragma unroll
-    for (int u = 0; u < kCount; ++u)
-      b[u] = load_block<T, kTarget, kWhole>(in, at + 8 * (int)threadIdx.x + kStep * u);
-#pragma unroll
-    for (int u = 0; u < kCount; ++u)
-      put_gradient<T, kTarget, kWhole, true>(g, b[u], in, at + 8 * (int)threadIdx.x + kStep * u,
-                                         o.g, r.kl_coef, w);
-  }
+  const int whole = in.legal ? 0 : in.cols / kChunk * kChunk;  // (of blocks that kAll is true of)
+  int at = (in.cols - 1) / kChunk * kChunk;
+  for (; at >= whole; at -= kChunk)
+    put_blocks<T, kTarget, kWhole, false, kCount, kStep>(g, in, at, o.g, r.kl_coef, w);
+  for (; at >= 0; at -= kChunk)
+    put_blocks<T, kTarget, kWhole, true, kCount, kStep>(g, in, at, o.g, r.kl_coef, w);
   if (taken >= 0 && o.g.inv_s != 0.0f && (int)threadIdx.x == (taken / 8) % kThreads)
     put_taken(g, in, o.g, z_taken, taken, r.kl_coef, w);
 }
@@ -584,7 +623,7 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(omq_policy_rows r, int b
   float z_taken;
   const int taken = taken_of<T>(r, row, action_of(r, row), &z_taken);
   T* to = grad + row * in.cols;
-  put_gradient<T, kTarget, kWhole, false>(to, b, in, col, g, r.kl_coef, w);
+  put_gradient<T, kTarget, kWhole, false, false>(to, b, in, col, g, r.kl_coef, w);
   if (taken >= 0 && g.inv_s != 0.0f && taken / 8 == col / 8)
     put_taken(to, in, g, z_taken, taken, r.kl_coef, w);
 }
