@@ -12,8 +12,8 @@
 // the order of the pieces.  No atomics on floating-point values: the result is the same at every
 // call.
 //
-// Measured, bfloat16: 115200 tokens of 675 rows, 256 columns 33 us (15 us sort, 14 us sums at 4.2
-// TB/s, 5 us join); 131071 tokens of 65536 rows, 1024 columns 123 us (33 us sort in two passes,
+// Measured, bfloat16: 115200 tokens of 675 rows, 256 columns 31 us (13 us sort, 14 us sums at 4.2
+// TB/s, 5 us join); 131071 tokens of 65536 rows, 1024 columns 120 us (29 us sort in two passes,
 // 90 us sums at 4.5 TB/s, 5 us join).  The sums are bound by memory, the sort by the latency of its
 // three short launches a pass.
 #include "net_common.h"
@@ -264,62 +264,78 @@ __global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__
   }
 }
 
-// Step 3: every pair to its place.
+// Step 3: every pair to its place.  Eight waves of two rounds; the waves' counters of a tile have
+// 16 bits, two to a word.  (5.4 to 6.2 us for 115200 tokens, 6.9 to 8 with four waves of four
+// rounds and counters of 32 bits.)
 template <class Id>
-__global__ __launch_bounds__(256) void digit_scatter_kernel(
+__global__ __launch_bounds__(512) void digit_scatter_kernel(
     const Id* __restrict__ ids, const uint2* __restrict__ in, int64_t tokens, int64_t vocab,
     int shift, int bits, int bins, const uint32_t* __restrict__ counts,
     const uint32_t* __restrict__ totals, uint2* __restrict__ out) {
-  constexpr int kWaves = 4, kRounds = kTile / 256, kBins = 1 << kMaxDigitBits;
-  __shared__ uint32_t next[kWaves][kBins];
+  constexpr int kThreads = 512, kWaves = kThreads / kWave, kRounds = kTile / kThreads;
+  constexpr int kBins = 1 << kMaxDigitBits;
+  __shared__ uint32_t next[kWaves][kBins / 2];
   __shared__ uint32_t base[kBins];
   __shared__ uint32_t wave_sums[kWaves];
   const uint32_t mask = (1u << bits) - 1;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int64_t first = (int64_t)blockIdx.x * kTile + wave * (kTile / kWaves);
+  const int words = (bins + 1) / 2;
   uint2 mine[kRounds];
-  uint32_t before[kBins / 256];  // of this thread's digits, in the tiles before
+  uint32_t before[kBins / kThreads];  // of this thread's digits, in the tiles before
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int64_t t = first + r * kWave + lane;
     if (t < tokens) mine[r] = in ? in[t] : make_uint2(key_of(ids, t, vocab), (uint32_t)t);
   }
 #pragma unroll
-  for (int k = 0; k < kBins / 256; ++k) {
-    const int j = k * 256 + threadIdx.x;
+  for (int k = 0; k < kBins / kThreads; ++k) {
+    const int j = k * kThreads + threadIdx.x;
     if (j < bins) {
       before[k] = counts[(int64_t)blockIdx.x * bins + j];
       base[j] = totals[j];
-      for (int w = 0; w < kWaves; ++w) next[w][j] = 0;
     }
   }
+  for (int j = threadIdx.x; j < words; j += kThreads)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) next[w][j] = 0;
   __syncthreads();
-  block_scan<256>(base, bins, wave_sums);
+  block_scan<kThreads>(base, bins, wave_sums);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
-    if (first + r * kWave + lane < tokens)
-      atomicAdd(&next[wave][(mine[r].x >> shift) & mask], 1u);
+    if (first + r * kWave + lane < tokens) {
+      const uint32_t d = (mine[r].x >> shift) & mask;
+      atomicAdd(&next[wave][d >> 1], 1u << (16 * (d & 1)));
+    }
+#pragma unroll
+  for (int k = 0; k < kBins / kThreads; ++k) {
+    const int j = k * kThreads + threadIdx.x;
+    if (j < bins) base[j] += before[k];
+  }
   __syncthreads();
+  for (int j = threadIdx.x; j < words; j += kThreads) {
+    uint32_t at = 0, c[kWaves];
 #pragma unroll
-  for (int k = 0; k < kBins / 256; ++k) {
-    const int j = k * 256 + threadIdx.x;
-    if (j < bins) {
-      uint32_t at = base[j] + before[k], c[kWaves];
+    for (int w = 0; w < kWaves; ++w) c[w] = next[w][j];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) c[w] = next[w][j];
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        next[w][j] = at;
-        at += c[w];
-      }
+    for (int w = 0; w < kWaves; ++w) {
+      next[w][j] = at;
+      at += c[w];  // (both halves: a tile has fewer than 2^16 pairs)
     }
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const bool here = first + r * kWave + lane < tokens;
-    const uint32_t digit = here ? (mine[r].x >> shift) & mask : 0u;
-    const uint32_t at = take_places(digit, bits, here, next[wave]);
+    const uint32_t d = here ? (mine[r].x >> shift) & mask : 0u;
+    const uint64_t same = match_digit(d, bits, __ballot(here));
+    const int below = lanes_below(same);
+    uint32_t* word = &next[wave][d >> 1];
+    uint32_t at = 0;
+    if (here) at = base[d] + ((*word >> (16 * (d & 1))) & 0xFFFFu) + below;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (here && below == 0) atomicAdd(word, (uint32_t)__popcll(same) << (16 * (d & 1)));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (here) out[at] = mine[r];
   }
 }
@@ -650,7 +666,7 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   p.lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : dim <= 256 ? 32 : 64;
   p.col_tiles = (int)ceil_div(dim, 8 * p.lanes);
   // Pieces for 2048 waves, of 16 to 1024 items.  Fewer leave memory idle, more are more partial
-  // sums: 115200 tokens of 675 rows and 256 columns take 34 us, 38 with 1024 waves and 40 with
+  // sums: 115200 tokens of 675 rows and 256 columns took 34 us, 38 with 1024 waves and 40 with
   // 4096; 131071 of 65536 rows and 1024 columns 125, 135 and 129.
   const int64_t items = tokens + vocab;
   const int64_t wanted = ceil_div(2048ll * (kWave / p.lanes), p.col_tiles);
@@ -699,7 +715,7 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
                                                               p.digit_bits, bins, counts);
     digit_scan_kernel<<<(uint32_t)ceil_div(bins, kWave), 1024, 0, st>>>(counts, (int)p.tiles, bins,
                                                                       totals);
-    digit_scatter_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(
+    digit_scatter_kernel<Id><<<(uint32_t)p.tiles, 512, 0, st>>>(
         ids, in, tokens, vocab, shift, p.digit_bits, bins, counts, totals, to);
     in = to;
   }
