@@ -12,7 +12,8 @@
  * fixed order (no floating-point atomics).
  *
  * Arrays of rows are given with a row stride in ELEMENTS; the elements of a row are adjacent.
- * No alignment beyond the element's own is needed.  Sums, statistics and intermediate values are
+ * No alignment beyond the element's own is needed, but workspaces (and `stats`) begin on a 16-byte
+ * boundary.  Sums, statistics and intermediate values are
  * float32; a result is rounded to its type once.
  */
 #ifndef OMQ_NET_OPS_H

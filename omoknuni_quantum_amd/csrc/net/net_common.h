@@ -272,6 +272,9 @@ inline dim3 grid_of(int64_t blocks, int threads) {
 int net_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int net_status(const char* what);  // of the launches made since the last call
 
+// Workspaces and the rows' statistics hold 16-byte records.
+inline bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool dtype_known(int d) { return d == OMQ_NET_F32 || d == OMQ_NET_BF16 || d == OMQ_NET_F16; }
 inline int dtype_size(int d) { return d == OMQ_NET_F32 ? 4 : 2; }

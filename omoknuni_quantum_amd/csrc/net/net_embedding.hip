@@ -843,6 +843,8 @@ int omq_token_embedding_grad(const void* grad, int64_t grad_stride, int dtype, c
   if (p.bytes > 0 && (workspace_bytes < p.bytes || !workspace))
     return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes, %lld needed", name,
                     (long long)workspace_bytes, (long long)p.bytes);
+  if (p.bytes > 0 && !on_16_bytes(workspace))
+    return net_fail(OMQ_NET_E_ARG, "%s: workspace is not on a 16-byte boundary", name);
   if (!out || (tokens > 0 && (!grad || !ids)))
     return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   hipStream_t st = (hipStream_t)stream;

@@ -804,6 +804,8 @@ int check_workspace(const char* name, const SpanPlan& p, const void* ws, int64_t
   if (p.bytes > 0 && (!ws || bytes < p.bytes))
     return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes, %lld needed", name,
                     (long long)bytes, (long long)p.bytes);
+  if (p.bytes > 0 && !on_16_bytes(ws))
+    return net_fail(OMQ_NET_E_ARG, "%s: workspace is not on a 16-byte boundary", name);
   return OMQ_NET_OK;
 }
 
@@ -828,6 +830,8 @@ int omq_clipped_policy_loss(const omq_policy_rows* r, float* loss, float* logp, 
   const SpanPlan p = span_plan(r->rows, r->actions);
   if (int rc = check_workspace(name, p, workspace, workspace_bytes)) return rc;
   if (!loss || !logp || !kl) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  if (!on_16_bytes(stats))
+    return net_fail(OMQ_NET_E_ARG, "%s: stats is not on a 16-byte boundary", name);
   hipStream_t st = (hipStream_t)stream;
   const LossOut o{loss, logp, kl, stats};
   switch (way_of(*r)) {
@@ -844,6 +848,8 @@ int omq_clipped_policy_loss_grad(const omq_policy_rows* r, const float* stats,
   if (int rc = check_rows(name, r)) return rc;
   if (r->rows == 0) return OMQ_NET_OK;
   if (!stats || !grad) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  if (!on_16_bytes(stats))
+    return net_fail(OMQ_NET_E_ARG, "%s: stats is not on a 16-byte boundary", name);
   launch_grad(*r, stats, row_weight, grad, (hipStream_t)stream);
   return net_status(name);
 }

@@ -130,6 +130,8 @@ def test_c_entry_points_refuse():
                                          None), str(need))
     refused(lib.omq_token_embedding_grad(ptr, 8, 1, ptr, 0, 1000, 5, 8, 1.0, ptr, 2, ptr, need,
                                          None), "types")
+    refused(lib.omq_token_embedding_grad(ptr, 8, 0, ptr, 0, 1000, 5, 8, 1.0, ptr, 0, ptr, need,
+                                         None), "16-byte")
     refused(lib.omq_dropout(ptr, 4, 8, 0, 1.01, 0, 0, ptr, None), "outside")
     refused(lib.omq_dropout(ptr, 4, 0, 0, 0.5, 0, 0, ptr, None), "dim 0")
     big = 16385
@@ -151,6 +153,11 @@ def test_c_entry_points_refuse():
     assert need > 0
     refused(lib.omq_clipped_policy_loss(ctypes.byref(r), ptr, ptr, ptr, None, ptr, need - 1, None),
             str(need))
+    refused(lib.omq_clipped_policy_loss(ctypes.byref(r), ptr, ptr, ptr, None, ptr, need, None),
+            "16-byte")
+    refused(lib.omq_clipped_policy_loss(ctypes.byref(r), ptr, ptr, ptr, ptr, 16, need, None),
+            "stats")
+    refused(lib.omq_clipped_policy_loss_grad(ctypes.byref(r), ptr, None, ptr, None), "stats")
     refused(lib.omq_clipped_policy_loss(None, ptr, ptr, ptr, None, ptr, need, None), "null")
     r.target = r.ref_logp = ptr
     refused(lib.omq_clipped_policy_loss(ctypes.byref(r), ptr, ptr, ptr, None, ptr, need, None),
