@@ -15,7 +15,9 @@
 // Measured, bfloat16: 115200 tokens of 675 rows, 256 columns 31 us (13 us sort, 14 us sums at 4.2
 // TB/s, 5 us join); 131071 tokens of 65536 rows, 1024 columns 120 us (29 us sort in two passes,
 // 90 us sums at 4.5 TB/s, 5 us join).  The sums are bound by memory, the sort by the latency of its
-// three short launches a pass.
+// two or three short launches a pass.
+#include <type_traits>
+
 #include "net_common.h"
 
 namespace omq_net {
@@ -126,12 +128,12 @@ __device__ inline uint32_t take_places(uint32_t digit, int bits, bool here, uint
   return place;
 }
 
-// All passes of up to kThreads * kRounds tokens in one workgroup.  8-bit digits.
-template <class Id, int kThreads, int kRounds>
-__global__ __launch_bounds__(kThreads) void sort_small_kernel(const Id* __restrict__ ids, int tokens,
+// All passes of up to kSmallSort tokens in one workgroup.  8-bit digits.
+template <class Id>
+__global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__ ids, int tokens,
                                                           int64_t vocab, int bits,
                                                           uint2* __restrict__ pairs) {
-  constexpr int kWaves = kThreads / kWave;
+  constexpr int kThreads = 1024, kRounds = kSmallSort / kThreads, kWaves = kThreads / kWave;
   __shared__ uint2 kept[kThreads * kRounds];
   __shared__ uint32_t next[kWaves][256];
   __shared__ uint32_t base[256];
@@ -267,7 +269,13 @@ __global__ __launch_bounds__(1024) void digit_scan_kernel(uint32_t* __restrict__
 // Step 3: every pair to its place.  Eight waves of two rounds; the waves' counters of a tile have
 // 16 bits, two to a word.  (5.4 to 6.2 us for 115200 tokens, 6.9 to 8 with four waves of four
 // rounds and counters of 32 bits.)
-template <class Id>
+//
+// kScan: there was no step 2; the tiles are few (kScanTiles), and every workgroup adds the counts
+// of its digits over all of them itself.  16 tiles and two passes: 32 us for the whole gradient, 36
+// with step 2; 32 tiles: one pass 26.4 and 25.8, two passes 40 and 42; 113 tiles: 41 and 32.
+constexpr int kScanTiles = 32;
+
+template <class Id, bool kScan>
 __global__ __launch_bounds__(512) void digit_scatter_kernel(
     const Id* __restrict__ ids, const uint2* __restrict__ in, int64_t tokens, int64_t vocab,
     int shift, int bits, int bins, const uint32_t* __restrict__ counts,
@@ -291,7 +299,22 @@ __global__ __launch_bounds__(512) void digit_scatter_kernel(
 #pragma unroll
   for (int k = 0; k < kBins / kThreads; ++k) {
     const int j = k * kThreads + threadIdx.x;
-    if (j < bins) {
+    if (j < bins && kScan) {
+      uint32_t sum = 0, ahead = 0;
+      for (int t = 0; t < (int)gridDim.x; t += 8) {  // eight loads in flight, the last ones too
+        uint32_t c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          c[u] = counts[(int64_t)(t + u < (int)gridDim.x ? t + u : t) * bins + j];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          sum += t + u < (int)gridDim.x ? c[u] : 0u;
+          ahead += t + u < (int)blockIdx.x ? c[u] : 0u;
+        }
+      }
+      before[k] = ahead;
+      base[j] = sum;
+    } else if (j < bins) {
       before[k] = counts[(int64_t)blockIdx.x * bins + j];
       base[j] = totals[j];
     }
@@ -565,75 +588,119 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
 }
 
 // ---- few tokens -----------------------------------------------------------------------------
-// Up to 256 tokens take one launch: a workgroup has some rows of the vocabulary (and 512 columns),
-// picks the tokens of those rows out of all, in their order, and its waves take a row each in
-// turn.  225 tokens of 675 rows and 128 columns take 5 us a call, and 15 by the sorted way; 256
-// tokens of two rows 17 us either way.
-constexpr int kFewTokens = 256;
+// Few tokens take one launch: a workgroup has some rows of the vocabulary (and 512 columns), lists
+// the tokens of those rows out of all in their order, and its waves take a row each in turn; a row
+// of more than kHotRow tokens is taken by all waves, a stretch of the list each, whose sums are
+// added in order.
+//
+// Up to 1024 tokens, and up to kListedTokens where the vocabulary's rows have four or fewer on
+// average.  The work of a row of many tokens is not spread over workgroups here, so that more
+// tokens are sorted: 225 tokens of 675 rows and 128 columns take 5 us a call (15 sorted), 1000 of
+// 1083 rows 5 us (18), 1734 of 867 rows 5.5 us (24); but 2048 of two rows 43 us (17), 8000 of 1000
+// rows unevenly 91 us (24).
+constexpr int kListedTokens = 2048, kHotRow = 64;
 
-template <class T, class O, class Id, bool kWhole>
-__global__ __launch_bounds__(256) void sum_few_kernel(const T* __restrict__ grad,
-                                                      int64_t grad_stride,
-                                                      const Id* __restrict__ ids, int tokens,
-                                                      int64_t vocab, int dim, float scale,
-                                                      int rows, O* __restrict__ out) {
+bool use_list(int64_t tokens, int64_t vocab) {
+  return tokens <= 1024 || (tokens <= kListedTokens && tokens <= 4 * vocab);
+}
+
+template <class T, class O, class Id, bool kWhole, int kThreads>
+__global__ __launch_bounds__(kThreads) void sum_listed_kernel(
+    const T* __restrict__ grad, int64_t grad_stride, const Id* __restrict__ ids, int tokens,
+    int64_t vocab, int dim, float scale, int rows, O* __restrict__ out) {
   constexpr int kBatch = 8;  // rows of `grad` in flight
-  __shared__ uint32_t token_of[kFewTokens], row_of[kFewTokens];
-  __shared__ int counts[4];
+  constexpr int kWaves = kThreads / kWave;
+  extern __shared__ uint32_t listed[];  // [tokens] rows, then [tokens] tokens of 16 bits
+  __shared__ int counts[2][kWaves];
+  __shared__ F8 joined[kWave];
+  __shared__ int hot[kListedTokens / kHotRow], hot_rows;
+  uint32_t* row_of = listed;
+  uint16_t* token_of = reinterpret_cast<uint16_t*>(listed + tokens);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t row0 = (int64_t)blockIdx.x * rows;
-  int64_t at = -1;
-  if ((int)threadIdx.x < tokens) {
-    const int64_t id = (int64_t)ids[threadIdx.x];
-    if (id >= row0 && id < row0 + rows && id < vocab) at = id - row0;
-  }
-  const uint64_t here = __ballot(at >= 0);
-  if (lane == 0) counts[wave] = __popcll(here);
-  __syncthreads();
-  int total = 0, before = 0;
+  const int64_t end = row0 + rows < vocab ? row0 + rows : vocab;
+  if (threadIdx.x == 0) hot_rows = 0;
+  int total = 0;
+  int64_t next = (int)threadIdx.x < tokens ? (int64_t)ids[threadIdx.x] : -1;
+  for (int base = 0, turn = 0; base < tokens; base += kThreads, turn ^= 1) {
+    const int64_t id = next;
+    const int ahead = base + kThreads + (int)threadIdx.x;
+    next = ahead < tokens ? (int64_t)ids[ahead] : -1;
+    const bool mine = id >= row0 && id < end;
+    const uint64_t here = __ballot(mine);
+    if (lane == 0) counts[turn][wave] = __popcll(here);
+    __syncthreads();
+    int place = total + lanes_below(here);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w == wave) before = total;
-    total += counts[w];
-  }
-  if (at >= 0) {
-    const int place = before + lanes_below(here);
-    token_of[place] = threadIdx.x;
-    row_of[place] = (uint32_t)at;
+    for (int w = 0; w < kWaves; ++w) {
+      const int c = counts[turn][w];
+      place += w < wave ? c : 0;
+      total += c;
+    }
+    if (mine) {
+      token_of[place] = (uint16_t)(base + threadIdx.x);
+      row_of[place] = (uint32_t)(id - row0);
+    }
   }
   __syncthreads();
   total = __builtin_amdgcn_readfirstlane(total);
   const int col = 8 * ((int)blockIdx.y * kWave + lane);
-  for (int r = wave; r < rows && row0 + r < vocab; r += 4) {
-    F8 acc = {};
-    for (int base = 0; base < total; base += kWave) {
-      const bool listed = base + lane < total;
-      const uint32_t token = listed ? token_of[base + lane] : 0u;
-      uint64_t mine = __ballot(listed && row_of[base + lane] == (uint32_t)r);
+  const auto matches = [&](int r, int base, int to, uint32_t* token) {
+    const bool there = base + lane < to;
+    *token = there ? token_of[base + lane] : 0u;
+    return __ballot(there && row_of[base + lane] == (uint32_t)r);
+  };
+  const auto add = [&](F8 acc, int r, int from, int to) {  // the list's stretch [from, to)
+    for (int base = from; base < to; base += kWave) {
+      uint32_t token;
+      uint64_t mine = matches(r, base, to, &token);
       while (mine) {
         Reg8<T> v[kBatch];
-        int n = 0;
+        const int n = __popcll(mine);
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) {  // (the last token again where there are no more)
-          const int from = __builtin_ctzll(mine);
-          const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)token, from);
+        for (int e = 0; e < kBatch; ++e) {  // (the last one again where there are no more)
+          const uint32_t t =
+              (uint32_t)__builtin_amdgcn_readlane((int)token, __builtin_ctzll(mine));
           v[e] = load_raw<T, kWhole>(grad + (int64_t)t * grad_stride, col, dim);
-          if (n == e) {
-            n = e + 1;
-            if (mine & (mine - 1))
-              mine &= mine - 1;
-            else
-              n |= 0x100;  // the last one
-          }
+          if (mine & (mine - 1)) mine &= mine - 1;
         }
 #pragma unroll
         for (int e = 0; e < kBatch; ++e)
-          if (e < (n & 0xFF)) acc += widen<T, kWhole>(v[e], col, dim);
-        if (n & 0x100) mine = 0;
+          if (e < n) acc += widen<T, kWhole>(v[e], col, dim);
+        if (n <= kBatch) mine = 0;
       }
     }
+    return acc;
+  };
+  const auto put = [&](int r, F8 acc) {
     store8<O, kWhole>(out + (row0 + r) * dim, col, dim, acc * scale);
+  };
+  for (int r = wave; row0 + r < end; r += kWaves) {
+    int n = total;
+    if (total > kHotRow) {
+      n = 0;
+      uint32_t token;
+      for (int base = 0; base < total; base += kWave)
+        n += __popcll(matches(r, base, total, &token));
+    }
+    if (n <= kHotRow)
+      put(r, n ? add(F8{}, r, 0, total) : F8{});
+    else if (lane == 0)
+      hot[atomicAdd(&hot_rows, 1)] = r;
+  }
+  __syncthreads();
+  const int stretch = (total + kThreads - 1) / kThreads * kWave;  // of whole waves
+  for (int h = 0; h < hot_rows; ++h) {
+    const int r = __builtin_amdgcn_readfirstlane(hot[h]);
+    const int from = wave * stretch < total ? wave * stretch : total;
+    const F8 acc = add(F8{}, r, from, from + stretch < total ? from + stretch : total);
+    for (int w = 0; w < kWaves; ++w) {
+      if (w == wave) joined[lane] = w ? joined[lane] + acc : acc;
+      __syncthreads();
+    }
+    if (wave == 0) put(r, joined[lane]);
+    __syncthreads();
   }
 }
 
@@ -656,9 +723,17 @@ bool grad_sizes_ok(int64_t tokens, int64_t vocab, int64_t dim) {
          dim >= 1 && dim <= OMQ_NET_MAX_DIM;
 }
 
+// One workgroup's sort is one launch, a pass of the radix sort two.  2048 tokens of two rows and
+// 1024 columns take 17 us a call with it (20 without); 3000 of 50000 rows, whose radix sort has two
+// passes, 24 us (28); but 4096 of 1000 rows, which it has to pass twice and the radix sort once,
+// 25 us (23).
+bool use_small_sort(int64_t tokens, int passes) {
+  return tokens <= (passes > 1 ? kSmallSort : kSmallSort / 2);
+}
+
 GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   GradPlan p{};
-  if (tokens <= kFewTokens) return p;  // (no workspace)
+  if (use_list(tokens, vocab)) return p;  // (no workspace)
   while (p.bits < 32 && (vocab >> p.bits) != 0) ++p.bits;
   p.passes = (int)ceil_div(p.bits, kMaxDigitBits);
   p.digit_bits = (int)ceil_div(p.bits, p.passes);
@@ -675,7 +750,7 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   p.pieces = ceil_div(items, p.piece);
   int64_t at = 0;
   p.at_pairs[0] = take(&at, 8 * tokens);
-  const bool radix = tokens > kSmallSort;
+  const bool radix = !use_small_sort(tokens, p.passes);
   p.at_pairs[1] = take(&at, radix && p.passes > 1 ? 8 * tokens : 0);
   p.at_counts = take(&at, radix ? 4 * (p.tiles << p.digit_bits) : 0);
   p.at_totals = take(&at, radix ? 4ll << p.digit_bits : 0);
@@ -692,14 +767,8 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
                          hipStream_t st) {
   uint2* buf[2] = {reinterpret_cast<uint2*>(ws + p.at_pairs[0]),
                    reinterpret_cast<uint2*>(ws + p.at_pairs[1])};
-  if (tokens <= kSmallSort) {
-    const auto sort = [&](auto kernel, int threads) {
-      kernel<<<1, threads, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
-    };
-    if (tokens <= 1024)
-      sort(sort_small_kernel<Id, 1024, 1>, 1024);
-    else
-      sort(sort_small_kernel<Id, 1024, kSmallSort / 1024>, 1024);
+  if (use_small_sort(tokens, p.passes)) {
+    sort_small_kernel<Id><<<1, 1024, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
     return buf[0];
   }
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.at_counts);
@@ -713,9 +782,12 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
     const int bins = (int)(top < all ? top : all);
     digit_counts_kernel<Id><<<(uint32_t)p.tiles, 256, 0, st>>>(ids, in, tokens, vocab, shift,
                                                               p.digit_bits, bins, counts);
-    digit_scan_kernel<<<(uint32_t)ceil_div(bins, kWave), 1024, 0, st>>>(counts, (int)p.tiles, bins,
-                                                                      totals);
-    digit_scatter_kernel<Id><<<(uint32_t)p.tiles, 512, 0, st>>>(
+    const bool scan = p.tiles <= kScanTiles;
+    if (!scan)
+      digit_scan_kernel<<<(uint32_t)ceil_div(bins, kWave), 1024, 0, st>>>(counts, (int)p.tiles,
+                                                                        bins, totals);
+    const auto scatter = scan ? digit_scatter_kernel<Id, true> : digit_scatter_kernel<Id, false>;
+    scatter<<<(uint32_t)p.tiles, 512, 0, st>>>(
         ids, in, tokens, vocab, shift, p.digit_bits, bins, counts, totals, to);
     in = to;
   }
@@ -742,24 +814,21 @@ void launch_sums(const GradPlan& p, const void* grad, int64_t grad_stride, const
                                            static_cast<O*>(out));
 }
 
-template <class T, class O>
-void launch_few(const void* grad, int64_t grad_stride, const void* ids, int ids_are_64, int tokens,
-                int64_t vocab, int dim, float scale, void* out, hipStream_t st) {
-  const int64_t col_tiles = ceil_div(dim, 8 * kWave);
-  // rows for about 2048 workgroups, four or more (a wave's)
-  const int64_t rows = ceil_div(ceil_div(vocab * col_tiles, 2048), 4) * 4;
-  const dim3 grid((uint32_t)ceil_div(vocab, rows), (uint32_t)col_tiles);
-  const auto go = [&](auto id, auto kernel) {
-    using Id = decltype(id);
-    kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(grad), grad_stride,
-                                 static_cast<const Id*>(ids), tokens, vocab, dim, scale, (int)rows,
-                                 static_cast<O*>(out));
+template <class T, class O, class Id, bool kWhole>
+void launch_listed(const void* grad, int64_t grad_stride, const void* ids, int tokens,
+                   int64_t vocab, int dim, float scale, void* out, hipStream_t st) {
+  const auto go = [&](auto kernel, int threads, int64_t groups) {
+    const int64_t col_tiles = ceil_div(dim, 8 * kWave), waves = threads / kWave;
+    const int64_t rows = ceil_div(ceil_div(vocab * col_tiles, groups), waves) * waves;
+    const dim3 grid((uint32_t)ceil_div(vocab, rows), (uint32_t)col_tiles);
+    kernel<<<grid, threads, 6 * tokens, st>>>(
+        static_cast<const T*>(grad), grad_stride, static_cast<const Id*>(ids), tokens, vocab, dim,
+        scale, (int)rows, static_cast<O*>(out));
   };
-  const bool whole = dim % 8 == 0;
-  if (ids_are_64)
-    go(int64_t{}, whole ? sum_few_kernel<T, O, int64_t, true> : sum_few_kernel<T, O, int64_t, false>);
+  if (tokens <= 256)
+    go(sum_listed_kernel<T, O, Id, kWhole, 256>, 256, 2048);
   else
-    go(int32_t{}, whole ? sum_few_kernel<T, O, int32_t, true> : sum_few_kernel<T, O, int32_t, false>);
+    go(sum_listed_kernel<T, O, Id, kWhole, 1024>, 1024, 1024);
 }
 
 template <class T, class O, class... A>
@@ -849,17 +918,24 @@ int omq_token_embedding_grad(const void* grad, int64_t grad_stride, int dtype, c
     return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   hipStream_t st = (hipStream_t)stream;
   char* ws = static_cast<char*>(workspace);
-  const bool few = tokens <= kFewTokens;
+  const bool listed = use_list(tokens, vocab);
   const uint2* pairs = nullptr;
-  if (!few)
+  if (!listed)
     pairs = ids_are_64 ? sort_tokens(p, static_cast<const int64_t*>(ids), tokens, vocab, ws, st)
                        : sort_tokens(p, static_cast<const int32_t*>(ids), tokens, vocab, ws, st);
   const auto sums = [&](auto t, auto o) {
     using T = decltype(t);
     using O = decltype(o);
-    if (few)
-      launch_few<T, O>(grad, grad_stride, ids, ids_are_64, (int)tokens, vocab, (int)dim, scale, out,
-                       st);
+    const auto go = [&](auto id, auto whole) {
+      launch_listed<T, O, decltype(id), whole.value>(grad, grad_stride, ids, (int)tokens, vocab,
+                                                     (int)dim, scale, out, st);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (listed && ids_are_64)
+      dim % 8 == 0 ? go(int64_t{}, Yes{}) : go(int64_t{}, No{});
+    else if (listed)
+      dim % 8 == 0 ? go(int32_t{}, Yes{}) : go(int32_t{}, No{});
     else
       launch_sums_lanes<T, O>(p, grad, grad_stride, pairs, tokens, vocab, (int)dim, scale, out, ws,
                               st);

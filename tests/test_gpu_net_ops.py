@@ -80,11 +80,14 @@ def test_embedding_shapes_and_far_ids(device):
 
 
 GRAD_CASES = [
-    # tokens, vocab, dim, skew: no tokens; one; few; one vocabulary row; one workgroup's sorts;
-    # radix sorts of one, two and three passes; tokens of few rows and rows of few tokens
+    # tokens, vocab, dim, skew: no tokens; one; few, listed, with rows of many tokens and of none;
+    # one vocabulary row; one workgroup's sorts; radix sorts of one, two and three passes, with and
+    # without a launch for the scan; tokens of few rows and rows of few tokens
     (0, 5, 16, 1), (1, 1, 1, 1), (1, 3000, 40, 1), (225, 675, 128, 1), (256, 2, 600, 1),
-    (256, 20_000, 7, 2), (257, 2, 600, 1), (1024, 40, 24, 1), (1025, 300, 129, 1),
-    (4096, 1, 64, 1),
+    (256, 20_000, 7, 2), (257, 2, 600, 1), (1024, 40, 24, 1), (1024, 1, 8, 1), (1025, 300, 129, 1),
+    (1025, 200, 129, 1), (2048, 512, 600, 6), (2047, 5000, 3, 1), (2049, 5000, 48, 1),
+    (2048, 400, 33, 1), (4096, 2047, 16, 1), (4096, 2048, 16, 1), (4097, 2048, 16, 1),
+    (32_768, 300, 40, 1), (32_769, 300, 40, 1), (32_000, 3000, 40, 2), (4096, 1, 64, 1),
     (4096, 300, 33, 3), (4097, 3, 64, 1), (5000, 2047, 130, 1), (9000, 2048, 257, 4),
     (20_000, 70_000, 65, 3), (6000, 5_000_000, 8, 1), (50_000, 2, 513, 1), (30_001, 900, 1031, 2),
 ]

@@ -124,13 +124,13 @@ def test_c_entry_points_refuse():
     refused(lib.omq_token_embedding(ptr, 0, 4, ptr, 8, 5, 1 << 21, 0, 1.0, ptr, None), "too large",
             -3)
     refused(lib.omq_token_embedding(None, 0, 4, ptr, 8, 5, 8, 0, 1.0, ptr, None), "null")
-    need = lib.omq_token_embedding_grad_workspace(1000, 5, 8)
+    need = lib.omq_token_embedding_grad_workspace(3000, 5, 8)
     assert need > 0 and lib.omq_token_embedding_grad_workspace(-1, 5, 8) < 0
-    refused(lib.omq_token_embedding_grad(ptr, 8, 0, ptr, 0, 1000, 5, 8, 1.0, ptr, 0, ptr, need - 1,
+    refused(lib.omq_token_embedding_grad(ptr, 8, 0, ptr, 0, 3000, 5, 8, 1.0, ptr, 0, ptr, need - 1,
                                          None), str(need))
-    refused(lib.omq_token_embedding_grad(ptr, 8, 1, ptr, 0, 1000, 5, 8, 1.0, ptr, 2, ptr, need,
+    refused(lib.omq_token_embedding_grad(ptr, 8, 1, ptr, 0, 3000, 5, 8, 1.0, ptr, 2, ptr, need,
                                          None), "types")
-    refused(lib.omq_token_embedding_grad(ptr, 8, 0, ptr, 0, 1000, 5, 8, 1.0, ptr, 0, ptr, need,
+    refused(lib.omq_token_embedding_grad(ptr, 8, 0, ptr, 0, 3000, 5, 8, 1.0, ptr, 0, ptr, need,
                                          None), "16-byte")
     refused(lib.omq_dropout(ptr, 4, 8, 0, 1.01, 0, 0, ptr, None), "outside")
     refused(lib.omq_dropout(ptr, 4, 0, 0, 0.5, 0, 0, ptr, None), "dim 0")
