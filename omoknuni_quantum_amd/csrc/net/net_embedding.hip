@@ -128,12 +128,12 @@ __device__ inline uint32_t take_places(uint32_t digit, int bits, bool here, uint
   return place;
 }
 
-// All passes of up to kSmallSort tokens in one workgroup.  8-bit digits.
-template <class Id>
+// All passes of up to kTokens tokens in one workgroup.  8-bit digits.
+template <class Id, int kTokens>
 __global__ __launch_bounds__(1024) void sort_small_kernel(const Id* __restrict__ ids, int tokens,
                                                           int64_t vocab, int bits,
                                                           uint2* __restrict__ pairs) {
-  constexpr int kThreads = 1024, kRounds = kSmallSort / kThreads, kWaves = kThreads / kWave;
+  constexpr int kThreads = 1024, kRounds = kTokens / kThreads, kWaves = kThreads / kWave;
   __shared__ uint2 kept[kThreads * kRounds];
   __shared__ uint32_t next[kWaves][256];
   __shared__ uint32_t base[256];
@@ -724,9 +724,9 @@ bool grad_sizes_ok(int64_t tokens, int64_t vocab, int64_t dim) {
 }
 
 // One workgroup's sort is one launch, a pass of the radix sort two.  2048 tokens of two rows and
-// 1024 columns take 17 us a call with it (20 without); 3000 of 50000 rows, whose radix sort has two
-// passes, 24 us (28); but 4096 of 1000 rows, which it has to pass twice and the radix sort once,
-// 25 us (23).
+// 1024 columns take 16.5 us a call with it (18.4 without; 17.4 with the larger one's registers);
+// 3000 of 50000 rows, whose radix sort has two passes, 24 us (28); but 4096 of 1000 rows, which it
+// has to pass twice and the radix sort once, 25.5 us (22.5).
 bool use_small_sort(int64_t tokens, int passes) {
   return tokens <= (passes > 1 ? kSmallSort : kSmallSort / 2);
 }
@@ -768,7 +768,9 @@ const uint2* sort_tokens(const GradPlan& p, const Id* ids, int64_t tokens, int64
   uint2* buf[2] = {reinterpret_cast<uint2*>(ws + p.at_pairs[0]),
                    reinterpret_cast<uint2*>(ws + p.at_pairs[1])};
   if (use_small_sort(tokens, p.passes)) {
-    sort_small_kernel<Id><<<1, 1024, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
+    const auto sort = tokens <= kSmallSort / 2 ? sort_small_kernel<Id, kSmallSort / 2>
+                                               : sort_small_kernel<Id, kSmallSort>;
+    sort<<<1, 1024, 0, st>>>(ids, (int)tokens, vocab, p.bits, buf[0]);
     return buf[0];
   }
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.at_counts);
