@@ -342,7 +342,8 @@ __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coe
   F8 d = e * scale;
   if constexpr (kTarget) {
     // (fmaf where a product and a sum could be contracted one way here and another there: the
-    // gradient has the same bits whichever kernel forms it from the same statistics)
+    // gradient has the same bits whichever kernel forms it from the same statistics, but for rows
+    // in the registers of several waves, whose exponentials are about each wave's own base)
 #pragma unroll
     for (int j = 0; j < 8; ++j) d[j] = fmaf(-pi[j], w_coef, d[j]);
   }
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
     t.m = larger(t.m, largest(z[i]));
   }
   t.m = lanes_reduce<Max, (kThreads < kWave ? kThreads : kWave)>(t.m);
-  const float base = base_of(t.m);
+  const float m = t.m, base = base_of(m);  // (of this wave)
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     if constexpr (kTarget) {
@@ -413,7 +414,9 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
   if (lane == 0) write_row(o, row, loss, logp, kl, stats);
   if (!grad) return;
   const float w = row_weight ? row_weight[row] : 1.0f;
-  const float scale = w * o.g.push * o.g.inv_s * exp_fast(base - o.g.m);
+  // From the wave's base to the row's: 0 where the wave has no weight.  (Its base is 0 then, which
+  // may lie any distance above the row's.)
+  const float scale = w * o.g.push * o.g.inv_s * exp_fast(m - o.g.m);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int col = 8 * (lane + i * kThreads);

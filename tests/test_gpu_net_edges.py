@@ -1,0 +1,70 @@
+"""Edges of the policy network's operators on the GPU against their definitions in 64 bits
+(oracle/net_ref.py): infinities, rows without weight, large differences of log-probabilities.
+
+Tolerances are derived as in test_gpu_net_ops.py: u = 2^-24, counts of operations times u times a
+magnitude taken from the 64-bit reference, plus the rounding to the result's type."""
+import math
+
+import pytest
+import torch
+
+from omoknuni_quantum_amd import net_ops
+from oracle import net_ref
+from tests.test_gpu_net_ops import check_loss, gen, loss_inputs, randn, u
+
+pytestmark = pytest.mark.gpu
+
+
+def check_autograd(dev, args, want):
+    """The gradient of the two operators, from the statistics that the loss left, against that of
+    the one: finite, and the same but for the exponentials' roundings."""
+    z = dev["z"].detach().clone().requires_grad_()
+    loss, _, _ = net_ops.clipped_policy_loss(z, dev["act"], dev["adv"], dev["old"], **args)
+    (loss * dev["weight"]).sum().backward()
+    fused = net_ops.clipped_policy_loss_with_grad(dev["z"], dev["act"], dev["adv"], dev["old"],
+                                                  dev["weight"], **args)[3]
+    got, fused = z.grad.cpu().double(), fused.cpu().double()
+    assert bool(got.isfinite().all()) and bool(fused.isfinite().all())
+    # e^(z - m) in one exponential or in two: |z - m| below 40 in the logits that count, each
+    # product with log2(e) off by u relative; the target's part of a sum that may cancel
+    size = want["grad"].abs() * dev["weight"].cpu().double()[:, None]
+    if dev.get("target") is not None:
+        size = size + dev["target"].cpu().double() * args["kl_coef"]
+    size = size + 2 * want["prob"] * (want["slope"].abs()[:, None] + args["kl_coef"])
+    assert bool(((got - fused).abs() <= (4 * 40 + 4) * u * size + 2.0**-120).all())
+
+
+# ---- waves of a row without weight ----------------------------------------------------------
+@pytest.mark.parametrize("cols", [600, 1024, 4672, 8192, 16_384, 20_000, 80_000])
+@pytest.mark.parametrize("level", [-100.0, -1000.0])
+@pytest.mark.parametrize("kl", ["none", "sampled", "target"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_columns_of_minus_infinity_below_far_logits(device, cols, level, kl, masked):
+    """Logits that the caller masked with -inf, 512 columns and more of them, where the others are
+    far below zero: those actions have probability and gradient 0, whatever the largest logit."""
+    rows = 12
+    d = loss_inputs(rows, cols, torch.float32, kl, False, cols)
+    d["z"] = (d["z"] + level).float()
+    away = torch.zeros(rows, cols, dtype=torch.bool)
+    away[0::3, :512] = True
+    away[1::3, 512:] = True
+    away[2::3, 40:cols - 40] = True
+    d["z"][away] = -math.inf
+    if masked:
+        d["legal"] = torch.rand(rows, cols, generator=gen(cols)) < 0.7
+    open_ = ~away if not masked else ~away & d["legal"]
+    for i in range(rows):  # an action that can be taken
+        if 0 <= int(d["act"][i]) < cols:
+            d["act"][i] = int(open_[i].nonzero()[i % 7])
+    ref = net_ref.policy_loss(d["z"], d["act"], d["adv"], torch.zeros(rows), 0.2, 0.3, 0.0,
+                              legal=d["legal"])
+    d["old"] = (ref["logp"] + randn(gen(1), rows, scale=0.1)).float()
+    if kl == "sampled":
+        d["ref"] = (ref["logp"] + randn(gen(2), rows, scale=0.1)).float()
+    if kl == "target":
+        d["target"][away] = 0.0
+    coef = {"none": 0.0, "sampled": 0.3, "target": 1.0}[kl]
+    # (a bound relative to logits of 1000 over 800 terms decides nothing about the clipping)
+    dev, args, want = check_loss(device, d, coef, with_grad=cols <= 16_384 or level > -500)
+    assert bool(want["grad"].isfinite().all())
+    check_autograd(dev, args, want)
