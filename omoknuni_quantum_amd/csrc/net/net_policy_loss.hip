@@ -155,7 +155,8 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
     if (r.ref_logp) {
       const float d = (float)((double)r.ref_logp[row] - logp);
       o.kl = exp_above_line(d);
-      slope -= r.kl_coef * (o.kl + d);
+      // (without a coefficient the kl is only watched: it may overflow)
+      if (r.kl_coef != 0.0f) slope -= r.kl_coef * (o.kl + d);
     }
   }
   if (r.target) o.kl = (float)((double)t.tk + (t.tp != 0.0f ? (double)t.tp * log_s : 0.0));

@@ -10,7 +10,7 @@ import torch
 
 from omoknuni_quantum_amd import net_ops
 from oracle import net_ref
-from tests.test_gpu_net_ops import check_loss, gen, loss_inputs, randn, u
+from tests.test_gpu_net_ops import check_loss, gen, loss_inputs, randn, u, within
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,50 @@ def test_columns_of_minus_infinity_below_far_logits(device, cols, level, kl, mas
     dev, args, want = check_loss(device, d, coef, with_grad=cols <= 16_384 or level > -500)
     assert bool(want["grad"].isfinite().all())
     check_autograd(dev, args, want)
+
+
+# ---- the sampled kl's ends ------------------------------------------------------------------
+def sampled_rows(cols, rows, seed):
+    """Rows whose old log-probability is the present one: a ratio of 1, inside the clipping."""
+    g = gen(seed)
+    z = randn(g, rows, cols)
+    act = torch.randint(0, cols, (rows,), generator=g)
+    logp = net_ref.policy_loss(z, act, torch.zeros(rows), torch.zeros(rows), 0.2, 0.2,
+                               0.0)["logp"]
+    return z, act, torch.ones(rows), logp
+
+
+def sampled(device, z, act, adv, old, ref, coef, dtype=torch.float32):
+    args = dict(clip_low=0.2, clip_high=0.2, kl_coef=coef, ref_logp=ref.float().to(device))
+    rest = act.to(device), adv.to(device), old.float().to(device)
+    one = [t.cpu() for t in net_ops.clipped_policy_loss_with_grad(z.to(device), *rest, None,
+                                                                  **args)]
+    x = z.to(device).requires_grad_()
+    two = net_ops.clipped_policy_loss(x, *rest, **args)
+    two[0].backward(torch.ones_like(two[0]))
+    two = [t.detach().cpu() for t in (*two, x.grad)]
+    want = net_ref.policy_loss(z, act, adv, old.float(), 0.2, 0.2, coef, ref.float())
+    return (one, two), want
+
+
+def slope_bounds(want, act, coef, e_kl_slope):
+    """Of the gradient, rounded to float32: the slope's error at the taken action and, times the
+    probabilities, at the others, which have their own."""
+    rows, cols = want["grad"].shape
+    e_logp = 800 * u * (6.0 + math.log(cols))
+    e_slope = 2 * e_logp + 4 * u + coef * e_kl_slope
+    bound = want["prob"] * (want["slope"].abs() * 3 * e_logp + e_slope)[:, None]
+    bound[torch.arange(rows), act] += e_slope
+    return bound + 8 * u * want["grad"].abs()
+
+
+@pytest.mark.parametrize("cols", [9, 300, 1024, 20_000, 80_000])
+def test_sampled_kl_that_is_only_watched(device, cols):
+    """No coefficient: a kl that overflows reaches neither the loss nor the gradient."""
+    z, act, adv, logp = sampled_rows(cols, 6, cols)
+    outs, want = sampled(device, z, act, adv, logp, logp + 100.0, 0.0)
+    e_logp = 800 * u * (6.0 + math.log(cols))
+    for out in outs:
+        assert bool((out[2] == math.inf).all())
+        within(out[0], want["loss"], 2 * e_logp + 4 * u)
+        within(out[3], want["grad"], slope_bounds(want, act, 0.0, 0.0))
