@@ -118,16 +118,21 @@ __device__ inline double log_of_sum(float s) {
   return (double)k * 0.6931471805599453 + (double)(__builtin_amdgcn_logf(f) * kLn2);
 }
 
-// e^d - 1 - d without its cancellation about 0.
-__device__ inline float exp_above_line(float d) {
-  if (fabsf(d) > 0.5f) return expm1f(d) - d;
+// e^d - 1 and e^d - 1 - d, the latter without its cancellation about 0.
+__device__ inline float exp_above_line(float d, float* above_one) {
+  if (fabsf(d) > 0.5f) {
+    *above_one = expm1f(d);
+    return *above_one - d;
+  }
   float p = 1.0f / 40320.0f;  // Taylor; the next term is below 2^-24 of the sum
   p = fmaf(p, d, 1.0f / 5040.0f);
   p = fmaf(p, d, 1.0f / 720.0f);
   p = fmaf(p, d, 1.0f / 120.0f);
   p = fmaf(p, d, 1.0f / 24.0f);
   p = fmaf(p, d, 1.0f / 6.0f);
-  return d * d * fmaf(p, d, 0.5f);
+  p = d * d * fmaf(p, d, 0.5f);
+  *above_one = p + d;
+  return p;
 }
 
 // z_taken: the logit of the taken action, `taken`: it is legal and in range.  The differences of
@@ -154,9 +159,10 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
     if (one <= two || one != one) slope = -one;
     if (r.ref_logp) {
       const float d = (float)((double)r.ref_logp[row] - logp);
-      o.kl = exp_above_line(d);
+      float above_one;  // (not kl + d, which loses the bits of -1 where d is far below 0)
+      o.kl = exp_above_line(d, &above_one);
       // (without a coefficient the kl is only watched: it may overflow)
-      if (r.kl_coef != 0.0f) slope -= r.kl_coef * (o.kl + d);
+      if (r.kl_coef != 0.0f) slope -= r.kl_coef * above_one;
     }
   }
   if (r.target) o.kl = (float)((double)t.tk + (t.tp != 0.0f ? (double)t.tp * log_s : 0.0));

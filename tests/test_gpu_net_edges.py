@@ -115,3 +115,16 @@ def test_sampled_kl_that_is_only_watched(device, cols):
         assert bool((out[2] == math.inf).all())
         within(out[0], want["loss"], 2 * e_logp + 4 * u)
         within(out[3], want["grad"], slope_bounds(want, act, 0.0, 0.0))
+
+
+@pytest.mark.parametrize("cols", [9, 300, 1024, 20_000, 80_000])
+@pytest.mark.parametrize("d", [-1000.0, -1e6, -math.inf])
+def test_sampled_kl_far_below_the_action(device, cols, d):
+    """The derivative of e^d - 1 - d is -1 to the last bit there."""
+    z, act, adv, logp = sampled_rows(cols, 6, cols)
+    outs, want = sampled(device, z, act, adv, logp, logp + d, 0.3)
+    assert bool(want["grad"].isfinite().all())
+    e_logp = 800 * u * (6.0 + math.log(cols))
+    for out in outs:
+        within(out[2], want["kl"], 4 * u * abs(d) + 2 * e_logp if d > -math.inf else 0.0)
+        within(out[3], want["grad"], slope_bounds(want, act, 0.3, u))
