@@ -122,7 +122,7 @@ __device__ inline double log_of_sum(float s) {
 __device__ inline float exp_above_line(float d, float* above_one) {
   if (fabsf(d) > 0.5f) {
     *above_one = expm1f(d);
-    return *above_one - d;
+    return d == kInf ? kInf : *above_one - d;  // (not inf - inf)
   }
   float p = 1.0f / 40320.0f;  // Taylor; the next term is below 2^-24 of the sum
   p = fmaf(p, d, 1.0f / 5040.0f);

@@ -106,8 +106,9 @@ def policy_loss(logits, actions, advantages, old_logp, clip_low, clip_high, kl_c
     kl, grad = torch.zeros(n, dtype=torch.float64), torch.zeros_like(z)
     if ref_logp is not None:
         d = ref_logp.double() - logp
-        kl = torch.where(taken, torch.expm1(d) - d, 0.0)
-        slope = slope - torch.where(taken, kl_coef * torch.expm1(d), 0.0)
+        kl = torch.where(taken, torch.where(d == math.inf, d, torch.expm1(d) - d), 0.0)
+        if kl_coef:
+            slope = slope - torch.where(taken, kl_coef * torch.expm1(d), 0.0)
     if target is not None:
         pi = target.double()
         use = ok & live[:, None] & (pi > 0)

@@ -128,3 +128,26 @@ def test_sampled_kl_far_below_the_action(device, cols, d):
     for out in outs:
         within(out[2], want["kl"], 4 * u * abs(d) + 2 * e_logp if d > -math.inf else 0.0)
         within(out[3], want["grad"], slope_bounds(want, act, 0.3, u))
+
+
+@pytest.mark.parametrize("cols", [2, 300, 1024, 20_000, 80_000])
+def test_sampled_kl_of_an_action_without_weight(device, cols):
+    """A legal action of probability 0 was taken: the kl is infinite, as it is against a target."""
+    z, act, adv, logp = sampled_rows(cols, 5, cols)
+    z[torch.arange(5), act] = -math.inf
+    for coef in (0.0, 0.3):
+        outs, want = sampled(device, z, act, adv, logp, logp, coef)
+        assert bool((want["kl"] == math.inf).all())
+        for out in outs:
+            assert bool((out[1] == -math.inf).all()) and bool((out[2] == math.inf).all())
+            assert bool((out[0] == (math.inf if coef else 0.0)).all())
+            if not coef:
+                assert not bool(out[3].any())
+    # a reference that is infinitely more likely, only watched
+    z, act, adv, logp = sampled_rows(cols, 6, cols)
+    outs, _ = sampled(device, z, act, adv, logp, logp + math.inf, 0.0)
+    want = net_ref.policy_loss(z, act, adv, logp.float(), 0.2, 0.2, 0.0)
+    for out in outs:
+        assert bool((out[2] == math.inf).all())
+        within(out[0], want["loss"], 2 * 800 * u * (6.0 + math.log(cols)) + 4 * u)
+        within(out[3], want["grad"], slope_bounds(want, act, 0.0, 0.0))

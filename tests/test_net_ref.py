@@ -96,3 +96,15 @@ def test_dropout_mask_statistics(p):
         assert abs(float(pair.mean())) < 5 * p * (1 - p) / math.sqrt(pair.numel())
     other = net_ref.keep_mask(rows, dim, p, 123, 5).double() - (1 - p)
     assert abs(float((c * other).mean())) < 5 * p * (1 - p) / math.sqrt(n)
+
+
+@pytest.mark.parametrize("coef", [0.0, 0.5])
+def test_sampled_kl_of_an_action_without_weight_is_infinite(coef):
+    """e^d - 1 - d at d = inf: a legal action of probability 0, as it is against a target."""
+    z = torch.tensor([[-math.inf, 0.0, 1.0]])
+    got = net_ref.policy_loss(z, torch.tensor([0]), torch.ones(1), torch.zeros(1), 0.2, 0.2, coef,
+                              ref_logp=torch.tensor([-1.0]))
+    assert float(got["logp"][0]) == -math.inf and float(got["kl"][0]) == math.inf
+    assert float(got["loss"][0]) == (math.inf if coef else 0.0)
+    if not coef:
+        assert not bool(got["grad"].any())
