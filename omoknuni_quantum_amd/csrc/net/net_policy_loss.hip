@@ -172,8 +172,9 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
   o.g.others = t.rest * o.g.inv_s;
   o.g.slope = slope;
   o.g.push = (r.kl_coef != 0.0f ? r.kl_coef * t.tp : 0.0f) - slope;
-  // a row that adds nothing to the loss has no gradient, whatever its logits hold (padding)
-  if (slope == 0.0f && o.g.push == 0.0f && (!r.target || r.kl_coef == 0.0f)) o.g.inv_s = 0.0f;
+  // a row that adds nothing to the loss has no gradient, whatever its logits hold (padding; tp is
+  // 0 without a target, and where nothing in it is positive)
+  if (slope == 0.0f && o.g.push == 0.0f && (r.kl_coef == 0.0f || t.tp == 0.0f)) o.g.inv_s = 0.0f;
   return o;
 }
 

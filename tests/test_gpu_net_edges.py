@@ -151,3 +151,21 @@ def test_sampled_kl_of_an_action_without_weight(device, cols):
         assert bool((out[2] == math.inf).all())
         within(out[0], want["loss"], 2 * 800 * u * (6.0 + math.log(cols)) + 4 * u)
         within(out[3], want["grad"], slope_bounds(want, act, 0.0, 0.0))
+
+
+# ---- padding --------------------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [300, 1024, 20_000, 80_000])
+def test_padding_with_a_target_of_nothing(device, cols):
+    """A row without an action whose target is zero adds nothing to the loss: its gradient is 0
+    whatever its logits hold."""
+    z = torch.full((3, cols), float("nan"))
+    z[2] = 1.0
+    f, act = torch.ones(3, device=device), torch.full((3,), -1, device=device)
+    pi = torch.zeros(3, cols, device=device)
+    pi[1] = -1.0
+    one = net_ops.clipped_policy_loss_with_grad(z.to(device), act, f, f, kl_coef=1.0, target=pi)
+    x = z.to(device).requires_grad_()
+    two = net_ops.clipped_policy_loss(x, act, f, f, kl_coef=1.0, target=pi)
+    two[0].sum().backward()
+    for out in (one, (*two, x.grad)):
+        assert all(not bool(t.any()) for t in out)
