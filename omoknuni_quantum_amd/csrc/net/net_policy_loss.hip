@@ -89,17 +89,18 @@ struct RowGrad {
   float m, inv_s;  // p = e^(z - m) * inv_s; inv_s = 0: the row has no gradient
   float push, slope;
   float others;  // 1 - p of the taken action
+  float mass;    // kl_coef tp
 };
 
 // Its place in the statistics that the loss leaves for its gradient: eight floats a row.
 __device__ inline void write_stats(float4* stats, int64_t row, const RowGrad& g) {
   stats[2 * row] = make_float4(g.m, g.inv_s, g.push, g.slope);
-  stats[2 * row + 1] = make_float4(g.others, 0.0f, 0.0f, 0.0f);
+  stats[2 * row + 1] = make_float4(g.others, g.mass, 0.0f, 0.0f);
 }
 
 __device__ inline RowGrad read_stats(const float4* stats, int64_t row) {
-  const float4 a = stats[2 * row];
-  return RowGrad{a.x, a.y, a.z, a.w, stats[2 * row + 1].x};
+  const float4 a = stats[2 * row], b = stats[2 * row + 1];
+  return RowGrad{a.x, a.y, a.z, a.w, b.x, b.y};
 }
 
 struct RowOut {
@@ -171,7 +172,8 @@ __device__ inline RowOut finish_row(const omq_policy_rows& r, int64_t row, const
   o.g.inv_s = 1.0f / s;
   o.g.others = t.rest * o.g.inv_s;
   o.g.slope = slope;
-  o.g.push = (r.kl_coef != 0.0f ? r.kl_coef * t.tp : 0.0f) - slope;
+  o.g.mass = r.kl_coef != 0.0f ? r.kl_coef * t.tp : 0.0f;
+  o.g.push = o.g.mass - slope;
   // a row that adds nothing to the loss has no gradient, whatever its logits hold (padding; tp is
   // 0 without a target, and where nothing in it is positive)
   if (slope == 0.0f && o.g.push == 0.0f && (r.kl_coef == 0.0f || t.tp == 0.0f)) o.g.inv_s = 0.0f;
@@ -363,11 +365,12 @@ __device__ inline F8 gradient(F8 e, F8 pi, uint64_t ok, float scale, float w_coe
 }
 
 // The element of the taken action, in full; written by the thread that wrote its block, after it.
-// (push + slope) p + slope (1 - p), not push p + slope: the second cancels where p is near 1.
+// kl_coef tp p + slope (1 - p), not push p + slope, which cancels where p is near 1 and is NaN where
+// the slope overflows.
 template <class T>
 __device__ inline void put_taken(T* grad, const RowIn<T>& in, const RowGrad& g, float z_taken,
                                  int taken, float coef, float w) {
-  float d = fmaf(g.push + g.slope, exp_fast(z_taken - g.m) * g.inv_s, g.slope * g.others);
+  float d = fmaf(g.mass, exp_fast(z_taken - g.m) * g.inv_s, g.slope * g.others);
   if (in.target) d = fmaf(-larger(in.target[taken], 0.0f), coef, d);
   grad[taken] = (T)(w * d);
 }

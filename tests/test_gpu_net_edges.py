@@ -169,3 +169,16 @@ def test_padding_with_a_target_of_nothing(device, cols):
     two[0].sum().backward()
     for out in (one, (*two, x.grad)):
         assert all(not bool(t.any()) for t in out)
+
+
+def test_sampled_kl_that_overflows_has_an_infinite_gradient(device):
+    """e^100 and more is beyond float32: the gradient is -inf at the taken action and inf elsewhere."""
+    for cols in (64, 300, 1024, 20_000, 80_000):
+        z, act, adv, logp = sampled_rows(cols, 4, cols)
+        outs, _ = sampled(device, 0.01 * z, act, adv, logp, logp + 115.0, 0.3)
+        taken = torch.zeros(4, cols, dtype=torch.bool)
+        taken[torch.arange(4), act] = True
+        for out in outs:
+            assert bool((out[0] == math.inf).all()) and bool((out[2] == math.inf).all())
+            assert bool((out[3][taken] == -math.inf).all())
+            assert bool((out[3][~taken] == math.inf).all())
