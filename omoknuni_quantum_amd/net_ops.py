@@ -133,8 +133,8 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, p, seed, offset):
         y, h = _NORM(x, residual, weight, eps, p, seed, offset)
-        if h.numel() != x.numel():
-            h = x.clone() if x.numel() else x.new_empty(x.shape)
+        if h.shape != x.shape:  # (not given: it is x)
+            h = x.clone()
         ctx.save_for_backward(h, weight)
         ctx.args, ctx.has_residual = (eps, p, seed, offset), residual is not None
         ctx.set_materialize_grads(False)
