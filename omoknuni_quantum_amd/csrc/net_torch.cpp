@@ -17,6 +17,8 @@
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <array>
 #include <optional>
@@ -434,13 +436,70 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> clipped_policy_loss_w
   return {loss, logp, kl, grad};
 }
 
+// ---- registration ---------------------------------------------------------------------------
+// The operators have no derivatives of their own (net_ops.py's autograd functions call them): a
+// tangent is refused, and a backward pass through one raises.  Without this kernel torch drops
+// tangents without a word and leaves gradients out with a warning.  (torch's fallback for operators
+// without a derivative does the same and takes 0.1 to 0.4 us more of a call.)
+template <auto Fn>
+struct NoDerivative;
+
+template <class R, class... A, R (*Fn)(A...)>
+struct NoDerivative<Fn> {
+  static std::string& name() {
+    static std::string given;
+    return given;
+  }
+
+  template <class T>
+  static const at::Tensor* tensor(const T& t) {
+    if constexpr (std::is_same_v<T, at::Tensor>) return &t;
+    else if constexpr (std::is_same_v<T, OptTensor>) return get(t);
+    else return nullptr;
+  }
+
+  static void record(const std::shared_ptr<torch::autograd::Node>& node, at::Tensor& out) {
+    torch::autograd::set_history(out, node);
+  }
+
+  template <class... T>
+  static void record(const std::shared_ptr<torch::autograd::Node>& node, std::tuple<T...>& out) {
+    std::apply([&](auto&... t) { (record(node, t), ...); }, out);
+  }
+
+  static R call(c10::DispatchKeySet keys, A... args) {
+    static const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow(name().c_str(), "").template typed<R(A...)>();
+    const at::Tensor* tensors[] = {tensor(args)...};
+    bool needed = false;
+    for (const at::Tensor* t : tensors) {
+      if (!t) continue;
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), name(),
+                                  " has no forward-mode derivative");
+      needed = needed || t->requires_grad();
+    }
+    R out = op.redispatch(keys & c10::after_autograd_keyset, args...);
+    if (needed && at::GradMode::is_enabled()) {
+      const std::shared_ptr<torch::autograd::Node> node(new torch::autograd::NotImplemented(name()),
+                                                        torch::autograd::deleteNode);
+      torch::autograd::edge_list edges;
+      for (const at::Tensor* t : tensors)
+        if (t) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+      node->set_next_edges(std::move(edges));
+      record(node, out);
+    }
+    return out;
+  }
+};
+
 // Defines `name` with one function for HIP, host (which it refuses) and meta tensors.
-template <class Fn>
-void define(torch::Library& m, const std::string& name, const std::string& schema, Fn fn) {
+template <auto Fn>
+void define(torch::Library& m, const std::string& name, const std::string& schema) {
   m.def((name + schema).c_str());
-  m.impl(name.c_str(), torch::dispatch(c10::DispatchKey::CUDA, fn));
-  m.impl(name.c_str(), torch::dispatch(c10::DispatchKey::CPU, fn));
-  m.impl(name.c_str(), torch::dispatch(c10::DispatchKey::Meta, fn));
+  for (const auto key : {c10::DispatchKey::CUDA, c10::DispatchKey::CPU, c10::DispatchKey::Meta})
+    m.impl(name.c_str(), torch::dispatch(key, Fn));
+  NoDerivative<Fn>::name() = "omq_net::" + name;
+  m.impl(name.c_str(), torch::dispatch(c10::DispatchKey::Autograd, &NoDerivative<Fn>::call));
 }
 
 const std::string kLossArgs =
@@ -450,31 +509,24 @@ const std::string kLossArgs =
 }  // namespace
 
 TORCH_LIBRARY(omq_net, m) {
-  define(m, "token_embedding", "(Tensor ids, Tensor weight, float scale) -> Tensor",
-         token_embedding);
-  define(m, "token_embedding_grad",
-         "(Tensor grad, Tensor ids, int num_embeddings, float scale, ScalarType? dtype) -> Tensor",
-         token_embedding_grad);
-  define(m, "dropout", "(Tensor x, float p, int seed, int offset) -> Tensor", dropout);
-  define(m, "add_rms_norm",
+  define<token_embedding>(m, "token_embedding",
+                          "(Tensor ids, Tensor weight, float scale) -> Tensor");
+  define<token_embedding_grad>(m, "token_embedding_grad",
+         "(Tensor grad, Tensor ids, int num_embeddings, float scale, ScalarType? dtype) -> Tensor");
+  define<dropout>(m, "dropout", "(Tensor x, float p, int seed, int offset) -> Tensor");
+  define<add_rms_norm>(m, "add_rms_norm",
          "(Tensor x, Tensor? residual, Tensor weight, float eps, float p, int seed, int offset) "
-         "-> (Tensor, Tensor)",
-         add_rms_norm);
-  define(m, "add_rms_norm_fp8",
+         "-> (Tensor, Tensor)");
+  define<add_rms_norm_fp8>(m, "add_rms_norm_fp8",
          "(Tensor x, Tensor? residual, Tensor weight, float eps, int group) "
-         "-> (Tensor, Tensor, Tensor)",
-         add_rms_norm_fp8);
-  define(m, "add_rms_norm_grad",
+         "-> (Tensor, Tensor, Tensor)");
+  define<add_rms_norm_grad>(m, "add_rms_norm_grad",
          "(Tensor grad_y, Tensor? grad_h, Tensor h, Tensor weight, float eps, float p, int seed, "
-         "int offset) -> (Tensor, Tensor, Tensor)",
-         add_rms_norm_grad);
-  define(m, "clipped_policy_loss",
-         "(" + kLossArgs + ", bool want_stats) -> (Tensor, Tensor, Tensor, Tensor)",
-         clipped_policy_loss);
-  define(m, "clipped_policy_loss_grad",
-         "(" + kLossArgs + ", Tensor stats, Tensor? row_weight) -> Tensor",
-         clipped_policy_loss_grad);
-  define(m, "clipped_policy_loss_with_grad",
-         "(" + kLossArgs + ", Tensor? row_weight) -> (Tensor, Tensor, Tensor, Tensor)",
-         clipped_policy_loss_with_grad);
+         "int offset) -> (Tensor, Tensor, Tensor)");
+  define<clipped_policy_loss>(m, "clipped_policy_loss",
+         "(" + kLossArgs + ", bool want_stats) -> (Tensor, Tensor, Tensor, Tensor)");
+  define<clipped_policy_loss_grad>(m, "clipped_policy_loss_grad",
+         "(" + kLossArgs + ", Tensor stats, Tensor? row_weight) -> Tensor");
+  define<clipped_policy_loss_with_grad>(m, "clipped_policy_loss_with_grad",
+         "(" + kLossArgs + ", Tensor? row_weight) -> (Tensor, Tensor, Tensor, Tensor)");
 }

@@ -13,7 +13,8 @@ caller's current HIP stream:
 The four that training uses are differentiable; their gradients are also functions of their own
 (``token_embedding_grad``, ``add_rms_norm_grad``, ``clipped_policy_loss_with_grad``; dropout is its
 own gradient) for a program that runs its backward pass by hand.  Every gradient is a function of
-its inputs alone, bit for bit: sums run in a fixed order.
+its inputs alone, bit for bit: sums run in a fixed order.  There are no second derivatives and no
+forward-mode ones, and none of the other functions: those raise.
 
 Elements are float32, bfloat16 or float16.  Sums and statistics are kept in float32, and a result
 is rounded once.  Tensors of rows (the last dimension) may be slices of wider ones as long as the
@@ -121,7 +122,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tens
     The mask is a function of (seed, offset, the element's row and column along the last
     dimension) and is formed again in the backward pass; give each use of a step its own offset.
     Elements that are dropped are 0 whatever x holds there.  Differentiable in x.  (A HIP graph
-    records seed and offset as they are: every replay drops the same elements.)"""
+    records seed and offset as they are: every replay drops the same elements.  So does every
+    example under torch.vmap, which is a call on that example with the same arguments.)"""
     seed, offset = _word(seed), _word(offset)
     if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, float(p), seed, offset)
@@ -174,7 +176,7 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
 
     scales: float32, x's shape with the last dimension 1 (group 0: one scale for a row) or
     ceil(dim / 128) (group 128: one for every 128 columns); a scale is the group's largest |y| /
-    448, at least 2^-126.  Not differentiable."""
+    448, at least 2^-126.  Not differentiable: a backward pass through its results raises."""
     q, scales, h = _NORM_FP8(x, residual, weight, eps, group)
     return q, scales, (x if residual is None else h)
 
