@@ -6,8 +6,10 @@ other's), looked up in one table; two kinds of layer alternate on the residual, 
 the cells and one over the channels, each behind a root-mean-square norm of the residual sum; the
 policy is one logit per cell, the value a mean over the cells.
 
-* ``evaluate_batch(features)`` (the protocol of ``MCTS``): the norms before the channel products
-  give them their input in 8 bits with a scale for every row, and so are those products' weights.
+* ``evaluator()`` has ``evaluate_batch(features)`` (the protocol of ``MCTS``): the norms before the
+  channel products give them their input in 8 bits with a scale for every row, and so are those
+  products' weights.  It holds the weights as they were when it was made; the network's own
+  ``evaluate_batch`` lays them out at every call.
 * ``train_step(...)``: dropout on every branch (fused into the norms), the clipped policy loss
   against the searches' policies over the legal cells, the table's gradient over sorted tokens.
 
@@ -24,6 +26,15 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import net_ops
+
+
+def position_tokens(features: torch.Tensor) -> torch.Tensor:
+    """int32 [positions, cells] of feature planes [positions, planes, board, board]: plane 0
+    holds the mover's stones, plane 1 the other's."""
+    own, other = features[:, 0].flatten(1), features[:, 1].flatten(1)
+    content = own + 2 * other
+    cell = torch.arange(content.shape[1], device=content.device)
+    return (3 * cell + content).to(torch.int32)
 
 
 class _Block(nn.Module):
@@ -62,21 +73,16 @@ class TokenPolicy(nn.Module):
             self.policy = nn.Linear(dim, 1)
             self.value = nn.Linear(dim, 1)
         self.steps = 0
-        self._serving = None
         self.to(device)
 
     # ---- training --------------------------------------------------------------------------
     def tokens(self, features: torch.Tensor) -> torch.Tensor:
-        """int32 [positions, cells] of feature planes [positions, planes, board, board]: plane 0
-        holds the mover's stones, plane 1 the other's."""
-        own, other = features[:, 0].flatten(1), features[:, 1].flatten(1)
-        content = own + 2 * other
-        cell = torch.arange(content.shape[1], device=content.device)
-        return (3 * cell + content).to(torch.int32)
+        """position_tokens(features)."""
+        return position_tokens(features)
 
     def forward(self, tokens: torch.Tensor):
         """(logits [positions, cells], values [positions]) for training; a new dropout mask for
-        every step and branch."""
+        every branch and every value of `steps`, which train_step counts."""
         p = self.p if self.training else 0.0
         use = self.steps * (2 * len(self.blocks) + 1)
         branch = net_ops.token_embedding(tokens, self.table, math.sqrt(self.dim))
@@ -110,45 +116,48 @@ class TokenPolicy(nn.Module):
         return dict(zip(("loss", "policy", "kl", "value"), said))
 
     # ---- serving ---------------------------------------------------------------------------
-    # The serving weights are laid out at the first use after the parameters may have changed:
-    # a training mode set, a state loaded, the module moved or converted.
-    def train(self, mode: bool = True):
-        self._serving = None
-        return super().train(mode)
+    def evaluator(self) -> "Evaluator":
+        """The network for serving, with its weights as they are now: make another one when they
+        have changed."""
+        return Evaluator(self)
 
-    def load_state_dict(self, *args, **kw):
-        self._serving = None
-        return super().load_state_dict(*args, **kw)
+    def serve(self, tokens: torch.Tensor):
+        """evaluator().serve(tokens)."""
+        return self.evaluator().serve(tokens)
 
-    def _apply(self, *args, **kw):
-        self._serving = None
-        return super()._apply(*args, **kw)
+    def evaluate_batch(self, features: torch.Tensor):
+        """evaluator().evaluate_batch(features)."""
+        return self.evaluator().evaluate_batch(features)
 
-    def _weights(self):
-        """The parameters as the evaluator uses them: bfloat16, the channel products' weights in
-        8 bits with a scale per output column."""
-        if self.training:  # (parameters may change at any time)
-            self.eval()
-        if self._serving is None:
-            bf = torch.bfloat16
-            blocks = []
-            for b in self.blocks:
-                w = b.up.weight.detach()
-                scale = (w.abs().amax(1, keepdim=True) / 448.0).clamp_(min=2.0**-126)
-                blocks.append((b.norm_cells.detach().to(bf), b.cells.weight.detach().to(bf),
-                               b.norm_channels.detach().to(bf),
-                               (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous(),
-                               b.down.weight.detach().to(bf)))
-            self._serving = (self.table.detach().to(bf), blocks, self.norm_out.detach().to(bf))
-        return self._serving
+
+class Evaluator:
+    """A TokenPolicy's weights laid out for serving, copies all: bfloat16, the channel products'
+    weights in 8 bits with a scale per output column, the heads in float32.  Without dropout,
+    whatever mode the network is in."""
+
+    @torch.no_grad()
+    def __init__(self, net: TokenPolicy):
+        def copy(p, dtype=torch.bfloat16):
+            return p.detach().to(dtype, copy=True)
+
+        self.input_channels, self.dim = net.input_channels, net.dim
+        self.table, self.norm_out = copy(net.table), copy(net.norm_out)
+        self.blocks = []
+        for b in net.blocks:
+            w = b.up.weight.detach().float()
+            scale = (w.abs().amax(1, keepdim=True) / 448.0).clamp_(min=2.0**-126)
+            self.blocks.append((copy(b.norm_cells), copy(b.cells.weight), copy(b.norm_channels),
+                                (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous(),
+                                copy(b.down.weight)))
+        self.heads = [(copy(h.weight, torch.float32), copy(h.bias, torch.float32))
+                      for h in (net.policy, net.value)]
 
     @torch.no_grad()
     def serve(self, tokens: torch.Tensor):
-        """forward without dropout, in bfloat16 and 8 bits."""
-        table, blocks, norm_out = self._weights()
-        branch, h = net_ops.token_embedding(tokens, table, math.sqrt(self.dim)), None
+        """(logits, values) as TokenPolicy.forward without dropout, in bfloat16 and 8 bits."""
+        branch, h = net_ops.token_embedding(tokens, self.table, math.sqrt(self.dim)), None
         b, c, d = branch.shape
-        for norm_cells, cells, norm_channels, up, up_scale, down in blocks:
+        for norm_cells, cells, norm_channels, up, up_scale, down in self.blocks:
             y, h = net_ops.add_rms_norm(branch, h, norm_cells)
             y = F.linear(y.transpose(1, 2).reshape(b * d, c), cells)
             y = y.view(b, d, c).transpose(1, 2).contiguous()
@@ -156,13 +165,15 @@ class TokenPolicy(nn.Module):
             y = torch._scaled_mm(q.view(b * c, d), up.t(), scale_a=scales.view(b * c, 1),
                                  scale_b=up_scale, out_dtype=torch.bfloat16)
             branch = F.linear(F.gelu(y), down).view(b, c, d)
-        y, _ = net_ops.add_rms_norm(branch, h, norm_out)
+        y, _ = net_ops.add_rms_norm(branch, h, self.norm_out)
         y = y.float()
-        return self.policy(y)[..., 0], torch.tanh(self.value(y.mean(1)))[:, 0]
+        policy, value = self.heads
+        return (F.linear(y, *policy)[..., 0],
+                torch.tanh(F.linear(y.mean(1), *value))[:, 0])
 
     def evaluate_batch(self, features: torch.Tensor):
         """(policies [positions, cells], values [positions]) of feature planes."""
-        logits, values = self.serve(self.tokens(features))
+        logits, values = self.serve(position_tokens(features))
         occupied = (features[:, 0] + features[:, 1]).flatten(1) > 0
         return torch.softmax(logits.masked_fill_(occupied, -math.inf), 1), values
 
@@ -181,7 +192,8 @@ def searched_positions(net: TokenPolicy, positions: int, simulations: int, stone
                         virtual_loss=3.0, game_type=GameType.GOMOKU, board_size=bs,
                         device="cuda", num_trees=positions, seed=seed,
                         max_tree_nodes=1024 + 2 * simulations * bs * bs)
-    policies = MCTS(config, net).search_batch(boards)
+    evaluator = net.evaluator()
+    policies = MCTS(config, evaluator).search_batch(boards)
     device = net.table.device
     flat = torch.from_numpy(np.ascontiguousarray(boards).reshape(positions, -1)).to(device)
     # player 1 moves on an even number of stones
@@ -193,7 +205,7 @@ def searched_positions(net: TokenPolicy, positions: int, simulations: int, stone
     g = torch.Generator(device=device).manual_seed(seed)
     actions = torch.multinomial(target, 1, generator=g)[:, 0]
     with torch.no_grad():
-        logits = net.serve(tokens)[0].masked_fill(~legal, -math.inf)
+        logits = evaluator.serve(tokens)[0].masked_fill(~legal, -math.inf)
         old = torch.log_softmax(logits, 1).gather(1, actions[:, None])[:, 0]
     return tokens, target, legal, actions, old
 
