@@ -31,10 +31,10 @@ from .. import net_ops
 def position_tokens(features: torch.Tensor) -> torch.Tensor:
     """int32 [positions, cells] of feature planes [positions, planes, board, board]: plane 0
     holds the mover's stones, plane 1 the other's."""
-    own, other = features[:, 0].flatten(1), features[:, 1].flatten(1)
-    content = own + 2 * other
-    cell = torch.arange(content.shape[1], device=content.device)
-    return (3 * cell + content).to(torch.int32)
+    # (in whole numbers: bfloat16 planes would round tokens above 256)
+    own, other = (features[:, k].flatten(1).to(torch.int32) for k in (0, 1))
+    cell = torch.arange(own.shape[1], device=own.device, dtype=torch.int32)
+    return 3 * cell + own + 2 * other
 
 
 class _Block(nn.Module):
