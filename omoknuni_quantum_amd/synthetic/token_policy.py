@@ -172,10 +172,12 @@ class Evaluator:
                 torch.tanh(F.linear(y.mean(1), *value))[:, 0])
 
     def evaluate_batch(self, features: torch.Tensor):
-        """(policies [positions, cells], values [positions]) of feature planes."""
+        """(policies [positions, cells], values [positions]) of feature planes.  The policy of a
+        full board is zero."""
         logits, values = self.serve(position_tokens(features))
         occupied = (features[:, 0] + features[:, 1]).flatten(1) > 0
-        return torch.softmax(logits.masked_fill_(occupied, -math.inf), 1), values
+        policies = torch.softmax(logits.masked_fill_(occupied, -math.inf), 1)
+        return policies.masked_fill_(occupied, 0.0), values  # (NaN where all are)
 
 
 def searched_positions(net: TokenPolicy, positions: int, simulations: int, stones: int,

@@ -97,3 +97,19 @@ def test_an_evaluator_keeps_its_weights(device):
         change(net)
         assert all(torch.equal(a, b) for a, b in zip(evaluator.evaluate_batch(f), first))
     assert not torch.equal(net.evaluate_batch(f)[0], first[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_policies_of_full_boards_are_zero(device, dtype):
+    """A row that the mask leaves nothing of has no policy, and the others theirs."""
+    f = planes(5, device, dtype)
+    f[1, 0], f[1, 1] = 1, 0
+    f[3, 0] = 1 - f[3, 1]
+    policies, values = network(device).evaluate_batch(f)
+    occupied = ((f[:, 0] + f[:, 1]) > 0).flatten(1)
+    full = torch.tensor([False, True, False, True, False], device=device)
+    assert torch.equal(occupied.all(1), full)
+    assert not bool(policies[occupied].any())
+    # 49 float32 terms
+    assert float((policies.double().sum(1) - (~full).double()).abs().max()) < 60 * 2.0**-24
+    assert bool(values.isfinite().all())
