@@ -167,7 +167,8 @@ int omq_clipped_policy_loss(const omq_policy_rows* r, float* loss, float* logp, 
 int omq_clipped_policy_loss_grad(const omq_policy_rows* r, const float* stats,
                                  const float* row_weight, void* grad, void* stream);
 
-/* Both at once, the logits read from memory once. */
+/* Both at once.  Rows of up to 16384 actions (8192 with a target) are read once, longer ones
+ * twice. */
 int omq_clipped_policy_loss_with_grad(const omq_policy_rows* r, const float* row_weight,
                                       float* loss, float* logp, float* kl, void* grad,
                                       void* workspace, int64_t workspace_bytes, void* stream);

@@ -597,7 +597,13 @@ __global__ __launch_bounds__(1024) void join_pieces_kernel(const Piece* __restri
 // average.  The work of a row of many tokens is not spread over workgroups here, so that more
 // tokens are sorted: 225 tokens of 675 rows and 128 columns take 5 us a call (15 sorted), 1000 of
 // 1083 rows 5 us (18), 1734 of 867 rows 5.5 us (24); but 2048 of two rows 43 us (17), 8000 of 1000
-// rows unevenly 91 us (24).
+// rows unevenly 91 us (24).  A workgroup has a wave's row at least, so that few rows are few
+// workgroups.  With 1024 columns, listed and sorted, us:
+//                  2 rows      16 rows     64 rows     675 rows
+//   256 tokens     13   14.5   6    15     5.3  14.5   5.3  17
+//   512 tokens     17   15.5   15   15     7    16     5.4  18
+//   1024 tokens    23   17     47   15.5   10   16     5.3  19
+// (The smallest board's table has 147 rows.)
 constexpr int kListedTokens = 2048, kHotRow = 64;
 
 bool use_list(int64_t tokens, int64_t vocab) {
@@ -723,10 +729,11 @@ bool grad_sizes_ok(int64_t tokens, int64_t vocab, int64_t dim) {
          dim >= 1 && dim <= OMQ_NET_MAX_DIM;
 }
 
-// One workgroup's sort is one launch, a pass of the radix sort two.  2048 tokens of two rows and
-// 1024 columns take 16.5 us a call with it (18.4 without; 17.4 with the larger one's registers);
-// 3000 of 50000 rows, whose radix sort has two passes, 24 us (28); but 4096 of 1000 rows, which it
-// has to pass twice and the radix sort once, 25.5 us (22.5).
+// One workgroup's sort is one launch, a pass of the radix sort two.  1100 tokens of 200 rows and
+// 1024 columns take 15.8 us a call with it (19 without; 16.8 with the larger one's registers); 3000
+// of 50000 rows and 256 columns, whose radix sort has two passes, 24.7 us (30.3); but 4096 of 1000
+// rows, which it has to pass twice and the radix sort once, 25.5 us (22.5), and 2048 of 400 rows,
+// the same, 21 us (20.2).
 bool use_small_sort(int64_t tokens, int passes) {
   return tokens <= (passes > 1 ? kSmallSort : kSmallSort / 2);
 }
@@ -741,8 +748,8 @@ GradPlan grad_plan(int64_t tokens, int64_t vocab, int64_t dim) {
   p.lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : dim <= 256 ? 32 : 64;
   p.col_tiles = (int)ceil_div(dim, 8 * p.lanes);
   // Pieces for 2048 waves, of 16 to 1024 items.  Fewer leave memory idle, more are more partial
-  // sums: 115200 tokens of 675 rows and 256 columns took 34 us, 38 with 1024 waves and 40 with
-  // 4096; 131071 of 65536 rows and 1024 columns 125, 135 and 129.
+  // sums: 115200 tokens of 675 rows and 256 columns take 32 us, 36 with 1024 waves and 38 with
+  // 4096; 131071 of 65536 rows and 1024 columns 116, 129 and 122.
   const int64_t items = tokens + vocab;
   const int64_t wanted = ceil_div(2048ll * (kWave / p.lanes), p.col_tiles);
   p.piece = ceil_div(items, wanted);

@@ -38,6 +38,9 @@ constexpr int block_of() {
   return kThreads <= kWave ? 256 : kThreads;
 }
 
+// v times the rounded inverse of the scale, not the quotient: a value on a tie of two 8-bit numbers
+// may go to either (1e-5 of the values of bfloat16 rows; the last bit of the norm's root moves
+// twice as many).
 __device__ inline uint2 to_fp8(F8 v, float inv) {
   v *= inv;
   uint2 r;

@@ -11,7 +11,7 @@
 //
 // Bound by memory, and for rows of a few hundred actions by the instructions of a row as well
 // (32768 rows of 362 bfloat16 with target and mask 31 us, 3.4 TB/s).  Measured with gradient: 4096
-// rows of 4672 36 us (4.7 TB/s), 4096 of 131072 without target 445 us (4.8 TB/s); without: 4096 of
+// rows of 4672 36 us (4.7 TB/s), 4096 of 131072 without target 437 us (4.9 TB/s); without: 4096 of
 // 4672 27 us (4.9 TB/s).  Three ways through a row:
 //   - short rows are held in registers: the base, the sums and the gradient come from one load;
 //   - a long row is read twice by its workgroup, for the sums and for the gradient, the second
@@ -35,6 +35,8 @@ struct Stats {
 
 __device__ inline Stats no_stats() { return Stats{-kInf, 0.0f, 0.0f, 0.0f}; }
 
+// e^x from one product and the instruction of 2^x: the product's rounding makes a relative error of
+// about |x| 2^-24 (4e-6 at -60, in a term of 1e-26 of the largest), and results below 2^-126 are 0.
 __device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // The base that the sums of a part with base m were formed about.
@@ -442,14 +444,15 @@ __global__ __launch_bounds__(block_of<kThreads>()) void loss_rows_kernel(
 
 // ---- long rows ------------------------------------------------------------------------------
 // Blocks that a thread has in flight: four of rows that are whole blocks (4096 rows of 131072
-// bfloat16 with gradient: 431 us, 442 with one), else one (4096 of 100003: 409 us, 479 with four;
-// 2018 of 87390 float32: 304 and 345 us: blocks at odd addresses take two lines each).
+// bfloat16 with gradient: 437 us, 453 with one; 2000 of 65536 float32: 231 and 267 us; but 1024 of
+// 20000 bfloat16: 24 and 17 us), else one (4096 of 100003: 402 us, 482 with four; 2018 of 87390
+// float32: 308 and 351 us: blocks at odd addresses take two lines each).
 template <bool kTarget, bool kWhole>
 constexpr int kInFlight = kWhole && !kTarget ? 4 : 1;
 
 // kAll: the blocks are whole and every action is legal, so that nothing is masked.  Long rows
 // without a mask are made of such blocks but for their end.  (4096 rows of 131072 bfloat16 with
-// gradient: the masks are a third of the instructions and 8 of 439 us.)
+// gradient: the masks are a third of the instructions and 7 of 444 us.)
 template <class T, bool kTarget, bool kWhole, bool kAll>
 __device__ inline F8 logits_of(const Block<T, kTarget>& b, const RowIn<T>& in, int col,
                                uint64_t ok) {
@@ -656,8 +659,9 @@ constexpr int64_t kRowActions = 16384, kRowActionsTarget = 8192;
 // 13 us cut; 128 rows of 131072 the same).
 constexpr int64_t kLongRows = 128, kWideActions = 65536;
 // A workgroup of 1024 threads for rows over kWideActions, so that the rows under way stay in the
-// last-level cache (4096 rows of 131072 bfloat16: 449 us, 484 with 512 threads), and where there
-// are fewer rows than compute units; else 512 (4096 rows of 32768: 113 us, 117 with 1024).
+// last-level cache (4096 rows of 131072 bfloat16: 437 us, 447 with 512 threads), and where there
+// are fewer rows than compute units (128 rows of 65536: 12 us, 13 with 512); else 512 (4096 rows of
+// 32768: 103 us, 128 with 1024).
 bool wide_row(int64_t rows, int64_t actions) { return actions > kWideActions || rows < 256; }
 
 template <bool kTarget, class F>

@@ -18,7 +18,8 @@ forward-mode ones, and none of the other functions: those raise.
 
 Elements are float32, bfloat16 or float16.  Sums and statistics are kept in float32, and a result
 is rounded once.  Tensors of rows (the last dimension) may be slices of wider ones as long as the
-rows' elements are adjacent and the rows equally far apart; other arguments must be contiguous.
+rows' elements are adjacent and the rows equally far apart; other arguments, and dropout's x, must
+be contiguous.
 There is no CPU implementation: tensors must be on a HIP device, and a missing library raises.
 """
 from __future__ import annotations
@@ -246,8 +247,9 @@ def clipped_policy_loss_with_grad(logits: torch.Tensor, actions: torch.Tensor,
                                   ref_logp: torch.Tensor | None = None,
                                   target: torch.Tensor | None = None,
                                   legal: torch.Tensor | None = None):
-    """(loss, logp, kl, grad): clipped_policy_loss and, from the same read of the logits, the
-    gradient by the logits of sum(row_weight * loss) (row_weight float32 [rows], None: ones), for
-    a program that goes on with ``logits.backward(grad)``."""
+    """(loss, logp, kl, grad): clipped_policy_loss and the gradient by the logits of
+    sum(row_weight * loss) (row_weight float32 [rows], None: ones), for a program that goes on with
+    ``logits.backward(grad)``.  One launch but for few very long rows; rows of up to 16384 actions
+    (8192 with a target) are read once."""
     return _LOSS_WITH_GRAD(logits, actions, advantages, old_logp, clip_low, clip_high, kl_coef,
                            ref_logp, target, legal, row_weight)
