@@ -118,7 +118,7 @@ class TokenPolicy(nn.Module):
     # ---- serving ---------------------------------------------------------------------------
     def evaluator(self) -> "Evaluator":
         """The network for serving, with its weights as they are now: make another one when they
-        have changed."""
+        have changed.  (Making one takes 0.2 ms, 32 positions of 15 x 15 cells 0.5 ms.)"""
         return Evaluator(self)
 
     def serve(self, tokens: torch.Tensor):

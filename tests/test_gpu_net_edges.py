@@ -182,3 +182,19 @@ def test_sampled_kl_that_overflows_has_an_infinite_gradient(device):
             assert bool((out[0] == math.inf).all()) and bool((out[2] == math.inf).all())
             assert bool((out[3][taken] == -math.inf).all())
             assert bool((out[3][~taken] == math.inf).all())
+
+
+# ---- a backward pass by hand ----------------------------------------------------------------
+def test_logits_that_go_on_backwards_with_the_gradient(device):
+    """logits.backward(grad) from rows that record gradients; the loss itself has no backward."""
+    g = gen(31)
+    x, w = randn(g, 20, 16).to(device), randn(g, 16, 225).to(device).requires_grad_()
+    act, f = torch.randint(0, 225, (20,), generator=g).to(device), randn(g, 20).to(device)
+    logits = x @ w
+    loss, logp, kl, grad = net_ops.clipped_policy_loss_with_grad(logits, act, f, f)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        loss.sum().backward(retain_graph=True)
+    logits.backward(grad)
+    with torch.no_grad():
+        want = x.t() @ net_ops.clipped_policy_loss_with_grad(x @ w, act, f, f)[3]
+    assert torch.equal(w.grad, want) and not w.grad.requires_grad
