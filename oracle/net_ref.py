@@ -86,8 +86,11 @@ def policy_loss(logits, actions, advantages, old_logp, clip_low, clip_high, kl_c
     n, a = z.shape
     ok = legal if legal is not None else torch.ones(n, a, dtype=torch.bool)
     ok = ok.bool()
-    live = (ok & (z > -math.inf)).any(1)
+    live = (ok & (z != -math.inf)).any(1)  # (a NaN is not left out)
     z = torch.where(ok, z, -math.inf)
+    # (about the largest logit, so that rows far from zero keep the bits of log-probabilities)
+    top = torch.where(z.isnan(), -math.inf, z).amax(1, keepdim=True)
+    z = z - torch.where(top.isfinite(), top, 0.0)
     lse = torch.where(live, torch.logsumexp(torch.where(live[:, None], z, 0.0), 1), 0.0)
     logq = torch.where(ok & live[:, None], z - lse[:, None], -math.inf)
     prob = torch.exp(logq)
@@ -120,5 +123,6 @@ def policy_loss(logits, actions, advantages, old_logp, clip_low, clip_high, kl_c
         loss = loss + kl_coef * kl
     grad = grad - slope[:, None] * prob
     grad[rows, at] += torch.where(taken, slope, 0.0)
+    grad = torch.where(ok, grad, 0.0)  # (whatever a row of NaN holds)
     return {"loss": loss, "logp": logp, "kl": kl, "ratio": ratio, "grad": grad, "taken": taken,
             "prob": prob, "slope": slope}

@@ -198,3 +198,58 @@ def test_logits_that_go_on_backwards_with_the_gradient(device):
     with torch.no_grad():
         want = x.t() @ net_ops.clipped_policy_loss_with_grad(x @ w, act, f, f)[3]
     assert torch.equal(w.grad, want) and not w.grad.requires_grad
+
+
+# ---- logits at the type's lowest value ------------------------------------------------------
+@pytest.mark.parametrize("cols", [49, 600, 4672, 16_384, 20_000, 80_000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kl", ["none", "target"])
+def test_logits_masked_with_the_lowest_value(device, cols, dtype, kl):
+    """By the caller, in part of a row (those actions have probability 0) or in all of it (all
+    have the same)."""
+    rows = 12
+    d = loss_inputs(rows, cols, dtype, kl, False, cols + 1)
+    low = torch.finfo(dtype).min
+    away = torch.rand(rows, cols, generator=gen(cols)) < 0.5
+    away[0::4] = True
+    away[1::4] = False
+    away[1::4, :min(cols - 9, 512)] = True
+    d["z"][away] = low
+    inside = (d["act"] >= 0) & (d["act"] < cols)
+    for i in range(rows):  # an action that can be taken
+        if inside[i] and i % 4:
+            d["act"][i] = int((~away[i]).nonzero()[i % 5])
+    if kl == "target":
+        d["target"][away & (torch.arange(rows) % 4 != 0)[:, None]] = 0.0
+    top = torch.where(away.all(1), math.log(cols), 20.0 + math.log(cols))
+    ref = net_ref.policy_loss(d["z"], d["act"], d["adv"], torch.zeros(rows), 0.2, 0.3, 0.0)
+    d["old"] = (ref["logp"] + randn(gen(3), rows, scale=0.1)).float()
+    dev = {k: v.to(device) for k, v in d.items() if v is not None}
+    coef = 1.0 if kl == "target" else 0.0
+    want = net_ref.policy_loss(d["z"], d["act"], d["adv"], d["old"], 0.2, 0.3, coef,
+                               target=d.get("target"))
+    args = dict(clip_low=0.2, clip_high=0.3, kl_coef=coef, target=dev.get("target"), legal=None)
+    out = net_ops.clipped_policy_loss_with_grad(dev["z"], dev["act"], dev["adv"], dev["old"],
+                                                dev["weight"], **args)
+    # sums of at most 800 terms in a row, about the largest logit
+    e_logp = 800 * u * (top + 1.0)
+    within(out[1], want["logp"], e_logp)
+    if kl == "target":
+        within(out[2], want["kl"], 2 * e_logp * (1.0 + d["target"].double().sum(1)))
+    x = dev["z"].clone().requires_grad_()
+    two = net_ops.clipped_policy_loss(x, dev["act"], dev["adv"], dev["old"], **args)
+    (two[0] * dev["weight"]).sum().backward()
+    # rows clear of the clipping's bounds, where the gradient jumps
+    e_ratio = want["ratio"] * (2 * e_logp + 4 * u)
+    edge = torch.minimum((want["ratio"] - 0.8).abs(), (want["ratio"] - 1.3).abs())
+    sure = edge > 2 * e_ratio + 1e-9
+    assert float(sure.double().mean()) > 0.7
+    e_slope = d["adv"].double().abs() * e_ratio
+    bound = want["prob"] * ((want["slope"].abs() + coef) * 3 * e_logp + e_slope)[:, None]
+    bound[torch.arange(rows), d["act"].clamp(0, cols - 1)] += e_slope
+    if kl == "target":
+        bound = bound + 4 * u * d["target"].double()
+    w = d["weight"].double()[:, None]
+    bound = w * (bound + 8 * u * want["grad"].abs())
+    for grad in (out[3], x.grad):
+        within(grad[sure.to(device)], (want["grad"] * w)[sure], bound[sure])

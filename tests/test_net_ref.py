@@ -108,3 +108,20 @@ def test_sampled_kl_of_an_action_without_weight_is_infinite(coef):
     assert float(got["loss"][0]) == (math.inf if coef else 0.0)
     if not coef:
         assert not bool(got["grad"].any())
+
+
+def test_loss_definition_far_from_zero_and_of_nan():
+    """Logits at the type's lowest value keep the bits of their log-probabilities, NaN among the
+    legal logits reaches the results, and illegal actions have gradient 0 all the same."""
+    low = torch.finfo(torch.float32).min
+    z = torch.tensor([[low] * 4, [math.nan] * 4, [math.nan, 1.0, 2.0, 3.0]])
+    legal = torch.tensor([[True] * 4, [True] * 3 + [False], [True, True, False, True]])
+    f = torch.ones(3)
+    got = net_ref.policy_loss(z, torch.tensor([2, 1, 1]), f, -math.log(4.0) * f, 0.2, 0.2, 0.0,
+                              legal=legal)
+    assert float(got["logp"][0]) == pytest.approx(-math.log(4.0), rel=1e-12)
+    assert got["grad"][0].tolist() == pytest.approx([0.25, 0.25, -0.75, 0.25], rel=1e-6)
+    for row in (1, 2):
+        assert math.isnan(got["logp"][row]) and math.isnan(got["loss"][row])
+        assert torch.equal(got["grad"][row].isnan(), legal[row])
+        assert not bool(got["grad"][row][~legal[row]].any())
