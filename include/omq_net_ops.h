@@ -133,7 +133,9 @@ int omq_add_rms_norm_grad(const void* grad_y, int64_t grad_y_stride, const void*
  * logit is above -infinity has loss, logp, kl and gradient 0.  Logits and targets of illegal
  * actions are never used, whatever they hold; a target that is not positive adds nothing whatever
  * its logq.  A row that adds nothing to the loss (padding) has gradient 0 whatever its logits
- * hold; elsewhere a NaN among the legal logits reaches the row's results. */
+ * hold; elsewhere a NaN among the legal logits reaches the row's results.  A legal action whose
+ * logit is -infinity has logp -infinity when it is taken, and a sampled kl of +infinity; where
+ * kl_coef is 0 the kl reaches neither loss nor gradient, whatever it is. */
 typedef struct omq_policy_rows {
   int64_t rows;
   int64_t actions;        /* columns */

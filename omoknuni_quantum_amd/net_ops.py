@@ -231,6 +231,7 @@ def clipped_policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages:
     actions int32/int64 [rows]; advantages, old_logp, ref_logp float32 [rows]; target float32
     [rows, actions], not together with ref_logp.  A row whose action is outside [0, actions) or
     not legal has logp 0 and only the target's kl; a row without a legal action has 0 throughout.
+    A kl_coef of 0 leaves the kl out of loss and gradient, whatever it is (it may be infinite).
     What illegal actions' logits and targets hold is never used.  Differentiable in logits through
     loss; logp and kl carry no gradient."""
     if logits.requires_grad and torch.is_grad_enabled():
