@@ -1,8 +1,10 @@
 /*
  * omq_net_ops.h -- C ABI of the MI355X (gfx950) operators of a policy network over board tokens
  * (libomq_net_ops.so): the token embedding and its gradient, the root-mean-square norm of a
- * residual sum with dropout, its 8-bit output and its gradients, dropout, and the clipped policy
- * loss over legal actions with its gradient.
+ * residual sum with dropout, its 8-bit output and its gradients, dropout, the clipped policy
+ * loss over legal actions with its gradient, the norm of queries and keys with the rotation by
+ * their positions and its gradients, attention and its gradients, and the log-probabilities of
+ * given tokens with the entropy, the best alternatives and their gradient.
  *
  * Conventions, those of omq_tree_ops.h: every array is a DEVICE pointer owned by the caller;
  * an entry point launches on the HIP stream it is given and returns without synchronising, keeps
@@ -25,7 +27,7 @@
 extern "C" {
 #endif
 
-#define OMQ_NET_ABI_VERSION 1
+#define OMQ_NET_ABI_VERSION 2
 
 #define OMQ_NET_OK 0
 #define OMQ_NET_E_ARG (-1)    /* invalid argument (size, type, null pointer, workspace) */
@@ -44,6 +46,10 @@ extern "C" {
 #define OMQ_NET_MAX_DIM (1 << 20)     /* columns of an embedding row, of a dropout row */
 #define OMQ_NET_MAX_ACTIONS (1 << 30) /* columns of a policy loss's row */
 #define OMQ_NET_MAX_COUNT 2147483647  /* rows, tokens, vocabulary */
+#define OMQ_NET_MAX_ROTARY_DIM 256    /* columns of a rotated head */
+#define OMQ_NET_MAX_AXES 4            /* axes of its positions */
+#define OMQ_NET_MAX_HEAD_DIM 128      /* columns of a head of the attention */
+#define OMQ_NET_MAX_TOP 32            /* alternatives of a row */
 
 int omq_net_abi_version(void);
 const char* omq_net_last_error(void);
@@ -174,6 +180,133 @@ int omq_clipped_policy_loss_grad(const omq_policy_rows* r, const float* stats,
 int omq_clipped_policy_loss_with_grad(const omq_policy_rows* r, const float* row_weight,
                                       float* loss, float* logp, float* kl, void* grad,
                                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Heads of queries and keys, normed each over its columns and rotated by the token's position:
+ *   n = x / sqrt(mean(x^2) + eps) * weight       (n = x where there are no weights)
+ *   out: pair j of the first 2 * pairs columns of n, (a, b), becomes
+ *        (a cos t - b sin t, b cos t + a sin t),  t = position[axis of j] * frequencies[j];
+ *        the columns behind them stay.
+ * Pair j is the columns (j, j + pairs), or (2j, 2j + 1) with `interleaved`.  Axis a holds the pairs
+ * from section_end[a-1] (0 for the first) to section_end[a]; the last section ends at `pairs`.
+ * The angle is formed in 64 bits and reduced to one turn before it is rounded.
+ *   q, k        [tokens, heads, dim] of dtype; a token's heads and the tokens at their strides
+ *   weights     [dim] of weight_dtype (dtype or OMQ_NET_F32), both or neither
+ *   positions   int32 or int64 [position_rows, axes]; token i has row i % position_rows
+ *   frequencies float64 [pairs], radians per unit of the position */
+typedef struct omq_rotary {
+  int64_t tokens, position_rows;
+  const void *q, *k;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  const void *q_weight, *k_weight;
+  const void* positions;
+  const double* frequencies;
+  int32_t q_heads, k_heads, dim, pairs, axes;
+  int32_t section_end[OMQ_NET_MAX_AXES];
+  int32_t positions_are_64, interleaved, dtype, weight_dtype;
+  float eps;
+} omq_rotary;
+
+/* q_out, k_out: [tokens, heads, dim] of dtype, contiguous. */
+int omq_head_norm_rotary(const omq_rotary* r, void* q_out, void* k_out, void* stream);
+
+/* Bytes of workspace of omq_head_norm_rotary_grad; negative for what it refuses. */
+int64_t omq_head_norm_rotary_grad_workspace(const omq_rotary* r);
+
+/* Gradients from the same q and k and the gradients of the outputs (contiguous):
+ *   grad_q, grad_k              [tokens, heads, dim] of dtype, contiguous
+ *   grad_q_weight, grad_k_weight  [dim] of weight_dtype; NULL where there are no weights */
+int omq_head_norm_rotary_grad(const omq_rotary* r, const void* grad_q_out, const void* grad_k_out,
+                              void* grad_q, void* grad_k, void* grad_q_weight,
+                              void* grad_k_weight, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+/* Attention of sequences: with the query i and the key j of a sequence of lq queries and lk keys,
+ *   out_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  lse_i = log sum_j exp(scale q_i.k_j)
+ * over the keys that i sees: all, or j <= i + lk - lq with `causal` (the last query sees every
+ * key).  A query that sees none has out 0 and lse -infinity, and so have rows of no sequence.
+ * Query head h attends to key head h / (q_heads / k_heads).
+ *
+ * Either a batch (q_starts NULL): sequence s has the queries q + s * q_seq_stride, q_len of them,
+ * and room for k_len keys at k + s * k_seq_stride.  Or packed (q_starts and k_starts given, int32
+ * [sequences + 1], not falling): sequence s has the rows q_starts[s] to q_starts[s + 1] of q and
+ * k_starts[s] to k_starts[s + 1] of k; q_len and k_len are the rows of all.  k_lengths (int32
+ * [sequences] or NULL) gives how many of a sequence's keys are in use, from the first.  Starts
+ * and lengths out of range are cut to the range; what rows behind a sequence's keys hold is never
+ * used.
+ *   q       rows of [q_heads, dim], at q_row_stride; its heads at q_head_stride; k, v alike
+ *   out     [rows of q, q_heads, dim], contiguous
+ *   lse     float32 [rows of q, q_heads], contiguous
+ * Products are formed from the elements' type and summed in float32; p is rounded to the elements'
+ * type before it multiplies v, as are the gradients of the scores before they multiply k and q. */
+typedef struct omq_attention_args {
+  int64_t sequences, q_len, k_len;
+  const void *q, *k, *v;
+  int64_t q_seq_stride, q_row_stride, q_head_stride;
+  int64_t k_seq_stride, k_row_stride, k_head_stride;
+  int64_t v_seq_stride, v_row_stride, v_head_stride;
+  const int32_t *q_starts, *k_starts, *k_lengths;
+  int32_t q_heads, k_heads, dim, dtype, causal;
+  float scale; /* finite, above 0 */
+} omq_attention_args;
+
+/* Bytes of workspace of omq_attention_forward; negative for what it refuses. */
+int64_t omq_attention_forward_workspace(const omq_attention_args* a);
+
+/* lse may be NULL when it is not wanted. */
+int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of omq_attention_grad; negative for what it refuses. */
+int64_t omq_attention_grad_workspace(const omq_attention_args* a);
+
+/* Gradients of sum(grad_out * out) from the forward pass's out and lse.
+ *   grad_out, out, grad_q  as out above
+ *   grad_k, grad_v         [rows of k (all of them), k_heads, dim], contiguous; 0 for rows of no
+ *                          sequence and behind a sequence's keys */
+int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const void* out,
+                       const float* lse, void* grad_q, void* grad_k, void* grad_v,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* What a policy says of given tokens.  With logq the log-softmax of a row over its legal tokens L:
+ *   logp     = logq[token]; 0 for a token outside [0, vocab) or not legal
+ *   entropy  = -sum over L of e^logq logq
+ *   top      the `top` most probable tokens of L, by falling logit and rising index among equals:
+ *            their logq and their indices; -infinity and -1 where L has fewer of probability
+ *            above 0
+ * A row without a legal token whose logit is above -infinity has logp and entropy 0 and no
+ * alternatives.  What the logits of other tokens hold is never used.  A NaN or +infinity among the
+ * legal logits makes the row's logp (of a legal token), entropy and top_logp NaN, its alternatives
+ * being those of its other logits (a NaN is never one).
+ *   logits  [rows, vocab] of dtype, logits_stride apart
+ *   legal   [rows, vocab], non-zero = legal, legal_stride apart; NULL: all are
+ *   tokens  int32 or int64 [rows] */
+typedef struct omq_logprob_rows {
+  int64_t rows, vocab;
+  const void* logits;
+  int64_t logits_stride;
+  const uint8_t* legal;
+  int64_t legal_stride;
+  const void* tokens;
+  int32_t dtype, tokens_are_64;
+} omq_logprob_rows;
+
+/* logp, entropy: float32 [rows].  top_logp float32, top_tokens int64 [rows, top] (0 <= top <=
+ * OMQ_NET_MAX_TOP; NULL for 0).  stats: float32 [rows, OMQ_NET_STATS] on a 16-byte boundary for
+ * omq_token_logprobs_grad, or NULL. */
+int omq_token_logprobs(const omq_logprob_rows* r, int32_t top, float* logp, float* entropy,
+                       float* top_logp, int64_t* top_tokens, float* stats, void* stream);
+
+/* grad [rows, vocab] of the logits' type, contiguous: the gradient of sum(logp_weight * logp +
+ * entropy_weight * entropy); 0 at tokens that are not legal, and in a row whose two weights are 0.
+ * Weights float32 [rows]; NULL: 0.  stats: from omq_token_logprobs on the same rows. */
+int omq_token_logprobs_grad(const omq_logprob_rows* r, const float* stats,
+                            const float* logp_weight, const float* entropy_weight, void* grad,
+                            void* stream);
+
+/* Both at once; rows of up to 16384 tokens are read once. */
+int omq_token_logprobs_with_grad(const omq_logprob_rows* r, const float* logp_weight,
+                                 const float* entropy_weight, float* logp, float* entropy,
+                                 void* grad, void* stream);
 
 #ifdef __cplusplus
 }

@@ -141,7 +141,7 @@ def edges_workspace_ints(num_nodes: int) -> int:
 
 # ---- libomq_net_ops.so (include/omq_net_ops.h) ----------------------------------------------
 NET_LIB_PATH = os.path.join(_HERE, "libomq_net_ops.so")
-NET_ABI_VERSION = 1
+NET_ABI_VERSION = 2
 OMQ_NET_F32, OMQ_NET_BF16, OMQ_NET_F16 = 0, 1, 2
 _i64, _u64, _f32, _f64, _int = (ctypes.c_int64, ctypes.c_uint64, ctypes.c_float, ctypes.c_double,
                                 ctypes.c_int)
@@ -157,7 +157,39 @@ class OmqPolicyRows(ctypes.Structure):
     ]
 
 
+class OmqRotary(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("position_rows", _i64), ("q", _p), ("k", _p),
+        ("q_token_stride", _i64), ("q_head_stride", _i64), ("k_token_stride", _i64),
+        ("k_head_stride", _i64), ("q_weight", _p), ("k_weight", _p), ("positions", _p),
+        ("frequencies", _p), ("q_heads", _i32), ("k_heads", _i32), ("dim", _i32), ("pairs", _i32),
+        ("axes", _i32), ("section_end", _i32 * 4), ("positions_are_64", _i32),
+        ("interleaved", _i32), ("dtype", _i32), ("weight_dtype", _i32), ("eps", _f32),
+    ]
+
+
+class OmqAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("sequences", _i64), ("q_len", _i64), ("k_len", _i64), ("q", _p), ("k", _p), ("v", _p),
+        ("q_seq_stride", _i64), ("q_row_stride", _i64), ("q_head_stride", _i64),
+        ("k_seq_stride", _i64), ("k_row_stride", _i64), ("k_head_stride", _i64),
+        ("v_seq_stride", _i64), ("v_row_stride", _i64), ("v_head_stride", _i64),
+        ("q_starts", _p), ("k_starts", _p), ("k_lengths", _p), ("q_heads", _i32),
+        ("k_heads", _i32), ("dim", _i32), ("dtype", _i32), ("causal", _i32), ("scale", _f32),
+    ]
+
+
+class OmqLogprobRows(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("vocab", _i64), ("logits", _p), ("logits_stride", _i64), ("legal", _p),
+        ("legal_stride", _i64), ("tokens", _p), ("dtype", _i32), ("tokens_are_64", _i32),
+    ]
+
+
 _RP = ctypes.POINTER(OmqPolicyRows)
+_HP = ctypes.POINTER(OmqRotary)
+_AP = ctypes.POINTER(OmqAttentionArgs)
+_LP = ctypes.POINTER(OmqLogprobRows)
 NET_SIGNATURES = {
     "omq_net_abi_version": (_int, []),
     "omq_net_last_error": (ctypes.c_char_p, []),
@@ -177,6 +209,16 @@ NET_SIGNATURES = {
     "omq_clipped_policy_loss": (_int, [_RP, _p, _p, _p, _p, _p, _i64, _p]),
     "omq_clipped_policy_loss_grad": (_int, [_RP, _p, _p, _p, _p]),
     "omq_clipped_policy_loss_with_grad": (_int, [_RP, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "omq_head_norm_rotary": (_int, [_HP, _p, _p, _p]),
+    "omq_head_norm_rotary_grad_workspace": (_i64, [_HP]),
+    "omq_head_norm_rotary_grad": (_int, [_HP, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "omq_attention_forward_workspace": (_i64, [_AP]),
+    "omq_attention_forward": (_int, [_AP, _p, _p, _p, _i64, _p]),
+    "omq_attention_grad_workspace": (_i64, [_AP]),
+    "omq_attention_grad": (_int, [_AP, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "omq_token_logprobs": (_int, [_LP, _i32, _p, _p, _p, _p, _p, _p]),
+    "omq_token_logprobs_grad": (_int, [_LP, _p, _p, _p, _p, _p]),
+    "omq_token_logprobs_with_grad": (_int, [_LP, _p, _p, _p, _p, _p, _p]),
 }
 
 

@@ -1,0 +1,183 @@
+// Attention with grouped heads over batches, packed sequences and caches (gfx950).
+//
+// One pass over the keys with the running maximum m and sum l of a row's softmax:
+//   s_ij = scale q_i.k_j;  m' = max(m, s);  l' = e^(m - m') l + sum e^(s - m');
+//   o' = e^(m - m') o + sum e^(s - m') v;   out = o / l,  lse = m + log l
+// A workgroup has 128 rows (queries x heads of a group), a wave 32 of them, in registers: queries,
+// the sums of the output and the softmax's m and l.  64 keys and values at a time pass through
+// LDS.  Probabilities are at most 1 and are rounded to the elements' type for the second product:
+// relative to a row's output that is half a step of the type at most, as the output's own
+// rounding; m and l are float32.
+#include "net_attention.h"
+
+namespace omq_net {
+namespace {
+
+template <class T, int kDim>
+__global__ __launch_bounds__(kWaves* kWave) void attention_kernel(AttentionArgs args) {
+  using L = Tile<T, kDim>;
+  __shared__ __attribute__((aligned(16))) char keys[L::kBytes];
+  __shared__ __attribute__((aligned(16))) char values[L::kBytes];
+  __shared__ int bad[2];
+  const omq_attention_args& a = args.a;
+  const int64_t block = block_index();
+  const int64_t slot = block / a.k_heads;
+  if (slot >= args.slots) return;
+  const int kv = (int)(block % a.k_heads), group = args.group;
+  int64_t tile;
+  Sequence q;
+  if (a.q_starts) {
+    q = sequence_of(args, find_piece(a.q_starts, a.sequences, a.q_len, group, kTileRows, slot,
+                                     &tile));
+  } else {
+    q = sequence_of(args, slot / args.batch_tiles);
+    tile = slot % args.batch_tiles;
+  }
+  const int64_t rows = (int64_t)q.lq * group, r0 = tile * kTileRows;
+  if (tile < 0 || r0 >= rows) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+
+  // this lane's row; lanes behind the last one do it again and store nothing
+  const int64_t mine = r0 + kWaveRows * wave + (lane & 31);
+  const bool there = mine < rows;
+  const int64_t row = there ? mine : rows - 1;
+  const int query = (int)(row / group), head = kv * group + (int)(row % group);
+  const int shift = q.lk - q.lq;
+  const int limit = a.causal ? cut(query + shift + 1, 0, q.lk) : q.lk;  // the keys that it sees
+  const int first_query = (int)(r0 / group);
+  const int64_t last_row = r0 + kTileRows < rows ? r0 + kTileRows - 1 : rows - 1;
+  const int most = a.causal ? cut((int)(last_row / group) + shift + 1, 0, q.lk) : q.lk;
+  const int least = a.causal ? cut(first_query + shift + 1, 0, q.lk) : q.lk;
+
+  typename L::Frag qf[L::kChunks];
+  load_row<T, kDim>(qf, static_cast<const T*>(a.q) + q.q_at + query * a.q_row_stride +
+                            head * a.q_head_stride, a.dim);
+  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + kv * a.k_head_stride;
+  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + kv * a.v_head_stride;
+
+  F16 o[kDim / 32] = {};
+  float m = -kInf32, l = 0.0f;  // l: over this half's keys
+  for (int k0 = 0, turn = 0; k0 < most; k0 += kTileKeys, turn ^= 1) {
+    const int left = q.lk - k0;
+    __syncthreads();
+    if (threadIdx.x == 0) bad[turn ^ 1] = 0;
+    load_tile<T, kDim>(keys, left, a.dim,
+                       [&](int i) { return k_rows + (int64_t)(k0 + i) * a.k_row_stride; });
+    const bool found = load_tile<T, kDim>(
+        values, left, a.dim, [&](int i) { return v_rows + (int64_t)(k0 + i) * a.v_row_stride; });
+    if (found) bad[turn] = 1;
+    __syncthreads();
+    const bool cuts = k0 + kTileKeys > least;  // some row does not see all of the tile
+    const bool careful = cuts && bad[turn];
+    F16 s[2];
+    float top = -kInf32;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = F16{};
+#pragma unroll
+      for (int c = 0; c < L::kChunks; ++c) s[b] = mma(L::row(keys, 32 * b, c), qf[c], s[b]);
+      if (cuts) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * b + result_row(r) >= limit) s[b][r] = -kInf32;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    }
+    top = fmaxf(fmaxf(top, other_half(top)), m);
+    const float base = top == -kInf32 ? 0.0f : top;
+    const float keep = __builtin_amdgcn_exp2f((m - base) * args.score_scale);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = __builtin_amdgcn_exp2f((s[b][r] - base) * args.score_scale);
+        l += s[b][r];
+      }
+      F16 seen = {};
+      if (careful) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) seen[r] = k0 + 32 * b + result_row(r) < limit ? 1.0f : 0.0f;
+      }
+      add_columns<T, kDim>(o, values, 32 * b, s[b], seen, careful);
+    }
+  }
+  l += other_half(l);
+  if (!there) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t out_row = (q.q_first + query) * a.q_heads + head;
+  store_column<T, kDim>(static_cast<T*>(args.out) + out_row * a.dim, o, inv, a.dim);
+  if (args.lse && lane < 32)
+    args.lse[out_row] =
+        l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+}
+
+}  // namespace
+
+int check_attention(const char* name, const omq_attention_args* a) {
+  if (!a) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  if (!dtype_known(a->dtype)) return net_fail(OMQ_NET_E_ARG, "%s: heads of type %d", name, a->dtype);
+  if (a->sequences < 0 || a->q_len < 0 || a->k_len < 0 || a->q_heads < 1 || a->k_heads < 1 ||
+      a->dim < 1 || a->q_heads % a->k_heads)
+    return net_fail(OMQ_NET_E_ARG,
+                    "%s: sequences %lld, queries %lld, keys %lld, heads %d over %d, dim %d", name,
+                    (long long)a->sequences, (long long)a->q_len, (long long)a->k_len, a->q_heads,
+                    a->k_heads, a->dim);
+  const int64_t n = a->q_starts ? 1 : a->sequences;
+  const int64_t most = OMQ_NET_MAX_COUNT;
+  if (a->dim > OMQ_NET_MAX_HEAD_DIM || a->sequences > most || a->q_len > most || a->k_len > most ||
+      a->q_len * a->q_heads > most || a->k_len * a->q_heads > most ||
+      (n > 0 && (a->q_len * a->q_heads > most / n || a->k_len * a->q_heads > most / n)))
+    return net_fail(OMQ_NET_E_LIMIT,
+                    "%s: sequences %lld of %lld queries and %lld keys, %d heads (rows of heads at "
+                    "most %d), dim %d (at most %d)",
+                    name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len,
+                    a->q_heads, OMQ_NET_MAX_COUNT, a->dim, OMQ_NET_MAX_HEAD_DIM);
+  if (!(a->scale > 0.0f && a->scale < kInf32))
+    return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be finite and above 0", name, a->scale);
+  if (!a->q_starts != !a->k_starts)
+    return net_fail(OMQ_NET_E_ARG, "%s: starts of queries and keys, or of neither", name);
+  if (a->q_seq_stride < 0 || a->q_row_stride < 0 || a->q_head_stride < 0 || a->k_seq_stride < 0 ||
+      a->k_row_stride < 0 || a->k_head_stride < 0 || a->v_seq_stride < 0 || a->v_row_stride < 0 ||
+      a->v_head_stride < 0)
+    return net_fail(OMQ_NET_E_ARG, "%s: negative stride", name);
+  const bool queries = a->q_len > 0 && n > 0, keys = a->k_len > 0 && n > 0;
+  if ((queries && !a->q) || (keys && (!a->k || !a->v)))
+    return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  return OMQ_NET_OK;
+}
+
+}  // namespace omq_net
+
+using namespace omq_net;
+
+extern "C" {
+
+int64_t omq_attention_forward_workspace(const omq_attention_args* a) {
+  return check_attention("omq_attention_forward_workspace", a);
+}
+
+int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  const char* name = "omq_attention_forward";
+  if (int rc = check_attention(name, a)) return rc;
+  if (a->q_len == 0 || (a->sequences == 0 && !a->q_starts)) return OMQ_NET_OK;
+  if (!out) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
+  (void)workspace, (void)workspace_bytes;
+  AttentionArgs args = attention_layout(*a);
+  tiles_of(&args, a->q_len, args.group, kTileRows);
+  args.out = out, args.lse = lse;
+  const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
+  with_head(a->dtype, a->dim, [&](auto t, auto dim) {
+    attention_kernel<decltype(t), dim.value>
+        <<<grid, kWaves * kWave, 0, (hipStream_t)stream>>>(args);
+  });
+  return net_status(name);
+}
+
+}  // extern "C"

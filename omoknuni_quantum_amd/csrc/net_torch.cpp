@@ -6,6 +6,9 @@
 //   omq_net::add_rms_norm, omq_net::add_rms_norm_fp8, omq_net::add_rms_norm_grad
 //   omq_net::dropout
 //   omq_net::clipped_policy_loss, omq_net::clipped_policy_loss_grad, omq_net::clipped_policy_loss_with_grad
+//   omq_net::head_norm_rotary, omq_net::head_norm_rotary_grad
+//   omq_net::attention, omq_net::attention_grad
+//   omq_net::token_logprobs, omq_net::token_logprobs_grad, omq_net::token_logprobs_with_grad
 //
 // Tensors must be on one HIP device; host tensors are refused (there is no CPU implementation).
 // On meta tensors the operators give the shapes only.
@@ -20,7 +23,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -436,6 +441,346 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> clipped_policy_loss_w
   return {loss, logp, kl, grad};
 }
 
+// ---- norm and rotation of heads -------------------------------------------------------------
+// The strides of a tensor [..., heads, dim] as tokens of heads: the elements of a head must be
+// adjacent and the leading dimensions one run of equally spaced tokens.
+std::pair<int64_t, int64_t> token_strides(const char* name, const char* arg, const at::Tensor& t) {
+  int64_t stride = -1, expected = 0;
+  bool ok = t.size(-1) == 1 || t.stride(-1) == 1;
+  for (int64_t i = t.dim() - 3; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (stride < 0)
+      stride = t.stride(i);
+    else
+      ok = ok && t.stride(i) == expected;
+    expected = t.stride(i) * t.size(i);
+  }
+  TORCH_CHECK(ok || t.numel() == 0, "omq_net::", name, ": the heads of ", arg,
+              " must have adjacent elements and its tokens equal distances (use .contiguous())");
+  return {stride < 0 ? 0 : stride, t.stride(-2)};
+}
+
+omq_rotary rotary_args(const char* name, const at::Tensor& q, const at::Tensor& k,
+                       const at::Tensor& positions, const at::Tensor& frequencies,
+                       const OptTensor& q_weight, const OptTensor& k_weight, double eps,
+                       at::IntArrayRef sections, bool interleaved) {
+  const at::Tensor *qw = get(q_weight), *kw = get(k_weight);
+  const c10::Device dev = common_device(name, {&q, &k, &positions, &frequencies, qw, kw});
+  omq_rotary r{};
+  TORCH_CHECK(q.dim() >= 2 && k.dim() == q.dim() &&
+                  q.sizes().slice(0, q.dim() - 2) == k.sizes().slice(0, k.dim() - 2) &&
+                  q.size(-1) == k.size(-1) && q.size(-1) >= 1 && q.size(-2) >= 1 && k.size(-2) >= 1,
+              "omq_net::", name, ": q and k must be [..., heads, dim] of the same tokens and dim, not ",
+              q.sizes(), " and ", k.sizes());
+  TORCH_CHECK(q.scalar_type() == k.scalar_type(), "omq_net::", name, ": q and k must be of one type");
+  r.dtype = type_of(name, "q", q);
+  r.dim = (int)std::min<int64_t>(q.size(-1), INT32_MAX);
+  r.q_heads = (int)std::min<int64_t>(q.size(-2), INT32_MAX);
+  r.k_heads = (int)std::min<int64_t>(k.size(-2), INT32_MAX);
+  r.tokens = 1;
+  for (int64_t i = 0; i < q.dim() - 2; ++i) r.tokens *= q.size(i);
+  std::tie(r.q_token_stride, r.q_head_stride) = token_strides(name, "q", q);
+  std::tie(r.k_token_stride, r.k_head_stride) = token_strides(name, "k", k);
+  r.positions_are_64 = ids_are_64(name, "positions", positions);
+  TORCH_CHECK(positions.dim() >= 1 && positions.dim() <= q.dim() - 1, "omq_net::", name,
+              ": positions must be [..., axes] over the last dimensions of the tokens");
+  const auto rows = positions.sizes().slice(0, positions.dim() - 1);
+  TORCH_CHECK(rows == q.sizes().slice(q.dim() - 2 - rows.size(), rows.size()), "omq_net::", name,
+              ": positions must be [..., axes] over the last dimensions of the tokens ", q.sizes(),
+              ", not ", positions.sizes());
+  r.position_rows = 1;
+  for (const int64_t n : rows) r.position_rows *= n;
+  const int64_t axes = positions.size(-1);
+  TORCH_CHECK((int64_t)sections.size() == axes && axes >= 1 && axes <= OMQ_NET_MAX_AXES, "omq_net::",
+              name, ": sections must give the pairs of each of the ", axes, " axes (1 to ",
+              OMQ_NET_MAX_AXES, "), not ", sections);
+  int64_t pairs = 0;
+  for (int64_t i = 0; i < axes; ++i) {
+    TORCH_CHECK(sections[i] >= 0 && sections[i] <= r.dim, "omq_net::", name, ": sections ", sections);
+    pairs += sections[i];
+    r.section_end[i] = (int)pairs;
+  }
+  r.axes = (int)axes;
+  r.pairs = (int)pairs;
+  TORCH_CHECK(frequencies.dim() == 1 && frequencies.size(0) == pairs &&
+                  frequencies.scalar_type() == at::kDouble && frequencies.is_contiguous(),
+              "omq_net::", name, ": frequencies must be contiguous float64 [", pairs,
+              "], the sum of the sections");
+  TORCH_CHECK(2 * pairs <= r.dim, "omq_net::", name, ": ", pairs, " pairs in a head of ", r.dim);
+  TORCH_CHECK(!qw == !kw, "omq_net::", name, ": weights of q and k, or of neither");
+  r.weight_dtype = qw ? check_weight(name, *qw, q) : r.dtype;
+  if (kw) {
+    check_weight(name, *kw, k);
+    TORCH_CHECK(kw->scalar_type() == qw->scalar_type(), "omq_net::", name,
+                ": the weights must be of one type");
+  }
+  r.interleaved = interleaved;
+  r.eps = (float)eps;
+  if (!dev.is_meta()) {
+    r.q = q.data_ptr();
+    r.k = k.data_ptr();
+    if (qw) r.q_weight = qw->data_ptr(), r.k_weight = kw->data_ptr();
+    r.positions = positions.data_ptr();
+    r.frequencies = frequencies.data_ptr<double>();
+  }
+  return r;
+}
+
+std::tuple<at::Tensor, at::Tensor> head_norm_rotary(const at::Tensor& q, const at::Tensor& k,
+                                                    const at::Tensor& positions,
+                                                    const at::Tensor& frequencies,
+                                                    const OptTensor& q_weight,
+                                                    const OptTensor& k_weight, double eps,
+                                                    at::IntArrayRef sections, bool interleaved) {
+  const char* name = "head_norm_rotary";
+  const omq_rotary r = rotary_args(name, q, k, positions, frequencies, q_weight, k_weight, eps,
+                                   sections, interleaved);
+  const c10::Device dev = q.device();
+  const Guard guard(dev);
+  at::Tensor q_out = fresh(q.sizes(), q.scalar_type(), dev);
+  at::Tensor k_out = fresh(k.sizes(), k.scalar_type(), dev);
+  if (dev.is_meta()) return {q_out, k_out};
+  check_rc(omq_head_norm_rotary(&r, q_out.data_ptr(), k_out.data_ptr(), stream_of(dev)),
+           "omq_head_norm_rotary");
+  return {q_out, k_out};
+}
+
+// (grad_q, grad_k, grad_q_weight, grad_k_weight); the last two are empty without weights
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> head_norm_rotary_grad(
+    const at::Tensor& grad_q, const at::Tensor& grad_k, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& positions, const at::Tensor& frequencies, const OptTensor& q_weight,
+    const OptTensor& k_weight, double eps, at::IntArrayRef sections, bool interleaved) {
+  const char* name = "head_norm_rotary_grad";
+  const omq_rotary r = rotary_args(name, q, k, positions, frequencies, q_weight, k_weight, eps,
+                                   sections, interleaved);
+  common_device(name, {&q, &grad_q, &grad_k});
+  check_same(name, "grad_q", grad_q, q);
+  check_same(name, "grad_k", grad_k, k);
+  TORCH_CHECK(grad_q.is_contiguous() && grad_k.is_contiguous(), "omq_net::", name,
+              ": gradients must be contiguous");
+  const at::Tensor* w = get(q_weight);
+  const c10::Device dev = q.device();
+  const Guard guard(dev);
+  at::Tensor gq = fresh(q.sizes(), q.scalar_type(), dev), gk = fresh(k.sizes(), k.scalar_type(), dev);
+  const at::ScalarType w_type = w ? w->scalar_type() : q.scalar_type();
+  at::Tensor gqw = fresh({w ? w->size(0) : 0}, w_type, dev);
+  at::Tensor gkw = fresh({w ? w->size(0) : 0}, w_type, dev);
+  if (dev.is_meta()) return {gq, gk, gqw, gkw};
+  const int64_t bytes = omq_head_norm_rotary_grad_workspace(&r);
+  TORCH_CHECK(bytes >= 0, omq_net_last_error());
+  const Workspace ws(name, bytes, dev);
+  check_rc(omq_head_norm_rotary_grad(&r, grad_q.data_ptr(), grad_k.data_ptr(), gq.data_ptr(),
+                                     gk.data_ptr(), w ? gqw.data_ptr() : nullptr,
+                                     w ? gkw.data_ptr() : nullptr, ws.data(), ws.bytes,
+                                     stream_of(dev)),
+           "omq_head_norm_rotary_grad");
+  return {gq, gk, gqw, gkw};
+}
+
+// ---- attention ------------------------------------------------------------------------------
+const int32_t* index_row(const char* name, const char* arg, const at::Tensor& t, int64_t n) {
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && t.is_contiguous(),
+              "omq_net::", name, ": ", arg, " must be contiguous int32 [", n, "]");
+  return t.is_meta() ? nullptr : t.data_ptr<int32_t>();
+}
+
+omq_attention_args attention_args(const char* name, const at::Tensor& q, const at::Tensor& k,
+                                  const at::Tensor& v, double scale, bool causal,
+                                  const OptTensor& q_starts, const OptTensor& k_starts,
+                                  const OptTensor& k_lengths) {
+  const at::Tensor *qs = get(q_starts), *ks = get(k_starts), *kl = get(k_lengths);
+  const c10::Device dev = common_device(name, {&q, &k, &v, qs, ks, kl});
+  omq_attention_args a{};
+  TORCH_CHECK((q.dim() == 4 && !qs) || (q.dim() == 3 && qs), "omq_net::", name,
+              ": q must be [sequences, queries, heads, dim], or [queries, heads, dim] with q_starts");
+  TORCH_CHECK(!qs == !ks, "omq_net::", name, ": starts of queries and keys, or of neither");
+  TORCH_CHECK(k.dim() == q.dim() && k.sizes() == v.sizes() && k.size(-1) == q.size(-1) &&
+                  (q.dim() == 3 || k.size(0) == q.size(0)),
+              "omq_net::", name, ": k and v must have q's sequences and dim, not ", k.sizes(), " and ",
+              v.sizes(), " with ", q.sizes());
+  TORCH_CHECK(q.size(-1) >= 1 && q.size(-2) >= 1 && k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0,
+              "omq_net::", name, ": heads of queries (", q.size(-2),
+              ") must be a multiple of those of keys (", k.size(-2), ")");
+  a.dtype = type_of(name, "q", q);
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "omq_net::",
+              name, ": q, k and v must be of one type");
+  for (const auto& [arg, t] : {std::pair<const char*, const at::Tensor*>{"q", &q}, {"k", &k}, {"v", &v}})
+    TORCH_CHECK(t->size(-1) == 1 || t->stride(-1) == 1 || t->numel() == 0, "omq_net::", name,
+                ": the elements of a head of ", arg, " must be adjacent (use .contiguous())");
+  a.q_len = q.size(-3);
+  a.k_len = k.size(-3);
+  a.q_heads = (int)std::min<int64_t>(q.size(-2), INT32_MAX);
+  a.k_heads = (int)std::min<int64_t>(k.size(-2), INT32_MAX);
+  a.dim = (int)std::min<int64_t>(q.size(-1), INT32_MAX);
+  if (qs) {
+    TORCH_CHECK(qs->dim() == 1 && qs->size(0) >= 1, "omq_net::", name,
+                ": q_starts must be [sequences + 1]");
+    a.sequences = qs->size(0) - 1;
+    a.q_starts = index_row(name, "q_starts", *qs, a.sequences + 1);
+    a.k_starts = index_row(name, "k_starts", *ks, a.sequences + 1);
+  } else {
+    a.sequences = q.size(0);
+    a.q_seq_stride = q.stride(0), a.k_seq_stride = k.stride(0), a.v_seq_stride = v.stride(0);
+  }
+  if (kl) a.k_lengths = index_row(name, "k_lengths", *kl, a.sequences);
+  a.q_row_stride = q.stride(-3), a.k_row_stride = k.stride(-3), a.v_row_stride = v.stride(-3);
+  a.q_head_stride = q.stride(-2), a.k_head_stride = k.stride(-2), a.v_head_stride = v.stride(-2);
+  TORCH_CHECK(scale > 0.0 && std::isfinite((float)scale) && (float)scale > 0.0f, "omq_net::", name,
+              ": scale ", scale, " must be finite and above 0");
+  a.scale = (float)scale;
+  a.causal = causal;
+  if (!dev.is_meta()) a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
+  return a;
+}
+
+// (out, lse); lse is empty where it is not wanted
+std::tuple<at::Tensor, at::Tensor> attention(const at::Tensor& q, const at::Tensor& k,
+                                             const at::Tensor& v, double scale, bool causal,
+                                             const OptTensor& q_starts, const OptTensor& k_starts,
+                                             const OptTensor& k_lengths, bool want_lse) {
+  const char* name = "attention";
+  const omq_attention_args a =
+      attention_args(name, q, k, v, scale, causal, q_starts, k_starts, k_lengths);
+  const c10::Device dev = q.device();
+  const Guard guard(dev);
+  at::Tensor out = fresh(q.sizes(), q.scalar_type(), dev);
+  at::Tensor lse = want_lse ? fresh(q.sizes().slice(0, q.dim() - 1), at::kFloat, dev)
+                            : fresh({0}, at::kFloat, dev);
+  if (dev.is_meta()) return {out, lse};
+  const int64_t bytes = omq_attention_forward_workspace(&a);
+  TORCH_CHECK(bytes >= 0, omq_net_last_error());
+  const Workspace ws(name, bytes, dev);
+  check_rc(omq_attention_forward(&a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+                                 ws.data(), ws.bytes, stream_of(dev)),
+           "omq_attention_forward");
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_grad(
+    const at::Tensor& grad_out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& out, const at::Tensor& lse, double scale, bool causal,
+    const OptTensor& q_starts, const OptTensor& k_starts, const OptTensor& k_lengths) {
+  const char* name = "attention_grad";
+  const omq_attention_args a =
+      attention_args(name, q, k, v, scale, causal, q_starts, k_starts, k_lengths);
+  common_device(name, {&q, &grad_out, &out, &lse});
+  check_same(name, "grad_out", grad_out, q);
+  check_same(name, "out", out, q);
+  TORCH_CHECK(lse.sizes() == q.sizes().slice(0, q.dim() - 1) && lse.scalar_type() == at::kFloat,
+              "omq_net::", name, ": lse must be float32 ", q.sizes().slice(0, q.dim() - 1));
+  TORCH_CHECK(grad_out.is_contiguous() && out.is_contiguous() && lse.is_contiguous(), "omq_net::",
+              name, ": grad_out, out and lse must be contiguous");
+  const c10::Device dev = q.device();
+  const Guard guard(dev);
+  at::Tensor gq = fresh(q.sizes(), q.scalar_type(), dev);
+  at::Tensor gk = fresh(k.sizes(), k.scalar_type(), dev);
+  at::Tensor gv = fresh(v.sizes(), v.scalar_type(), dev);
+  if (dev.is_meta()) return {gq, gk, gv};
+  const int64_t bytes = omq_attention_grad_workspace(&a);
+  TORCH_CHECK(bytes >= 0, omq_net_last_error());
+  const Workspace ws(name, bytes, dev);
+  check_rc(omq_attention_grad(&a, grad_out.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+                              gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), ws.data(), ws.bytes,
+                              stream_of(dev)),
+           "omq_attention_grad");
+  return {gq, gk, gv};
+}
+
+// ---- log-probabilities of tokens ------------------------------------------------------------
+omq_logprob_rows logprob_rows(const char* name, const at::Tensor& logits, const at::Tensor& tokens,
+                              const OptTensor& legal) {
+  const at::Tensor* ok = get(legal);
+  const c10::Device dev = common_device(name, {&logits, &tokens, ok});
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1, "omq_net::", name,
+              ": logits must be [rows, vocabulary]");
+  omq_logprob_rows r{};
+  r.rows = logits.size(0);
+  r.vocab = logits.size(1);
+  r.dtype = type_of(name, "logits", logits);
+  r.logits_stride = row_stride(name, "logits", logits);
+  r.tokens_are_64 = ids_are_64(name, "tokens", tokens);
+  TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) == r.rows, "omq_net::", name, ": tokens must be [",
+              r.rows, "]");
+  if (ok) {
+    TORCH_CHECK(ok->sizes() == logits.sizes() && ok->scalar_type() == at::kBool, "omq_net::", name,
+                ": legal must be bool ", logits.sizes());
+    r.legal_stride = row_stride(name, "legal", *ok);
+  }
+  if (!dev.is_meta()) {
+    r.logits = logits.data_ptr();
+    r.tokens = tokens.data_ptr();
+    if (ok) r.legal = reinterpret_cast<const uint8_t*>(ok->data_ptr<bool>());
+  }
+  return r;
+}
+
+// (logp, entropy, top_logp, top_tokens, stats)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
+    const at::Tensor& logits, const at::Tensor& tokens, const OptTensor& legal, int64_t top,
+    bool want_stats) {
+  const char* name = "token_logprobs";
+  const omq_logprob_rows r = logprob_rows(name, logits, tokens, legal);
+  TORCH_CHECK(top >= 0 && top <= OMQ_NET_MAX_TOP, "omq_net::", name, ": top ", top, " outside [0, ",
+              OMQ_NET_MAX_TOP, "]");
+  const c10::Device dev = logits.device();
+  const Guard guard(dev);
+  at::Tensor logp = fresh({r.rows}, at::kFloat, dev), entropy = fresh({r.rows}, at::kFloat, dev);
+  at::Tensor top_logp = fresh({r.rows, top}, at::kFloat, dev);
+  at::Tensor top_tokens = fresh({r.rows, top}, at::kLong, dev);
+  at::Tensor stats = fresh({want_stats ? r.rows : 0, OMQ_NET_STATS}, at::kFloat, dev);
+  if (dev.is_meta()) return {logp, entropy, top_logp, top_tokens, stats};
+  check_rc(omq_token_logprobs(&r, (int32_t)top, logp.data_ptr<float>(), entropy.data_ptr<float>(),
+                              top ? top_logp.data_ptr<float>() : nullptr,
+                              top ? top_tokens.data_ptr<int64_t>() : nullptr,
+                              want_stats ? stats.data_ptr<float>() : nullptr, stream_of(dev)),
+           "omq_token_logprobs");
+  return {logp, entropy, top_logp, top_tokens, stats};
+}
+
+at::Tensor token_logprobs_grad(const at::Tensor& logits, const at::Tensor& tokens,
+                               const OptTensor& legal, const at::Tensor& stats,
+                               const OptTensor& logp_weight, const OptTensor& entropy_weight) {
+  const char* name = "token_logprobs_grad";
+  const omq_logprob_rows r = logprob_rows(name, logits, tokens, legal);
+  const at::Tensor *wl = get(logp_weight), *we = get(entropy_weight);
+  common_device(name, {&logits, &stats, wl, we});
+  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == OMQ_NET_STATS &&
+                  stats.scalar_type() == at::kFloat && stats.is_contiguous(),
+              "omq_net::", name, ": stats must be those of token_logprobs");
+  const float* l = wl ? row_floats(name, "logp_weight", *wl, r.rows) : nullptr;
+  const float* e = we ? row_floats(name, "entropy_weight", *we, r.rows) : nullptr;
+  const c10::Device dev = logits.device();
+  const Guard guard(dev);
+  at::Tensor grad = fresh({r.rows, r.vocab}, logits.scalar_type(), dev);
+  if (dev.is_meta()) return grad;
+  check_rc(omq_token_logprobs_grad(&r, stats.data_ptr<float>(), l, e, grad.data_ptr(),
+                                   stream_of(dev)),
+           "omq_token_logprobs_grad");
+  return grad;
+}
+
+// (logp, entropy, grad)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> token_logprobs_with_grad(
+    const at::Tensor& logits, const at::Tensor& tokens, const OptTensor& legal,
+    const OptTensor& logp_weight, const OptTensor& entropy_weight) {
+  const char* name = "token_logprobs_with_grad";
+  const omq_logprob_rows r = logprob_rows(name, logits, tokens, legal);
+  const at::Tensor *wl = get(logp_weight), *we = get(entropy_weight);
+  common_device(name, {&logits, wl, we});
+  const float* l = wl ? row_floats(name, "logp_weight", *wl, r.rows) : nullptr;
+  const float* e = we ? row_floats(name, "entropy_weight", *we, r.rows) : nullptr;
+  const c10::Device dev = logits.device();
+  const Guard guard(dev);
+  at::Tensor logp = fresh({r.rows}, at::kFloat, dev), entropy = fresh({r.rows}, at::kFloat, dev);
+  at::Tensor grad = fresh({r.rows, r.vocab}, logits.scalar_type(), dev);
+  if (dev.is_meta()) return {logp, entropy, grad};
+  check_rc(omq_token_logprobs_with_grad(&r, l, e, logp.data_ptr<float>(),
+                                        entropy.data_ptr<float>(), grad.data_ptr(),
+                                        stream_of(dev)),
+           "omq_token_logprobs_with_grad");
+  return {logp, entropy, grad};
+}
+
 // ---- registration ---------------------------------------------------------------------------
 // The operators have no derivatives of their own (net_ops.py's autograd functions call them): a
 // tangent is refused, and a backward pass through one raises.  Without this kernel torch drops
@@ -505,6 +850,11 @@ void define(torch::Library& m, const std::string& name, const std::string& schem
 const std::string kLossArgs =
     "Tensor logits, Tensor actions, Tensor advantages, Tensor old_logp, float clip_low, "
     "float clip_high, float kl_coef, Tensor? ref_logp, Tensor? target, Tensor? legal";
+const std::string kRotaryArgs =
+    "Tensor positions, Tensor frequencies, Tensor? q_weight, Tensor? k_weight, float eps, "
+    "int[] sections, bool interleaved";
+const std::string kAttentionArgs =
+    "float scale, bool causal, Tensor? q_starts, Tensor? k_starts, Tensor? k_lengths";
 
 }  // namespace
 
@@ -529,4 +879,23 @@ TORCH_LIBRARY(omq_net, m) {
          "(" + kLossArgs + ", Tensor stats, Tensor? row_weight) -> Tensor");
   define<clipped_policy_loss_with_grad>(m, "clipped_policy_loss_with_grad",
          "(" + kLossArgs + ", Tensor? row_weight) -> (Tensor, Tensor, Tensor, Tensor)");
+  define<head_norm_rotary>(m, "head_norm_rotary",
+         "(Tensor q, Tensor k, " + kRotaryArgs + ") -> (Tensor, Tensor)");
+  define<head_norm_rotary_grad>(m, "head_norm_rotary_grad",
+         "(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, " + kRotaryArgs +
+         ") -> (Tensor, Tensor, Tensor, Tensor)");
+  define<attention>(m, "attention", "(Tensor q, Tensor k, Tensor v, " + kAttentionArgs +
+         ", bool want_lse) -> (Tensor, Tensor)");
+  define<attention_grad>(m, "attention_grad",
+         "(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, " +
+         kAttentionArgs + ") -> (Tensor, Tensor, Tensor)");
+  define<token_logprobs>(m, "token_logprobs",
+         "(Tensor logits, Tensor tokens, Tensor? legal, int top, bool want_stats) "
+         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  define<token_logprobs_grad>(m, "token_logprobs_grad",
+         "(Tensor logits, Tensor tokens, Tensor? legal, Tensor stats, Tensor? logp_weight, "
+         "Tensor? entropy_weight) -> Tensor");
+  define<token_logprobs_with_grad>(m, "token_logprobs_with_grad",
+         "(Tensor logits, Tensor tokens, Tensor? legal, Tensor? logp_weight, "
+         "Tensor? entropy_weight) -> (Tensor, Tensor, Tensor)");
 }

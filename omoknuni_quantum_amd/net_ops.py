@@ -9,15 +9,20 @@ caller's current HIP stream:
     add_rms_norm_fp8(x, residual, weight, eps, group)   the same for serving, y in 8 bits
     dropout(x, p, seed, offset)                         dropout whose mask is never stored
     clipped_policy_loss(logits, actions, ...)           the policy loss over legal actions
+    head_norm_rotary(q, k, positions, frequencies, ...) heads normed and rotated by position
+    attention(q, k, v, ...)                             attention: batches, packed rows, caches
+    token_logprobs(logits, tokens, legal, top)          log-probabilities, entropy, alternatives
 
-The four that training uses are differentiable; their gradients are also functions of their own
-(``token_embedding_grad``, ``add_rms_norm_grad``, ``clipped_policy_loss_with_grad``; dropout is its
-own gradient) for a program that runs its backward pass by hand.  Every gradient is a function of
+Those that training uses (all but add_rms_norm_fp8) are differentiable; their gradients are also
+functions of their own (``token_embedding_grad``, ``add_rms_norm_grad``,
+``clipped_policy_loss_with_grad``, ``head_norm_rotary_grad``, ``attention_grad``,
+``token_logprobs_with_grad``; dropout is its own gradient) for a program that runs its backward
+pass by hand.  Every gradient is a function of
 its inputs alone, bit for bit: sums run in a fixed order.  There are no second derivatives and no
 forward-mode ones, and none of the other functions: those raise.
 
 Elements are float32, bfloat16 or float16.  Sums and statistics are kept in float32, and a result
-is rounded once.  Tensors of rows (the last dimension) may be slices of wider ones as long as the
+is rounded once (attention also rounds what its matrix products take).  Tensors of rows (the last dimension) may be slices of wider ones as long as the
 rows' elements are adjacent and the rows equally far apart; other arguments, and dropout's x, must
 be contiguous.
 There is no CPU implementation: tensors must be on a HIP device, and a missing library raises.
@@ -57,6 +62,13 @@ _NORM_GRAD = torch.ops.omq_net.add_rms_norm_grad.default
 _LOSS = torch.ops.omq_net.clipped_policy_loss.default
 _LOSS_GRAD = torch.ops.omq_net.clipped_policy_loss_grad.default
 _LOSS_WITH_GRAD = torch.ops.omq_net.clipped_policy_loss_with_grad.default
+_ROTARY = torch.ops.omq_net.head_norm_rotary.default
+_ROTARY_GRAD = torch.ops.omq_net.head_norm_rotary_grad.default
+_ATTENTION = torch.ops.omq_net.attention.default
+_ATTENTION_GRAD = torch.ops.omq_net.attention_grad.default
+_LOGPROBS = torch.ops.omq_net.token_logprobs.default
+_LOGPROBS_GRAD = torch.ops.omq_net.token_logprobs_grad.default
+_LOGPROBS_WITH_GRAD = torch.ops.omq_net.token_logprobs_with_grad.default
 
 
 def _word(x: int) -> int:
@@ -254,3 +266,188 @@ def clipped_policy_loss_with_grad(logits: torch.Tensor, actions: torch.Tensor,
     (8192 with a target) are read once."""
     return _LOSS_WITH_GRAD(logits, actions, advantages, old_logp, clip_low, clip_high, kl_coef,
                            ref_logp, target, legal, row_weight)
+
+
+# ---- norm and rotation of heads -------------------------------------------------------------
+def rotary_frequencies(sections, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """float64 [sum of sections]: for an axis of n pairs base^(-j / n), j = 0 ... n - 1 (radians per
+    unit of the position), the axes one after another."""
+    parts = [float(base) ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in sections]
+    return torch.cat(parts).to(device)
+
+
+class _HeadNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved):
+        ctx.save_for_backward(q, k, positions, frequencies, q_weight, k_weight)
+        ctx.args = eps, sections, interleaved
+        return _ROTARY(q, k, positions, frequencies, q_weight, k_weight, *ctx.args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_q, grad_k):
+        gq, gk, gqw, gkw = _ROTARY_GRAD(_rows(grad_q), _rows(grad_k), *ctx.saved_tensors, *ctx.args)
+        if ctx.saved_tensors[4] is None:
+            gqw = gkw = None
+        return gq, gk, None, None, gqw, gkw, None, None, None
+
+
+def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                     frequencies: torch.Tensor, q_weight: torch.Tensor | None = None,
+                     k_weight: torch.Tensor | None = None, eps: float = 1e-6, sections=None,
+                     interleaved: bool = False):
+    """(q', k'): each head x of q [..., q_heads, dim] and k [..., k_heads, dim] normed,
+    n = x / sqrt(mean(x^2) + eps) * weight, and its first 2 * pairs columns rotated by the token's
+    position: a pair (a, b) of n becomes (a cos t - b sin t, b cos t + a sin t), t = position *
+    frequency.  The columns behind them stay.
+
+    q_weight, k_weight: [dim], of the heads' type or float32; both None: no norm.
+    positions: int32 or int64 [..., axes], over all leading dimensions of q and k, or over the last
+    of them (then they serve each of the dimensions before: [cells, 2] for a batch of boards).
+    sections: the number of pairs that each axis turns, one axis' pairs after another's (None: one
+    axis, all of `frequencies`); frequencies: float64 [their sum], see rotary_frequencies.
+    Pair j is the columns (j, j + pairs), or (2j, 2j + 1) with interleaved.  The angle is formed in
+    64 bits, so that far positions keep their phase.
+
+    q and k may be slices of one product's output: a head's elements must be adjacent and the
+    tokens equally far apart.  At most 256 columns and 4 axes.  Differentiable in q, k and the
+    weights."""
+    sections = (frequencies.shape[0],) if sections is None else tuple(int(n) for n in sections)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                    (q_weight is not None and q_weight.requires_grad) or
+                                    (k_weight is not None and k_weight.requires_grad)):
+        return _HeadNormRotary.apply(q, k, positions, frequencies, q_weight, k_weight, float(eps),
+                                     sections, bool(interleaved))
+    return _ROTARY(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
+
+
+def head_norm_rotary_grad(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.Tensor,
+                          k: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor,
+                          q_weight: torch.Tensor | None = None,
+                          k_weight: torch.Tensor | None = None, eps: float = 1e-6, sections=None,
+                          interleaved: bool = False):
+    """(grad_q, grad_k, grad_q_weight, grad_k_weight) of head_norm_rotary from its arguments and
+    the gradients of its two results (contiguous).  The last two are None without weights."""
+    sections = (frequencies.shape[0],) if sections is None else tuple(int(n) for n in sections)
+    gq, gk, gqw, gkw = _ROTARY_GRAD(grad_q, grad_k, q, k, positions, frequencies, q_weight,
+                                    k_weight, eps, sections, interleaved)
+    return (gq, gk, gqw, gkw) if q_weight is not None else (gq, gk, None, None)
+
+
+# ---- attention ------------------------------------------------------------------------------
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, q_starts, k_starts, k_lengths):
+        out, lse = _ATTENTION(q, k, v, scale, causal, q_starts, k_starts, k_lengths, True)
+        ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts, k_lengths)
+        ctx.args = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, q_starts, k_starts, k_lengths = ctx.saved_tensors
+        gq, gk, gv = _ATTENTION_GRAD(_rows(grad), q, k, v, out, lse, *ctx.args, q_starts, k_starts,
+                                     k_lengths)
+        return gq, gk, gv, None, None, None, None, None
+
+
+def _attention_args(q, scale, q_starts, k_starts):
+    return (q.shape[-1] ** -0.5 if scale is None else float(scale),
+            q_starts if k_starts is None else k_starts)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
+              causal: bool = False, q_starts: torch.Tensor | None = None,
+              k_starts: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None):
+    """softmax(scale * q k^T) v for each sequence and head, of q's shape.
+
+    A batch: q [sequences, queries, q_heads, dim], k and v [sequences, keys, k_heads, dim].
+    Packed sequences of different lengths: q [rows, q_heads, dim], k and v [rows, k_heads, dim];
+    sequence s has the rows q_starts[s] to q_starts[s + 1] of q and k_starts[s] to k_starts[s + 1]
+    of k and v (int32 [sequences + 1] on the device, not falling; k_starts None: q_starts).
+    k_lengths (int32 [sequences] on the device) gives how many of a sequence's keys are in use,
+    from the first: caches with room left, or a padded batch.
+
+    q_heads is a multiple of k_heads; each run of q_heads / k_heads query heads shares a key head.
+    causal: a sequence's last query sees all its keys, and each before it one key less.  A query
+    that sees no key, and a row of no sequence, has 0.  What keys that are hidden from a query hold
+    (infinities and NaN too) does not reach its result.  scale None: 1 / sqrt(dim).
+
+    Scores and sums are float32; probabilities are rounded to the elements' type before they
+    multiply v.  Head elements must be adjacent; other strides are free.  At most 128 columns.
+    Differentiable in q, k and v (keys that are not in use have gradient 0)."""
+    scale, k_starts = _attention_args(q, scale, q_starts, k_starts)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, scale, bool(causal), q_starts, k_starts, k_lengths)
+    return _ATTENTION(q, k, v, scale, causal, q_starts, k_starts, k_lengths, False)[0]
+
+
+def attention_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       scale: float | None = None, causal: bool = False,
+                       q_starts: torch.Tensor | None = None, k_starts: torch.Tensor | None = None,
+                       k_lengths: torch.Tensor | None = None):
+    """(out, lse) of attention; lse float32, q's shape without dim: the logarithm of the sum of the
+    exponentials of a row's scores (-inf where it sees no key).  For attention_grad."""
+    scale, k_starts = _attention_args(q, scale, q_starts, k_starts)
+    return _ATTENTION(q, k, v, scale, causal, q_starts, k_starts, k_lengths, True)
+
+
+def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   out: torch.Tensor, lse: torch.Tensor, scale: float | None = None,
+                   causal: bool = False, q_starts: torch.Tensor | None = None,
+                   k_starts: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None):
+    """(grad_q, grad_k, grad_v) of attention from its arguments, the gradient of out, and out and
+    lse of attention_with_lse.  The gradients of the scores are rounded to the elements' type
+    before they multiply k and q."""
+    scale, k_starts = _attention_args(q, scale, q_starts, k_starts)
+    return _ATTENTION_GRAD(grad_out, q, k, v, out, lse, scale, causal, q_starts, k_starts,
+                           k_lengths)
+
+
+# ---- log-probabilities of tokens ------------------------------------------------------------
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, legal, top):
+        logp, entropy, top_logp, top_tokens, stats = _LOGPROBS(logits, tokens, legal, top, True)
+        ctx.save_for_backward(logits, tokens, legal, stats)
+        ctx.mark_non_differentiable(top_logp, top_tokens)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logp, grad_entropy, _top_logp, _top_tokens):
+        grads = [None if g is None else _rows(g) for g in (grad_logp, grad_entropy)]
+        return _LOGPROBS_GRAD(*ctx.saved_tensors, *grads), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, legal: torch.Tensor | None = None,
+                   top: int = 0):
+    """(logp, entropy, top_logp, top_tokens) of a policy's rows.
+
+    With logq the log-softmax of a row over its legal tokens: logp = logq[token], entropy =
+    -sum e^logq logq, and the `top` (at most 32) most probable tokens with their logq, by falling
+    logit and rising index among equals.  logp and entropy float32 [rows]; top_logp float32 and
+    top_tokens int64 [rows, top], -inf and -1 where fewer tokens have a probability.
+
+    logits [rows, vocabulary] float32/bfloat16/float16; tokens int32/int64 [rows]; legal bool like
+    logits (None: all).  A token outside the vocabulary (padding) or not legal has logp 0, as
+    clipped_policy_loss has it; a row without a legal token has 0 throughout and no alternatives.
+    What the logits of illegal tokens hold is never used.  A NaN or an infinity above 0 among the
+    legal ones makes the row's results NaN.  Differentiable in logits through logp and entropy (a
+    policy-gradient term and an entropy bonus)."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogprobs.apply(logits, tokens, legal, int(top))
+    return _LOGPROBS(logits, tokens, legal, top, False)[:4]
+
+
+def token_logprobs_with_grad(logits: torch.Tensor, tokens: torch.Tensor,
+                             logp_weight: torch.Tensor | None = None,
+                             entropy_weight: torch.Tensor | None = None,
+                             legal: torch.Tensor | None = None):
+    """(logp, entropy, grad): those of token_logprobs and the gradient by the logits of
+    sum(logp_weight * logp + entropy_weight * entropy) (float32 [rows] each, None: 0), for a
+    program that goes on with ``logits.backward(grad)``.  One launch; rows of up to 16384 tokens
+    are read once.  A row whose weights are 0 has no gradient, whatever its logits hold."""
+    return _LOGPROBS_WITH_GRAD(logits, tokens, legal, logp_weight, entropy_weight)

@@ -126,3 +126,109 @@ def policy_loss(logits, actions, advantages, old_logp, clip_low, clip_high, kl_c
     grad = torch.where(ok, grad, 0.0)  # (whatever a row of NaN holds)
     return {"loss": loss, "logp": logp, "kl": kl, "ratio": ratio, "grad": grad, "taken": taken,
             "prob": prob, "slope": slope}
+
+
+# ---- norm and rotation of heads -------------------------------------------------------------
+def _rotation(positions, frequencies, sections, dim, interleaved):
+    """The rotation of each token as a matrix [tokens, dim, dim]."""
+    pairs = sum(sections)
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    r = torch.eye(dim, dtype=torch.float64).repeat(positions.shape[0], 1, 1)
+    for j in range(pairs):
+        t = positions[:, axis[j]].double() * frequencies[j]
+        a, b = (2 * j, 2 * j + 1) if interleaved else (j, j + pairs)
+        r[:, a, a] = r[:, b, b] = torch.cos(t)
+        r[:, a, b], r[:, b, a] = -torch.sin(t), torch.sin(t)
+    return r
+
+
+def head_norm_rotary(x, positions, frequencies, weight, eps, sections, interleaved):
+    """One of q and k: x [tokens, heads, dim], positions [tokens, axes]."""
+    x = x.double()
+    if weight is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * weight.double()
+    r = _rotation(positions, frequencies, sections, x.shape[-1], interleaved)
+    return torch.matmul(r[:, None], x[..., None])[..., 0]
+
+
+def head_norm_rotary_grad(g, x, positions, frequencies, weight, eps, sections, interleaved):
+    """(grad_x, grad_weight)."""
+    r = _rotation(positions, frequencies, sections, x.shape[-1], interleaved)
+    d = torch.matmul(r.transpose(1, 2)[:, None], g.double()[..., None])[..., 0]
+    if weight is None:
+        return d, None
+    x, w = x.double(), weight.double()
+    root = torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+    n = x / root
+    dn = d * w
+    return (dn - n * (dn * n).mean(-1, keepdim=True)) / root, (d * n).sum((0, 1))
+
+
+# ---- attention ------------------------------------------------------------------------------
+def attention(q, k, v, scale, causal, grad=None):
+    """One sequence: q [queries, q_heads, dim], k and v [keys, k_heads, dim] (those in use).
+    (out, lse), and with `grad` the gradients of q, k and v.  Hidden keys take no part, whatever
+    they hold."""
+    lq, heads, dim = q.shape
+    lk, group = k.shape[0], heads // k.shape[1]
+    q, k, v = q.double(), k.double(), v.double()
+    out = torch.zeros(lq, heads, dim, dtype=torch.float64)
+    lse = torch.full((lq, heads), -math.inf, dtype=torch.float64)
+    back = [torch.zeros_like(t) for t in (q, k, v)]
+    for h in range(heads):
+        for i in range(lq):
+            n = min(max(i + 1 + lk - lq, 0), lk) if causal else lk
+            if n == 0:
+                continue
+            kk, vv = k[:n, h // group], v[:n, h // group]
+            s = scale * (kk @ q[i, h])
+            lse[i, h] = torch.logsumexp(s, 0)
+            p = torch.exp(s - lse[i, h])
+            out[i, h] = p @ vv
+            if grad is not None:
+                g = grad[i, h].double()
+                dp = vv @ g
+                ds = p * (dp - (p * dp).sum()) * scale
+                back[0][i, h] = ds @ kk
+                back[1][:n, h // group] += ds[:, None] * q[i, h]
+                back[2][:n, h // group] += p[:, None] * g
+    return (out, lse) if grad is None else (out, lse, *back)
+
+
+# ---- log-probabilities of tokens ------------------------------------------------------------
+def token_logprobs(logits, tokens, legal, top, a=None, b=None):
+    """(logp, entropy, top_logp, top_tokens, gradient of sum(a logp + b entropy)), a row at a
+    time."""
+    rows, vocab = logits.shape
+    logp, entropy = torch.zeros(rows, dtype=torch.float64), torch.zeros(rows, dtype=torch.float64)
+    top_logp = torch.full((rows, top), -math.inf, dtype=torch.float64)
+    top_tokens = torch.full((rows, top), -1, dtype=torch.int64)
+    grad = torch.zeros(rows, vocab, dtype=torch.float64)
+    for i in range(rows):
+        z = logits[i].double()
+        ok = legal[i].bool() if legal is not None else torch.ones(vocab, dtype=torch.bool)
+        t = int(tokens[i])
+        given = 0 <= t < vocab and bool(ok[t])
+        if not bool((z[ok] != -math.inf).any()):  # (a NaN is not)
+            continue
+        zl = z.masked_fill(~ok, -math.inf)
+        logq = torch.log_softmax(zl, 0)
+        p = torch.exp(logq)
+        plogp = torch.where(p == 0, 0.0, p * logq)
+        entropy[i] = -plogp.sum()
+        if given:
+            logp[i] = logq[t]
+        order = sorted((j for j in range(vocab) if bool(ok[j]) and float(z[j]) > -math.inf),
+                       key=lambda j: (-float(z[j]), j))[:top] if top else []
+        for j, at in enumerate(order):
+            top_logp[i, j], top_tokens[i, j] = logq[at], at
+        wl = float(a[i]) if a is not None and given else 0.0
+        we = float(b[i]) if b is not None else 0.0
+        if wl or we:
+            g = -wl * p - we * torch.where(p == 0, 0.0, p * (logq + entropy[i]))
+            if given:
+                g[t] += wl
+            grad[i] = torch.where(ok & (z != -math.inf), g, 0.0)
+            if given:
+                grad[i, t] = g[t]
+    return logp, entropy, top_logp, top_tokens, grad
