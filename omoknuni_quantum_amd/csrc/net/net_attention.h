@@ -36,6 +36,8 @@ struct AttentionArgs {
   int64_t slots;    // tiles a key head, some of them empty
   int64_t batch_tiles;  // tiles of a sequence of a batch
   float score_scale;    // scale * log2 e
+  uint32_t group_mul;   // a row's query is umulhi(row, group_mul) >> group_shift; 0: the row
+  int group_shift;
   void* out;
   float* lse;
   const void* grad_out;
@@ -44,6 +46,11 @@ struct AttentionArgs {
   float* delta;     // [rows of q, q_heads]: sum of grad_out * out
   void *grad_q, *grad_k, *grad_v;
 };
+
+// The query of a row and its head in the group.
+__device__ inline int query_of(const AttentionArgs& args, int row) {
+  return args.group_mul ? (int)(__umulhi((uint32_t)row, args.group_mul) >> args.group_shift) : row;
+}
 
 // ---- sequences ------------------------------------------------------------------------------
 // A sequence's rows in the arrays; lk: its keys in use, of `room`.
@@ -117,6 +124,78 @@ __device__ inline Sequence sequence_of(const AttentionArgs& args, int64_t s) {
   return q;
 }
 
+// The tile of a launch by rows of queries: its sequence and number, or false.  Those of the last rows
+// come first: in a causal sequence they see the most keys.
+struct Place {
+  Sequence q;
+  int kv;
+  int64_t tile;
+};
+
+__device__ inline bool place_of_queries(const AttentionArgs& args, int tile_rows, Place* p) {
+  const omq_attention_args& a = args.a;
+  const int64_t block = block_index();
+  int64_t slot = block / a.k_heads;
+  if (slot >= args.slots) return false;
+  slot = args.slots - 1 - slot;
+  p->kv = (int)(block % a.k_heads);
+  if (a.q_starts) {
+    p->q = sequence_of(args, find_piece(a.q_starts, a.sequences, a.q_len, args.group, tile_rows,
+                                        slot, &p->tile));
+  } else {
+    p->q = sequence_of(args, slot % a.sequences);
+    p->tile = slot / a.sequences;
+  }
+  return p->tile >= 0 && p->tile * tile_rows < (int64_t)p->q.lq * args.group;
+}
+
+// The same by keys, the first ones first: in a causal sequence the most queries see them.
+__device__ inline bool place_of_keys(const AttentionArgs& args, int tile_rows, Place* p) {
+  const omq_attention_args& a = args.a;
+  const int64_t block = block_index();
+  const int64_t slot = block / a.k_heads;
+  if (slot >= args.slots) return false;
+  p->kv = (int)(block % a.k_heads);
+  if (a.q_starts) {
+    p->q = sequence_of(args,
+                       find_piece(a.k_starts, a.sequences, a.k_len, 1, tile_rows, slot, &p->tile));
+  } else {
+    p->q = sequence_of(args, slot % a.sequences);
+    p->tile = slot / a.sequences;
+  }
+  return p->tile >= 0 && p->tile * tile_rows < p->q.room;
+}
+
+// What a lane's row sees of its sequence, and which keys the rows of its wave see.
+struct Rows {
+  int query, head;   // of the row, or of the last one
+  bool there;
+  int limit;         // keys that the row sees
+  int least, most;   // that all of the wave's rows see, and that some do
+  int block_most;    // that some row of the workgroup sees
+};
+
+__device__ inline Rows rows_of(const AttentionArgs& args, const Sequence& q, int kv, int r0,
+                               int rows) {
+  const int shift = q.lk - q.lq, lane = threadIdx.x & 63;
+  const int first = r0 + kWaveRows * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto sees = [&](int row) {
+    return args.a.causal ? cut(query_of(args, row < rows ? row : rows - 1) + shift + 1, 0, q.lk)
+                         : q.lk;
+  };
+  Rows x;
+  const int mine = first + (lane & 31);
+  x.there = mine < rows;
+  const int row = x.there ? mine : rows - 1;
+  x.query = query_of(args, row);
+  x.head = kv * args.group + row - x.query * args.group;
+  x.limit = sees(row);
+  x.least = sees(first);
+  x.most = first < rows ? sees(first + kWaveRows - 1) : 0;
+  x.block_most = sees(r0 + kTileRows - 1);
+  return x;
+}
+
 // ---- products -------------------------------------------------------------------------------
 // 16 bytes a lane are an operand: kChunk columns of the sum, half of them in each half of the wave.
 template <class T>
@@ -142,47 +221,64 @@ __device__ inline F16 mma(F4 a, F4 b, F16 c) {
   return c;
 }
 
-// A tile in LDS: rows of kDim columns, 16 bytes between them, so that 16 rows' 16 bytes of one
-// column lie in different banks.
+// A tile in LDS: kTileKeys rows of kDim columns, their 16-byte chunks exchanged within a row (chunk
+// c of row r at place c ^ swap(r)) so that neither the chunks of one column from 16 rows nor a
+// column's elements from four rows and 32 columns share banks.  Rows follow each other without
+// gaps, as loads from memory straight into LDS need it.
 template <class T, int kDim>
 struct Tile {
   using Frag = typename Operand<T>::Frag;
   static constexpr int kChunk = Operand<T>::kChunk;
-  static constexpr int kPitch = kDim * (int)sizeof(T) + 16;
-  static constexpr int kChunks = kDim / kChunk;   // operands of a row
+  static constexpr int kPitch = kDim * (int)sizeof(T);
+  static constexpr int kPer = kPitch / 16;           // chunks of a row
+  static constexpr int kChunks = kDim / kChunk;      // operands of a row
   static constexpr int kParts = kWaveRows / kChunk;  // operands of 32 rows down a column
   static constexpr int kBytes = kTileKeys * kPitch;
 
-  // Chunk c of the row row0 + lane % 32.
+  __device__ static int swap(int r) {
+    if constexpr (kPer == 4) return (r >> 2) & 3;
+    if constexpr (sizeof(T) == 2)
+      return kPer == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+    else
+      return kPer == 8 ? (r >> 1) & 7
+                       : (((r >> 2) & 1) << 3) | (((r >> 3) & 1) << 2) | (r & 3);
+  }
+  __device__ static int place(int r, int chunk) { return r * kPitch + ((chunk ^ swap(r)) << 4); }
+
+  // Chunk c of the row row0 + lane % 32 (row0 a multiple of 32).
   __device__ static Frag row(const char* tile, int row0, int c) {
     const int lane = threadIdx.x & 63;
-    const char* p = tile + (row0 + (lane & 31)) * kPitch + (c * kChunk + (lane >> 5) * (kChunk / 2)) *
-                                                               (int)sizeof(T);
-    return *reinterpret_cast<const Frag*>(p);
+    const int at = place(lane & 31, lane >> 5) ^ (c << 5);
+    return *reinterpret_cast<const Frag*>(tile + row0 * kPitch + at);
   }
 
-  // Column col0 + lane % 32 of part t of the rows from row0, in the order of a product's registers.
+  // Column col0 + lane % 32 of part t of the rows from row0, in the order of a product's registers
+  // (row0 and col0 multiples of 32).
   __device__ static Frag column(const char* tile, int row0, int col0, int t) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     if constexpr (sizeof(T) == 2) {
       // 16 lanes address four rows of 16 columns, and get a column of four rows each
-      const int r = row0 + 16 * t + 4 * half + ((lane & 15) >> 2);
-      const int c = col0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const char* p = tile + r * kPitch + c * 2;
+      const int r = 4 * half + ((lane & 15) >> 2), c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const char* p = tile + (row0 + 16 * t) * kPitch;
+      const int lo = (place(r, c >> 3) + (c & 4) * 2) ^ (col0 << 1);
+      const int hi = (place(r + 8, c >> 3) + (c & 4) * 2) ^ (col0 << 1);
       using S4 = short __attribute__((ext_vector_type(4)));
       using Lds = __attribute__((address_space(3))) S4;
       struct Both {
         S4 lo, hi;
       } v;
-      v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)p);
-      v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + 8 * kPitch));
+      v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + lo));
+      v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + hi));
       return __builtin_bit_cast(Frag, v);
     } else {
       Frag f;
+      const int c = lane & 31;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f[i] = *reinterpret_cast<const float*>(tile + (row0 + 8 * t + 4 * half + i) * kPitch +
-                                               (col0 + (lane & 31)) * 4);
+      for (int i = 0; i < 4; ++i) {
+        const int r = (8 * t + i) % 16 + 4 * half;
+        const int at = (place(r, c >> 2) + (c & 3) * 4) ^ (col0 << 2);
+        f[i] = *reinterpret_cast<const float*>(tile + (row0 + (8 * t + i) / 16 * 16) * kPitch + at);
+      }
       return f;
     }
   }
@@ -208,42 +304,69 @@ __device__ inline float other_half(float x) {
 }
 
 // ---- values that are not finite -------------------------------------------------------------
-// A hidden key's probability is 0, and 0 times an infinity or a NaN is NaN.  Tiles that a mask cuts
-// are looked over while they are loaded, and where one holds such a value the product takes 0 in
-// its place and adds what visible ones make of the result from a second product: of a code of the
+// A hidden key's probability is 0, and 0 times an infinity or a NaN is NaN.  In tiles that a mask
+// cuts, the operands are looked over, and where one holds such a value the product takes 0 in its
+// place and adds what visible ones make of the result from a second product: of a code of the
 // value (NaN 1, infinities 64 and 4096: sums of 32 of them, exact in every type) and of 1 where the
 // key is seen.
-template <class T>
-__device__ inline bool not_finite(T x) {
-  const float f = (float)x;
-  return !(__builtin_fabsf(f) < kInf32);
-}
-
-template <class T>
-__device__ inline bool any_not_finite(const Reg8<T>& v) {
-  bool any = false;
+// Not 0 where one of an operand's values is not finite: its exponent's bits are all set, and one
+// more carries out of them.
+template <class T, class Frag>
+__device__ inline uint32_t not_finite_bits(const Frag& v) {
+  constexpr uint32_t kExp = sizeof(T) == 4            ? 0x7F800000u
+                            : std::is_same_v<T, bf16> ? 0x7F807F80u
+                                                      : 0x7C007C00u;
+  constexpr uint32_t kOne = sizeof(T) == 4            ? 0x00800000u
+                            : std::is_same_v<T, bf16> ? 0x00800080u
+                                                      : 0x04000400u;
+  using U4 = uint32_t __attribute__((ext_vector_type(4)));
+  const U4 x = __builtin_bit_cast(U4, v);
+  uint32_t bad = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) any = any || not_finite(v[j]);
-  return any;
+  for (int i = 0; i < 4; ++i) bad |= (x[i] & kExp) + kOne;
+  return bad & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
 }
 
-// acc += (columns of the tile's 32 rows from row0) x w; careful: as above, w being 0 where `seen`
-// is.
-template <class T, int kDim>
-__device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int row0,
-                                   const F16& w, const F16& seen, bool careful) {
+// acc += (columns of the tile's 32 rows from row0) x w; cuts: w is 0 where seen(r) is false for
+// its register r.  kTwice: w to twice the type's bits, what its rounding leaves in a second product.
+template <class T, int kDim, bool kTwice, class Seen>
+__device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int row0, const F16& w,
+                                   bool cuts, Seen&& seen) {
   using L = Tile<T, kDim>;
-  typename L::Frag part[L::kParts];
+  constexpr bool kRest = kTwice && sizeof(T) == 2;
+  typename L::Frag part[L::kParts], rest[kRest ? L::kParts : 1];
 #pragma unroll
-  for (int t = 0; t < L::kParts; ++t) part[t] = L::part(w, t);
-  if (!careful) {
+  for (int t = 0; t < L::kParts; ++t) {
+    part[t] = L::part(w, t);
+    if constexpr (kRest) {
+      F16 left = w;
+#pragma unroll
+      for (int i = 0; i < L::kChunk / 2; ++i) left[t * (L::kChunk / 2) + i] -= (float)part[t][i];
+      rest[t] = L::part(left, t);
+    }
+  }
+  uint32_t bad = 0;
+  if (cuts) {
 #pragma unroll
     for (int d = 0; d < kDim / 32; ++d)
 #pragma unroll
       for (int t = 0; t < L::kParts; ++t)
-        acc[d] = mma(L::column(tile, row0, 32 * d, t), part[t], acc[d]);
+        bad |= not_finite_bits<T>(L::column(tile, row0, 32 * d, t));
+  }
+  if (!cuts || __builtin_expect(!__any(bad), 1)) {
+#pragma unroll
+    for (int d = 0; d < kDim / 32; ++d)
+#pragma unroll
+      for (int t = 0; t < L::kParts; ++t) {
+        const typename L::Frag v = L::column(tile, row0, 32 * d, t);
+        acc[d] = mma(v, part[t], acc[d]);
+        if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
+      }
     return;
   }
+  F16 ones;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ones[r] = seen(r) ? 1.0f : 0.0f;
 #pragma unroll
   for (int d = 0; d < kDim / 32; ++d) {
     F16 codes = {};
@@ -252,65 +375,113 @@ __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int 
       typename L::Frag v = L::column(tile, row0, 32 * d, t), code;
 #pragma unroll
       for (int i = 0; i < L::kChunk / 2; ++i) {
-        const float f = (float)v[i];
-        const bool bad = not_finite(v[i]);
-        code[i] = (T)(!bad ? 0.0f : f != f ? 1.0f : f > 0.0f ? 64.0f : 4096.0f);
-        v[i] = bad ? (T)0.0f : v[i];
+        const float f = (float)v[i], size = __builtin_fabsf(f);
+        const float inf = f > 0.0f ? 64.0f : 4096.0f;
+        code[i] = (T)(size < kInf32 ? 0.0f : size == kInf32 ? inf : 1.0f);
+        v[i] = size < kInf32 ? v[i] : (T)0.0f;
       }
       acc[d] = mma(v, part[t], acc[d]);
-      codes = mma(code, L::part(seen, t), codes);
+      if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
+      codes = mma(code, L::part(ones, t), codes);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int n = (int)codes[r];
-      if (n & 63) acc[d][r] = __builtin_nanf("");
-      if (n & (63 << 6)) acc[d][r] += kInf32;
-      if (n >> 12) acc[d][r] -= kInf32;
+      const float up = n & (63 << 6) ? kInf32 : 0.0f, down = n >> 12 ? -kInf32 : 0.0f;
+      acc[d][r] += (n & 63 ? __builtin_nanf("") : up) + down;
     }
   }
 }
 
 // ---- loading and storing --------------------------------------------------------------------
-// Eight columns of a row that is there, 0 from column dim on.
-template <class T>
+// Eight columns of a row that is there, 0 from column dim on; kWhole: dim is a multiple of 8.
+template <class T, bool kWhole>
 __device__ inline Reg8<T> load_piece(const T* row, int col, int dim) {
-  if (dim % 8 == 0) return block_of_raw<T, true>(load_raw<T, true>(row, col, dim), col, dim);
-  return block_of_raw<T, false>(load_raw<T, false>(row, col, dim), col, dim);
+  return block_of_raw<T, kWhole>(load_raw<T, kWhole>(row, col, dim), col, dim);
 }
 
 // The operands of a row: its chunks, 0 from column dim on.
-template <class T, int kDim>
+template <class T, int kDim, bool kWhole>
 __device__ inline void load_row(typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
                                 const T* row, int dim) {
   const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
   for (int c = 0; c < kDim / Operand<T>::kChunk; ++c) {
     if constexpr (sizeof(T) == 2) {
-      f[c] = load_piece(row, 16 * c + 8 * half, dim);
+      f[c] = load_piece<T, kWhole>(row, 16 * c + 8 * half, dim);
     } else {
-      const Reg8<T> v = load_piece(row, 8 * c, dim);
+      const Reg8<T> v = load_piece<T, kWhole>(row, 8 * c, dim);
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[c][i] = half ? v[4 + i] : v[i];
     }
   }
 }
 
-// Loads kTileKeys rows into LDS, zeros for rows from `rows` on (of which there is at least one);
-// row_at(i): row i < rows.  True where a value is not finite.
-template <class T, int kDim, class RowAt>
-__device__ inline bool load_tile(char* tile, int rows, int dim, RowAt&& row_at) {
-  constexpr int kPieces = kDim / 8;
-  bool bad = false;
+// Whether rows are whole chunks of 16 bytes on such a boundary, which can be loaded straight into
+// LDS.
+inline bool chunks_aligned(int dtype, int64_t dim, std::initializer_list<const void*> pointers,
+                           std::initializer_list<int64_t> strides) {
+  const int64_t size = dtype_size(dtype);
+  bool ok = dim % 8 == 0;
+  for (const void* p : pointers) ok = ok && on_16_bytes(p);
+  for (const int64_t s : strides) ok = ok && s * size % 16 == 0;
+  return ok;
+}
+
+inline bool direct_tiles(const omq_attention_args& a) {
+  return chunks_aligned(a.dtype, a.dim, {a.k, a.v},
+                        {a.k_seq_stride, a.k_row_stride, a.k_head_stride, a.v_seq_stride,
+                         a.v_row_stride, a.v_head_stride});
+}
+
+// Zeros where a tile's rows have no column (from dim on): before the first load_tile, and a
+// barrier between the two.
+template <class T, int kDim>
+__device__ inline void clear_tile(char* tile, int dim) {
+  if (dim == kDim) return;
+  for (int i = threadIdx.x; i < Tile<T, kDim>::kBytes / 16; i += kWaves * kWave)
+    *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
+}
+
+// Loads kTileKeys rows into LDS, the last of `rows` (at least one) again in place of those behind
+// it; row_at(i): row i < rows.  kDirect: chunks_aligned; the loads are under way when this returns.
+template <class T, int kDim, bool kDirect, class RowAt>
+__device__ inline void load_tile(char* tile, int rows, int dim, RowAt&& row_at) {
+  using L = Tile<T, kDim>;
+  if constexpr (kDirect) {
+    constexpr int kEach = 16 / (int)sizeof(T);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-  for (int i = threadIdx.x; i < kTileKeys * kPieces; i += kWaves * kWave) {
-    const int r = i / kPieces, col = i % kPieces * 8;
-    Reg8<T> v = load_piece<T>(row_at(r < rows ? r : rows - 1), col, dim);
-    if (r >= rows) v = Reg8<T>{};
-    bad = bad || any_not_finite<T>(v);
-    using Out __attribute__((aligned(16))) = Reg8<T>;
-    *reinterpret_cast<Out*>(tile + r * Tile<T, kDim>::kPitch + col * (int)sizeof(T)) = v;
+    for (int i = 0; i < L::kBytes / (kWaves * kWave * 16); ++i) {
+      const int from = (i * kWaves + wave) * kWave * 16;  // this wave's 64 chunks
+      const int at = from + 16 * (threadIdx.x & 63);
+      const int r = at / L::kPitch, chunk = (at / 16 % L::kPer) ^ L::swap(r);
+      if (chunk * kEach < dim)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(row_at(r < rows ? r : rows - 1) +
+                                                            chunk * kEach),
+            (__attribute__((address_space(3))) void*)(tile + from), 16, 0, 0);
+    }
+  } else {
+    constexpr int kPieces = kDim / 8;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kTileKeys * kPieces; i += kWaves * kWave) {
+      const int r = i / kPieces, col = i % kPieces * 8;
+      const Reg8<T> v = load_piece<T, false>(row_at(r < rows ? r : rows - 1), col, dim);
+      using Frag = typename L::Frag;
+      Frag f[sizeof(T) / 2];
+      __builtin_memcpy(f, &v, sizeof(v));
+#pragma unroll
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+        *reinterpret_cast<Frag*>(tile + L::place(r, col * (int)sizeof(T) / 16 + h)) = f[h];
+    }
   }
-  return bad;
+}
+
+// The loads into LDS of this wave have arrived, and all waves come here.
+__device__ inline void tiles_ready() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
 }
 
 // Stores a lane's column of a result [kDim columns of a row, 32 rows] as a row, times `scale`.
@@ -342,6 +513,12 @@ inline AttentionArgs attention_layout(const omq_attention_args& a) {
   r.a = a;
   r.group = a.q_heads / a.k_heads;
   r.score_scale = a.scale * kLog2E;
+  if (r.group > 1) {  // exact for rows below 2^31
+    int log = 0;
+    while ((1ll << log) < r.group) ++log;
+    r.group_mul = (uint32_t)((1ull << (31 + log)) / r.group + 1);
+    r.group_shift = log - 1;
+  }
   return r;
 }
 
@@ -353,13 +530,17 @@ inline void tiles_of(AttentionArgs* r, int64_t rows, int64_t group, int64_t tile
                            : r->batch_tiles * r->a.sequences;
 }
 
+// f(element, columns that are held, whether tiles go straight into LDS) for a launch.
 template <class F>
-void with_head(int dtype, int dim, F&& f) {
+void with_head(int dtype, int dim, bool direct, F&& f) {
+  const auto loaded = [&](auto t, auto held) {
+    if (direct) return f(t, held, std::true_type{});
+    return f(t, held, std::false_type{});
+  };
   const auto sized = [&](auto t) {
-    using T = decltype(t);
-    if (dim <= 32) return f(T{}, std::integral_constant<int, 32>{});
-    if (dim <= 64) return f(T{}, std::integral_constant<int, 64>{});
-    return f(T{}, std::integral_constant<int, 128>{});
+    if (dim <= 32) return loaded(t, std::integral_constant<int, 32>{});
+    if (dim <= 64) return loaded(t, std::integral_constant<int, 64>{});
+    return loaded(t, std::integral_constant<int, 128>{});
   };
   if (dtype == OMQ_NET_F32) return sized(float{});
   if (dtype == OMQ_NET_BF16) return sized(bf16{});

@@ -13,63 +13,50 @@
 namespace omq_net {
 namespace {
 
-template <class T, int kDim>
-__global__ __launch_bounds__(kWaves* kWave) void attention_kernel(AttentionArgs args) {
+// Probabilities are formed about a maximum that follows the running one only where that has grown
+// by more than a factor of 2^8: the sums' rescaling, a product for each of a row's columns, is
+// left out for most tiles, and a probability is at most 2^8 (float16 holds 2^15).
+constexpr float kLag = 8.0f;
+
+template <class T, int kDim, bool kDirect>
+__global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(16))) char keys[L::kBytes];
-  __shared__ __attribute__((aligned(16))) char values[L::kBytes];
-  __shared__ int bad[2];
+  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
   const omq_attention_args& a = args.a;
-  const int64_t block = block_index();
-  const int64_t slot = block / a.k_heads;
-  if (slot >= args.slots) return;
-  const int kv = (int)(block % a.k_heads), group = args.group;
-  int64_t tile;
-  Sequence q;
-  if (a.q_starts) {
-    q = sequence_of(args, find_piece(a.q_starts, a.sequences, a.q_len, group, kTileRows, slot,
-                                     &tile));
-  } else {
-    q = sequence_of(args, slot / args.batch_tiles);
-    tile = slot % args.batch_tiles;
+  Place at;
+  if (!place_of_queries(args, kTileRows, &at)) return;
+  const Sequence& q = at.q;
+  const int rows = (int)((int64_t)q.lq * args.group), lane = threadIdx.x & 63;
+  const Rows x = rows_of(args, q, at.kv, (int)(at.tile * kTileRows), rows);
+
+  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
+  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
+  const auto load = [&](int k0, int turn) {
+    load_tile<T, kDim, kDirect>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+      return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
+    });
+    load_tile<T, kDim, kDirect>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+      return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
+    });
+  };
+  if (kDirect && a.dim < kDim) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
+    __syncthreads();
   }
-  const int64_t rows = (int64_t)q.lq * group, r0 = tile * kTileRows;
-  if (tile < 0 || r0 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-
-  // this lane's row; lanes behind the last one do it again and store nothing
-  const int64_t mine = r0 + kWaveRows * wave + (lane & 31);
-  const bool there = mine < rows;
-  const int64_t row = there ? mine : rows - 1;
-  const int query = (int)(row / group), head = kv * group + (int)(row % group);
-  const int shift = q.lk - q.lq;
-  const int limit = a.causal ? cut(query + shift + 1, 0, q.lk) : q.lk;  // the keys that it sees
-  const int first_query = (int)(r0 / group);
-  const int64_t last_row = r0 + kTileRows < rows ? r0 + kTileRows - 1 : rows - 1;
-  const int most = a.causal ? cut((int)(last_row / group) + shift + 1, 0, q.lk) : q.lk;
-  const int least = a.causal ? cut(first_query + shift + 1, 0, q.lk) : q.lk;
-
+  if (x.block_most > 0) load(0, 0);
   typename L::Frag qf[L::kChunks];
-  load_row<T, kDim>(qf, static_cast<const T*>(a.q) + q.q_at + query * a.q_row_stride +
-                            head * a.q_head_stride, a.dim);
-  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + kv * a.k_head_stride;
-  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + kv * a.v_head_stride;
+  load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
+                            x.head * a.q_head_stride, a.dim);
 
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;  // l: over this half's keys
-  for (int k0 = 0, turn = 0; k0 < most; k0 += kTileKeys, turn ^= 1) {
-    const int left = q.lk - k0;
-    __syncthreads();
-    if (threadIdx.x == 0) bad[turn ^ 1] = 0;
-    load_tile<T, kDim>(keys, left, a.dim,
-                       [&](int i) { return k_rows + (int64_t)(k0 + i) * a.k_row_stride; });
-    const bool found = load_tile<T, kDim>(
-        values, left, a.dim, [&](int i) { return v_rows + (int64_t)(k0 + i) * a.v_row_stride; });
-    if (found) bad[turn] = 1;
-    __syncthreads();
-    const bool cuts = k0 + kTileKeys > least;  // some row does not see all of the tile
-    const bool careful = cuts && bad[turn];
+  for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
+    tiles_ready();
+    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, turn ^ 1);
+    if (k0 >= x.most) continue;
+    const char *keys = tiles[turn][0], *values = tiles[turn][1];
+    const bool cuts = k0 + kTileKeys > x.least;  // some row does not see all of the tile
     F16 s[2];
     float top = -kInf32;
 #pragma unroll
@@ -77,40 +64,45 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_kernel(AttentionArgs 
       s[b] = F16{};
 #pragma unroll
       for (int c = 0; c < L::kChunks; ++c) s[b] = mma(L::row(keys, 32 * b, c), qf[c], s[b]);
-      if (cuts) {
+    }
+    if (cuts) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + result_row(r) >= limit) s[b][r] = -kInf32;
-      }
+          if (k0 + 32 * b + result_row(r) >= x.limit) s[b][r] = -kInf32;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    }
-    top = fmaxf(fmaxf(top, other_half(top)), m);
-    const float base = top == -kInf32 ? 0.0f : top;
-    const float keep = __builtin_amdgcn_exp2f((m - base) * args.score_scale);
-    m = top;
-    l *= keep;
+    top = fmaxf(top, other_half(top));
+    if (__any((top - m) * args.score_scale > kLag)) {  // (m is -inf at first)
+      const float next = fmaxf(m, top);
+      const float keep =
+          next == -kInf32 ? 1.0f : __builtin_amdgcn_exp2f((m - next) * args.score_scale);
+      m = next;
+      l *= keep;
 #pragma unroll
-    for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
+      for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
+    }
+    const float base = m == -kInf32 ? 0.0f : m * args.score_scale;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f((s[b][r] - base) * args.score_scale);
+        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], args.score_scale, -base));
         l += s[b][r];
       }
-      F16 seen = {};
-      if (careful) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) seen[r] = k0 + 32 * b + result_row(r) < limit ? 1.0f : 0.0f;
-      }
-      add_columns<T, kDim>(o, values, 32 * b, s[b], seen, careful);
+      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, [&](int r) {
+        return k0 + 32 * b + result_row(r) < x.limit;
+      });
     }
   }
   l += other_half(l);
-  if (!there) return;
+  if (!x.there) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int64_t out_row = (q.q_first + query) * a.q_heads + head;
+  const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   store_column<T, kDim>(static_cast<T*>(args.out) + out_row * a.dim, o, inv, a.dim);
   if (args.lse && lane < 32)
     args.lse[out_row] =
@@ -173,8 +165,8 @@ int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, vo
   tiles_of(&args, a->q_len, args.group, kTileRows);
   args.out = out, args.lse = lse;
   const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
-  with_head(a->dtype, a->dim, [&](auto t, auto dim) {
-    attention_kernel<decltype(t), dim.value>
+  with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
+    attention_kernel<decltype(t), dim.value, direct.value>
         <<<grid, kWaves * kWave, 0, (hipStream_t)stream>>>(args);
   });
   return net_status(name);

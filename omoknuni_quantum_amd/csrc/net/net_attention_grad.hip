@@ -7,79 +7,68 @@
 // split over workgroups, which would take atomics or float32 copies of dq; every result is the
 // same bits at every call.  Rows of queries that share a key head are rows of one sum.
 // ds is rounded to the elements' type for its products, times scale, without which float16 would
-// overflow earlier.
+// overflow earlier.  Its sum over a row is 0 but for what the rounding of out took from delta, which
+// the first launch so finds and the second has again; dq, for which that comes too late, has ds to
+// twice the type's bits instead.  (With neither, the gradients are off by 1.6 times their own
+// rounding and more, with both by 1.3 and 1.4 times.)
 #include "net_attention.h"
 
 namespace omq_net {
 namespace {
 
-template <class T, int kDim>
+template <class T, int kDim, bool kDirect>
 __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(16))) char keys[L::kBytes];
-  __shared__ __attribute__((aligned(16))) char values[L::kBytes];
-  __shared__ int bad[2];
+  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
   const omq_attention_args& a = args.a;
-  const int64_t block = block_index();
-  const int64_t slot = block / a.k_heads;
-  if (slot >= args.slots) return;
-  const int kv = (int)(block % a.k_heads), group = args.group;
-  int64_t tile;
-  Sequence q;
-  if (a.q_starts) {
-    q = sequence_of(args, find_piece(a.q_starts, a.sequences, a.q_len, group, kTileRows, slot,
-                                     &tile));
-  } else {
-    q = sequence_of(args, slot / args.batch_tiles);
-    tile = slot % args.batch_tiles;
-  }
-  const int64_t rows = (int64_t)q.lq * group, r0 = tile * kTileRows;
-  if (tile < 0 || r0 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-  const int64_t mine = r0 + kWaveRows * wave + (lane & 31);
-  const bool there = mine < rows;
-  const int64_t row = there ? mine : rows - 1;
-  const int query = (int)(row / group), head = kv * group + (int)(row % group);
-  const int shift = q.lk - q.lq;
-  const int limit = a.causal ? cut(query + shift + 1, 0, q.lk) : q.lk;
-  const int64_t last_row = r0 + kTileRows < rows ? r0 + kTileRows - 1 : rows - 1;
-  const int most = a.causal ? cut((int)(last_row / group) + shift + 1, 0, q.lk) : q.lk;
-  const int least = a.causal ? cut((int)(r0 / group) + shift + 1, 0, q.lk) : q.lk;
+  Place at;
+  if (!place_of_queries(args, kTileRows, &at)) return;
+  const Sequence& q = at.q;
+  const int rows = (int)((int64_t)q.lq * args.group), lane = threadIdx.x & 63;
+  const Rows x = rows_of(args, q, at.kv, (int)(at.tile * kTileRows), rows);
 
+  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
+  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
+  const auto load = [&](int k0, int turn) {
+    load_tile<T, kDim, kDirect>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+      return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
+    });
+    load_tile<T, kDim, kDirect>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+      return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
+    });
+  };
+  if (kDirect && a.dim < kDim) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
+    __syncthreads();
+  }
+  if (x.block_most > 0) load(0, 0);
   typename L::Frag qf[L::kChunks], gf[L::kChunks];
-  load_row<T, kDim>(qf, static_cast<const T*>(a.q) + q.q_at + query * a.q_row_stride +
-                            head * a.q_head_stride, a.dim);
-  const int64_t out_row = (q.q_first + query) * a.q_heads + head;
-  load_row<T, kDim>(gf, static_cast<const T*>(args.grad_out) + out_row * a.dim, a.dim);
+  load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
+                                     x.head * a.q_head_stride, a.dim);
+  const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
+  load_row<T, kDim, kDirect>(gf, static_cast<const T*>(args.grad_out) + out_row * a.dim, a.dim);
   float delta = 0.0f;
   {
     typename L::Frag of[L::kChunks];
-    load_row<T, kDim>(of, static_cast<const T*>(args.out_in) + out_row * a.dim, a.dim);
+    load_row<T, kDim, kDirect>(of, static_cast<const T*>(args.out_in) + out_row * a.dim, a.dim);
 #pragma unroll
     for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
       for (int i = 0; i < L::kChunk / 2; ++i) delta = fmaf((float)gf[c][i], (float)of[c][i], delta);
   }
   delta += other_half(delta);
-  if (there && lane < 32) args.delta[out_row] = delta;
   const float lse = args.lse_in[out_row];
   const float base = lse == -kInf32 ? 0.0f : lse * kLog2E;
 
-  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + kv * a.k_head_stride;
-  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + kv * a.v_head_stride;
   F16 dq[kDim / 32] = {};
-  for (int k0 = 0, turn = 0; k0 < most; k0 += kTileKeys, turn ^= 1) {
-    const int left = q.lk - k0;
-    __syncthreads();
-    if (threadIdx.x == 0) bad[turn ^ 1] = 0;
-    const bool found = load_tile<T, kDim>(
-        keys, left, a.dim, [&](int i) { return k_rows + (int64_t)(k0 + i) * a.k_row_stride; });
-    load_tile<T, kDim>(values, left, a.dim,
-                       [&](int i) { return v_rows + (int64_t)(k0 + i) * a.v_row_stride; });
-    if (found) bad[turn] = 1;
-    __syncthreads();
-    const bool cuts = k0 + kTileKeys > least, careful = cuts && bad[turn];
+  float rest = 0.0f;  // sum p (g.v - delta): what out's rounding took from delta
+  for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
+    tiles_ready();
+    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, turn ^ 1);
+    if (k0 >= x.most) continue;
+    const char *keys = tiles[turn][0], *values = tiles[turn][1];
+    const bool cuts = k0 + kTileKeys > x.least;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       F16 s = {}, dp = {};
@@ -87,128 +76,155 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
       for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 32 * b, c), qf[c], s);
 #pragma unroll
       for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(values, 32 * b, c), gf[c], dp);
-      F16 seen = {};
+      const auto seen = [&](int r) { return k0 + 32 * b + result_row(r) < x.limit; };
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
-        s[r] = p * (dp[r] - delta) * a.scale;
-        if (cuts) {
-          const bool sees = k0 + 32 * b + result_row(r) < limit;
-          s[r] = sees ? s[r] : 0.0f;
-          seen[r] = sees ? 1.0f : 0.0f;
-        }
+        s[r] = p * (dp[r] - delta);
       }
-      add_columns<T, kDim>(dq, keys, 32 * b, s, seen, careful);
+      if (cuts) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = seen(r) ? s[r] : 0.0f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        rest += s[r];
+        s[r] *= a.scale;
+      }
+      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, seen);
     }
   }
-  if (there)
-    store_column<T, kDim>(static_cast<T*>(args.grad_q) + out_row * a.dim, dq, 1.0f, a.dim);
+  rest += other_half(rest);
+  if (!x.there) return;
+  if (lane < 32) args.delta[out_row] = delta + rest;
+  store_column<T, kDim>(static_cast<T*>(args.grad_q) + out_row * a.dim, dq, 1.0f, a.dim);
 }
 
 // A workgroup has 128 keys, a wave 32 of them; 64 rows of queries at a time pass through LDS.
-template <class T, int kDim>
+template <class T, int kDim, bool kDirect>
 __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(16))) char queries[L::kBytes];
-  __shared__ __attribute__((aligned(16))) char grads[L::kBytes];
-  __shared__ __attribute__((aligned(16))) float bases[kTileKeys], deltas[kTileKeys];
-  __shared__ __attribute__((aligned(16))) int limits[kTileKeys];
-  __shared__ int bad[2];
+  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // queries, gradients
+  __shared__ __attribute__((aligned(16))) float bases[2][kTileKeys], deltas[2][kTileKeys];
+  __shared__ __attribute__((aligned(16))) int limits[2][kTileKeys];
   const omq_attention_args& a = args.a;
-  const int64_t block = block_index();
-  const int64_t slot = block / a.k_heads;
-  if (slot >= args.slots) return;
-  const int kv = (int)(block % a.k_heads), group = args.group;
-  int64_t tile;
-  Sequence q;
-  if (a.q_starts) {
-    q = sequence_of(args, find_piece(a.k_starts, a.sequences, a.k_len, 1, kTileRows, slot, &tile));
-  } else {
-    q = sequence_of(args, slot / args.batch_tiles);
-    tile = slot % args.batch_tiles;
-  }
-  const int64_t j0 = tile * kTileRows;
-  if (tile < 0 || j0 >= q.room) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-  const int mine = (int)j0 + kWaveRows * wave + (lane & 31);
-  const bool there = mine < q.room, used = mine < q.lk;
+  Place at;
+  if (!place_of_keys(args, kTileRows, &at)) return;
+  const Sequence& q = at.q;
+  const int j0 = (int)(at.tile * kTileRows), group = args.group, kv = at.kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int from = j0 + kWaveRows * wave, mine = from + (lane & 31);
+  const bool there = mine < q.room;
   const int key = there ? mine : q.room - 1;
   const int shift = q.lk - q.lq;
-  const int64_t rows = (int64_t)q.lq * group;
-
-  typename L::Frag kf[L::kChunks], vf[L::kChunks];
-  load_row<T, kDim>(kf, static_cast<const T*>(a.k) + q.k_at + key * a.k_row_stride +
-                            kv * a.k_head_stride, a.dim);
-  load_row<T, kDim>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
-                            kv * a.v_head_stride, a.dim);
-  F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
-  // the first row that sees a key of this tile; the last key of it that is in use
+  const int rows = (int)((int64_t)q.lq * group);
+  // the rows that see a key of the workgroup: from `first` (on a tile's boundary) to `end`
   int64_t first = 0;
-  if (a.causal && j0 > shift) first = (j0 - shift) * group / kTileKeys * kTileKeys;
-  const int last_key = (int)(j0 + kTileRows < q.lk ? j0 + kTileRows : q.lk) - 1;
-  const int64_t end = j0 < q.lk ? rows : 0;
-  int turn = 0;
-  for (int64_t r0 = first; r0 < end; r0 += kTileKeys, turn ^= 1) {
-    const int left = rows - r0 < kTileKeys ? (int)(rows - r0) : kTileKeys;
-    const auto query_of = [&](int i) { return (int)((r0 + i) / group); };
-    const auto head_of = [&](int i) { return kv * group + (int)((r0 + i) % group); };
-    __syncthreads();
-    if (threadIdx.x == 0) bad[turn ^ 1] = 0;
-    bool found = load_tile<T, kDim>(queries, left, a.dim, [&](int i) {
-      return static_cast<const T*>(a.q) + q.q_at + query_of(i) * a.q_row_stride +
-             head_of(i) * a.q_head_stride;
-    });
-    found |= load_tile<T, kDim>(grads, left, a.dim, [&](int i) {
-      return static_cast<const T*>(args.grad_out) +
-             ((q.q_first + query_of(i)) * a.q_heads + head_of(i)) * a.dim;
-    });
-    if (found) bad[turn] = 1;
+  if (a.causal && j0 > shift)
+    first = (int64_t)(j0 - shift) * group / kTileKeys * kTileKeys;
+  const int end = j0 < q.lk ? rows : 0;
+
+  const T* q_rows = static_cast<const T*>(a.q) + q.q_at + kv * group * a.q_head_stride;
+  const int64_t out_first = q.q_first * a.q_heads + kv * group;
+  const T* g_rows = static_cast<const T*>(args.grad_out) + out_first * a.dim;
+  // row r's place in q, and in arrays of rows of heads
+  const auto q_place = [&](int r) {
+    const int query = query_of(args, r);
+    return query * a.q_row_stride + (r - query * group) * a.q_head_stride;
+  };
+  const auto out_place = [&](int r) {
+    const int query = query_of(args, r);
+    return (int64_t)query * a.q_heads + (r - query * group);
+  };
+  const auto load = [&](int r0, int turn) {
+    load_tile<T, kDim, kDirect>(tiles[turn][0], rows - r0, a.dim,
+                                [&](int i) { return q_rows + q_place(r0 + i); });
+    load_tile<T, kDim, kDirect>(tiles[turn][1], rows - r0, a.dim,
+                                [&](int i) { return g_rows + out_place(r0 + i) * a.dim; });
+  };
+  // what the first wave brings of a tile's rows
+  float lse = 0.0f, delta = 0.0f;
+  const auto fetch = [&](int r0) {
     if (threadIdx.x < kTileKeys) {
-      const int i = threadIdx.x < left ? threadIdx.x : left - 1;
-      const int64_t at = (q.q_first + query_of(i)) * a.q_heads + head_of(i);
-      const float lse = args.lse_in[at];
-      bases[threadIdx.x] = lse == -kInf32 ? 0.0f : lse * kLog2E;
-      deltas[threadIdx.x] = args.delta[at];
-      limits[threadIdx.x] = (int)threadIdx.x >= left ? 0
-                            : a.causal ? cut(query_of(i) + shift + 1, 0, q.lk) : q.lk;
+      const int64_t i = out_first + out_place(r0 + lane < rows ? r0 + lane : rows - 1);
+      lse = args.lse_in[i], delta = args.delta[i];
     }
+  };
+  const auto put = [&](int r0, int turn) {
+    if (threadIdx.x < kTileKeys) {
+      const int r = r0 + lane;
+      bases[turn][lane] = lse == -kInf32 ? 0.0f : lse * kLog2E;
+      deltas[turn][lane] = delta;
+      limits[turn][lane] = r >= rows ? 0
+                           : a.causal ? cut(query_of(args, r) + shift + 1, 0, q.lk)
+                                      : q.lk;
+    }
+  };
+  if (kDirect && a.dim < kDim) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
     __syncthreads();
-    const bool cuts = left < kTileKeys || j0 + kTileRows > q.lk ||
-                      (a.causal && last_key >= query_of(0) + shift + 1);
-    const bool careful = cuts && bad[turn];
+  }
+  if (first < end) {
+    load((int)first, 0);
+    fetch((int)first);
+    put((int)first, 0);
+  }
+  typename L::Frag kf[L::kChunks], vf[L::kChunks];
+  load_row<T, kDim, kDirect>(kf, static_cast<const T*>(a.k) + q.k_at + key * a.k_row_stride +
+                                     kv * a.k_head_stride, a.dim);
+  load_row<T, kDim, kDirect>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
+                                     kv * a.v_head_stride, a.dim);
+  F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
+  int turn = 0;
+  for (int64_t next = first; next < end; next += kTileKeys, turn ^= 1) {
+    const int r0 = (int)next;
+    const bool more = next + kTileKeys < end;
+    tiles_ready();
+    if (more) load(r0 + kTileKeys, turn ^ 1), fetch(r0 + kTileKeys);
+    const char *queries = tiles[turn][0], *grads = tiles[turn][1];
+    // some row does not see all of the wave's keys; or none does
+    const int low = limits[turn][0], high = limits[turn][kTileKeys - 1];
+    const bool cuts = r0 + kTileKeys > rows || from + kWaveRows > q.lk ||
+                      from + kWaveRows > __builtin_amdgcn_readfirstlane(low);
+    if (from < __builtin_amdgcn_readfirstlane(high) || r0 + kTileKeys > rows) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      F16 s = {}, dp = {};
+      for (int b = 0; b < 2; ++b) {
+        F16 s = {}, dp = {};
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c), kf[c], s);
+        for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c), kf[c], s);
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c), vf[c], dp);
-      F16 p, seen = {};
+        for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c), vf[c], dp);
+        const auto seen = [&](int r) { return mine < limits[turn][32 * b + result_row(r)]; };
+        F16 p;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = 32 * b + result_row(r);
-        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -bases[i]));
-        s[r] = p[r] * (dp[r] - deltas[i]) * a.scale;
-        if (cuts) {
-          const bool sees = mine < limits[i];
-          p[r] = sees ? p[r] : 0.0f;
-          s[r] = sees ? s[r] : 0.0f;
-          seen[r] = sees ? 1.0f : 0.0f;
+        for (int r = 0; r < 16; ++r) {
+          const int i = 32 * b + result_row(r);
+          p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -bases[turn][i]));
+          s[r] = p[r] * (dp[r] - deltas[turn][i]) * a.scale;
         }
+        if (cuts) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool sees = seen(r);
+            p[r] = sees ? p[r] : 0.0f;
+            s[r] = sees ? s[r] : 0.0f;
+          }
+        }
+        add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, seen);
+        add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, seen);
       }
-      add_columns<T, kDim>(dv, grads, 32 * b, p, seen, careful);
-      add_columns<T, kDim>(dk, queries, 32 * b, s, seen, careful);
     }
+    if (more) put(r0 + kTileKeys, turn ^ 1);
   }
   if (!there) return;
-  if (!used) {  // (whatever the queries hold)
+  if (mine >= q.lk) {  // (whatever the queries hold)
 #pragma unroll
     for (int d = 0; d < kDim / 32; ++d) dk[d] = F16{}, dv[d] = F16{};
   }
-  const int64_t at = ((q.k_first + key) * a.k_heads + kv) * a.dim;
-  store_column<T, kDim>(static_cast<T*>(args.grad_k) + at, dk, 1.0f, a.dim);
-  store_column<T, kDim>(static_cast<T*>(args.grad_v) + at, dv, 1.0f, a.dim);
+  const int64_t out = ((q.k_first + key) * a.k_heads + kv) * a.dim;
+  store_column<T, kDim>(static_cast<T*>(args.grad_k) + out, dk, 1.0f, a.dim);
+  store_column<T, kDim>(static_cast<T*>(args.grad_v) + out, dv, 1.0f, a.dim);
 }
 
 int64_t delta_bytes(const omq_attention_args& a) {
@@ -249,15 +265,19 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
   if (queries) {
     tiles_of(&args, a->q_len, args.group, kTileRows);
     const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
-    with_head(a->dtype, a->dim, [&](auto t, auto dim) {
-      attention_grad_q_kernel<decltype(t), dim.value><<<grid, kWaves * kWave, 0, st>>>(args);
+    with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
+      attention_grad_q_kernel<decltype(t), dim.value, direct.value>
+          <<<grid, kWaves * kWave, 0, st>>>(args);
     });
   }
   if (keys) {
     tiles_of(&args, a->k_len, 1, kTileRows);
     const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
-    with_head(a->dtype, a->dim, [&](auto t, auto dim) {
-      attention_grad_kv_kernel<decltype(t), dim.value><<<grid, kWaves * kWave, 0, st>>>(args);
+    const bool rows_direct = chunks_aligned(a->dtype, a->dim, {a->q, grad_out},
+                                            {a->q_seq_stride, a->q_row_stride, a->q_head_stride});
+    with_head(a->dtype, a->dim, rows_direct, [&](auto t, auto dim, auto direct) {
+      attention_grad_kv_kernel<decltype(t), dim.value, direct.value>
+          <<<grid, kWaves * kWave, 0, st>>>(args);
     });
   }
   return net_status(name);
