@@ -50,10 +50,12 @@ def build_library(out: str | None = None, verbose: bool = False) -> str:
 
 
 # The policy network's operators (csrc/net) are a library of their own: plain -O3, so that sums
-# of products contract into FMA.
+# of products contract into FMA.  The results of matrix instructions stay in vector registers: they
+# are copied there otherwise in kernels of one wave a SIMD (the attention's gradient).
 NET_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    "-mllvm", "-amdgpu-mfma-vgpr-form",
 ]
 
 

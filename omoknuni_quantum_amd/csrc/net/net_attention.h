@@ -305,14 +305,13 @@ __device__ inline float other_half(float x) {
 
 // ---- values that are not finite -------------------------------------------------------------
 // A hidden key's probability is 0, and 0 times an infinity or a NaN is NaN.  In tiles that a mask
-// cuts, the operands are looked over, and where one holds such a value the product takes 0 in its
-// place and adds what visible ones make of the result from a second product: of a code of the
-// value (NaN 1, infinities 64 and 4096: sums of 32 of them, exact in every type) and of 1 where the
-// key is seen.
-// Not 0 where one of an operand's values is not finite: its exponent's bits are all set, and one
-// more carries out of them.
+// cuts, products take 0 in place of such values, and note it; what those among them that are seen
+// make of a result is added when it has been stored (add_hidden).
+//
+// Puts 0 in place of an operand's values that are not finite (all bits of the exponent set: one
+// more carries out of them) and says in `found` where there was one.
 template <class T, class Frag>
-__device__ inline uint32_t not_finite_bits(const Frag& v) {
+__device__ inline Frag finite_only(const Frag& v, uint32_t& found) {
   constexpr uint32_t kExp = sizeof(T) == 4            ? 0x7F800000u
                             : std::is_same_v<T, bf16> ? 0x7F807F80u
                                                       : 0x7C007C00u;
@@ -320,18 +319,22 @@ __device__ inline uint32_t not_finite_bits(const Frag& v) {
                             : std::is_same_v<T, bf16> ? 0x00800080u
                                                       : 0x04000400u;
   using U4 = uint32_t __attribute__((ext_vector_type(4)));
-  const U4 x = __builtin_bit_cast(U4, v);
-  uint32_t bad = 0;
+  U4 x = __builtin_bit_cast(U4, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (x[i] & kExp) + kOne;
-  return bad & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bad = ((x[i] & kExp) + kOne) & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
+    found |= bad;
+    // (the sign's bit and those below it)
+    x[i] &= sizeof(T) == 4 ? ~(uint32_t)((int32_t)bad >> 31) : ~((bad << 1) - (bad >> 15));
+  }
+  return __builtin_bit_cast(Frag, x);
 }
 
-// acc += (columns of the tile's 32 rows from row0) x w; cuts: w is 0 where seen(r) is false for
-// its register r.  kTwice: w to twice the type's bits, what its rounding leaves in a second product.
-template <class T, int kDim, bool kTwice, class Seen>
+// acc += (columns of the tile's 32 rows from row0) x w; cuts: a mask cuts the tile.  kTwice: w to
+// twice the type's bits, what its rounding leaves in a second product.
+template <class T, int kDim, bool kTwice>
 __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int row0, const F16& w,
-                                   bool cuts, Seen&& seen) {
+                                   bool cuts, uint32_t& found) {
   using L = Tile<T, kDim>;
   constexpr bool kRest = kTwice && sizeof(T) == 2;
   typename L::Frag part[L::kParts], rest[kRest ? L::kParts : 1];
@@ -345,50 +348,36 @@ __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int 
       rest[t] = L::part(left, t);
     }
   }
-  uint32_t bad = 0;
-  if (cuts) {
-#pragma unroll
-    for (int d = 0; d < kDim / 32; ++d)
-#pragma unroll
-      for (int t = 0; t < L::kParts; ++t)
-        bad |= not_finite_bits<T>(L::column(tile, row0, 32 * d, t));
-  }
-  if (!cuts || __builtin_expect(!__any(bad), 1)) {
+  const auto add = [&](auto cut) {
 #pragma unroll
     for (int d = 0; d < kDim / 32; ++d)
 #pragma unroll
       for (int t = 0; t < L::kParts; ++t) {
-        const typename L::Frag v = L::column(tile, row0, 32 * d, t);
+        typename L::Frag v = L::column(tile, row0, 32 * d, t);
+        if constexpr (cut.value) v = finite_only<T>(v, found);
         acc[d] = mma(v, part[t], acc[d]);
         if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
       }
-    return;
-  }
-  F16 ones;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) ones[r] = seen(r) ? 1.0f : 0.0f;
-#pragma unroll
-  for (int d = 0; d < kDim / 32; ++d) {
-    F16 codes = {};
-#pragma unroll
-    for (int t = 0; t < L::kParts; ++t) {
-      typename L::Frag v = L::column(tile, row0, 32 * d, t), code;
-#pragma unroll
-      for (int i = 0; i < L::kChunk / 2; ++i) {
-        const float f = (float)v[i], size = __builtin_fabsf(f);
-        const float inf = f > 0.0f ? 64.0f : 4096.0f;
-        code[i] = (T)(size < kInf32 ? 0.0f : size == kInf32 ? inf : 1.0f);
-        v[i] = size < kInf32 ? v[i] : (T)0.0f;
-      }
-      acc[d] = mma(v, part[t], acc[d]);
-      if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
-      codes = mma(code, L::part(ones, t), codes);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int n = (int)codes[r];
-      const float up = n & (63 << 6) ? kInf32 : 0.0f, down = n >> 12 ? -kInf32 : 0.0f;
-      acc[d][r] += (n & 63 ? __builtin_nanf("") : up) + down;
+  };
+  if (cuts)
+    add(std::true_type{});
+  else
+    add(std::false_type{});
+}
+
+// Adds to a stored row what the values that are not finite make of it, of the rows from `from` to
+// `to` of a factor that it sees: themselves (a factor of probabilities), or NaN.  (Rows of tiles
+// that no mask cut may be among them: an infinity twice is one.)
+template <class T, bool kNan, class RowAt>
+__device__ inline void add_hidden(T* row, int dim, int from, int to, RowAt&& row_at) {
+#pragma unroll 1
+  for (int j = from; j < to; ++j) {
+    const T* p = row_at(j);
+#pragma unroll 1
+    for (int d = 0; d < dim; ++d) {
+      const float x = (float)p[d];
+      if (!(__builtin_fabsf(x) < kInf32))
+        row[d] = (T)((float)row[d] + (kNan ? __builtin_nanf("") : x));
     }
   }
 }
@@ -449,18 +438,22 @@ template <class T, int kDim, bool kDirect, class RowAt>
 __device__ inline void load_tile(char* tile, int rows, int dim, RowAt&& row_at) {
   using L = Tile<T, kDim>;
   if constexpr (kDirect) {
-    constexpr int kEach = 16 / (int)sizeof(T);
+    constexpr int kEach = 16 / (int)sizeof(T), kStep = kWaves * kWave * 16;  // bytes at a time
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = (int)threadIdx.x / L::kPer, place = threadIdx.x % L::kPer;
+    // (the places of a row repeat with the steps where those are 16 rows or more)
+    constexpr bool kSame = kStep / L::kPitch >= 16;
+    if (!kSame || (place ^ L::swap(r0)) * kEach < dim) {
 #pragma unroll
-    for (int i = 0; i < L::kBytes / (kWaves * kWave * 16); ++i) {
-      const int from = (i * kWaves + wave) * kWave * 16;  // this wave's 64 chunks
-      const int at = from + 16 * (threadIdx.x & 63);
-      const int r = at / L::kPitch, chunk = (at / 16 % L::kPer) ^ L::swap(r);
-      if (chunk * kEach < dim)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(row_at(r < rows ? r : rows - 1) +
-                                                            chunk * kEach),
-            (__attribute__((address_space(3))) void*)(tile + from), 16, 0, 0);
+      for (int i = 0; i < L::kBytes / kStep; ++i) {
+        const int r = r0 + i * (kStep / L::kPitch), chunk = place ^ L::swap(kSame ? r0 : r);
+        if (kSame || chunk * kEach < dim)
+          __builtin_amdgcn_global_load_lds(
+              (const __attribute__((address_space(1))) void*)(row_at(r < rows ? r : rows - 1) +
+                                                              chunk * kEach),
+              (__attribute__((address_space(3))) void*)(tile + i * kStep + wave * kWave * 16), 16,
+              0, 0);
+      }
     }
   } else {
     constexpr int kPieces = kDim / 8;

@@ -51,6 +51,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
 
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;  // l: over this half's keys
+  uint32_t found = 0;
   for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
     tiles_ready();
     if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, turn ^ 1);
@@ -94,16 +95,18 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
         s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], args.score_scale, -base));
         l += s[b][r];
       }
-      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, [&](int r) {
-        return k0 + 32 * b + result_row(r) < x.limit;
-      });
+      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, found);
     }
   }
   l += other_half(l);
   if (!x.there) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
-  store_column<T, kDim>(static_cast<T*>(args.out) + out_row * a.dim, o, inv, a.dim);
+  T* out = static_cast<T*>(args.out) + out_row * a.dim;
+  store_column<T, kDim>(out, o, inv, a.dim);
+  if (__builtin_expect(__any(found != 0), 0) && lane < 32)
+    add_hidden<T, false>(out, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
+                         [=](int j) { return v_rows + j * a.v_row_stride; });
   if (args.lse && lane < 32)
     args.lse[out_row] =
         l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);

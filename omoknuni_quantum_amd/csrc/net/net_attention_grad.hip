@@ -62,6 +62,7 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
   const float base = lse == -kInf32 ? 0.0f : lse * kLog2E;
 
   F16 dq[kDim / 32] = {};
+  uint32_t found = 0;
   float rest = 0.0f;  // sum p (g.v - delta): what out's rounding took from delta
   for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
     tiles_ready();
@@ -91,13 +92,17 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
         rest += s[r];
         s[r] *= a.scale;
       }
-      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, seen);
+      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, found);
     }
   }
   rest += other_half(rest);
   if (!x.there) return;
   if (lane < 32) args.delta[out_row] = delta + rest;
-  store_column<T, kDim>(static_cast<T*>(args.grad_q) + out_row * a.dim, dq, 1.0f, a.dim);
+  T* grad = static_cast<T*>(args.grad_q) + out_row * a.dim;
+  store_column<T, kDim>(grad, dq, 1.0f, a.dim);
+  if (__builtin_expect(__any(found != 0), 0) && lane < 32)
+    add_hidden<T, true>(grad, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
+                        [=](int j) { return k_rows + j * a.k_row_stride; });
 }
 
 // A workgroup has 128 keys, a wave 32 of them; 64 rows of queries at a time pass through LDS.
@@ -176,6 +181,7 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
   load_row<T, kDim, kDirect>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
                                      kv * a.v_head_stride, a.dim);
   F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
+  uint32_t found_q = 0, found_g = 0;
   int turn = 0;
   for (int64_t next = first; next < end; next += kTileKeys, turn ^= 1) {
     const int r0 = (int)next;
@@ -211,8 +217,8 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
             s[r] = sees ? s[r] : 0.0f;
           }
         }
-        add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, seen);
-        add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, seen);
+        add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g);
+        add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q);
       }
     }
     if (more) put(r0 + kTileKeys, turn ^ 1);
@@ -223,8 +229,16 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
     for (int d = 0; d < kDim / 32; ++d) dk[d] = F16{}, dv[d] = F16{};
   }
   const int64_t out = ((q.k_first + key) * a.k_heads + kv) * a.dim;
-  store_column<T, kDim>(static_cast<T*>(args.grad_k) + out, dk, 1.0f, a.dim);
-  store_column<T, kDim>(static_cast<T*>(args.grad_v) + out, dv, 1.0f, a.dim);
+  T *grad_k = static_cast<T*>(args.grad_k) + out, *grad_v = static_cast<T*>(args.grad_v) + out;
+  store_column<T, kDim>(grad_k, dk, 1.0f, a.dim);
+  store_column<T, kDim>(grad_v, dv, 1.0f, a.dim);
+  if (__builtin_expect(__any((found_q | found_g) != 0), 0) && lane < 32 && mine < q.lk) {
+    const int64_t least = a.causal && mine > shift ? (int64_t)(mine - shift) * group : 0;
+    const int sees = least < rows ? (int)least : rows;  // the first row that sees this key
+    add_hidden<T, true>(grad_k, a.dim, sees, rows, [=](int r) { return q_rows + q_place(r); });
+    add_hidden<T, false>(grad_v, a.dim, sees, rows,
+                         [=](int r) { return g_rows + out_place(r) * a.dim; });
+  }
 }
 
 int64_t delta_bytes(const omq_attention_args& a) {
