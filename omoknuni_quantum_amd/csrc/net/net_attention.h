@@ -36,6 +36,10 @@ struct AttentionArgs {
   int64_t slots;    // tiles a key head, some of them empty
   int64_t batch_tiles;  // tiles of a sequence of a batch
   float score_scale;    // scale * log2 e
+  int splits;           // parts of a sequence's keys, each a workgroup's
+  float* parts;         // [splits, rows of out, dim] sums, and behind them
+  float2* part_stats;   // [splits, rows of out] maximum and sum of the exponentials
+  int64_t out_rows;
   uint32_t group_mul;   // a row's query is umulhi(row, group_mul) >> group_shift; 0: the row
   int group_shift;
   void* out;
@@ -132,9 +136,9 @@ struct Place {
   int64_t tile;
 };
 
-__device__ inline bool place_of_queries(const AttentionArgs& args, int tile_rows, Place* p) {
+__device__ inline bool place_of_queries(const AttentionArgs& args, int tile_rows, int64_t block,
+                                        Place* p) {
   const omq_attention_args& a = args.a;
-  const int64_t block = block_index();
   int64_t slot = block / a.k_heads;
   if (slot >= args.slots) return false;
   slot = args.slots - 1 - slot;
@@ -175,6 +179,7 @@ struct Rows {
   int block_most;    // that some row of the workgroup sees
 };
 
+template <int kTileRows_ = kTileRows>
 __device__ inline Rows rows_of(const AttentionArgs& args, const Sequence& q, int kv, int r0,
                                int rows) {
   const int shift = q.lk - q.lq, lane = threadIdx.x & 63;
@@ -192,7 +197,7 @@ __device__ inline Rows rows_of(const AttentionArgs& args, const Sequence& q, int
   x.limit = sees(row);
   x.least = sees(first);
   x.most = first < rows ? sees(first + kWaveRows - 1) : 0;
-  x.block_most = sees(r0 + kTileRows - 1);
+  x.block_most = sees(r0 + kTileRows_ - 1);
   return x;
 }
 
@@ -368,8 +373,8 @@ __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int 
 // Adds to a stored row what the values that are not finite make of it, of the rows from `from` to
 // `to` of a factor that it sees: themselves (a factor of probabilities), or NaN.  (Rows of tiles
 // that no mask cut may be among them: an infinity twice is one.)
-template <class T, bool kNan, class RowAt>
-__device__ inline void add_hidden(T* row, int dim, int from, int to, RowAt&& row_at) {
+template <class T, bool kNan, class O, class RowAt>
+__device__ inline void add_hidden(O* row, int dim, int from, int to, RowAt&& row_at) {
 #pragma unroll 1
   for (int j = from; j < to; ++j) {
     const T* p = row_at(j);
@@ -377,7 +382,7 @@ __device__ inline void add_hidden(T* row, int dim, int from, int to, RowAt&& row
     for (int d = 0; d < dim; ++d) {
       const float x = (float)p[d];
       if (!(__builtin_fabsf(x) < kInf32))
-        row[d] = (T)((float)row[d] + (kNan ? __builtin_nanf("") : x));
+        row[d] = (O)((float)row[d] + (kNan ? __builtin_nanf("") : x));
     }
   }
 }
@@ -425,27 +430,34 @@ inline bool direct_tiles(const omq_attention_args& a) {
 
 // Zeros where a tile's rows have no column (from dim on): before the first load_tile, and a
 // barrier between the two.
-template <class T, int kDim>
+template <class T, int kDim, int kThreads = kWaves * kWave, int kRows = kTileKeys>
 __device__ inline void clear_tile(char* tile, int dim) {
   if (dim == kDim) return;
-  for (int i = threadIdx.x; i < Tile<T, kDim>::kBytes / 16; i += kWaves * kWave)
+  for (int i = threadIdx.x; i < kRows * Tile<T, kDim>::kPitch / 16; i += kThreads)
     *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
 }
 
-// Loads kTileKeys rows into LDS, the last of `rows` (at least one) again in place of those behind
-// it; row_at(i): row i < rows.  kDirect: chunks_aligned; the loads are under way when this returns.
-template <class T, int kDim, bool kDirect, class RowAt>
+// Loads kRows rows into LDS, the last of `rows` (at least one) again in place of those behind it;
+// row_at(i): row i < rows.  kDirect: chunks_aligned; the loads are under way when this returns,
+// tile_loads of them for every wave.
+template <class T, int kDim, int kThreads, int kRows>
+constexpr int tile_loads() {
+  return kRows * Tile<T, kDim>::kPitch / (kThreads * 16);
+}
+
+template <class T, int kDim, bool kDirect, int kThreads = kWaves * kWave, int kRows = kTileKeys,
+          class RowAt>
 __device__ inline void load_tile(char* tile, int rows, int dim, RowAt&& row_at) {
   using L = Tile<T, kDim>;
   if constexpr (kDirect) {
-    constexpr int kEach = 16 / (int)sizeof(T), kStep = kWaves * kWave * 16;  // bytes at a time
+    constexpr int kEach = 16 / (int)sizeof(T), kStep = kThreads * 16;  // bytes at a time
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r0 = (int)threadIdx.x / L::kPer, place = threadIdx.x % L::kPer;
     // (the places of a row repeat with the steps where those are 16 rows or more)
     constexpr bool kSame = kStep / L::kPitch >= 16;
     if (!kSame || (place ^ L::swap(r0)) * kEach < dim) {
 #pragma unroll
-      for (int i = 0; i < L::kBytes / kStep; ++i) {
+      for (int i = 0; i < tile_loads<T, kDim, kThreads, kRows>(); ++i) {
         const int r = r0 + i * (kStep / L::kPitch), chunk = place ^ L::swap(kSame ? r0 : r);
         if (kSame || chunk * kEach < dim)
           __builtin_amdgcn_global_load_lds(
@@ -458,7 +470,7 @@ __device__ inline void load_tile(char* tile, int rows, int dim, RowAt&& row_at) 
   } else {
     constexpr int kPieces = kDim / 8;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < kTileKeys * kPieces; i += kWaves * kWave) {
+    for (int i = threadIdx.x; i < kRows * kPieces; i += kThreads) {
       const int r = i / kPieces, col = i % kPieces * 8;
       const Reg8<T> v = load_piece<T, false>(row_at(r < rows ? r : rows - 1), col, dim);
       using Frag = typename L::Frag;

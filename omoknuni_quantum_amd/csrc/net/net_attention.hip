@@ -24,7 +24,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
   const omq_attention_args& a = args.a;
   Place at;
-  if (!place_of_queries(args, kTileRows, &at)) return;
+  if (!place_of_queries(args, kTileRows, block_index(), &at)) return;
   const Sequence& q = at.q;
   const int rows = (int)((int64_t)q.lq * args.group), lane = threadIdx.x & 63;
   const Rows x = rows_of(args, q, at.kv, (int)(at.tile * kTileRows), rows);
@@ -112,6 +112,175 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
         l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
 }
 
+// ---- few rows ---------------------------------------------------------------------------------
+// Where a sequence has few rows (single tokens over a cache), bound by reading its keys and values:
+// a workgroup is one wave, with 32 rows and a part of the keys, 32 of them at a time, loaded while
+// the 32 before are attended to.  The parts' sums are joined in their order by a second launch.
+constexpr int kPartKeys = 32;
+
+template <class T, int kDim, bool kDirect>
+__global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args) {
+  using L = Tile<T, kDim>;
+  constexpr int kLoads = 2 * tile_loads<T, kDim, kWave, kPartKeys>();
+  static_assert(kLoads < 64);
+  __shared__ __attribute__((aligned(1024))) char tiles[2][2][kPartKeys * L::kPitch];
+  const omq_attention_args& a = args.a;
+  const int64_t block = block_index();
+  const int split = (int)(block % args.splits);
+  Place at;
+  if (!place_of_queries(args, kWaveRows, block / args.splits, &at)) return;
+  const Sequence& q = at.q;
+  const int rows = (int)((int64_t)q.lq * args.group), lane = threadIdx.x;
+  const Rows x = rows_of<kWaveRows>(args, q, at.kv, (int)(at.tile * kWaveRows), rows);
+  // this part's keys
+  const int tiles_in_all = (x.most + kPartKeys - 1) / kPartKeys;
+  const int each = (tiles_in_all + args.splits - 1) / args.splits;
+  const int64_t begin64 = (int64_t)split * each * kPartKeys;
+  const int begin = begin64 < x.most ? (int)begin64 : x.most;
+  const int end = begin + each * kPartKeys < x.most ? begin + each * kPartKeys : x.most;
+
+  const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
+  const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
+  const auto load = [&](int k0, int turn) {
+    load_tile<T, kDim, kDirect, kWave, kPartKeys>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+      return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
+    });
+    load_tile<T, kDim, kDirect, kWave, kPartKeys>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+      return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
+    });
+  };
+  if (kDirect && a.dim < kDim) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) clear_tile<T, kDim, kWave, kPartKeys>(tiles[t / 2][t % 2], a.dim);
+    __syncthreads();
+  }
+  typename L::Frag qf[L::kChunks];
+  load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
+                                     x.head * a.q_head_stride, a.dim);
+  if (begin < end) load(begin, 0);
+  F16 o[kDim / 32] = {};
+  float m = -kInf32, l = 0.0f;
+  uint32_t found = 0;
+  for (int k0 = begin, turn = 0; k0 < end; k0 += kPartKeys, turn ^= 1) {
+    if (k0 + kPartKeys < end) {
+      load(k0 + kPartKeys, turn ^ 1);
+      // this tile's loads have arrived when no more are under way than the next one's
+      __builtin_amdgcn_s_waitcnt((kLoads & 15) | 0x0F70 | ((kLoads >> 4) << 14));
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+    // (a barrier would wait for the next tile; LDS accesses of one wave are in order)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    const char *keys = tiles[turn][0], *values = tiles[turn][1];
+    const bool cuts = k0 + kPartKeys > x.least;
+    F16 s = {};
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 0, c), qf[c], s);
+    if (cuts) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (k0 + result_row(r) >= x.limit) s[r] = -kInf32;
+    }
+    float top = -kInf32;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(top, other_half(top));
+    if (__any((top - m) * args.score_scale > kLag)) {
+      const float next = fmaxf(m, top);
+      const float keep =
+          next == -kInf32 ? 1.0f : __builtin_amdgcn_exp2f((m - next) * args.score_scale);
+      m = next;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
+    }
+    const float base = m == -kInf32 ? 0.0f : m * args.score_scale;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
+      l += s[r];
+    }
+    add_columns<T, kDim, false>(o, values, 0, s, cuts, found);
+  }
+  l += other_half(l);
+  if (!x.there) return;
+  const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
+  const int least = x.least / kPartKeys * kPartKeys;
+  const int from = begin > least ? begin : least, to = end < x.limit ? end : x.limit;
+  const bool hidden = __any(found != 0) && lane < 32;
+  const auto value = [=](int j) { return v_rows + j * a.v_row_stride; };
+  if (args.splits == 1) {
+    T* out = static_cast<T*>(args.out) + out_row * a.dim;
+    store_column<T, kDim>(out, o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
+    if (hidden) add_hidden<T, false>(out, a.dim, from, to, value);
+    if (args.lse && lane < 32)
+      args.lse[out_row] =
+          l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+    return;
+  }
+  const int64_t part = split * args.out_rows + out_row;
+  store_column<float, kDim>(args.parts + part * a.dim, o, 1.0f, a.dim);
+  if (hidden) add_hidden<T, false>(args.parts + part * a.dim, a.dim, from, to, value);
+  if (lane < 32) args.part_stats[part] = make_float2(m, l);
+}
+
+// A row of the output from its parts (at most 64), a wave a row.
+template <class T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs args) {
+  const int64_t row = block_index() * 4 + row_slot<kWave>();
+  if (row >= args.out_rows) return;
+  const int lane = threadIdx.x & 63, dim = args.a.dim;
+  float2 mine = make_float2(-kInf32, 0.0f);
+  if (lane < args.splits) mine = args.part_stats[lane * args.out_rows + row];
+  const float m = lanes_reduce<Max, kWave>(mine.x);
+  // (a part without keys has a sum of 0; NaN is a sum)
+  const float w = mine.x == -kInf32 ? (mine.y == 0.0f ? 0.0f : 1.0f)
+                                    : __builtin_amdgcn_exp2f((mine.x - m) * args.score_scale);
+  const float l = lanes_reduce<Sum, kWave>(mine.y == 0.0f ? 0.0f : w * mine.y);
+  const float scale = l == 0.0f ? 0.0f : w / l;
+  float x[2] = {};
+  for (int s = 0; s < args.splits; ++s) {
+    const float f = __shfl(scale, s);
+    const float* part = args.parts + (s * args.out_rows + row) * dim;
+    if (f != 0.0f) {  // (a part without keys is zeros; of weight 0, nothing beside the others)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < dim) x[i] = fmaf(f, part[lane + 64 * i], x[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < dim)
+      static_cast<T*>(args.out)[row * dim + lane + 64 * i] = (T)x[i];
+  if (args.lse && lane == 0)
+    args.lse[row] =
+        l == 0.0f ? -kInf32 : fmaf(m, args.a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+}
+
+// Whether a call takes the kernel for few rows, and with how many parts.
+bool few_rows(const omq_attention_args& a, int* splits, int64_t* out_rows) {
+  const int64_t group = a.q_heads / a.k_heads, n = a.q_starts ? a.sequences : 1;
+  const int64_t all = a.q_starts ? 1 : a.sequences;
+  *out_rows = all * a.q_len * a.q_heads;
+  const int64_t rows = n > 0 ? ceil_div(a.q_len * group, n) : 0;  // (of a sequence, in the mean)
+  const int64_t keys = n > 0 ? ceil_div(a.k_len, n) : 0;
+  const int64_t sequences = a.sequences > 0 ? a.sequences : 1;
+  const int64_t wide = ceil_div(rows, kTileRows) * sequences * a.k_heads;
+  *splits = 1;
+  if (rows > kWaveRows && (wide >= 256 || keys < 512)) return false;
+  const int64_t units = ceil_div(rows > 0 ? rows : 1, kWaveRows) * sequences * a.k_heads;
+  int64_t parts = ceil_div(4096, units);
+  const int64_t most = ceil_div(keys, 4 * kPartKeys);
+  parts = parts < most ? parts : most;
+  *splits = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+  return true;
+}
+
+int64_t parts_bytes(const omq_attention_args& a, int splits, int64_t out_rows) {
+  return splits > 1 ? splits * out_rows * (a.dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
 }  // namespace
 
 int check_attention(const char* name, const omq_attention_args* a) {
@@ -154,7 +323,10 @@ using namespace omq_net;
 extern "C" {
 
 int64_t omq_attention_forward_workspace(const omq_attention_args* a) {
-  return check_attention("omq_attention_forward_workspace", a);
+  if (const int rc = check_attention("omq_attention_forward_workspace", a)) return rc;
+  int splits;
+  int64_t out_rows;
+  return few_rows(*a, &splits, &out_rows) ? parts_bytes(*a, splits, out_rows) : 0;
 }
 
 int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, void* workspace,
@@ -163,15 +335,40 @@ int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, vo
   if (int rc = check_attention(name, a)) return rc;
   if (a->q_len == 0 || (a->sequences == 0 && !a->q_starts)) return OMQ_NET_OK;
   if (!out) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
-  (void)workspace, (void)workspace_bytes;
   AttentionArgs args = attention_layout(*a);
-  tiles_of(&args, a->q_len, args.group, kTileRows);
   args.out = out, args.lse = lse;
-  const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
+  const bool few = few_rows(*a, &args.splits, &args.out_rows);
+  const int64_t need = few ? parts_bytes(*a, args.splits, args.out_rows) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || !on_16_bytes(workspace)))
+    return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes at %p, %lld on a 16-byte boundary "
+                    "needed", name, (long long)workspace_bytes, workspace, (long long)need);
+  hipStream_t st = (hipStream_t)stream;
+  if (!few) {
+    tiles_of(&args, a->q_len, args.group, kTileRows);
+    const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
+    with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
+      attention_kernel<decltype(t), dim.value, direct.value><<<grid, kWaves * kWave, 0, st>>>(args);
+    });
+    return net_status(name);
+  }
+  tiles_of(&args, a->q_len, args.group, kWaveRows);
+  if (need > 0) {
+    args.part_stats = static_cast<float2*>(workspace);
+    args.parts = static_cast<float*>(workspace) + 2 * args.splits * args.out_rows;
+  }
+  const dim3 grid = grid_of(args.slots * a->k_heads * args.splits, kWave);
   with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
-    attention_kernel<decltype(t), dim.value, direct.value>
-        <<<grid, kWaves * kWave, 0, (hipStream_t)stream>>>(args);
+    attention_few_kernel<decltype(t), dim.value, direct.value><<<grid, kWave, 0, st>>>(args);
   });
+  if (args.splits > 1) {
+    const dim3 rows = grid_of(ceil_div(args.out_rows, 4), 256);
+    if (a->dtype == OMQ_NET_F32)
+      attention_join_kernel<float><<<rows, 256, 0, st>>>(args);
+    else if (a->dtype == OMQ_NET_BF16)
+      attention_join_kernel<bf16><<<rows, 256, 0, st>>>(args);
+    else
+      attention_join_kernel<f16><<<rows, 256, 0, st>>>(args);
+  }
   return net_status(name);
 }
 

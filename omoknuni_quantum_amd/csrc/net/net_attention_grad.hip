@@ -22,7 +22,7 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
   __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
   const omq_attention_args& a = args.a;
   Place at;
-  if (!place_of_queries(args, kTileRows, &at)) return;
+  if (!place_of_queries(args, kTileRows, block_index(), &at)) return;
   const Sequence& q = at.q;
   const int rows = (int)((int64_t)q.lq * args.group), lane = threadIdx.x & 63;
   const Rows x = rows_of(args, q, at.kv, (int)(at.tile * kTileRows), rows);
