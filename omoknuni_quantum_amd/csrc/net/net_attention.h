@@ -30,6 +30,14 @@ constexpr int kWaveRows = 32;           // rows of the stationary side that a wa
 constexpr int kTileRows = kWaves * kWaveRows;
 constexpr int kTileKeys = 64;           // rows of the moving side in LDS
 
+// Waves a SIMD that a kernel's registers have to leave room for: two, so that one's products run
+// while the other forms its probabilities (float32 heads of 128 columns: their operands alone take
+// the registers of one).
+template <class T, int kDim>
+constexpr int waves_per_simd() {
+  return sizeof(T) == 4 && kDim > 64 ? 1 : 2;
+}
+
 struct AttentionArgs {
   omq_attention_args a;
   int group;        // query heads of a key head
@@ -154,9 +162,9 @@ __device__ inline bool place_of_queries(const AttentionArgs& args, int tile_rows
 }
 
 // The same by keys, the first ones first: in a causal sequence the most queries see them.
-__device__ inline bool place_of_keys(const AttentionArgs& args, int tile_rows, Place* p) {
+__device__ inline bool place_of_keys(const AttentionArgs& args, int tile_rows, int64_t block,
+                                     Place* p) {
   const omq_attention_args& a = args.a;
-  const int64_t block = block_index();
   const int64_t slot = block / a.k_heads;
   if (slot >= args.slots) return false;
   p->kv = (int)(block % a.k_heads);

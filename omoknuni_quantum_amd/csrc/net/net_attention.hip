@@ -19,9 +19,10 @@ namespace {
 constexpr float kLag = 8.0f;
 
 template <class T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionArgs args) {
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
+  __shared__ __attribute__((aligned(1024))) char keys0[L::kBytes], keys1[L::kBytes];
+  __shared__ __attribute__((aligned(1024))) char values0[L::kBytes], values1[L::kBytes];
   const omq_attention_args& a = args.a;
   Place at;
   if (!place_of_queries(args, kTileRows, block_index(), &at)) return;
@@ -31,20 +32,20 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
 
   const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
   const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
-  const auto load = [&](int k0, int turn) {
-    load_tile<T, kDim, kDirect>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+  const auto load = [&](int k0, char* keys, char* values) {
+    load_tile<T, kDim, kDirect>(keys, q.lk - k0, a.dim, [&](int i) {
       return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
     });
-    load_tile<T, kDim, kDirect>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+    load_tile<T, kDim, kDirect>(values, q.lk - k0, a.dim, [&](int i) {
       return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
     });
   };
   if (kDirect && a.dim < kDim) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
+    clear_tile<T, kDim>(keys0, a.dim), clear_tile<T, kDim>(keys1, a.dim);
+    clear_tile<T, kDim>(values0, a.dim), clear_tile<T, kDim>(values1, a.dim);
     __syncthreads();
   }
-  if (x.block_most > 0) load(0, 0);
+  if (x.block_most > 0) load(0, keys0, values0);
   typename L::Frag qf[L::kChunks];
   load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
                             x.head * a.q_head_stride, a.dim);
@@ -52,11 +53,11 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;  // l: over this half's keys
   uint32_t found = 0;
-  for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
+  const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
+                        char* next_values) __attribute__((always_inline)) {
     tiles_ready();
-    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, turn ^ 1);
-    if (k0 >= x.most) continue;
-    const char *keys = tiles[turn][0], *values = tiles[turn][1];
+    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
+    if (k0 >= x.most) return;
     const bool cuts = k0 + kTileKeys > x.least;  // some row does not see all of the tile
     F16 s[2];
     float top = -kInf32;
@@ -97,6 +98,12 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void attention_kernel(AttentionAr
       }
       add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, found);
     }
+  };
+  // (two steps a turn, so that the tiles' arrays are told apart: the compiler would wait for all
+  // loads under way before it reads an array that they may write)
+  for (int k0 = 0; k0 < x.block_most; k0 += 2 * kTileKeys) {
+    step(k0, keys0, values0, keys1, values1);
+    if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
   l += other_half(l);
   if (!x.there) return;
@@ -123,7 +130,9 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
   using L = Tile<T, kDim>;
   constexpr int kLoads = 2 * tile_loads<T, kDim, kWave, kPartKeys>();
   static_assert(kLoads < 64);
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][kPartKeys * L::kPitch];
+  constexpr int kBytes = kPartKeys * L::kPitch;
+  __shared__ __attribute__((aligned(1024))) char keys0[kBytes], keys1[kBytes];
+  __shared__ __attribute__((aligned(1024))) char values0[kBytes], values1[kBytes];
   const omq_attention_args& a = args.a;
   const int64_t block = block_index();
   const int split = (int)(block % args.splits);
@@ -141,29 +150,30 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
 
   const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
   const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
-  const auto load = [&](int k0, int turn) {
-    load_tile<T, kDim, kDirect, kWave, kPartKeys>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+  const auto load = [&](int k0, char* keys, char* values) {
+    load_tile<T, kDim, kDirect, kWave, kPartKeys>(keys, q.lk - k0, a.dim, [&](int i) {
       return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
     });
-    load_tile<T, kDim, kDirect, kWave, kPartKeys>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+    load_tile<T, kDim, kDirect, kWave, kPartKeys>(values, q.lk - k0, a.dim, [&](int i) {
       return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
     });
   };
   if (kDirect && a.dim < kDim) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) clear_tile<T, kDim, kWave, kPartKeys>(tiles[t / 2][t % 2], a.dim);
+    for (char* t : {keys0, keys1, values0, values1})
+      clear_tile<T, kDim, kWave, kPartKeys>(t, a.dim);
     __syncthreads();
   }
   typename L::Frag qf[L::kChunks];
   load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
                                      x.head * a.q_head_stride, a.dim);
-  if (begin < end) load(begin, 0);
+  if (begin < end) load(begin, keys0, values0);
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;
   uint32_t found = 0;
-  for (int k0 = begin, turn = 0; k0 < end; k0 += kPartKeys, turn ^= 1) {
+  const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
+                        char* next_values) __attribute__((always_inline)) {
     if (k0 + kPartKeys < end) {
-      load(k0 + kPartKeys, turn ^ 1);
+      load(k0 + kPartKeys, next_keys, next_values);
       // this tile's loads have arrived when no more are under way than the next one's
       __builtin_amdgcn_s_waitcnt((kLoads & 15) | 0x0F70 | ((kLoads >> 4) << 14));
     } else {
@@ -172,7 +182,6 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     // (a barrier would wait for the next tile; LDS accesses of one wave are in order)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    const char *keys = tiles[turn][0], *values = tiles[turn][1];
     const bool cuts = k0 + kPartKeys > x.least;
     F16 s = {};
 #pragma unroll
@@ -202,6 +211,10 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
       l += s[r];
     }
     add_columns<T, kDim, false>(o, values, 0, s, cuts, found);
+  };
+  for (int k0 = begin; k0 < end; k0 += 2 * kPartKeys) {  // (as above)
+    step(k0, keys0, values0, keys1, values1);
+    if (k0 + kPartKeys < end) step(k0 + kPartKeys, keys1, values1, keys0, values0);
   }
   l += other_half(l);
   if (!x.there) return;

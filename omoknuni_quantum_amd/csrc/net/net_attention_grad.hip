@@ -17,9 +17,10 @@ namespace omq_net {
 namespace {
 
 template <class T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(AttentionArgs args) {
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_q_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // keys, values
+  __shared__ __attribute__((aligned(1024))) char keys0[L::kBytes], keys1[L::kBytes];
+  __shared__ __attribute__((aligned(1024))) char values0[L::kBytes], values1[L::kBytes];
   const omq_attention_args& a = args.a;
   Place at;
   if (!place_of_queries(args, kTileRows, block_index(), &at)) return;
@@ -29,20 +30,20 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
 
   const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
   const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
-  const auto load = [&](int k0, int turn) {
-    load_tile<T, kDim, kDirect>(tiles[turn][0], q.lk - k0, a.dim, [&](int i) {
+  const auto load = [&](int k0, char* keys, char* values) {
+    load_tile<T, kDim, kDirect>(keys, q.lk - k0, a.dim, [&](int i) {
       return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
     });
-    load_tile<T, kDim, kDirect>(tiles[turn][1], q.lk - k0, a.dim, [&](int i) {
+    load_tile<T, kDim, kDirect>(values, q.lk - k0, a.dim, [&](int i) {
       return v_rows + (int64_t)(k0 + i) * a.v_row_stride;
     });
   };
   if (kDirect && a.dim < kDim) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
+    clear_tile<T, kDim>(keys0, a.dim), clear_tile<T, kDim>(keys1, a.dim);
+    clear_tile<T, kDim>(values0, a.dim), clear_tile<T, kDim>(values1, a.dim);
     __syncthreads();
   }
-  if (x.block_most > 0) load(0, 0);
+  if (x.block_most > 0) load(0, keys0, values0);
   typename L::Frag qf[L::kChunks], gf[L::kChunks];
   load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
                                      x.head * a.q_head_stride, a.dim);
@@ -64,11 +65,11 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
   F16 dq[kDim / 32] = {};
   uint32_t found = 0;
   float rest = 0.0f;  // sum p (g.v - delta): what out's rounding took from delta
-  for (int k0 = 0, turn = 0; k0 < x.block_most; k0 += kTileKeys, turn ^= 1) {
+  const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
+                        char* next_values) __attribute__((always_inline)) {
     tiles_ready();
-    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, turn ^ 1);
-    if (k0 >= x.most) continue;
-    const char *keys = tiles[turn][0], *values = tiles[turn][1];
+    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
+    if (k0 >= x.most) return;
     const bool cuts = k0 + kTileKeys > x.least;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -94,6 +95,11 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
       }
       add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, found);
     }
+  };
+  // (two steps a turn: as in the forward kernel)
+  for (int k0 = 0; k0 < x.block_most; k0 += 2 * kTileKeys) {
+    step(k0, keys0, values0, keys1, values1);
+    if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
   rest += other_half(rest);
   if (!x.there) return;
@@ -105,16 +111,25 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_q_kernel(Attenti
                         [=](int j) { return k_rows + j * a.k_row_stride; });
 }
 
+// What a row of queries brings to the gradients by keys: the base of its probabilities, its delta,
+// and the keys that it sees.
+struct RowStats {
+  float base[kTileKeys], delta[kTileKeys];
+  int limit[kTileKeys];
+};
+
 // A workgroup has 128 keys, a wave 32 of them; 64 rows of queries at a time pass through LDS.
-template <class T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(AttentionArgs args) {
+// kKeys, kValues: the sums that it forms.
+template <class T, int kDim, bool kDirect, bool kKeys, bool kValues>
+__device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArgs& args,
+                                                              int64_t block, char* queries0,
+                                                              char* queries1, char* grads0,
+                                                              char* grads1, RowStats& stats0,
+                                                              RowStats& stats1) {
   using L = Tile<T, kDim>;
-  __shared__ __attribute__((aligned(1024))) char tiles[2][2][L::kBytes];  // queries, gradients
-  __shared__ __attribute__((aligned(16))) float bases[2][kTileKeys], deltas[2][kTileKeys];
-  __shared__ __attribute__((aligned(16))) int limits[2][kTileKeys];
   const omq_attention_args& a = args.a;
   Place at;
-  if (!place_of_keys(args, kTileRows, &at)) return;
+  if (!place_of_keys(args, kTileRows, block, &at)) return;
   const Sequence& q = at.q;
   const int j0 = (int)(at.tile * kTileRows), group = args.group, kv = at.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -141,13 +156,13 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
     const int query = query_of(args, r);
     return (int64_t)query * a.q_heads + (r - query * group);
   };
-  const auto load = [&](int r0, int turn) {
-    load_tile<T, kDim, kDirect>(tiles[turn][0], rows - r0, a.dim,
+  const auto load = [&](int r0, char* queries, char* grads) {
+    load_tile<T, kDim, kDirect>(queries, rows - r0, a.dim,
                                 [&](int i) { return q_rows + q_place(r0 + i); });
-    load_tile<T, kDim, kDirect>(tiles[turn][1], rows - r0, a.dim,
+    load_tile<T, kDim, kDirect>(grads, rows - r0, a.dim,
                                 [&](int i) { return g_rows + out_place(r0 + i) * a.dim; });
   };
-  // what the first wave brings of a tile's rows
+  // the first wave brings what belongs to a tile's rows
   float lse = 0.0f, delta = 0.0f;
   const auto fetch = [&](int r0) {
     if (threadIdx.x < kTileKeys) {
@@ -155,73 +170,83 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
       lse = args.lse_in[i], delta = args.delta[i];
     }
   };
-  const auto put = [&](int r0, int turn) {
+  const auto put = [&](int r0, RowStats& stats) {
     if (threadIdx.x < kTileKeys) {
       const int r = r0 + lane;
-      bases[turn][lane] = lse == -kInf32 ? 0.0f : lse * kLog2E;
-      deltas[turn][lane] = delta;
-      limits[turn][lane] = r >= rows ? 0
-                           : a.causal ? cut(query_of(args, r) + shift + 1, 0, q.lk)
-                                      : q.lk;
+      stats.base[lane] = lse == -kInf32 ? 0.0f : lse * kLog2E;
+      stats.delta[lane] = delta;
+      stats.limit[lane] = r >= rows ? 0
+                          : a.causal ? cut(query_of(args, r) + shift + 1, 0, q.lk)
+                                     : q.lk;
     }
   };
   if (kDirect && a.dim < kDim) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) clear_tile<T, kDim>(tiles[t / 2][t % 2], a.dim);
+    clear_tile<T, kDim>(queries0, a.dim), clear_tile<T, kDim>(queries1, a.dim);
+    clear_tile<T, kDim>(grads0, a.dim), clear_tile<T, kDim>(grads1, a.dim);
     __syncthreads();
   }
   if (first < end) {
-    load((int)first, 0);
+    load((int)first, queries0, grads0);
     fetch((int)first);
-    put((int)first, 0);
+    put((int)first, stats0);
   }
-  typename L::Frag kf[L::kChunks], vf[L::kChunks];
+  typename L::Frag kf[L::kChunks], vf[kKeys ? L::kChunks : 1];
   load_row<T, kDim, kDirect>(kf, static_cast<const T*>(a.k) + q.k_at + key * a.k_row_stride +
                                      kv * a.k_head_stride, a.dim);
-  load_row<T, kDim, kDirect>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
-                                     kv * a.v_head_stride, a.dim);
+  if constexpr (kKeys)
+    load_row<T, kDim, kDirect>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
+                                       kv * a.v_head_stride, a.dim);
   F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
   uint32_t found_q = 0, found_g = 0;
-  int turn = 0;
-  for (int64_t next = first; next < end; next += kTileKeys, turn ^= 1) {
+  const auto step = [&](int64_t next, const char* queries, const char* grads,
+                        const RowStats& stats, char* next_queries, char* next_grads,
+                        RowStats& next_stats) __attribute__((always_inline)) {
     const int r0 = (int)next;
     const bool more = next + kTileKeys < end;
     tiles_ready();
-    if (more) load(r0 + kTileKeys, turn ^ 1), fetch(r0 + kTileKeys);
-    const char *queries = tiles[turn][0], *grads = tiles[turn][1];
+    if (more) load(r0 + kTileKeys, next_queries, next_grads), fetch(r0 + kTileKeys);
     // some row does not see all of the wave's keys; or none does
-    const int low = limits[turn][0], high = limits[turn][kTileKeys - 1];
-    const bool cuts = r0 + kTileKeys > rows || from + kWaveRows > q.lk ||
-                      from + kWaveRows > __builtin_amdgcn_readfirstlane(low);
-    if (from < __builtin_amdgcn_readfirstlane(high) || r0 + kTileKeys > rows) {
+    const int low = a.causal ? query_of(args, r0) + shift + 1 : q.lk;
+    const int high = a.causal ? query_of(args, r0 + kTileKeys - 1) + shift + 1 : q.lk;
+    const bool cuts = r0 + kTileKeys > rows || from + kWaveRows > q.lk || from + kWaveRows > low;
+    if (from < high && from < q.lk) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         F16 s = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c), kf[c], s);
+        if constexpr (kKeys) {
 #pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c), vf[c], dp);
-        const auto seen = [&](int r) { return mine < limits[turn][32 * b + result_row(r)]; };
+          for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c), vf[c], dp);
+        }
         F16 p;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = 32 * b + result_row(r);
-          p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -bases[turn][i]));
-          s[r] = p[r] * (dp[r] - deltas[turn][i]) * a.scale;
+        for (int r = 0; r < 16; ++r)
+          p[r] = __builtin_amdgcn_exp2f(
+              fmaf(s[r], args.score_scale, -stats.base[32 * b + result_row(r)]));
+        if constexpr (kKeys) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[r] = p[r] * (dp[r] - stats.delta[32 * b + result_row(r)]) * a.scale;
         }
         if (cuts) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const bool sees = seen(r);
+            const bool sees = mine < stats.limit[32 * b + result_row(r)];
             p[r] = sees ? p[r] : 0.0f;
             s[r] = sees ? s[r] : 0.0f;
           }
         }
-        add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g);
-        add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q);
+        if constexpr (kValues) add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g);
+        if constexpr (kKeys) add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q);
       }
     }
-    if (more) put(r0 + kTileKeys, turn ^ 1);
+    if (more) put(r0 + kTileKeys, next_stats);
+  };
+  for (int64_t r0 = first; r0 < end; r0 += 2 * kTileKeys) {  // (as in the forward kernel)
+    step(r0, queries0, grads0, stats0, queries1, grads1, stats1);
+    if (r0 + kTileKeys < end)
+      step(r0 + kTileKeys, queries1, grads1, stats1, queries0, grads0, stats0);
   }
   if (!there) return;
   if (mine >= q.lk) {  // (whatever the queries hold)
@@ -230,15 +255,43 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_grad_kv_kernel(Attent
   }
   const int64_t out = ((q.k_first + key) * a.k_heads + kv) * a.dim;
   T *grad_k = static_cast<T*>(args.grad_k) + out, *grad_v = static_cast<T*>(args.grad_v) + out;
-  store_column<T, kDim>(grad_k, dk, 1.0f, a.dim);
-  store_column<T, kDim>(grad_v, dv, 1.0f, a.dim);
+  if constexpr (kKeys) store_column<T, kDim>(grad_k, dk, 1.0f, a.dim);
+  if constexpr (kValues) store_column<T, kDim>(grad_v, dv, 1.0f, a.dim);
   if (__builtin_expect(__any((found_q | found_g) != 0), 0) && lane < 32 && mine < q.lk) {
     const int64_t least = a.causal && mine > shift ? (int64_t)(mine - shift) * group : 0;
     const int sees = least < rows ? (int)least : rows;  // the first row that sees this key
-    add_hidden<T, true>(grad_k, a.dim, sees, rows, [=](int r) { return q_rows + q_place(r); });
-    add_hidden<T, false>(grad_v, a.dim, sees, rows,
-                         [=](int r) { return g_rows + out_place(r) * a.dim; });
+    if constexpr (kKeys)
+      add_hidden<T, true>(grad_k, a.dim, sees, rows, [=](int r) { return q_rows + q_place(r); });
+    if constexpr (kValues)
+      add_hidden<T, false>(grad_v, a.dim, sees, rows,
+                           [=](int r) { return g_rows + out_place(r) * a.dim; });
   }
+}
+
+// Sums of 128 columns are a workgroup's each, of the keys or of the values (scores are formed in
+// both: five products in place of four): with both a wave has no room for a second one on its SIMD,
+// whose products run while the first forms its probabilities.
+template <int kDim>
+constexpr bool sums_apart() {
+  return kDim > 64;
+}
+
+template <class T, int kDim, bool kDirect>
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_kv_kernel(AttentionArgs args) {
+  using L = Tile<T, kDim>;
+  __shared__ __attribute__((aligned(1024))) char queries0[L::kBytes], queries1[L::kBytes];
+  __shared__ __attribute__((aligned(1024))) char grads0[L::kBytes], grads1[L::kBytes];
+  __shared__ __attribute__((aligned(16))) RowStats stats0, stats1;
+  const int64_t block = block_index();
+  if constexpr (!sums_apart<kDim>())
+    grad_kv<T, kDim, kDirect, true, true>(args, block, queries0, queries1, grads0, grads1, stats0,
+                                          stats1);
+  else if (block % 2 == 0)
+    grad_kv<T, kDim, kDirect, true, false>(args, block / 2, queries0, queries1, grads0, grads1,
+                                           stats0, stats1);
+  else
+    grad_kv<T, kDim, kDirect, false, true>(args, block / 2, queries0, queries1, grads0, grads1,
+                                           stats0, stats1);
 }
 
 int64_t delta_bytes(const omq_attention_args& a) {
@@ -286,10 +339,11 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
   }
   if (keys) {
     tiles_of(&args, a->k_len, 1, kTileRows);
-    const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
     const bool rows_direct = chunks_aligned(a->dtype, a->dim, {a->q, grad_out},
                                             {a->q_seq_stride, a->q_row_stride, a->q_head_stride});
     with_head(a->dtype, a->dim, rows_direct, [&](auto t, auto dim, auto direct) {
+      const int64_t blocks = args.slots * a->k_heads * (sums_apart<dim.value>() ? 2 : 1);
+      const dim3 grid = grid_of(blocks, kWaves * kWave);
       attention_grad_kv_kernel<decltype(t), dim.value, direct.value>
           <<<grid, kWaves * kWave, 0, st>>>(args);
     });
