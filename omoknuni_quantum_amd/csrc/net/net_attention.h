@@ -44,6 +44,7 @@ struct AttentionArgs {
   int64_t slots;    // tiles a key head, some of them empty
   int64_t batch_tiles;  // tiles of a sequence of a batch
   float score_scale;    // scale * log2 e
+  int even;             // the moving side's rows are EvenRows
   int splits;           // parts of a sequence's keys, each a workgroup's
   float* parts;         // [splits, rows of out, dim] sums, and behind them
   float2* part_stats;   // [splits, rows of out] maximum and sum of the exponentials
@@ -258,39 +259,51 @@ struct Tile {
   }
   __device__ static int place(int r, int chunk) { return r * kPitch + ((chunk ^ swap(r)) << 4); }
 
+  // Where a lane's operands are: of row lane % 32, and of its columns.  An operand's own address is
+  // one exclusive or away (swap is a permutation of a row's bits); `renew` keeps the compiler from
+  // forming all of them before a loop, for which there are no registers.
+  struct Lane {
+    int row, column;
+    __device__ Lane() {
+      const int lane = threadIdx.x & 63, half = lane >> 5;
+      row = place(lane & 31, half);
+      if constexpr (sizeof(T) == 2) {
+        // 16 lanes address four rows of 16 columns, and get a column of four rows each
+        const int c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        column = place(4 * half + ((lane & 15) >> 2), c >> 3) + (c & 4) * 2;
+      } else {
+        column = place(4 * half, (lane & 31) >> 2) + (lane & 3) * 4;
+      }
+    }
+    __device__ void renew() { asm volatile("" : "+v"(row), "+v"(column)); }
+  };
+
   // Chunk c of the row row0 + lane % 32 (row0 a multiple of 32).
-  __device__ static Frag row(const char* tile, int row0, int c) {
-    const int lane = threadIdx.x & 63;
-    const int at = place(lane & 31, lane >> 5) ^ (c << 5);
-    return *reinterpret_cast<const Frag*>(tile + row0 * kPitch + at);
+  __device__ static Frag row(const char* tile, int row0, int c, const Lane& lane) {
+    return *reinterpret_cast<const Frag*>(tile + row0 * kPitch + (lane.row ^ (c << 5)));
   }
 
   // Column col0 + lane % 32 of part t of the rows from row0, in the order of a product's registers
   // (row0 and col0 multiples of 32).
-  __device__ static Frag column(const char* tile, int row0, int col0, int t) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
+  __device__ static Frag column(const char* tile, int row0, int col0, int t, const Lane& lane) {
     if constexpr (sizeof(T) == 2) {
-      // 16 lanes address four rows of 16 columns, and get a column of four rows each
-      const int r = 4 * half + ((lane & 15) >> 2), c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
       const char* p = tile + (row0 + 16 * t) * kPitch;
-      const int lo = (place(r, c >> 3) + (c & 4) * 2) ^ (col0 << 1);
-      const int hi = (place(r + 8, c >> 3) + (c & 4) * 2) ^ (col0 << 1);
+      const int lo = lane.column ^ (col0 << 1), hi = lo ^ (swap(8) << 4);
       using S4 = short __attribute__((ext_vector_type(4)));
       using Lds = __attribute__((address_space(3))) S4;
       struct Both {
         S4 lo, hi;
       } v;
       v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + lo));
-      v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + hi));
+      v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + 8 * kPitch + hi));
       return __builtin_bit_cast(Frag, v);
     } else {
       Frag f;
-      const int c = lane & 31;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = (8 * t + i) % 16 + 4 * half;
-        const int at = (place(r, c >> 2) + (c & 3) * 4) ^ (col0 << 2);
-        f[i] = *reinterpret_cast<const float*>(tile + (row0 + (8 * t + i) / 16 * 16) * kPitch + at);
+        const int r = 8 * t + i;
+        f[i] = *reinterpret_cast<const float*>(
+            tile + (row0 + r) * kPitch + (lane.column ^ (swap(r) << 4) ^ (col0 << 2)));
       }
       return f;
     }
@@ -347,7 +360,8 @@ __device__ inline Frag finite_only(const Frag& v, uint32_t& found) {
 // twice the type's bits, what its rounding leaves in a second product.
 template <class T, int kDim, bool kTwice>
 __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int row0, const F16& w,
-                                   bool cuts, uint32_t& found) {
+                                   bool cuts, uint32_t& found,
+                                   const typename Tile<T, kDim>::Lane& lane) {
   using L = Tile<T, kDim>;
   constexpr bool kRest = kTwice && sizeof(T) == 2;
   typename L::Frag part[L::kParts], rest[kRest ? L::kParts : 1];
@@ -366,7 +380,7 @@ __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int 
     for (int d = 0; d < kDim / 32; ++d)
 #pragma unroll
       for (int t = 0; t < L::kParts; ++t) {
-        typename L::Frag v = L::column(tile, row0, 32 * d, t);
+        typename L::Frag v = L::column(tile, row0, 32 * d, t, lane);
         if constexpr (cut.value) v = finite_only<T>(v, found);
         acc[d] = mma(v, part[t], acc[d]);
         if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
@@ -491,6 +505,58 @@ __device__ inline void load_tile(char* tile, int rows, int dim, RowAt&& row_at) 
   }
 }
 
+// A lane's place in the rows of a tile that are all there and lie as far apart at every step of its
+// loads: bytes from the tile's first row, the same for every tile.  A load then has a scalar
+// address and a 32-bit one, where a lane's rows otherwise take some ten instructions a load.
+template <class T, int kDim>
+struct EvenRows {
+  using L = Tile<T, kDim>;
+  static constexpr int kStep = kWaves * kWave * 16;
+  static constexpr int kRowsAStep = kStep / L::kPitch;
+  static constexpr int kPeriod = kRowsAStep >= 16 ? 1 : 16 / kRowsAStep;  // of a row's places
+  static constexpr int kEach = 16 / (int)sizeof(T);
+  uint32_t own[kPeriod];
+  bool on;  // the lane has columns (kPeriod 1; all lanes have where the columns are kDim)
+
+  // Whether rows can be taken so: at most 2^31 bytes apart.
+  static bool possible(int dim, int64_t farthest) {
+    return (kPeriod == 1 || dim == kDim) && farthest * (int64_t)sizeof(T) < (1ll << 31);
+  }
+
+  // at(r): elements from the first row to row r.
+  template <class At>
+  __device__ EvenRows(int dim, At&& at) {
+    const int r = (int)threadIdx.x / L::kPer, place = threadIdx.x % L::kPer;
+#pragma unroll
+    for (int i = 0; i < kPeriod; ++i) {
+      const int chunk = place ^ L::swap(r + i * kRowsAStep);
+      own[i] = (uint32_t)((at(r) + chunk * kEach) * (int64_t)sizeof(T));
+      on = kPeriod > 1 || chunk * kEach < dim;
+    }
+  }
+
+  // first: the tile's first row; step: elements from a load's rows to the next one's.
+  __device__ __attribute__((always_inline)) void load(char* tile, const T* first,
+                                                      int64_t step) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < L::kBytes / kStep; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(
+                                                              first + i * step) +
+                                                          own[i % kPeriod]),
+          (__attribute__((address_space(3))) void*)(tile + i * kStep + wave * kWave * 16), 16, 0,
+          0);
+  }
+};
+
+template <class T, int kDim>
+bool even_keys(const omq_attention_args& a) {
+  const int64_t far = a.k_row_stride > a.v_row_stride ? a.k_row_stride : a.v_row_stride;
+  return EvenRows<T, kDim>::possible(a.dim, far < (1ll << 31) ? kTileKeys * far + kDim : far);
+}
+
 // The loads into LDS of this wave have arrived, and all waves come here.
 __device__ inline void tiles_ready() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -498,7 +564,8 @@ __device__ inline void tiles_ready() {
 }
 
 // Stores a lane's column of a result [kDim columns of a row, 32 rows] as a row, times `scale`.
-template <class T, int kDim>
+// kWhole: dim is a multiple of 8.
+template <class T, int kDim, bool kWhole>
 __device__ inline void store_column(T* row, const F16 (&x)[kDim / 32], float scale, int dim) {
 #pragma unroll
   for (int d = 0; d < kDim / 32; ++d)
@@ -506,11 +573,11 @@ __device__ inline void store_column(T* row, const F16 (&x)[kDim / 32], float sca
     for (int r = 0; r < 16; r += 4) {
       const int col = 32 * d + result_row(r);
       using V4 __attribute__((aligned(sizeof(T)))) = T __attribute__((ext_vector_type(4)));
-      if (col + 4 <= dim) {
+      if (kWhole ? col < dim : col + 4 <= dim) {
         *reinterpret_cast<V4*>(row + col) =
             V4{(T)(x[d][r] * scale), (T)(x[d][r + 1] * scale), (T)(x[d][r + 2] * scale),
                (T)(x[d][r + 3] * scale)};
-      } else {
+      } else if (!kWhole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (col + i < dim) row[col + i] = (T)(x[d][r + i] * scale);

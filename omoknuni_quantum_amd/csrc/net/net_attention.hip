@@ -32,7 +32,15 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 
   const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
   const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
+  const EvenRows<T, kDim> k_own(a.dim, [&](int r) { return r * a.k_row_stride; });
+  const EvenRows<T, kDim> v_own(a.dim, [&](int r) { return r * a.v_row_stride; });
   const auto load = [&](int k0, char* keys, char* values) {
+    if (kDirect && args.even && q.lk - k0 >= kTileKeys) {
+      constexpr int kRowsAStep = EvenRows<T, kDim>::kRowsAStep;
+      k_own.load(keys, k_rows + k0 * a.k_row_stride, kRowsAStep * a.k_row_stride);
+      v_own.load(values, v_rows + k0 * a.v_row_stride, kRowsAStep * a.v_row_stride);
+      return;
+    }
     load_tile<T, kDim, kDirect>(keys, q.lk - k0, a.dim, [&](int i) {
       return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
     });
@@ -53,9 +61,11 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;  // l: over this half's keys
   uint32_t found = 0;
+  typename L::Lane own;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
     tiles_ready();
+    own.renew();
     if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
     if (k0 >= x.most) return;
     const bool cuts = k0 + kTileKeys > x.least;  // some row does not see all of the tile
@@ -65,7 +75,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     for (int b = 0; b < 2; ++b) {
       s[b] = F16{};
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) s[b] = mma(L::row(keys, 32 * b, c), qf[c], s[b]);
+      for (int c = 0; c < L::kChunks; ++c) s[b] = mma(L::row(keys, 32 * b, c, own), qf[c], s[b]);
     }
     if (cuts) {
 #pragma unroll
@@ -96,7 +106,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
         s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], args.score_scale, -base));
         l += s[b][r];
       }
-      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, found);
+      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, found, own);
     }
   };
   // (two steps a turn, so that the tiles' arrays are told apart: the compiler would wait for all
@@ -110,7 +120,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   T* out = static_cast<T*>(args.out) + out_row * a.dim;
-  store_column<T, kDim>(out, o, inv, a.dim);
+  store_column<T, kDim, kDirect>(out, o, inv, a.dim);
   if (__builtin_expect(__any(found != 0), 0) && lane < 32)
     add_hidden<T, false>(out, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                          [=](int j) { return v_rows + j * a.v_row_stride; });
@@ -170,6 +180,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
   F16 o[kDim / 32] = {};
   float m = -kInf32, l = 0.0f;
   uint32_t found = 0;
+  typename L::Lane own;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
     if (k0 + kPartKeys < end) {
@@ -182,10 +193,11 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     // (a barrier would wait for the next tile; LDS accesses of one wave are in order)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
+    own.renew();
     const bool cuts = k0 + kPartKeys > x.least;
     F16 s = {};
 #pragma unroll
-    for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 0, c), qf[c], s);
+    for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 0, c, own), qf[c], s);
     if (cuts) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -210,7 +222,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
       s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
       l += s[r];
     }
-    add_columns<T, kDim, false>(o, values, 0, s, cuts, found);
+    add_columns<T, kDim, false>(o, values, 0, s, cuts, found, own);
   };
   for (int k0 = begin; k0 < end; k0 += 2 * kPartKeys) {  // (as above)
     step(k0, keys0, values0, keys1, values1);
@@ -225,7 +237,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
   const auto value = [=](int j) { return v_rows + j * a.v_row_stride; };
   if (args.splits == 1) {
     T* out = static_cast<T*>(args.out) + out_row * a.dim;
-    store_column<T, kDim>(out, o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
+    store_column<T, kDim, kDirect>(out, o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
     if (hidden) add_hidden<T, false>(out, a.dim, from, to, value);
     if (args.lse && lane < 32)
       args.lse[out_row] =
@@ -233,7 +245,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     return;
   }
   const int64_t part = split * args.out_rows + out_row;
-  store_column<float, kDim>(args.parts + part * a.dim, o, 1.0f, a.dim);
+  store_column<float, kDim, kDirect>(args.parts + part * a.dim, o, 1.0f, a.dim);
   if (hidden) add_hidden<T, false>(args.parts + part * a.dim, a.dim, from, to, value);
   if (lane < 32) args.part_stats[part] = make_float2(m, l);
 }
@@ -360,6 +372,7 @@ int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, vo
     tiles_of(&args, a->q_len, args.group, kTileRows);
     const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
     with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
+      args.even = even_keys<decltype(t), dim.value>(*a);
       attention_kernel<decltype(t), dim.value, direct.value><<<grid, kWaves * kWave, 0, st>>>(args);
     });
     return net_status(name);

@@ -30,7 +30,15 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 
   const T* k_rows = static_cast<const T*>(a.k) + q.k_at + at.kv * a.k_head_stride;
   const T* v_rows = static_cast<const T*>(a.v) + q.v_at + at.kv * a.v_head_stride;
+  const EvenRows<T, kDim> k_own(a.dim, [&](int r) { return r * a.k_row_stride; });
+  const EvenRows<T, kDim> v_own(a.dim, [&](int r) { return r * a.v_row_stride; });
   const auto load = [&](int k0, char* keys, char* values) {
+    if (kDirect && args.even && q.lk - k0 >= kTileKeys) {
+      constexpr int kRowsAStep = EvenRows<T, kDim>::kRowsAStep;
+      k_own.load(keys, k_rows + k0 * a.k_row_stride, kRowsAStep * a.k_row_stride);
+      v_own.load(values, v_rows + k0 * a.v_row_stride, kRowsAStep * a.v_row_stride);
+      return;
+    }
     load_tile<T, kDim, kDirect>(keys, q.lk - k0, a.dim, [&](int i) {
       return k_rows + (int64_t)(k0 + i) * a.k_row_stride;
     });
@@ -64,10 +72,13 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 
   F16 dq[kDim / 32] = {};
   uint32_t found = 0;
-  float rest = 0.0f;  // sum p (g.v - delta): what out's rounding took from delta
+  const float shift = delta * a.scale;
+  float rest = 0.0f;  // sum of ds: scale times what out's rounding took from delta
+  typename L::Lane own;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
     tiles_ready();
+    own.renew();
     if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
     if (k0 >= x.most) return;
     const bool cuts = k0 + kTileKeys > x.least;
@@ -75,25 +86,22 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     for (int b = 0; b < 2; ++b) {
       F16 s = {}, dp = {};
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 32 * b, c), qf[c], s);
+      for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 32 * b, c, own), qf[c], s);
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(values, 32 * b, c), gf[c], dp);
+      for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(values, 32 * b, c, own), gf[c], dp);
       const auto seen = [&](int r) { return k0 + 32 * b + result_row(r) < x.limit; };
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
-        s[r] = p * (dp[r] - delta);
+        s[r] = p * fmaf(dp[r], a.scale, -shift);
       }
       if (cuts) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = seen(r) ? s[r] : 0.0f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        rest += s[r];
-        s[r] *= a.scale;
-      }
-      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, found);
+      for (int r = 0; r < 16; ++r) rest += s[r];
+      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, found, own);
     }
   };
   // (two steps a turn: as in the forward kernel)
@@ -103,16 +111,16 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   }
   rest += other_half(rest);
   if (!x.there) return;
-  if (lane < 32) args.delta[out_row] = delta + rest;
+  if (lane < 32) args.delta[out_row] = delta + rest / a.scale;
   T* grad = static_cast<T*>(args.grad_q) + out_row * a.dim;
-  store_column<T, kDim>(grad, dq, 1.0f, a.dim);
+  store_column<T, kDim, kDirect>(grad, dq, 1.0f, a.dim);
   if (__builtin_expect(__any(found != 0), 0) && lane < 32)
     add_hidden<T, true>(grad, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                         [=](int j) { return k_rows + j * a.k_row_stride; });
 }
 
-// What a row of queries brings to the gradients by keys: the base of its probabilities, its delta,
-// and the keys that it sees.
+// What a row of queries brings to the gradients by keys: the base of its probabilities, its delta
+// times scale, and the keys that it sees.
 struct RowStats {
   float base[kTileKeys], delta[kTileKeys];
   int limit[kTileKeys];
@@ -156,7 +164,16 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
     const int query = query_of(args, r);
     return (int64_t)query * a.q_heads + (r - query * group);
   };
+  const EvenRows<T, kDim> q_own(a.dim, q_place);
+  const EvenRows<T, kDim> g_own(a.dim, [&](int r) { return out_place(r) * a.dim; });
   const auto load = [&](int r0, char* queries, char* grads) {
+    if (kDirect && args.even && rows - r0 >= kTileKeys) {
+      const int queries_a_step = EvenRows<T, kDim>::kRowsAStep / group, query = query_of(args, r0);
+      q_own.load(queries, q_rows + query * a.q_row_stride, queries_a_step * a.q_row_stride);
+      const int64_t heads = (int64_t)a.q_heads * a.dim;
+      g_own.load(grads, g_rows + query * heads, queries_a_step * heads);
+      return;
+    }
     load_tile<T, kDim, kDirect>(queries, rows - r0, a.dim,
                                 [&](int i) { return q_rows + q_place(r0 + i); });
     load_tile<T, kDim, kDirect>(grads, rows - r0, a.dim,
@@ -174,7 +191,7 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
     if (threadIdx.x < kTileKeys) {
       const int r = r0 + lane;
       stats.base[lane] = lse == -kInf32 ? 0.0f : lse * kLog2E;
-      stats.delta[lane] = delta;
+      stats.delta[lane] = delta * a.scale;
       stats.limit[lane] = r >= rows ? 0
                           : a.causal ? cut(query_of(args, r) + shift + 1, 0, q.lk)
                                      : q.lk;
@@ -198,12 +215,14 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
                                        kv * a.v_head_stride, a.dim);
   F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
   uint32_t found_q = 0, found_g = 0;
+  typename L::Lane own;
   const auto step = [&](int64_t next, const char* queries, const char* grads,
                         const RowStats& stats, char* next_queries, char* next_grads,
                         RowStats& next_stats) __attribute__((always_inline)) {
     const int r0 = (int)next;
     const bool more = next + kTileKeys < end;
     tiles_ready();
+    own.renew();
     if (more) load(r0 + kTileKeys, next_queries, next_grads), fetch(r0 + kTileKeys);
     // some row does not see all of the wave's keys; or none does
     const int low = a.causal ? query_of(args, r0) + shift + 1 : q.lk;
@@ -214,10 +233,10 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
       for (int b = 0; b < 2; ++b) {
         F16 s = {}, dp = {};
 #pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c), kf[c], s);
+        for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c, own), kf[c], s);
         if constexpr (kKeys) {
 #pragma unroll
-          for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c), vf[c], dp);
+          for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c, own), vf[c], dp);
         }
         F16 p;
 #pragma unroll
@@ -227,7 +246,7 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
         if constexpr (kKeys) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            s[r] = p[r] * (dp[r] - stats.delta[32 * b + result_row(r)]) * a.scale;
+            s[r] = p[r] * fmaf(dp[r], a.scale, -stats.delta[32 * b + result_row(r)]);
         }
         if (cuts) {
 #pragma unroll
@@ -237,8 +256,8 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
             s[r] = sees ? s[r] : 0.0f;
           }
         }
-        if constexpr (kValues) add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g);
-        if constexpr (kKeys) add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q);
+        if constexpr (kValues) add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g, own);
+        if constexpr (kKeys) add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q, own);
       }
     }
     if (more) put(r0 + kTileKeys, next_stats);
@@ -255,8 +274,8 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
   }
   const int64_t out = ((q.k_first + key) * a.k_heads + kv) * a.dim;
   T *grad_k = static_cast<T*>(args.grad_k) + out, *grad_v = static_cast<T*>(args.grad_v) + out;
-  if constexpr (kKeys) store_column<T, kDim>(grad_k, dk, 1.0f, a.dim);
-  if constexpr (kValues) store_column<T, kDim>(grad_v, dv, 1.0f, a.dim);
+  if constexpr (kKeys) store_column<T, kDim, kDirect>(grad_k, dk, 1.0f, a.dim);
+  if constexpr (kValues) store_column<T, kDim, kDirect>(grad_v, dv, 1.0f, a.dim);
   if (__builtin_expect(__any((found_q | found_g) != 0), 0) && lane < 32 && mine < q.lk) {
     const int64_t least = a.causal && mine > shift ? (int64_t)(mine - shift) * group : 0;
     const int sees = least < rows ? (int)least : rows;  // the first row that sees this key
@@ -333,6 +352,7 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
     tiles_of(&args, a->q_len, args.group, kTileRows);
     const dim3 grid = grid_of(args.slots * a->k_heads, kWaves * kWave);
     with_head(a->dtype, a->dim, direct_tiles(*a), [&](auto t, auto dim, auto direct) {
+      args.even = even_keys<decltype(t), dim.value>(*a);
       attention_grad_q_kernel<decltype(t), dim.value, direct.value>
           <<<grid, kWaves * kWave, 0, st>>>(args);
     });
@@ -342,6 +362,14 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
     const bool rows_direct = chunks_aligned(a->dtype, a->dim, {a->q, grad_out},
                                             {a->q_seq_stride, a->q_row_stride, a->q_head_stride});
     with_head(a->dtype, a->dim, rows_direct, [&](auto t, auto dim, auto direct) {
+      // (rows of a group lie as far apart at every step that has whole groups)
+      using Even = EvenRows<decltype(t), dim.value>;
+      const int64_t far = a->q_row_stride < (1ll << 31) && a->q_head_stride < (1ll << 31)
+                              ? (kTileKeys + 1) * a->q_row_stride + args.group * a->q_head_stride
+                              : 1ll << 31;
+      const int64_t far_out = (kTileKeys + 1) * (int64_t)a->q_heads * a->dim;
+      args.even = Even::kRowsAStep % args.group == 0 &&
+                  Even::possible(a->dim, far > far_out ? far : far_out);
       const int64_t blocks = args.slots * a->k_heads * (sums_apart<dim.value>() ? 2 : 1);
       const dim3 grid = grid_of(blocks, kWaves * kWave);
       attention_grad_kv_kernel<decltype(t), dim.value, direct.value>
