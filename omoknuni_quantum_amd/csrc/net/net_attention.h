@@ -45,6 +45,7 @@ struct AttentionArgs {
   int64_t batch_tiles;  // tiles of a sequence of a batch
   float score_scale;    // scale * log2 e
   int even;             // the moving side's rows are EvenRows
+  int paired;           // (place_of_keys)
   int splits;           // parts of a sequence's keys, each a workgroup's
   float* parts;         // [splits, rows of out, dim] sums, and behind them
   float2* part_stats;   // [splits, rows of out] maximum and sum of the exponentials
@@ -162,12 +163,16 @@ __device__ inline bool place_of_queries(const AttentionArgs& args, int tile_rows
   return p->tile >= 0 && p->tile * tile_rows < (int64_t)p->q.lq * args.group;
 }
 
-// The same by keys, the first ones first: in a causal sequence the most queries see them.
+// The same by keys, the first ones first: in a causal sequence the most queries see them.  Where all
+// workgroups run at once, two on a compute unit (`paired`), the second half comes in the other
+// order, so that a long one shares its unit with a short one.
 __device__ inline bool place_of_keys(const AttentionArgs& args, int tile_rows, int64_t block,
                                      Place* p) {
   const omq_attention_args& a = args.a;
-  const int64_t slot = block / a.k_heads;
+  int64_t slot = block / a.k_heads;
   if (slot >= args.slots) return false;
+  const int64_t half = (args.slots + 1) / 2;
+  if (args.paired && slot >= half) slot = args.slots - 1 - (slot - half);
   p->kv = (int)(block % a.k_heads);
   if (a.q_starts) {
     p->q = sequence_of(args,

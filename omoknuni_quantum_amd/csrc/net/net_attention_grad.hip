@@ -287,6 +287,8 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
   }
 }
 
+constexpr int kComputeUnits = 256;
+
 // Sums of 128 columns are a workgroup's each, of the keys or of the values (scores are formed in
 // both: five products in place of four): with both a wave has no room for a second one on its SIMD,
 // whose products run while the first forms its probabilities.
@@ -371,6 +373,7 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
       args.even = Even::kRowsAStep % args.group == 0 &&
                   Even::possible(a->dim, far > far_out ? far : far_out);
       const int64_t blocks = args.slots * a->k_heads * (sums_apart<dim.value>() ? 2 : 1);
+      args.paired = a->causal && blocks > kComputeUnits && blocks <= 2 * kComputeUnits;
       const dim3 grid = grid_of(blocks, kWaves * kWave);
       attention_grad_kv_kernel<decltype(t), dim.value, direct.value>
           <<<grid, kWaves * kWave, 0, st>>>(args);
