@@ -361,13 +361,76 @@ __device__ inline Frag finite_only(const Frag& v, uint32_t& found) {
   return __builtin_bit_cast(Frag, x);
 }
 
-// acc += (columns of the tile's 32 rows from row0) x w; cuts: a mask cuts the tile.  kTwice: w to
-// twice the type's bits, what its rounding leaves in a second product.
-template <class T, int kDim, bool kTwice>
-__device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int row0, const F16& w,
-                                   bool cuts, uint32_t& found,
-                                   const typename Tile<T, kDim>::Lane& lane) {
+// Keeps the compiler from moving instructions across: reads of LDS are under way this far ahead of
+// the products that use them, and no further, for which there are no registers.
+__device__ __attribute__((always_inline)) inline void here() {
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Products of two blocks of 32 rows with 32 rows in registers, each of its own tile, the second
+// one's reads under way with the first one's products.
+template <class T, int kDim>
+__device__ __attribute__((always_inline)) inline void two_products(
+    F16& s, const char* tile, int row0, const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
+    F16& s2, const char* tile2, int row2,
+    const typename Operand<T>::Frag (&f2)[kDim / Operand<T>::kChunk],
+    const typename Tile<T, kDim>::Lane& lane) {
   using L = Tile<T, kDim>;
+  typename L::Frag a[L::kChunks], b[L::kChunks];
+#pragma unroll
+  for (int c = 0; c < L::kChunks; ++c) a[c] = L::row(tile, row0, c, lane);
+  here();
+  s = F16{}, s2 = F16{};
+#pragma unroll
+  for (int c = 0; c < L::kChunks; ++c) {
+    b[c] = L::row(tile2, row2, c, lane);
+    s = mma(a[c], f[c], s);
+  }
+  here();
+#pragma unroll
+  for (int c = 0; c < L::kChunks; ++c) s2 = mma(b[c], f2[c], s2);
+}
+
+template <class T, int kDim>
+__device__ __attribute__((always_inline)) inline void one_product(
+    F16& s, const char* tile, int row0, const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
+    const typename Tile<T, kDim>::Lane& lane) {
+  using L = Tile<T, kDim>;
+  typename L::Frag a[L::kChunks];
+#pragma unroll
+  for (int c = 0; c < L::kChunks; ++c) a[c] = L::row(tile, row0, c, lane);
+  here();
+  s = F16{};
+#pragma unroll
+  for (int c = 0; c < L::kChunks; ++c) s = mma(a[c], f[c], s);
+}
+
+// acc += (columns of the tile's 32 rows from row0) x w, a group of the columns' operands at a time;
+// the first group is read by `columns_ahead`, before w is formed.
+template <class T, int kDim>
+struct Columns {
+  using L = Tile<T, kDim>;
+  static constexpr int kAll = kDim / 32 * L::kParts, kGroup = kAll < 4 ? kAll : 4;
+  typename L::Frag v[kGroup];
+
+  __device__ __attribute__((always_inline)) void read(const char* tile, int row0, int group,
+                                                      const typename L::Lane& lane) {
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const int at = group * kGroup + i;
+      v[i] = L::column(tile, row0, at / L::kParts * 32, at % L::kParts, lane);
+    }
+  }
+};
+
+// cuts: a mask cuts the tile.  kTwice: w to twice the type's bits, what its rounding leaves in a
+// second product.
+template <class T, int kDim, bool kTwice>
+__device__ __attribute__((always_inline)) inline void add_columns(
+    F16 (&acc)[kDim / 32], Columns<T, kDim>& first, const char* tile, int row0, const F16& w,
+    bool cuts, uint32_t& found, const typename Tile<T, kDim>::Lane& lane) {
+  using L = Tile<T, kDim>;
+  using C = Columns<T, kDim>;
   constexpr bool kRest = kTwice && sizeof(T) == 2;
   typename L::Frag part[L::kParts], rest[kRest ? L::kParts : 1];
 #pragma unroll
@@ -380,21 +443,26 @@ __device__ inline void add_columns(F16 (&acc)[kDim / 32], const char* tile, int 
       rest[t] = L::part(left, t);
     }
   }
-  const auto add = [&](auto cut) {
+  C now = first;
 #pragma unroll
-    for (int d = 0; d < kDim / 32; ++d)
+  for (int g = 0; g < C::kAll / C::kGroup; ++g) {
+    C next;
+    here();
+    if (g + 1 < C::kAll / C::kGroup) next.read(tile, row0, g + 1, lane);
+    if (cuts) {
 #pragma unroll
-      for (int t = 0; t < L::kParts; ++t) {
-        typename L::Frag v = L::column(tile, row0, 32 * d, t, lane);
-        if constexpr (cut.value) v = finite_only<T>(v, found);
-        acc[d] = mma(v, part[t], acc[d]);
-        if constexpr (kRest) acc[d] = mma(v, rest[t], acc[d]);
-      }
-  };
-  if (cuts)
-    add(std::true_type{});
-  else
-    add(std::false_type{});
+      for (int i = 0; i < C::kGroup; ++i) now.v[i] = finite_only<T>(now.v[i], found);
+    }
+    here();
+#pragma unroll
+    for (int i = 0; i < C::kGroup; ++i) {
+      const int d = (g * C::kGroup + i) / L::kParts, t = (g * C::kGroup + i) % L::kParts;
+      acc[d] = mma(now.v[i], part[t], acc[d]);
+      if constexpr (kRest) acc[d] = mma(now.v[i], rest[t], acc[d]);
+    }
+    now = next;
+  }
+  here();
 }
 
 // Adds to a stored row what the values that are not finite make of it, of the rows from `from` to

@@ -18,6 +18,68 @@ namespace {
 // left out for most tiles, and a probability is at most 2^8 (float16 holds 2^15).
 constexpr float kLag = 8.0f;
 
+// A row's output so far: sums about the maximum m; l over this half's keys.
+template <int kDim>
+struct Softmax {
+  F16 o[kDim / 32] = {};
+  float m = -kInf32, l = 0.0f;
+  uint32_t found = 0;
+};
+
+__device__ inline float lse_of(float m, float l, float scale) {
+  return l == 0.0f ? -kInf32 : fmaf(m, scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+}
+
+// Attends to one or two blocks of 32 keys from k0, of which the row sees those below `limit`; cuts:
+// some row of the wave does not see all of them.
+template <class T, int kDim, int kBlocks>
+__device__ __attribute__((always_inline)) inline void attend(
+    Softmax<kDim>& x, const char* keys, const char* values,
+    const typename Operand<T>::Frag (&qf)[kDim / Operand<T>::kChunk], int k0, bool cuts, int limit,
+    float scale, const typename Tile<T, kDim>::Lane& lane) {
+  F16 s[kBlocks];
+  if constexpr (kBlocks == 2)
+    two_products<T, kDim>(s[0], keys, 0, qf, s[1], keys, 32, qf, lane);
+  else
+    one_product<T, kDim>(s[0], keys, 0, qf, lane);
+  Columns<T, kDim> columns;
+  columns.read(values, 0, 0, lane);
+  here();
+  if (cuts) {
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (k0 + 32 * b + result_row(r) >= limit) s[b][r] = -kInf32;
+  }
+  float top = -kInf32;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+  top = fmaxf(top, other_half(top));
+  if (__any((top - x.m) * scale > kLag)) {  // (m is -inf at first)
+    const float next = fmaxf(x.m, top);
+    const float keep = next == -kInf32 ? 1.0f : __builtin_amdgcn_exp2f((x.m - next) * scale);
+    x.m = next;
+    x.l *= keep;
+#pragma unroll
+    for (int d = 0; d < kDim / 32; ++d) x.o[d] *= keep;
+  }
+  const float base = x.m == -kInf32 ? 0.0f : x.m * scale;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    if (b > 0) columns.read(values, 32 * b, 0, lane);
+    here();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -base));
+      x.l += s[b][r];
+    }
+    add_columns<T, kDim, false>(x.o, columns, values, 32 * b, s[b], cuts, x.found, lane);
+  }
+}
+
 template <class T, int kDim, bool kDirect>
 __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
@@ -58,56 +120,16 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
                             x.head * a.q_head_stride, a.dim);
 
-  F16 o[kDim / 32] = {};
-  float m = -kInf32, l = 0.0f;  // l: over this half's keys
-  uint32_t found = 0;
+  Softmax<kDim> sum;
   typename L::Lane own;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
     tiles_ready();
     own.renew();
     if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
-    if (k0 >= x.most) return;
-    const bool cuts = k0 + kTileKeys > x.least;  // some row does not see all of the tile
-    F16 s[2];
-    float top = -kInf32;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = F16{};
-#pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) s[b] = mma(L::row(keys, 32 * b, c, own), qf[c], s[b]);
-    }
-    if (cuts) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + result_row(r) >= x.limit) s[b][r] = -kInf32;
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = fmaxf(top, other_half(top));
-    if (__any((top - m) * args.score_scale > kLag)) {  // (m is -inf at first)
-      const float next = fmaxf(m, top);
-      const float keep =
-          next == -kInf32 ? 1.0f : __builtin_amdgcn_exp2f((m - next) * args.score_scale);
-      m = next;
-      l *= keep;
-#pragma unroll
-      for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
-    }
-    const float base = m == -kInf32 ? 0.0f : m * args.score_scale;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], args.score_scale, -base));
-        l += s[b][r];
-      }
-      add_columns<T, kDim, false>(o, values, 32 * b, s[b], cuts, found, own);
-    }
+    if (k0 < x.most)
+      attend<T, kDim, 2>(sum, keys, values, qf, k0, k0 + kTileKeys > x.least, x.limit,
+                         args.score_scale, own);
   };
   // (two steps a turn, so that the tiles' arrays are told apart: the compiler would wait for all
   // loads under way before it reads an array that they may write)
@@ -115,18 +137,16 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     step(k0, keys0, values0, keys1, values1);
     if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
-  l += other_half(l);
+  const float l = sum.l + other_half(sum.l);
   if (!x.there) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   T* out = static_cast<T*>(args.out) + out_row * a.dim;
-  store_column<T, kDim, kDirect>(out, o, inv, a.dim);
-  if (__builtin_expect(__any(found != 0), 0) && lane < 32)
+  store_column<T, kDim, kDirect>(out, sum.o, inv, a.dim);
+  if (__builtin_expect(__any(sum.found != 0), 0) && lane < 32)
     add_hidden<T, false>(out, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                          [=](int j) { return v_rows + j * a.v_row_stride; });
-  if (args.lse && lane < 32)
-    args.lse[out_row] =
-        l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+  if (args.lse && lane < 32) args.lse[out_row] = lse_of(sum.m, l, a.scale);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -177,9 +197,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
   load_row<T, kDim, kDirect>(qf, static_cast<const T*>(a.q) + q.q_at + x.query * a.q_row_stride +
                                      x.head * a.q_head_stride, a.dim);
   if (begin < end) load(begin, keys0, values0);
-  F16 o[kDim / 32] = {};
-  float m = -kInf32, l = 0.0f;
-  uint32_t found = 0;
+  Softmax<kDim> sum;
   typename L::Lane own;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
@@ -194,60 +212,31 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
     own.renew();
-    const bool cuts = k0 + kPartKeys > x.least;
-    F16 s = {};
-#pragma unroll
-    for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 0, c, own), qf[c], s);
-    if (cuts) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (k0 + result_row(r) >= x.limit) s[r] = -kInf32;
-    }
-    float top = -kInf32;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = fmaxf(top, other_half(top));
-    if (__any((top - m) * args.score_scale > kLag)) {
-      const float next = fmaxf(m, top);
-      const float keep =
-          next == -kInf32 ? 1.0f : __builtin_amdgcn_exp2f((m - next) * args.score_scale);
-      m = next;
-      l *= keep;
-#pragma unroll
-      for (int d = 0; d < kDim / 32; ++d) o[d] *= keep;
-    }
-    const float base = m == -kInf32 ? 0.0f : m * args.score_scale;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
-      l += s[r];
-    }
-    add_columns<T, kDim, false>(o, values, 0, s, cuts, found, own);
+    attend<T, kDim, 1>(sum, keys, values, qf, k0, k0 + kPartKeys > x.least, x.limit,
+                       args.score_scale, own);
   };
   for (int k0 = begin; k0 < end; k0 += 2 * kPartKeys) {  // (as above)
     step(k0, keys0, values0, keys1, values1);
     if (k0 + kPartKeys < end) step(k0 + kPartKeys, keys1, values1, keys0, values0);
   }
-  l += other_half(l);
+  const float l = sum.l + other_half(sum.l);
   if (!x.there) return;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   const int least = x.least / kPartKeys * kPartKeys;
   const int from = begin > least ? begin : least, to = end < x.limit ? end : x.limit;
-  const bool hidden = __any(found != 0) && lane < 32;
+  const bool hidden = __any(sum.found != 0) && lane < 32;
   const auto value = [=](int j) { return v_rows + j * a.v_row_stride; };
   if (args.splits == 1) {
     T* out = static_cast<T*>(args.out) + out_row * a.dim;
-    store_column<T, kDim, kDirect>(out, o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
+    store_column<T, kDim, kDirect>(out, sum.o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
     if (hidden) add_hidden<T, false>(out, a.dim, from, to, value);
-    if (args.lse && lane < 32)
-      args.lse[out_row] =
-          l == 0.0f ? -kInf32 : fmaf(m, a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+    if (args.lse && lane < 32) args.lse[out_row] = lse_of(sum.m, l, a.scale);
     return;
   }
   const int64_t part = split * args.out_rows + out_row;
-  store_column<float, kDim, kDirect>(args.parts + part * a.dim, o, 1.0f, a.dim);
+  store_column<float, kDim, kDirect>(args.parts + part * a.dim, sum.o, 1.0f, a.dim);
   if (hidden) add_hidden<T, false>(args.parts + part * a.dim, a.dim, from, to, value);
-  if (lane < 32) args.part_stats[part] = make_float2(m, l);
+  if (lane < 32) args.part_stats[part] = make_float2(sum.m, l);
 }
 
 // A row of the output from its parts (at most 64), a wave a row.
@@ -278,9 +267,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs args)
   for (int i = 0; i < 2; ++i)
     if (lane + 64 * i < dim)
       static_cast<T*>(args.out)[row * dim + lane + 64 * i] = (T)x[i];
-  if (args.lse && lane == 0)
-    args.lse[row] =
-        l == 0.0f ? -kInf32 : fmaf(m, args.a.scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+  if (args.lse && lane == 0) args.lse[row] = lse_of(m, l, args.a.scale);
 }
 
 // Whether a call takes the kernel for few rows, and with how many parts.

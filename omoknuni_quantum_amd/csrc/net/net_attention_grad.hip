@@ -84,12 +84,11 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     const bool cuts = k0 + kTileKeys > x.least;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      F16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(keys, 32 * b, c, own), qf[c], s);
-#pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(values, 32 * b, c, own), gf[c], dp);
-      const auto seen = [&](int r) { return k0 + 32 * b + result_row(r) < x.limit; };
+      F16 s, dp;
+      two_products<T, kDim>(s, keys, 32 * b, qf, dp, values, 32 * b, gf, own);
+      Columns<T, kDim> columns;
+      columns.read(keys, 32 * b, 0, own);
+      here();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
@@ -97,11 +96,12 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
       }
       if (cuts) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = seen(r) ? s[r] : 0.0f;
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * b + result_row(r) >= x.limit) s[r] = 0.0f;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) rest += s[r];
-      add_columns<T, kDim, true>(dq, keys, 32 * b, s, cuts, found, own);
+      add_columns<T, kDim, true>(dq, columns, keys, 32 * b, s, cuts, found, own);
     }
   };
   // (two steps a turn: as in the forward kernel)
@@ -231,22 +231,20 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
     if (from < high && from < q.lk) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        F16 s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) s = mma(L::row(queries, 32 * b, c, own), kf[c], s);
-        if constexpr (kKeys) {
-#pragma unroll
-          for (int c = 0; c < L::kChunks; ++c) dp = mma(L::row(grads, 32 * b, c, own), vf[c], dp);
-        }
+        F16 s, dp;
+        if constexpr (kKeys)
+          two_products<T, kDim>(s, queries, 32 * b, kf, dp, grads, 32 * b, vf, own);
+        else
+          one_product<T, kDim>(s, queries, 32 * b, kf, own);
+        Columns<T, kDim> columns;
+        columns.read(kValues ? grads : queries, 32 * b, 0, own);
+        here();
         F16 p;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          p[r] = __builtin_amdgcn_exp2f(
-              fmaf(s[r], args.score_scale, -stats.base[32 * b + result_row(r)]));
-        if constexpr (kKeys) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[r] = p[r] * fmaf(dp[r], a.scale, -stats.delta[32 * b + result_row(r)]);
+        for (int r = 0; r < 16; ++r) {
+          const int i = 32 * b + result_row(r);
+          p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -stats.base[i]));
+          if constexpr (kKeys) s[r] = p[r] * fmaf(dp[r], a.scale, -stats.delta[i]);
         }
         if (cuts) {
 #pragma unroll
@@ -256,8 +254,12 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
             s[r] = sees ? s[r] : 0.0f;
           }
         }
-        if constexpr (kValues) add_columns<T, kDim, false>(dv, grads, 32 * b, p, cuts, found_g, own);
-        if constexpr (kKeys) add_columns<T, kDim, false>(dk, queries, 32 * b, s, cuts, found_q, own);
+        if constexpr (kValues)
+          add_columns<T, kDim, false>(dv, columns, grads, 32 * b, p, cuts, found_g, own);
+        if constexpr (kKeys) {
+          if constexpr (kValues) columns.read(queries, 32 * b, 0, own);
+          add_columns<T, kDim, false>(dk, columns, queries, 32 * b, s, cuts, found_q, own);
+        }
       }
     }
     if (more) put(r0 + kTileKeys, next_stats);
