@@ -424,11 +424,16 @@ struct Columns {
 };
 
 // cuts: a mask cuts the tile.  kTwice: w to twice the type's bits, what its rounding leaves in a
-// second product.
-template <class T, int kDim, bool kTwice>
+// second product.  beside(i): what runs beside product i of kAll.
+struct Nothing {
+  __device__ void operator()(int) const {}
+};
+
+template <class T, int kDim, bool kTwice, class Beside = Nothing>
 __device__ __attribute__((always_inline)) inline void add_columns(
     F16 (&acc)[kDim / 32], Columns<T, kDim>& first, const char* tile, int row0, const F16& w,
-    bool cuts, uint32_t& found, const typename Tile<T, kDim>::Lane& lane) {
+    bool cuts, uint32_t& found, const typename Tile<T, kDim>::Lane& lane,
+    Beside&& beside = Beside()) {
   using L = Tile<T, kDim>;
   using C = Columns<T, kDim>;
   constexpr bool kRest = kTwice && sizeof(T) == 2;
@@ -459,6 +464,7 @@ __device__ __attribute__((always_inline)) inline void add_columns(
       const int d = (g * C::kGroup + i) / L::kParts, t = (g * C::kGroup + i) % L::kParts;
       acc[d] = mma(now.v[i], part[t], acc[d]);
       if constexpr (kRest) acc[d] = mma(now.v[i], rest[t], acc[d]);
+      beside(g * C::kGroup + i);
     }
     now = next;
   }

@@ -67,16 +67,27 @@ __device__ __attribute__((always_inline)) inline void attend(
     for (int d = 0; d < kDim / 32; ++d) x.o[d] *= keep;
   }
   const float base = x.m == -kInf32 ? 0.0f : x.m * scale;
+  const auto form = [&](int b, int r) __attribute__((always_inline)) {
+    s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -base));
+    x.l += s[b][r];
+  };
+  here();
 #pragma unroll
-  for (int b = 0; b < kBlocks; ++b) {
-    if (b > 0) columns.read(values, 32 * b, 0, lane);
+  for (int r = 0; r < 16; ++r) form(0, r);
+  if constexpr (kBlocks == 1) {
+    add_columns<T, kDim, false>(x.o, columns, values, 0, s[0], cuts, x.found, lane);
+  } else {
+    // (a wave's products run while it forms the other block's probabilities)
+    constexpr int kAll = Columns<T, kDim>::kAll, kEach = 16 / kAll > 0 ? 16 / kAll : 1;
+    add_columns<T, kDim, false>(x.o, columns, values, 0, s[0], cuts, x.found, lane, [&](int i) {
+#pragma unroll
+      for (int r = 0; r < kEach; ++r)
+        if (i * kEach + r < 16) form(1, i * kEach + r);
+      here();
+    });
+    columns.read(values, 32, 0, lane);
     here();
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -base));
-      x.l += s[b][r];
-    }
-    add_columns<T, kDim, false>(x.o, columns, values, 32 * b, s[b], cuts, x.found, lane);
+    add_columns<T, kDim, false>(x.o, columns, values, 32, s[1], cuts, x.found, lane);
   }
 }
 
