@@ -1,7 +1,7 @@
 // The log-probabilities of given tokens over the legal ones, with the entropy and the best
 // alternatives, and their gradient (gfx950).
 //
-// Per row, about a base m near the largest legal logit, with x = z - m, rest = sum e^x and
+// Per row, about a base m at the largest legal logit, with x = z - m, rest = sum e^x and
 // xe = sum e^x x over the legal tokens but the given one, t, and s = rest + e^(x_t):
 //   logp    = x_t - log s
 //   entropy = log s - (xe + e^(x_t) x_t) / s
@@ -33,7 +33,9 @@ struct LogprobArgs {
   int top;
 };
 
-// Sums of a part of a row about its base; m is -inf while nothing in it has weight.
+// Sums of a part of a row about its largest logit m; m is -inf while nothing in it has weight.  An
+// exponential is 2^y, y = z log2 e - exponent_of(m), a product and a difference rounded once: what
+// the exponent of m was rounded by cancels however large the logits are.  xe is the sum of 2^y y.
 struct Sums {
   float m, rest, xe;
 };
@@ -42,10 +44,24 @@ __device__ inline Sums no_sums() { return Sums{-kInf, 0.0f, 0.0f}; }
 
 __device__ inline float base_of(float m) { return m == -kInf ? 0.0f : m; }
 
+// m log2 e, rounded to float32 as long as that holds it.
+__device__ inline double exponent_of(float m) {
+  return fabsf(m) < 0x1p126f ? (double)(m * kLog2e) : (double)m * (double)kLog2e;
+}
+
+// y of a logit, and of a part's m about another one's.
+__device__ inline float y_of(float z, float m) {
+  return fabsf(m) < 0x1p126f ? fmaf(z, kLog2e, -(m * kLog2e)) : (z - m) * kLog2e;
+}
+
+__device__ inline float y_between(float from, float to) {
+  return from == -kInf ? -kInf : (float)(exponent_of(from) - exponent_of(to));
+}
+
 // About another base, which is finite or that of a part without weight.
 __device__ inline void rebase(Sums& t, float m) {
   if (t.m != m) {
-    const float d = t.m - base_of(m), scale = exp_fast(d);
+    const float d = y_between(t.m, base_of(m)), scale = __builtin_amdgcn_exp2f(d);
     t.rest *= scale;
     t.xe = scale != 0.0f ? fmaf(d, t.rest, scale * t.xe) : t.rest;  // (0, or NaN; d may be -inf)
     t.m = m;
@@ -84,14 +100,34 @@ __device__ inline float largest_number(const F8& z) {
   return m;
 }
 
-// Adds a block of logits; `at`: the given token's place in it, if it is there.
-__device__ inline void add_block(Sums& t, const F8& z, float base, int at) {
+// Adds a block of logits about a base; `at`: the given token's place in it, if it is there.  y and
+// e: a logit's y, no less than -2^100, for which the products with e = 0 are 0, and 2^y.
+__device__ inline void exponentials(const F8& z, float base, F8& y, F8& e) {
+  if (fabsf(base) < 0x1p126f) {
+    const float exponent = base * kLog2e;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = fmaf(z[j], kLog2e, -exponent);
+  } else {
+    y = (z - base) * kLog2e;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float x = z[j] - base;
-    const float e = j == at ? 0.0f : exp_fast(x);
-    t.rest += e;
-    t.xe = fmaf(e, larger(x, -0x1p100f), t.xe);  // (0 for -inf; a NaN is in e)
+    e[j] = __builtin_amdgcn_exp2f(y[j]);  // (a NaN is kept here)
+    y[j] = larger(y[j], -0x1p100f);
+  }
+}
+
+__device__ inline void add_block(Sums& t, const F8& z, float base, int at, F8& y, F8& e) {
+  exponentials(z, base, y, e);
+  F8 added = e;
+  if ((uint32_t)at < 8u) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) added[j] = j == at ? 0.0f : e[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    t.rest += added[j];
+    t.xe = fmaf(added[j], y[j], t.xe);
   }
 }
 
@@ -103,11 +139,16 @@ struct RowEnd {
   bool live;
 };
 
+// log p of a legal logit.
+__device__ inline double logp_of(const RowEnd& o, float z) {
+  return ((double)z * (double)kLog2e - exponent_of(o.base)) * 0.6931471805599453 - o.log_s64;
+}
+
 __device__ inline RowEnd finish_row(const Sums& t, float z_token, bool given) {
   RowEnd o{};
   o.base = base_of(t.m);
-  const float x = given ? z_token - o.base : 0.0f;
-  const float e = given ? exp_fast(x) : 0.0f;
+  const float y = given ? y_of(z_token, o.base) : 0.0f;
+  const float e = given ? __builtin_amdgcn_exp2f(y) : 0.0f;
   const float s = t.rest + e;
   o.live = !(t.m == -kInf && s == 0.0f);
   if (!o.live) return o;
@@ -115,9 +156,9 @@ __device__ inline RowEnd finish_row(const Sums& t, float z_token, bool given) {
   o.log_s = (float)o.log_s64;
   o.inv_s = 1.0f / s;
   o.others = t.rest * o.inv_s;
-  const float xe = e != 0.0f ? fmaf(e, x, t.xe) : t.xe;
-  o.entropy = (float)(o.log_s64 - (double)xe * (double)o.inv_s);
-  if (given) o.logp = (float)((double)z_token - (double)o.base - o.log_s64);
+  const float xe = e != 0.0f ? fmaf(e, y, t.xe) : t.xe;
+  o.entropy = (float)(o.log_s64 - (double)xe * (double)o.inv_s * 0.6931471805599453);
+  if (given) o.logp = (float)logp_of(o, z_token);
   return o;
 }
 
@@ -138,21 +179,31 @@ __device__ inline int token_of(const omq_logprob_rows& r, int64_t row, float* z)
   return (int)a;
 }
 
-// The gradient of a block of logits but for the given token's.
-__device__ inline F8 gradient(const F8& z, const RowEnd& o, float a, float b) {
+// A row's gradient from its y and e about another base: but for the given token's it is
+// -p (a + b (log p + entropy)), p = e inv.
+struct RowSlope {
+  float inv, shift, slope;  // the bracket is slope * y + shift
+};
+
+__device__ inline RowSlope slope_of(const RowEnd& o, float base, float a, float b) {
+  // (about a base of -inf, that of a part without weight, y and e are those of base 0)
+  const float d = y_between(base_of(base), o.base);
+  const float scale = __builtin_amdgcn_exp2f(d);
+  if (scale == 0.0f) return {scale * o.inv_s, 0.0f, 0.0f};  // (d may be -inf)
+  return {scale * o.inv_s, fmaf(b, d * kLn2 - o.log_s + o.entropy, a), b * kLn2};
+}
+
+__device__ inline F8 gradient(const F8& y, const F8& e, const RowSlope& r) {
   F8 g;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x = z[j] - o.base;
-    const float p = exp_fast(x) * o.inv_s;
-    g[j] = -p * fmaf(b, larger(x, -0x1p100f) - o.log_s + o.entropy, a);
-  }
+  for (int j = 0; j < 8; ++j) g[j] = -(e[j] * r.inv) * fmaf(y[j], r.slope, r.shift);
   return g;
 }
 
 __device__ inline float gradient_of_token(const RowEnd& o, float z, float a, float b) {
-  const float x = z - o.base, p = exp_fast(x) * o.inv_s;
-  const float h = b != 0.0f ? b * p * (larger(x, -0x1p100f) - o.log_s + o.entropy) : 0.0f;
+  const float y = y_of(z, o.base), p = __builtin_amdgcn_exp2f(y) * o.inv_s;
+  const float h =
+      b != 0.0f ? b * p * (larger(y, -0x1p100f) * kLn2 - o.log_s + o.entropy) : 0.0f;
   return fmaf(a, o.others, -h);
 }
 
@@ -232,7 +283,7 @@ __device__ inline void best_of_row(const LogprobArgs& a, int64_t row, const RowE
   float* logp = a.top_logp + row * a.top;
   int64_t* tokens = a.top_tokens + row * a.top;
   const auto put = [&](int rank, uint64_t key) {
-    logp[rank] = (float)((double)logit_of(key) - (double)o.base - o.log_s64);
+    logp[rank] = (float)logp_of(o, logit_of(key));
     tokens[rank] = (int64_t)(0xFFFFFFFFu - (uint32_t)key);
   };
   const auto none = [&](int rank) { logp[rank] = -kInf, tokens[rank] = -1; };
@@ -266,7 +317,7 @@ __device__ inline void best_of_row(const LogprobArgs& a, int64_t row, const RowE
 }
 
 // ---- a row's results ------------------------------------------------------------------------
-__device__ inline void write_row(const LogprobArgs& a, int64_t row, const RowEnd& o, bool given) {
+__device__ inline void write_row(const LogprobArgs& a, int64_t row, const RowEnd& o) {
   a.logp[row] = o.logp;
   a.entropy[row] = o.entropy;
   if (a.stats) {
@@ -283,16 +334,18 @@ __device__ inline bool weights_of(const LogprobArgs& a, int64_t row, bool live, 
   return live && (*wl != 0.0f || *we != 0.0f);
 }
 
-// The gradient of the block at column col: of logits z (-inf where there is none).
+// Stores the gradient of the block at column col from its y and e.
 template <class T, bool kWhole, bool kStream>
-__device__ inline void put_gradient(T* grad, const F8& z, const RowEnd& o, bool some, float wl,
-                                    float we, int col, int cols, int token, float z_token) {
+__device__ inline void put_gradient(T* grad, const F8& y, const F8& e, const RowSlope& r,
+                                    const RowEnd& o, bool some, float wl, float we, int col,
+                                    int cols, int token, float z_token) {
   F8 g = {};
   if (some) {
-    g = gradient(z, o, wl, we);
-    // (a legal token's alone: 0 stands where z is -inf, and -0 does not)
+    g = gradient(y, e, r);
+    if (r.inv != r.inv) {  // (NaN reaches the legal logits alone)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = z[j] == -kInf ? 0.0f : g[j];
+      for (int j = 0; j < 8; ++j) g[j] = e[j] == 0.0f && y[j] == -0x1p100f ? 0.0f : g[j];
+    }
     if ((uint32_t)(token - col) < 8u) {
       const float gt = gradient_of_token(o, z_token, wl, we);
 #pragma unroll
@@ -334,23 +387,23 @@ __global__ __launch_bounds__(block_of<kThreads>()) void logprob_rows_kernel(Logp
   }
   const float mine = t.m;
   t.m = lanes_reduce<Max, kWave>(t.m);
-  const float base = base_of(t.m);
+  const float base = t.m;  // (of this wave)
+  F8 y[kVecs], e[kVecs];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int col = 8 * (lane + i * kThreads);
-    add_block(t, z[i], base, token - col);
-  }
+  for (int i = 0; i < kVecs; ++i)
+    add_block(t, z[i], base_of(base), token - 8 * (lane + i * kThreads), y[i], e[i]);
   row_join<kThreads>(t, smem);
   const RowEnd o = finish_row(t, z_token, token >= 0);
-  if (lane == 0) write_row(a, row, o, token >= 0);
+  if (lane == 0) write_row(a, row, o);
   if constexpr (kGrad) {
     float wl, we;
     const bool some = weights_of(a, row, o.live, token >= 0, &wl, &we);
+    const RowSlope r = slope_of(o, base, wl, we);
     T* grad = static_cast<T*>(a.grad) + row * a.r.vocab;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
-      put_gradient<T, kWhole, false>(grad, z[i], o, some, wl, we, 8 * (lane + i * kThreads),
-                                     in.cols, token, z_token);
+      put_gradient<T, kWhole, false>(grad, y[i], e[i], r, o, some, wl, we,
+                                     8 * (lane + i * kThreads), in.cols, token, z_token);
   } else if (a.top) {
     best_of_row<kThreads>(a, row, o, mine, space[slot], [&](auto&& f) {
 #pragma unroll
@@ -403,19 +456,25 @@ __global__ __launch_bounds__(kLongThreads) void logprob_long_kernel(LogprobArgs 
     if (m > t.m) rebase(t, m);
     const float base = base_of(t.m);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      add_block(t, z[u], base, (int)(token - at - (int64_t)u * kStep));
+    for (int u = 0; u < kAhead; ++u) {
+      F8 y, e;
+      add_block(t, z[u], base, (int)(token - at - (int64_t)u * kStep), y, e);
+    }
   }
   row_join<kLongThreads>(t, smem);
   const RowEnd o = finish_row(t, z_token, token >= 0);
-  if (threadIdx.x == 0) write_row(a, row, o, token >= 0);
+  if (threadIdx.x == 0) write_row(a, row, o);
   if constexpr (kGrad) {
     float wl, we;
     const bool some = weights_of(a, row, o.live, token >= 0, &wl, &we);
     T* grad = static_cast<T*>(a.grad) + row * a.r.vocab;
-    for (int64_t col = first; col < in.cols; col += kStep)
-      put_gradient<T, kWhole, true>(grad, logits_at<T, kWhole>(in, (int)col), o, some, wl, we,
-                                    (int)col, in.cols, token, z_token);
+    const RowSlope r = slope_of(o, o.base, wl, we);
+    for (int64_t col = first; col < in.cols; col += kStep) {
+      F8 y, e;
+      exponentials(logits_at<T, kWhole>(in, (int)col), o.base, y, e);
+      put_gradient<T, kWhole, true>(grad, y, e, r, o, some, wl, we, (int)col, in.cols, token,
+                                    z_token);
+    }
   } else if (a.top) {
     best_of_row<kLongThreads>(a, row, o, mine, space[0], [&](auto&& f) {
       for (int64_t col = first; col < in.cols; col += kStep) {
@@ -447,8 +506,11 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(LogprobArgs a, int64_
   const bool some = weights_of(a, row, more.y != 0.0f, token >= 0, &wl, &we);
   const F8 z = legal_logits<T, false, kWhole>(raw, in, col,
                                               ok_bytes<T, false, kWhole>(raw, in, col));
-  put_gradient<T, kWhole, false>(static_cast<T*>(a.grad) + row * a.r.vocab, z, o, some, wl, we, col,
-                                 in.cols, token, z_token);
+  F8 y, e;
+  exponentials(z, o.base, y, e);
+  put_gradient<T, kWhole, false>(static_cast<T*>(a.grad) + row * a.r.vocab, y, e,
+                                 slope_of(o, o.base, wl, we), o, some, wl, we, col, in.cols, token,
+                                 z_token);
 }
 
 // ---- launches -------------------------------------------------------------------------------
@@ -476,9 +538,11 @@ void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     const int64_t v = a.r.vocab;
     if (v <= 512) return launch_rows<T, 64, 1, kGrad>(a, st);
     if (v <= 1024) return launch_rows<T, 64, 2, kGrad>(a, st);
-    if (v <= 2048) return launch_rows<T, 256, 1, kGrad>(a, st);
+    if (v <= 2048) return launch_rows<T, 128, 2, kGrad>(a, st);
     if (v <= 4096) return launch_rows<T, 256, 2, kGrad>(a, st);
-    if (v <= 8192) return launch_rows<T, 1024, 1, kGrad>(a, st);
+    if (v <= 6144) return launch_rows<T, 256, 3, kGrad>(a, st);
+    if (v <= 8192) return launch_rows<T, 512, 2, kGrad>(a, st);
+    if (v <= 12288) return launch_rows<T, 512, 3, kGrad>(a, st);
     if (v <= 16384) return launch_rows<T, 1024, 2, kGrad>(a, st);
     const dim3 grid = grid_of(a.r.rows, kLongThreads);
     const auto kernel = v % 8 == 0 ? logprob_long_kernel<T, true, kGrad>
