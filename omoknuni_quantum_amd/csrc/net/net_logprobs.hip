@@ -18,6 +18,8 @@
 // Bound by memory: a row of up to 16384 tokens is held in registers; a longer one is read by a
 // workgroup, its alternatives from the few threads that hold them, and a second time for the
 // gradient.
+#include <type_traits>
+
 #include "net_logits.h"
 
 namespace omq_net {
@@ -228,7 +230,8 @@ struct TopSpace {
   float largest[kWaves > 1 ? kWaves : 1][kWave];
   uint64_t list[kListed];
   uint64_t best[2];
-  uint32_t count;
+  uint32_t count, reaching;
+  uint16_t thread[kThreads];  // that reach the bound, in a long row
 };
 
 // All threads of a row: a workgroup, or one wave, whose LDS accesses are in order.
@@ -255,12 +258,13 @@ __device__ inline float largest_but(float v, int top) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), __builtin_ctzll(at)));
 }
 
-// mine: the thread's largest logit.  each(f): f(logit, index) for the thread's logits.
-template <int kThreads, class Each>
+// mine: the thread's largest logit.  each(f): f(logit, index) for the thread's logits; some(reaches, f):
+// the same for those of the threads for which `reaches` is true, by whichever threads.
+template <int kThreads, class Each, class Some>
 __device__ inline void best_of_row(const LogprobArgs& a, int64_t row, const RowEnd& o, float mine,
-                                   TopSpace<kThreads>& sp, Each&& each) {
+                                   TopSpace<kThreads>& sp, Each&& each, Some&& some) {
   const int lane = threadIdx.x & (kWave - 1), thread = threadIdx.x % kThreads;
-  if (thread == 0) sp.count = 0;
+  if (thread == 0) sp.count = sp.reaching = 0;
   float v = mine;
   if constexpr (kThreads > kWave) {
     sp.largest[threadIdx.x / kWave][lane] = mine;
@@ -272,12 +276,11 @@ __device__ inline void best_of_row(const LogprobArgs& a, int64_t row, const RowE
   }
   const float bound = largest_but(v, a.top);
   const auto reaches = [&](float z) { return z >= bound && z > -kInf; };
-  if (reaches(mine))
-    each([&](float z, int index) {
-      if (!reaches(z)) return;
-      const uint32_t at = atomicAdd(&sp.count, 1u);
-      if (at < (uint32_t)kListed) sp.list[at] = key_of(z, index);
-    });
+  some(reaches(mine), [&](float z, int index) {
+    if (!reaches(z)) return;
+    const uint32_t at = atomicAdd(&sp.count, 1u);
+    if (at < (uint32_t)kListed) sp.list[at] = key_of(z, index);
+  });
   row_sync<kThreads>();
   const int n = (int)sp.count;
   float* logp = a.top_logp + row * a.top;
@@ -405,17 +408,20 @@ __global__ __launch_bounds__(block_of<kThreads>()) void logprob_rows_kernel(Logp
       put_gradient<T, kWhole, false>(grad, y[i], e[i], r, o, some, wl, we,
                                      8 * (lane + i * kThreads), in.cols, token, z_token);
   } else if (a.top) {
-    best_of_row<kThreads>(a, row, o, mine, space[slot], [&](auto&& f) {
+    const auto each = [&](auto&& f) {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) f(z[i][j], 8 * (lane + i * kThreads) + j);
+    };
+    best_of_row<kThreads>(a, row, o, mine, space[slot], each, [&](bool reaches, auto&& f) {
+      if (reaches) each(f);
     });
   }
 }
 
 // Rows that are longer: a workgroup reads kAhead blocks a thread at a time.
-constexpr int kLongThreads = 1024, kAhead = 4;
+constexpr int kAhead = 4;
 
 template <class T, bool kWhole>
 __device__ inline F8 logits_at(const RowIn<T>& in, int col) {
@@ -423,7 +429,7 @@ __device__ inline F8 logits_at(const RowIn<T>& in, int col) {
   return legal_logits<T, false, kWhole>(b, in, col, ok_bytes<T, false, kWhole>(b, in, col));
 }
 
-template <class T, bool kWhole, bool kGrad>
+template <class T, int kLongThreads, bool kWhole, bool kGrad>
 __global__ __launch_bounds__(kLongThreads) void logprob_long_kernel(LogprobArgs a) {
   __shared__ Sums smem[16];
   __shared__ TopSpace<kLongThreads> space[1];
@@ -476,13 +482,28 @@ __global__ __launch_bounds__(kLongThreads) void logprob_long_kernel(LogprobArgs 
                                     z_token);
     }
   } else if (a.top) {
-    best_of_row<kLongThreads>(a, row, o, mine, space[0], [&](auto&& f) {
-      for (int64_t col = first; col < in.cols; col += kStep) {
-        const F8 z = logits_at<T, kWhole>(in, (int)col);
+    const auto at = [&](int64_t col, auto&& f) {
+      const F8 z = logits_at<T, kWhole>(in, (int)col);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f(z[j], (int)col + j);
-      }
-    });
+      for (int j = 0; j < 8; ++j) f(z[j], (int)col + j);
+    };
+    // (the blocks of the threads that reach the bound are shared out: one after another they would
+    // take such a thread longer than the row's first reading took all)
+    TopSpace<kLongThreads>& sp = space[0];
+    best_of_row<kLongThreads>(
+        a, row, o, mine, sp,
+        [&](auto&& f) {
+          for (int64_t col = first; col < in.cols; col += kStep) at(col, f);
+        },
+        [&](bool reaches, auto&& f) {
+          if (reaches) sp.thread[atomicAdd(&sp.reaching, 1u)] = (uint16_t)threadIdx.x;
+          __syncthreads();
+          const int64_t blocks = (in.cols + kStep - 1) / kStep, all = sp.reaching * blocks;
+          for (int64_t i = threadIdx.x; i < all; i += kLongThreads) {
+            const int64_t col = 8 * (int64_t)sp.thread[i / blocks] + i % blocks * kStep;
+            if (col < in.cols) at(col, f);
+          }
+        });
   }
 }
 
@@ -544,10 +565,19 @@ void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     if (v <= 8192) return launch_rows<T, 512, 2, kGrad>(a, st);
     if (v <= 12288) return launch_rows<T, 512, 3, kGrad>(a, st);
     if (v <= 16384) return launch_rows<T, 1024, 2, kGrad>(a, st);
-    const dim3 grid = grid_of(a.r.rows, kLongThreads);
-    const auto kernel = v % 8 == 0 ? logprob_long_kernel<T, true, kGrad>
-                                   : logprob_long_kernel<T, false, kGrad>;
-    kernel<<<grid, kLongThreads, 0, st>>>(a);
+    // workgroups of 256 threads where there is one for each compute unit twice: a row's end (its
+    // sums' join, its alternatives) takes as long in all, and the other rows' loads go on
+    const auto go = [&](auto threads) {
+      constexpr int kThreads = threads.value;
+      const dim3 grid = grid_of(a.r.rows, kThreads);
+      const auto kernel = v % 8 == 0 ? logprob_long_kernel<T, kThreads, true, kGrad>
+                                     : logprob_long_kernel<T, kThreads, false, kGrad>;
+      kernel<<<grid, kThreads, 0, st>>>(a);
+    };
+    if (a.r.rows >= 512)
+      go(std::integral_constant<int, 256>{});
+    else
+      go(std::integral_constant<int, 1024>{});
   });
 }
 
