@@ -498,9 +498,11 @@ __global__ __launch_bounds__(kLongThreads) void logprob_long_kernel(LogprobArgs 
         [&](bool reaches, auto&& f) {
           if (reaches) sp.thread[atomicAdd(&sp.reaching, 1u)] = (uint16_t)threadIdx.x;
           __syncthreads();
-          const int64_t blocks = (in.cols + kStep - 1) / kStep, all = sp.reaching * blocks;
-          for (int64_t i = threadIdx.x; i < all; i += kLongThreads) {
-            const int64_t col = 8 * (int64_t)sp.thread[i / blocks] + i % blocks * kStep;
+          // (fewer than 2^27 + 1024 blocks: rows have at most 2^30 tokens)
+          const uint32_t blocks = (uint32_t)((in.cols - 1) / kStep + 1), all = sp.reaching * blocks;
+          for (uint32_t i = threadIdx.x; i < all; i += kLongThreads) {
+            const uint32_t who = i / blocks;
+            const int64_t col = 8 * (int64_t)sp.thread[who] + (int64_t)(i - who * blocks) * kStep;
             if (col < in.cols) at(col, f);
           }
         });

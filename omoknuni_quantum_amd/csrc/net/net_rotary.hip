@@ -7,9 +7,9 @@
 // Bound by memory: each element is read and written once.  A lane has eight pairs of columns (two
 // blocks of eight elements, which lie a half of the rotated columns apart, or side by side where
 // pairs are), or sixteen columns that do not rotate, and 1 to 32 lanes share a head, so that the
-// rotation needs no exchange between lanes.  A workgroup takes all heads of some tokens: it forms
-// the sines and cosines of the tokens' pairs once, in LDS, for all their heads (an angle costs
-// about as many instructions as a lane's norm).
+// rotation needs no exchange between lanes.  A workgroup takes all heads of queries or of keys of
+// some tokens: it forms the sines and cosines of the tokens' pairs once, in LDS, for all of them (an
+// angle costs about as many instructions as a lane's norm).
 #include <type_traits>
 
 #include "net_common.h"
@@ -18,16 +18,26 @@ namespace omq_net {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kGradGroups = 2048;
+
+// One of queries and keys: each has workgroups of its own, so that a thread has one weight and one
+// of the weights' sums.
+struct Side {
+  const void *x, *weight;
+  const void* g;       // gradient of the output
+  void* out;           // the gradient: of x
+  int64_t token_stride, head_stride;
+  int heads;
+  int tile;            // tokens of a workgroup
+  uint32_t magic;      // 2^32 / heads, rounded up; 0 for one head
+  int64_t tiles, groups;  // workgroups: of all tiles, or fewer that take turns
+};
 
 struct RotaryArgs {
   omq_rotary r;
-  void *q_out, *k_out;            // the gradient: of q and k
-  const void *gq, *gk;            // gradients of the outputs
-  float* partial;                 // [workgroups, 2, dim] sums of the weights' gradients, or NULL
+  Side side[2];
+  float* partial;                 // [workgroups, dim] sums of a weight's gradient, or NULL
   int turning, slots, lanes_log;  // lanes of a head that rotate, that work, and all (a power of 2)
-  int tile;                       // tokens of a workgroup
-  uint32_t heads_magic;           // 2^32 / heads, rounded up
-  int64_t tiles;
   float inv_dim;
 };
 
@@ -103,49 +113,49 @@ __device__ inline void rotate(F8& x, F8& y, const float2* cs, bool interleaved) 
 }
 
 template <class T, bool kWhole, bool kGrad>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+__global__ __launch_bounds__(kThreads, (kWhole ? 4 : 3)) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float4 shared[];
   float2* turn = reinterpret_cast<float2*>(shared);
-  const int lanes = 1 << a.lanes_log, heads = a.r.q_heads + a.r.k_heads, dim = a.r.dim;
+  const int64_t block = block_index();
+  const bool is_key = block >= a.side[0].groups;
+  const Side& side = a.side[is_key];
+  const int64_t group = is_key ? block - a.side[0].groups : block;
+  if (group >= side.groups) return;
+  const int lanes = 1 << a.lanes_log, heads = side.heads, dim = a.r.dim;
   const int own = threadIdx.x & (lanes - 1);
   const bool works = own < a.slots;
   const int slot = works ? own : 0;  // (lanes beyond a head load its first blocks, to no use)
   const Place at = place_of(a, slot);
   const int padded = 8 * ((a.r.pairs + 7) / 8);
-  const bool turns = slot < a.turning, weighted = a.r.q_weight != nullptr;
-  const bool w_f32 = a.r.weight_dtype == OMQ_NET_F32;
-  const int w_size = w_f32 ? 4 : (int)sizeof(T);
-  Weight8<T> wa[2] = {}, wb[2] = {};  // of queries and keys
+  const bool turns = slot < a.turning, weighted = side.weight != nullptr;
+  F8 w_u = {}, w_v = {};
   if (weighted) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const char* w = static_cast<const char*>(i ? a.r.k_weight : a.r.q_weight);
-      wa[i] = load_weight<T, kWhole>(w + at.seg_a * w_size, w_f32, at.col_a, at.len_a);
-      wb[i] = load_weight<T, kWhole>(w + at.seg_b * w_size, w_f32, at.col_b, at.len_b);
-    }
+    const bool w_f32 = a.r.weight_dtype == OMQ_NET_F32;
+    const int w_size = w_f32 ? 4 : (int)sizeof(T);
+    const char* w = static_cast<const char*>(side.weight);
+    w_u = widen<T, kWhole>(load_weight<T, kWhole>(w + at.seg_a * w_size, w_f32, at.col_a, at.len_a),
+                           w_f32, at.col_a, at.len_a);
+    w_v = widen<T, kWhole>(load_weight<T, kWhole>(w + at.seg_b * w_size, w_f32, at.col_b, at.len_b),
+                           w_f32, at.col_b, at.len_b);
   }
-  F8 dwa[kGrad ? 2 : 1] = {}, dwb[kGrad ? 2 : 1] = {};
-  for (int64_t tile = block_index(); tile < a.tiles;
-       tile += kGrad ? (int64_t)gridDim.x : a.tiles) {
-    const int64_t first = tile * a.tile, left = a.r.tokens - first;
-    const int tokens = left < a.tile ? (int)left : a.tile;
-    if (kGrad) __syncthreads();  // (the tile before has used its angles)
+  F8 dw_u = {}, dw_v = {};
+  for (int64_t tile = group; tile < side.tiles; tile += side.groups) {
+    const int64_t first = tile * side.tile, left = a.r.tokens - first;
+    const int tokens = left < side.tile ? (int)left : side.tile;
+    if (tile != group) __syncthreads();  // (the tile before has used its angles)
     form_angles(a, first, tokens, turn);
     __syncthreads();
     for (int i = threadIdx.x >> a.lanes_log; i < tokens * heads; i += kThreads >> a.lanes_log) {
-      const int t = (int)__umulhi((uint32_t)i, a.heads_magic), head = i - t * heads;
-      const bool key = head >= a.r.q_heads;
-      const int h = key ? head - a.r.q_heads : head;
+      const int t = side.magic ? (int)__umulhi((uint32_t)i, side.magic) : i, head = i - t * heads;
       const int64_t token = first + t;
-      const T* x = static_cast<const T*>(key ? a.r.k : a.r.q) +
-                   token * (key ? a.r.k_token_stride : a.r.q_token_stride) +
-                   h * (key ? a.r.k_head_stride : a.r.q_head_stride);
-      const int64_t flat = (token * (key ? a.r.k_heads : a.r.q_heads) + h) * dim;
+      const T* x = static_cast<const T*>(side.x) + token * side.token_stride +
+                   head * side.head_stride;
+      const int64_t flat = (token * heads + head) * dim;
       const auto raw_a = load_raw<T, kWhole>(x + at.seg_a, at.col_a, at.len_a);
       const auto raw_b = load_raw<T, kWhole>(x + at.seg_b, at.col_b, at.len_b);
       Reg8<T> g_a = {}, g_b = {};
       if constexpr (kGrad) {
-        const T* g = static_cast<const T*>(key ? a.gk : a.gq) + flat;
+        const T* g = static_cast<const T*>(side.g) + flat;
         g_a = load_raw<T, kWhole>(g + at.seg_a, at.col_a, at.len_a);
         g_b = load_raw<T, kWhole>(g + at.seg_b, at.col_b, at.len_b);
       }
@@ -161,11 +171,6 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         sq = head_sum(works ? sq : 0.0f, a.lanes_log);
         r = 1.0f / sqrtf(fmaf(sq, a.inv_dim, a.r.eps));
       }
-      F8 w_u = {}, w_v = {};
-      if (weighted) {
-        w_u = widen<T, kWhole>(key ? wa[1] : wa[0], w_f32, at.col_a, at.len_a);
-        w_v = widen<T, kWhole>(key ? wb[1] : wb[0], w_f32, at.col_b, at.len_b);
-      }
       float2 cs[8];
       if (turns) {
 #pragma unroll
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
           *reinterpret_cast<float4*>(&cs[j]) =
               *reinterpret_cast<const float4*>(&turn[t * padded + 8 * slot + j]);
       }
-      T* out = static_cast<T*>(key ? a.k_out : a.q_out) + flat;
+      T* out = static_cast<T*>(side.out) + flat;
       if constexpr (!kGrad) {
         if (weighted) u = u * r * w_u, v = v * r * w_v;
         if (turns) rotate<false>(u, v, cs, a.r.interleaved);
@@ -186,11 +191,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         F8 dv = widen<T, kWhole>(g_b, at.col_b, at.len_b);
         if (turns) rotate<true>(du, dv, cs, a.r.interleaved);
         if (weighted) {
-          const F8 su = du * u * r, sv = dv * v * r;
-          if (key)
-            dwa[1] += su, dwb[1] += sv;
-          else
-            dwa[0] += su, dwb[0] += sv;
+          dw_u += du * u * r, dw_v += dv * v * r;
           du *= w_u, dv *= w_v;
           float dot = 0.0f;
 #pragma unroll
@@ -210,53 +211,61 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   }
   if constexpr (kGrad) {
     if (!a.partial) return;
-    // the lane groups' sums, in their order: queries, then keys
+    // the lane groups' sums, in their order
     float* sum = reinterpret_cast<float*>(shared);
-    const int groups = kThreads >> a.lanes_log;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum[j * kThreads + threadIdx.x] = dwa[i][j];
-        sum[(8 + j) * kThreads + threadIdx.x] = dwb[i][j];
-      }
-      __syncthreads();
-      if ((int)threadIdx.x < dim) {
-        const int c = threadIdx.x, n = a.r.pairs;
-        int lane, e;  // the column's lane and its place among its sixteen
-        if (c >= 2 * n)
-          lane = a.turning + (c - 2 * n) / 16, e = (c - 2 * n) % 16;
-        else if (a.r.interleaved)
-          lane = c / 16, e = c % 16;
-        else
-          lane = (c < n ? c : c - n) / 8, e = (c < n ? c : c - n) % 8 + (c < n ? 0 : 8);
-        float s = 0.0f;
-        for (int g = 0; g < groups; ++g) s += sum[e * kThreads + (g << a.lanes_log) + lane];
-        a.partial[(block_index() * 2 + i) * dim + c] = s;
-      }
+    for (int j = 0; j < 8; ++j) {
+      sum[j * kThreads + threadIdx.x] = dw_u[j];
+      sum[(8 + j) * kThreads + threadIdx.x] = dw_v[j];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < dim) {
+      const int c = threadIdx.x, n = a.r.pairs;
+      int lane, e;  // the column's lane and its place among its sixteen
+      if (c >= 2 * n)
+        lane = a.turning + (c - 2 * n) / 16, e = (c - 2 * n) % 16;
+      else if (a.r.interleaved)
+        lane = c / 16, e = c % 16;
+      else
+        lane = (c < n ? c : c - n) / 8, e = (c < n ? c : c - n) % 8 + (c < n ? 0 : 8);
+      float s = 0.0f;
+      for (int g = 0; g < kThreads >> a.lanes_log; ++g)
+        s += sum[e * kThreads + (g << a.lanes_log) + lane];
+      a.partial[block * dim + c] = s;
     }
   }
 }
 
-// The weights' gradients from the workgroups' sums: 32 columns, 32 slices side by side, the slices
-// added in order.
+// The weights' gradients from the workgroups' sums (of queries, then of keys): 32 columns, 32 slices
+// side by side, the slices added in order.
 template <class O>
 __global__ __launch_bounds__(1024) void join_weights_kernel(const float* __restrict__ partial,
-                                                            int groups, int dim,
+                                                            int q_groups, int k_groups, int dim,
                                                             O* __restrict__ q, O* __restrict__ k) {
   __shared__ float part[32][33];
+  const int blocks = (dim + 31) / 32;
+  const bool is_key = (int)blockIdx.x >= blocks;
+  const int groups = is_key ? k_groups : q_groups;
+  if (is_key) partial += (int64_t)q_groups * dim;
   const int c = threadIdx.x % 32, slice = threadIdx.x / 32;
-  const int col = blockIdx.x * 32 + c;
+  const int col = ((int)blockIdx.x - (is_key ? blocks : 0)) * 32 + c;
   float s = 0.0f;
-  if (col < 2 * dim)
-    for (int g = slice; g < groups; g += 32) s += partial[(int64_t)g * 2 * dim + col];
+  if (col < dim)
+    for (int g = slice; g < groups; g += 32 * 8) {  // eight loads in flight, the last ones too
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = partial[(int64_t)(g + 32 * u < groups ? g + 32 * u : g) * dim + col];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += g + 32 * u < groups ? v[u] : 0.0f;
+    }
   part[slice][c] = s;
   __syncthreads();
-  if (threadIdx.x < 32 && col < 2 * dim) {
+  if (threadIdx.x < 32 && col < dim) {
     s = part[0][c];
     for (int i = 1; i < 32; ++i) s += part[i][c];
-    (col < dim ? q : k)[col < dim ? col : col - dim] = (O)s;
+    (is_key ? k : q)[col] = (O)s;
   }
 }
 
@@ -302,41 +311,39 @@ int check_rotary(const char* name, const omq_rotary* r) {
   return OMQ_NET_OK;
 }
 
-// How the heads are cut, but for the arrays of a call.
-RotaryArgs layout_of(const omq_rotary& r) {
+// How the heads are cut, but for the outputs of a call.
+RotaryArgs layout_of(const omq_rotary& r, bool grad) {
   RotaryArgs a{};
   a.r = r;
-  const int heads = r.q_heads + r.k_heads;
   a.turning = (r.pairs + 7) / 8;
   a.slots = a.turning + (r.dim - 2 * r.pairs + 15) / 16;
   while ((1 << a.lanes_log) < a.slots) ++a.lanes_log;
-  // four rounds of a workgroup's threads or one token, and fewer where the tokens are few
-  const int64_t lanes = (int64_t)heads << a.lanes_log;
-  int64_t tile = 4 * kThreads / lanes;
-  const int64_t few = r.tokens / 1024;
-  tile = tile < few ? tile : few;
-  tile = tile < 1 ? 1 : tile;
-  a.tile = (int)tile;
-  a.tiles = ceil_div(r.tokens, tile);
-  a.heads_magic = (uint32_t)((0x100000000ull + heads - 1) / heads);
   a.inv_dim = 1.0f / (float)r.dim;
+  a.side[0] = {r.q, r.q_weight, nullptr, nullptr, r.q_token_stride, r.q_head_stride, r.q_heads};
+  a.side[1] = {r.k, r.k_weight, nullptr, nullptr, r.k_token_stride, r.k_head_stride, r.k_heads};
+  for (Side& s : a.side) {
+    // four rounds of a workgroup's threads or one token, and fewer where the tokens are few
+    int64_t tile = 4 * kThreads / ((int64_t)s.heads << a.lanes_log);
+    tile = tile < r.tokens / 1024 ? tile : r.tokens / 1024;
+    s.tile = (int)(tile < 1 ? 1 : tile);
+    s.tiles = ceil_div(r.tokens, s.tile);
+    s.magic = s.heads > 1 ? (uint32_t)((0x100000000ull + s.heads - 1) / s.heads) : 0;
+    // (of the gradient: enough for the chip, few enough for their sums)
+    s.groups = grad && r.q_weight && s.tiles > kGradGroups ? kGradGroups : s.tiles;
+  }
   return a;
 }
 
-// Workgroups of the gradient: enough for the chip, few enough for their sums.
-int64_t grad_groups(const RotaryArgs& a) { return a.tiles < 2048 ? a.tiles : 2048; }
-
-size_t angle_bytes(const RotaryArgs& a) {
-  return (size_t)a.tile * 8 * ((a.r.pairs + 7) / 8) * sizeof(float2);
-}
+int64_t grad_groups(const RotaryArgs& a) { return a.side[0].groups + a.side[1].groups; }
 
 template <bool kGrad>
 void launch_rotary(const RotaryArgs& a, hipStream_t st) {
-  size_t bytes = angle_bytes(a);
+  const int n = a.r.pairs, rest = a.r.dim - 2 * n;
+  const int tile = a.side[0].tile > a.side[1].tile ? a.side[0].tile : a.side[1].tile;
+  size_t bytes = (size_t)tile * 8 * ((n + 7) / 8) * sizeof(float2);
   if (kGrad && a.partial && bytes < 16 * kThreads * sizeof(float))
     bytes = 16 * kThreads * sizeof(float);
-  const dim3 grid = kGrad ? dim3((uint32_t)grad_groups(a)) : grid_of(a.tiles, kThreads);
-  const int n = a.r.pairs, rest = a.r.dim - 2 * n;
+  const dim3 grid = grid_of(grad_groups(a), kThreads);
   const bool whole = (a.r.interleaved ? 2 * n : n) % 8 == 0 && rest % 8 == 0;
   with_type(a.r.dtype, [&](auto t) {
     using T = decltype(t);
@@ -357,8 +364,8 @@ int omq_head_norm_rotary(const omq_rotary* r, void* q_out, void* k_out, void* st
   if (int rc = check_rotary(name, r)) return rc;
   if (r->tokens == 0) return OMQ_NET_OK;
   if (!q_out || !k_out) return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
-  RotaryArgs a = layout_of(*r);
-  a.q_out = q_out, a.k_out = k_out;
+  RotaryArgs a = layout_of(*r, false);
+  a.side[0].out = q_out, a.side[1].out = k_out;
   launch_rotary<false>(a, (hipStream_t)stream);
   return net_status(name);
 }
@@ -367,7 +374,7 @@ int64_t omq_head_norm_rotary_grad_workspace(const omq_rotary* r) {
   const int rc = check_rotary("omq_head_norm_rotary_grad_workspace", r);
   if (rc) return rc;
   if (!r->q_weight) return 0;
-  return grad_groups(layout_of(*r)) * 2 * r->dim * (int64_t)sizeof(float);
+  return grad_groups(layout_of(*r, true)) * r->dim * (int64_t)sizeof(float);
 }
 
 int omq_head_norm_rotary_grad(const omq_rotary* r, const void* grad_q_out, const void* grad_k_out,
@@ -381,20 +388,22 @@ int omq_head_norm_rotary_grad(const omq_rotary* r, const void* grad_q_out, const
     return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
   if (r->tokens > 0 && (!grad_q_out || !grad_k_out || !grad_q || !grad_k))
     return net_fail(OMQ_NET_E_ARG, "%s: a null array", name);
-  RotaryArgs a = layout_of(*r);
-  const int64_t need = weighted ? grad_groups(a) * 2 * r->dim * (int64_t)sizeof(float) : 0;
+  RotaryArgs a = layout_of(*r, true);
+  const int64_t need = weighted ? grad_groups(a) * r->dim * (int64_t)sizeof(float) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need || !on_16_bytes(workspace)))
     return net_fail(OMQ_NET_E_ARG, "%s: workspace of %lld bytes at %p, %lld on a 16-byte boundary "
                     "needed", name, (long long)workspace_bytes, workspace, (long long)need);
-  a.gq = grad_q_out, a.gk = grad_k_out, a.q_out = grad_q, a.k_out = grad_k;
+  a.side[0].g = grad_q_out, a.side[1].g = grad_k_out;
+  a.side[0].out = grad_q, a.side[1].out = grad_k;
   a.partial = weighted ? static_cast<float*>(workspace) : nullptr;
   if (r->tokens > 0) launch_rotary<true>(a, (hipStream_t)stream);
   if (weighted)
     with_type(r->weight_dtype, [&](auto t) {
       using O = decltype(t);
-      join_weights_kernel<O><<<(uint32_t)ceil_div(2 * r->dim, 32), 1024, 0, (hipStream_t)stream>>>(
-          static_cast<const float*>(workspace), r->tokens > 0 ? (int)grad_groups(a) : 0, r->dim,
-          static_cast<O*>(grad_q_weight), static_cast<O*>(grad_k_weight));
+      const uint32_t grid = 2 * (uint32_t)ceil_div(r->dim, 32);
+      join_weights_kernel<O><<<grid, 1024, 0, (hipStream_t)stream>>>(
+          static_cast<const float*>(workspace), (int)a.side[0].groups, (int)a.side[1].groups,
+          r->dim, static_cast<O*>(grad_q_weight), static_cast<O*>(grad_k_weight));
     });
   return net_status(name);
 }
