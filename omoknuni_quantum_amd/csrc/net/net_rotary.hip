@@ -143,16 +143,30 @@ __global__ __launch_bounds__(kThreads, (kWhole ? 4 : 3)) void rotary_kernel(Rota
     const int64_t first = tile * side.tile, left = a.r.tokens - first;
     const int tokens = left < side.tile ? (int)left : side.tile;
     if (tile != group) __syncthreads();  // (the tile before has used its angles)
+    const int step = kThreads >> a.lanes_log, rows = tokens * heads;
+    const auto token_of = [&](int i) {
+      return side.magic ? (int)__umulhi((uint32_t)i, side.magic) : i;
+    };
+    Reg8<T> next_a, next_b;
+    const auto load = [&](int i) {
+      const int t = token_of(i);
+      const T* x = static_cast<const T*>(side.x) + (first + t) * side.token_stride +
+                   (i - t * heads) * side.head_stride;
+      next_a = load_raw<T, kWhole>(x + at.seg_a, at.col_a, at.len_a);
+      next_b = load_raw<T, kWhole>(x + at.seg_b, at.col_b, at.len_b);
+    };
+    // (the first heads are under way while the angles are formed, and the next ones later)
+    const int start = threadIdx.x >> a.lanes_log;
+    if (!kGrad && start < rows) load(start);
     form_angles(a, first, tokens, turn);
     __syncthreads();
-    for (int i = threadIdx.x >> a.lanes_log; i < tokens * heads; i += kThreads >> a.lanes_log) {
-      const int t = side.magic ? (int)__umulhi((uint32_t)i, side.magic) : i, head = i - t * heads;
+    for (int i = start; i < rows; i += step) {
+      const int t = token_of(i), head = i - t * heads;
       const int64_t token = first + t;
-      const T* x = static_cast<const T*>(side.x) + token * side.token_stride +
-                   head * side.head_stride;
       const int64_t flat = (token * heads + head) * dim;
-      const auto raw_a = load_raw<T, kWhole>(x + at.seg_a, at.col_a, at.len_a);
-      const auto raw_b = load_raw<T, kWhole>(x + at.seg_b, at.col_b, at.len_b);
+      if (kGrad) load(i);
+      const Reg8<T> raw_a = next_a, raw_b = next_b;
+      if (!kGrad && i + step < rows) load(i + step);
       Reg8<T> g_a = {}, g_b = {};
       if constexpr (kGrad) {
         const T* g = static_cast<const T*>(side.g) + flat;
