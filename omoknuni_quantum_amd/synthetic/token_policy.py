@@ -4,21 +4,25 @@ what the searches return: the operators of ``net_ops`` in one path.
 A position is one token per cell, ``3 * cell + content`` (0 empty, 1 the mover's stone, 2 the
 other's), looked up in one table; two kinds of layer alternate on the residual, a product over
 the cells and one over the channels, each behind a root-mean-square norm of the residual sum; the
-policy is one logit per cell, the value a mean over the cells.
+policy is one logit per cell, the value a mean over the cells.  With `heads` the cells attend to
+one another in place of the product: queries and keys normed and rotated by row and column.  Such
+a network takes boards of different sizes, packed one after another (``forward(tokens, starts)``).
 
 * ``evaluator()`` has ``evaluate_batch(features)`` (the protocol of ``MCTS``): the norms before the
   channel products give them their input in 8 bits with a scale for every row, and so are those
   products' weights.  It holds the weights as they were when it was made; the network's own
   ``evaluate_batch`` lays them out at every call.
 * ``train_step(...)``: dropout on every branch (fused into the norms), the clipped policy loss
-  against the searches' policies over the legal cells, the table's gradient over sorted tokens.
+  against the searches' policies over the legal cells (with an entropy bonus, if asked for), the
+  table's gradient over sorted tokens.
 
-``python -m omoknuni_quantum_amd.synthetic.token_policy`` searches a batch of random Gomoku
+``python -m omoknuni_quantum_amd.synthetic.token_policy [heads]`` searches a batch of random Gomoku
 positions, trains on the visit distributions and prints the loss of every step.
 """
 from __future__ import annotations
 
 import math
+import sys
 
 import numpy as np
 import torch
@@ -55,20 +59,82 @@ class _Block(nn.Module):
         return self.cells(rows).view(b, d, c).transpose(1, 2).contiguous()
 
 
+class _AttentionBlock(nn.Module):
+    """Attention over the cells, and a product over the channels (times `widen` and back)."""
+
+    def __init__(self, dim: int, widen: int, heads: int, kv_heads: int):
+        super().__init__()
+        self.heads, self.kv_heads, width = heads, kv_heads, dim // heads
+        self.norm_cells = nn.Parameter(torch.ones(dim))
+        self.norm_channels = nn.Parameter(torch.ones(dim))
+        self.qkv = nn.Linear(dim, (heads + 2 * kv_heads) * width, bias=False)
+        self.norm_q = nn.Parameter(torch.ones(width))
+        self.norm_k = nn.Parameter(torch.ones(width))
+        self.out = nn.Linear(dim, dim, bias=False)
+        self.up = nn.Linear(dim, widen * dim, bias=False)
+        self.down = nn.Linear(widen * dim, dim, bias=False)
+
+    def mix(self, y, rotation, starts=None):
+        """Over the cells of y [positions, cells, dim], or [rows, dim] of the positions that begin
+        at `starts`; rotation: RotaryTable.of's."""
+        return _attend(y, self.qkv.weight, self.norm_q, self.norm_k, self.out.weight, self.heads,
+                       self.kv_heads, rotation, starts)
+
+
+def _attend(y, qkv, norm_q, norm_k, out, heads, kv_heads, rotation, starts):
+    q, k, v = F.linear(y, qkv).unflatten(-1, (heads + 2 * kv_heads, -1)).split(
+        (heads, kv_heads, kv_heads), -2)
+    positions, frequencies, sections = rotation
+    q, k = net_ops.head_norm_rotary(q, k, positions, frequencies, norm_q, norm_k,
+                                    sections=sections)
+    return F.linear(net_ops.attention(q, k, v, q_starts=starts).flatten(-2), out)
+
+
+class RotaryTable:
+    """The rotation of heads of `width` columns by a cell's row and column, half of the pairs each."""
+
+    def __init__(self, board_size: int, width: int):
+        pairs = width // 2
+        self.board, self.sections, self.held = board_size, (pairs - pairs // 2, pairs // 2), {}
+
+    def of(self, tokens: torch.Tensor, packed: bool):
+        """(positions, frequencies, sections) of a batch, or of packed tokens 3 * cell + content."""
+        device = tokens.device
+        if device not in self.held:
+            cell = torch.arange(self.board**2, dtype=torch.int32, device=device)
+            self.held[device] = (self._places(cell),
+                                 net_ops.rotary_frequencies(self.sections, 100.0, device))
+        positions, frequencies = self.held[device]
+        return self._places(tokens // 3) if packed else positions, frequencies, self.sections
+
+    def _places(self, cell):
+        return torch.stack((cell // self.board, cell % self.board), -1).int()
+
+
 class TokenPolicy(nn.Module):
-    """The network, its evaluator and its training step."""
+    """The network, its evaluator and its training step.  heads: 0, or the heads of the attention
+    over the cells (a divisor of dim); kv_heads: those of its keys and values (as many)."""
 
     input_channels = 18
 
     def __init__(self, board_size: int = 15, dim: int = 128, blocks: int = 3, widen: int = 2,
-                 dropout: float = 0.1, seed: int = 0, device: str = "cuda"):
+                 dropout: float = 0.1, seed: int = 0, device: str = "cuda", heads: int = 0,
+                 kv_heads: int | None = None):
         super().__init__()
         self.board, self.dim, self.p, self.seed = board_size, dim, dropout, seed
+        self.heads = heads
+        kv_heads = kv_heads or heads
+        if heads and (dim % heads or heads % kv_heads):
+            raise ValueError(f"dim {dim}, heads {heads}, kv_heads {kv_heads}: each must divide the "
+                             "one before")
+        self.rotation = RotaryTable(board_size, dim // heads) if heads else None
         c = board_size * board_size
         with torch.random.fork_rng(devices=[]):
             torch.manual_seed(seed)
             self.table = nn.Parameter(torch.randn(3 * c, dim) / dim)
-            self.blocks = nn.ModuleList(_Block(c, dim, widen) for _ in range(blocks))
+            self.blocks = nn.ModuleList(
+                _AttentionBlock(dim, widen, heads, kv_heads) if heads else _Block(c, dim, widen)
+                for _ in range(blocks))
             self.norm_out = nn.Parameter(torch.ones(dim))
             self.policy = nn.Linear(dim, 1)
             self.value = nn.Linear(dim, 1)
@@ -80,40 +146,64 @@ class TokenPolicy(nn.Module):
         """position_tokens(features)."""
         return position_tokens(features)
 
-    def forward(self, tokens: torch.Tensor):
+    def forward(self, tokens: torch.Tensor, starts: torch.Tensor | None = None):
         """(logits [positions, cells], values [positions]) for training; a new dropout mask for
-        every branch and every value of `steps`, which train_step counts."""
+        every branch and every value of `steps`, which train_step counts.
+
+        starts (int32 [positions + 1], of a network with heads): tokens are [rows], the positions
+        packed one after another, of boards of at most board_size; a cell is numbered as on the
+        largest board, row * board_size + column.  The logits are [rows] then."""
+        if starts is not None and not self.heads:
+            raise ValueError("packed positions need a network with heads")
         p = self.p if self.training else 0.0
         use = self.steps * (2 * len(self.blocks) + 1)
         branch = net_ops.token_embedding(tokens, self.table, math.sqrt(self.dim))
+        rotation = self.rotation.of(tokens, starts is not None) if self.heads else None
         h = None
         for block in self.blocks:
             y, h = net_ops.add_rms_norm(branch, h, block.norm_cells, p=p, seed=self.seed,
                                         offset=use)
-            y, h = net_ops.add_rms_norm(block.mix(y), h, block.norm_channels, p=p,
-                                        seed=self.seed, offset=use + 1)
+            y = block.mix(y, rotation, starts) if self.heads else block.mix(y)
+            y, h = net_ops.add_rms_norm(y, h, block.norm_channels, p=p, seed=self.seed,
+                                        offset=use + 1)
             branch = block.down(F.gelu(block.up(y)))
             use += 2
         y, _ = net_ops.add_rms_norm(branch, h, self.norm_out, p=p, seed=self.seed, offset=use)
-        return self.policy(y)[..., 0], torch.tanh(self.value(y.mean(1)))[:, 0]
+        mean = y.mean(1) if starts is None else self._means(y, starts)
+        return self.policy(y)[..., 0], torch.tanh(self.value(mean))[:, 0]
+
+    def _means(self, y, starts):
+        """The means of packed positions' rows: what a query of zeros attends to."""
+        n = starts.shape[0] - 1
+        y = y.unflatten(-1, (self.heads, -1))
+        ask = y.new_zeros(n, *y.shape[1:])
+        one = torch.arange(n + 1, dtype=torch.int32, device=y.device)
+        return net_ops.attention(ask, torch.zeros_like(y), y, q_starts=one,
+                                 k_starts=starts).flatten(-2)
 
     def train_step(self, optimizer, tokens, target, legal, actions, advantages, old_logp, outcome,
-                   clip: float = 0.2, kl_coef: float = 1.0) -> dict:
+                   clip: float = 0.2, kl_coef: float = 1.0, entropy_coef: float = 0.0) -> dict:
         """One step on positions with the searches' policies `target` [positions, cells], the
         moves played, their advantages and log-probabilities when they were played, and the
-        games' outcomes.  Returns the losses."""
+        games' outcomes.  entropy_coef: the weight of the policies' mean entropy over the legal
+        cells, which is taken off the loss.  Returns the losses (and the entropy, with a weight)."""
         self.train()
         logits, values = self(tokens)
         loss, _, kl = net_ops.clipped_policy_loss(logits, actions, advantages, old_logp, clip,
                                                   clip, kl_coef, target=target, legal=legal)
         value_loss = F.mse_loss(values, outcome)
         total = loss.mean() + value_loss
+        more = {}
+        if entropy_coef:
+            more["entropy"] = net_ops.token_logprobs(logits, actions, legal)[1].mean()
+            total = total - entropy_coef * more["entropy"]
         optimizer.zero_grad(set_to_none=True)
         total.backward()
         optimizer.step()
         self.steps += 1
-        said = torch.stack((total, loss.mean(), kl.mean(), value_loss)).detach().tolist()
-        return dict(zip(("loss", "policy", "kl", "value"), said))
+        said = torch.stack((total, loss.mean(), kl.mean(), value_loss,
+                            *more.values())).detach().tolist()
+        return dict(zip(("loss", "policy", "kl", "value", *more), said))
 
     # ---- serving ---------------------------------------------------------------------------
     def evaluator(self) -> "Evaluator":
@@ -141,12 +231,15 @@ class Evaluator:
             return p.detach().to(dtype, copy=True)
 
         self.input_channels, self.dim = net.input_channels, net.dim
+        self.rotation = net.rotation
         self.table, self.norm_out = copy(net.table), copy(net.norm_out)
         self.blocks = []
         for b in net.blocks:
             w = b.up.weight.detach().float()
             scale = (w.abs().amax(1, keepdim=True) / 448.0).clamp_(min=2.0**-126)
-            self.blocks.append((copy(b.norm_cells), copy(b.cells.weight), copy(b.norm_channels),
+            mix = ((copy(b.qkv.weight), copy(b.norm_q), copy(b.norm_k), copy(b.out.weight),
+                    b.heads, b.kv_heads) if net.heads else copy(b.cells.weight))
+            self.blocks.append((copy(b.norm_cells), mix, copy(b.norm_channels),
                                 (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous(),
                                 copy(b.down.weight)))
         self.heads = [(copy(h.weight, torch.float32), copy(h.bias, torch.float32))
@@ -157,10 +250,14 @@ class Evaluator:
         """(logits, values) as TokenPolicy.forward without dropout, in bfloat16 and 8 bits."""
         branch, h = net_ops.token_embedding(tokens, self.table, math.sqrt(self.dim)), None
         b, c, d = branch.shape
-        for norm_cells, cells, norm_channels, up, up_scale, down in self.blocks:
+        rotation = self.rotation.of(tokens, False) if self.rotation else None
+        for norm_cells, mix, norm_channels, up, up_scale, down in self.blocks:
             y, h = net_ops.add_rms_norm(branch, h, norm_cells)
-            y = F.linear(y.transpose(1, 2).reshape(b * d, c), cells)
-            y = y.view(b, d, c).transpose(1, 2).contiguous()
+            if rotation:
+                y = _attend(y, *mix, rotation, None)
+            else:
+                y = F.linear(y.transpose(1, 2).reshape(b * d, c), mix)
+                y = y.view(b, d, c).transpose(1, 2).contiguous()
             q, scales, h = net_ops.add_rms_norm_fp8(y, h, norm_channels)
             y = torch._scaled_mm(q.view(b * c, d), up.t(), scale_a=scales.view(b * c, 1),
                                  scale_b=up_scale, out_dtype=torch.bfloat16)
@@ -178,6 +275,18 @@ class Evaluator:
         occupied = (features[:, 0] + features[:, 1]).flatten(1) > 0
         policies = torch.softmax(logits.masked_fill_(occupied, -math.inf), 1)
         return policies.masked_fill_(occupied, 0.0), values  # (NaN where all are)
+
+
+    @torch.no_grad()
+    def best_moves(self, features: torch.Tensor, top: int = 5):
+        """(moves int64 [positions, top], their log-probabilities, the policy's entropy [positions])
+        of feature planes: the most probable free cells (-1 and -inf where there are fewer)."""
+        tokens = position_tokens(features)
+        logits, _ = self.serve(tokens)
+        free = (features[:, 0] + features[:, 1]).flatten(1) == 0
+        none = tokens.new_full(tokens.shape[:1], -1)
+        _, entropy, logp, moves = net_ops.token_logprobs(logits, none, free, top)
+        return moves, logp, entropy
 
 
 def searched_positions(net: TokenPolicy, positions: int, simulations: int, stones: int,
@@ -212,8 +321,8 @@ def searched_positions(net: TokenPolicy, positions: int, simulations: int, stone
     return tokens, target, legal, actions, old
 
 
-def main(steps: int = 20, positions: int = 64) -> list:
-    net = TokenPolicy()
+def main(steps: int = 20, positions: int = 64, heads: int = 0) -> list:
+    net = TokenPolicy(heads=heads)
     optimizer = torch.optim.AdamW(net.parameters(), lr=2e-3)
     tokens, target, legal, actions, old = searched_positions(net, positions, 128, 60, 1)
     g = torch.Generator(device=tokens.device).manual_seed(2)
@@ -230,4 +339,4 @@ def main(steps: int = 20, positions: int = 64) -> list:
 
 
 if __name__ == "__main__":
-    main()
+    main(heads=int(sys.argv[1]) if len(sys.argv) > 1 else 0)
