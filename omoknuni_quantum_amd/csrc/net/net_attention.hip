@@ -67,9 +67,10 @@ __device__ __attribute__((always_inline)) inline void attend(
     for (int d = 0; d < kDim / 32; ++d) x.o[d] *= keep;
   }
   const float base = x.m == -kInf32 ? 0.0f : x.m * scale;
+  float l = 0.0f;  // (a sum of its own: each step of a long one would round at its size)
   const auto form = [&](int b, int r) __attribute__((always_inline)) {
     s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -base));
-    x.l += s[b][r];
+    l += s[b][r];
   };
   here();
 #pragma unroll
@@ -89,6 +90,7 @@ __device__ __attribute__((always_inline)) inline void attend(
     here();
     add_columns<T, kDim, false>(x.o, columns, values, 32, s[1], cuts, x.found, lane);
   }
+  x.l += l;
 }
 
 template <class T, int kDim, bool kDirect>

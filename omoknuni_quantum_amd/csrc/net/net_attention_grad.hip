@@ -9,8 +9,10 @@
 // ds is rounded to the elements' type for its products, times scale, without which float16 would
 // overflow earlier.  Its sum over a row is 0 but for what the rounding of out took from delta, which
 // the first launch so finds and the second has again; dq, for which that comes too late, has ds to
-// twice the type's bits instead.  (With neither, the gradients are off by 1.6 times their own
-// rounding and more, with both by 1.3 and 1.4 times.)
+// twice the type's bits instead, and rows that see few keys (of whose outs the roundings weigh
+// most) form their ds twice: where a workgroup's keys are two tiles, both stay in LDS and the first
+// time over them only corrects delta.  (With none of it, the gradients are off by 1.6 times their own
+// rounding and more, those of few keys by 2 and more; with all of it by 1.1 to 1.4 times.)
 #include "net_attention.h"
 
 namespace omq_net {
@@ -72,14 +74,44 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 
   F16 dq[kDim / 32] = {};
   uint32_t found = 0;
-  const float shift = delta * a.scale;
   float rest = 0.0f;  // sum of ds: scale times what out's rounding took from delta
   typename L::Lane own;
+  // the two products of 32 keys, and ds in place of s
+  const auto slopes = [&](int k0, int b, F16& s, const F16& dp, float shift, bool cuts)
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
+      s[r] = p * fmaf(dp[r], a.scale, -shift);
+    }
+    if (cuts) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (k0 + 32 * b + result_row(r) >= x.limit) s[r] = 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rest += s[r];
+  };
+  const bool twice = sizeof(T) == 2 && x.block_most <= 2 * kTileKeys;
+  if (twice) {
+    if (x.block_most > kTileKeys) load(kTileKeys, keys1, values1);
+    tiles_ready();
+#pragma unroll 1
+    for (int i = 0; i < 4 && 32 * i < x.most; ++i) {
+      F16 s, dp;
+      const char *keys = i < 2 ? keys0 : keys1, *values = i < 2 ? values0 : values1;
+      two_products<T, kDim>(s, keys, 32 * (i % 2), qf, dp, values, 32 * (i % 2), gf, own);
+      slopes(0, i, s, dp, delta * a.scale, 32 * i + 32 > x.least);
+    }
+    rest += other_half(rest);
+    delta += rest / a.scale, rest = 0.0f;
+  }
+  const float shift = delta * a.scale;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
                         char* next_values) __attribute__((always_inline)) {
     tiles_ready();
     own.renew();
-    if (k0 + kTileKeys < x.block_most) load(k0 + kTileKeys, next_keys, next_values);
+    if (k0 + kTileKeys < x.block_most && !twice) load(k0 + kTileKeys, next_keys, next_values);
     if (k0 >= x.most) return;
     const bool cuts = k0 + kTileKeys > x.least;
 #pragma unroll
@@ -89,18 +121,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
       Columns<T, kDim> columns;
       columns.read(keys, 32 * b, 0, own);
       here();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
-        s[r] = p * fmaf(dp[r], a.scale, -shift);
-      }
-      if (cuts) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + result_row(r) >= x.limit) s[r] = 0.0f;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) rest += s[r];
+      slopes(k0, b, s, dp, shift, cuts);
       add_columns<T, kDim, true>(dq, columns, keys, 32 * b, s, cuts, found, own);
     }
   };
