@@ -151,12 +151,13 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
   const float l = sum.l + other_half(sum.l);
+  const bool hidden = __any(sum.found != 0) && lane < 32;  // (a lane finds for other lanes' rows)
   if (!x.there) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   T* out = static_cast<T*>(args.out) + out_row * a.dim;
   store_column<T, kDim, kDirect>(out, sum.o, inv, a.dim);
-  if (__builtin_expect(__any(sum.found != 0), 0) && lane < 32)
+  if (__builtin_expect(hidden, 0))
     add_hidden<T, false>(out, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                          [=](int j) { return v_rows + j * a.v_row_stride; });
   if (args.lse && lane < 32) args.lse[out_row] = lse_of(sum.m, l, a.scale);
@@ -233,11 +234,11 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     if (k0 + kPartKeys < end) step(k0 + kPartKeys, keys1, values1, keys0, values0);
   }
   const float l = sum.l + other_half(sum.l);
+  const bool hidden = __any(sum.found != 0) && lane < 32;  // (as above)
   if (!x.there) return;
   const int64_t out_row = (q.q_first + x.query) * a.q_heads + x.head;
   const int least = x.least / kPartKeys * kPartKeys;
   const int from = begin > least ? begin : least, to = end < x.limit ? end : x.limit;
-  const bool hidden = __any(sum.found != 0) && lane < 32;
   const auto value = [=](int j) { return v_rows + j * a.v_row_stride; };
   if (args.splits == 1) {
     T* out = static_cast<T*>(args.out) + out_row * a.dim;
@@ -267,13 +268,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs args)
   const float l = lanes_reduce<Sum, kWave>(mine.y == 0.0f ? 0.0f : w * mine.y);
   const float scale = l == 0.0f ? 0.0f : w / l;
   float x[2] = {};
-  for (int s = 0; s < args.splits; ++s) {
-    const float f = __shfl(scale, s);
-    const float* part = args.parts + (s * args.out_rows + row) * dim;
-    if (f != 0.0f) {  // (a part without keys is zeros; of weight 0, nothing beside the others)
+  constexpr int kAhead = 8;  // (loads under way)
+  for (int s0 = 0; s0 < args.splits; s0 += kAhead) {
+    float part[kAhead][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < dim) x[i] = fmaf(f, part[lane + 64 * i], x[i]);
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = s0 + i < args.splits ? s0 + i : args.splits - 1;
+      const float* from = args.parts + (s * args.out_rows + row) * dim;
+      part[i][0] = from[lane < dim ? lane : 0];
+      part[i][1] = from[lane + 64 < dim ? lane + 64 : 0];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float f = s0 + i < args.splits ? __shfl(scale, s0 + i) : 0.0f;
+      // (a part without keys is zeros; of weight 0, nothing beside the others)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) x[d] = f != 0.0f ? fmaf(f, part[i][d], x[d]) : x[d];
     }
   }
 #pragma unroll
@@ -283,7 +293,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs args)
   if (args.lse && lane == 0) args.lse[row] = lse_of(m, l, args.a.scale);
 }
 
-// Whether a call takes the kernel for few rows, and with how many parts.
+// Whether a call takes the kernel for few rows, and with how many parts (all us, bf16 unless said).
+//  * Parts fill the chip where the pairs of heads and 32 rows do not, with 1024 waves: 64 tokens x 2
+//    heads over 2048 keys of 128: 27 (parts), 41 (wide); 16 x 8 heads x 64 rows over 2048 of 64: 24,
+//    31; twice and four times the waves cost 10 % and more there, of parts written and read.
+//  * 4096 waves where lengths differ and there are few rows to write (64 x 8 heads x 1 row over up
+//    to 4096: 60, with 1024 waves 93, wide 67), and for float32, whose products take 8 times as long
+//    (64 x 8 x 1 over 4096: 273, 350, 286).  Half the keys a part with elements of twice the size
+//    (512 keys of 64, float32: 13 for 18).
+//  * At least 4 parts and 2 KB of a column's keys: 128 rows x 8 heads over 512 of 64 take 10 either
+//    way, over 256 7 (wide) and 9.
+//  * Without parts it serves float32 with rows enough for the chip: 512 x 8 heads over 128 of 64: 81,
+//    wide 145, whose second wave on a SIMD has no registers (bf16: 23.6 and 24.8, but 64 x 8 heads x
+//    32 rows over 512: 15.8 and 13.9).
 bool few_rows(const omq_attention_args& a, int* splits, int64_t* out_rows) {
   const int64_t group = a.q_heads / a.k_heads, n = a.q_starts ? a.sequences : 1;
   const int64_t all = a.q_starts ? 1 : a.sequences;
@@ -291,15 +313,17 @@ bool few_rows(const omq_attention_args& a, int* splits, int64_t* out_rows) {
   const int64_t rows = n > 0 ? ceil_div(a.q_len * group, n) : 0;  // (of a sequence, in the mean)
   const int64_t keys = n > 0 ? ceil_div(a.k_len, n) : 0;
   const int64_t sequences = a.sequences > 0 ? a.sequences : 1;
-  const int64_t wide = ceil_div(rows, kTileRows) * sequences * a.k_heads;
-  *splits = 1;
-  if (rows > kWaveRows && (wide >= 256 || keys < 512)) return false;
   const int64_t units = ceil_div(rows > 0 ? rows : 1, kWaveRows) * sequences * a.k_heads;
-  int64_t parts = ceil_div(4096, units);
-  const int64_t most = ceil_div(keys, 4 * kPartKeys);
+  const int64_t size = dtype_size(a.dtype);
+  const bool uneven = a.q_starts || a.k_lengths;
+  const int64_t waves = rows <= kWaveRows && (size == 4 || (uneven && rows <= 8)) ? 4096 : 1024;
+  int64_t parts = waves / units;
+  const int64_t most = keys * size / (8 * kPartKeys);
   parts = parts < most ? parts : most;
-  *splits = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
-  return true;
+  parts = parts < 64 ? parts : 64;
+  const bool split = parts >= 4 && keys * size >= 2048;
+  *splits = split ? (int)parts : 1;
+  return split || (size == 4 && rows <= kWaveRows && units >= 512);
 }
 
 int64_t parts_bytes(const omq_attention_args& a, int splits, int64_t out_rows) {
@@ -318,7 +342,7 @@ int check_attention(const char* name, const omq_attention_args* a) {
                     (long long)a->sequences, (long long)a->q_len, (long long)a->k_len, a->q_heads,
                     a->k_heads, a->dim);
   const int64_t n = a->q_starts ? 1 : a->sequences;
-  const int64_t most = OMQ_NET_MAX_COUNT;
+  const int64_t most = OMQ_NET_MAX_COUNT - 4095;  // (a tile past the last is counted in 32 bits)
   if (a->dim > OMQ_NET_MAX_HEAD_DIM || a->sequences > most || a->q_len > most || a->k_len > most ||
       a->q_len * a->q_heads > most || a->k_len * a->q_heads > most ||
       (n > 0 && (a->q_len * a->q_heads > most / n || a->k_len * a->q_heads > most / n)))
@@ -326,7 +350,7 @@ int check_attention(const char* name, const omq_attention_args* a) {
                     "%s: sequences %lld of %lld queries and %lld keys, %d heads (rows of heads at "
                     "most %d), dim %d (at most %d)",
                     name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len,
-                    a->q_heads, OMQ_NET_MAX_COUNT, a->dim, OMQ_NET_MAX_HEAD_DIM);
+                    a->q_heads, (int)most, a->dim, OMQ_NET_MAX_HEAD_DIM);
   if (!(a->scale > 0.0f && a->scale < kInf32))
     return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be finite and above 0", name, a->scale);
   if (!a->q_starts != !a->k_starts)

@@ -131,11 +131,12 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
   rest += other_half(rest);
+  const bool hidden = __any(found != 0) && lane < 32;  // (a lane finds for other lanes' rows)
   if (!x.there) return;
   if (lane < 32) args.delta[out_row] = delta + rest / a.scale;
   T* grad = static_cast<T*>(args.grad_q) + out_row * a.dim;
   store_column<T, kDim, kDirect>(grad, dq, 1.0f, a.dim);
-  if (__builtin_expect(__any(found != 0), 0) && lane < 32)
+  if (__builtin_expect(hidden, 0))
     add_hidden<T, true>(grad, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                         [=](int j) { return k_rows + j * a.k_row_stride; });
 }
@@ -290,6 +291,7 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
     if (r0 + kTileKeys < end)
       step(r0 + kTileKeys, queries1, grads1, stats1, queries0, grads0, stats0);
   }
+  const bool hidden = __any((found_q | found_g) != 0) && lane < 32;  // (as above)
   if (!there) return;
   if (mine >= q.lk) {  // (whatever the queries hold)
 #pragma unroll
@@ -299,7 +301,7 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
   T *grad_k = static_cast<T*>(args.grad_k) + out, *grad_v = static_cast<T*>(args.grad_v) + out;
   if constexpr (kKeys) store_column<T, kDim, kDirect>(grad_k, dk, 1.0f, a.dim);
   if constexpr (kValues) store_column<T, kDim, kDirect>(grad_v, dv, 1.0f, a.dim);
-  if (__builtin_expect(__any((found_q | found_g) != 0), 0) && lane < 32 && mine < q.lk) {
+  if (__builtin_expect(hidden, 0) && mine < q.lk) {
     const int64_t least = a.causal && mine > shift ? (int64_t)(mine - shift) * group : 0;
     const int sees = least < rows ? (int)least : rows;  // the first row that sees this key
     if constexpr (kKeys)
