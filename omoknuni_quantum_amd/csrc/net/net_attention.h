@@ -523,6 +523,8 @@ inline bool chunks_aligned(int dtype, int64_t dim, std::initializer_list<const v
   return ok;
 }
 
+// Keys and values for the loads straight into LDS; others pass through registers.  8 x 8 heads of 1024
+// keys of 64 columns, bf16: 28 us straight, 52 with rows 2 bytes off (of 128: 45 and 92).
 inline bool direct_tiles(const omq_attention_args& a) {
   return chunks_aligned(a.dtype, a.dim, {a.k, a.v},
                         {a.k_seq_stride, a.k_row_stride, a.k_head_stride, a.v_seq_stride,

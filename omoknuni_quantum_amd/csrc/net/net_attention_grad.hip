@@ -6,6 +6,16 @@
 // keys (dk and dv).  Scores are formed in both, seven products in place of five, and no sum is
 // split over workgroups, which would take atomics or float32 copies of dq; every result is the
 // same bits at every call.  Rows of queries that share a key head are rows of one sum.
+//
+// Two causal sequences of 4096 with 16 heads over 4 of 128, bf16: 290 us by queries, 575 by keys
+// (950 and 600 TFLOP/s of what they multiply); 256 boards of 49 to 361 cells with 8 heads over 4 of
+// 64, float16: 107 and 144 us; 64 of 225 cells with 4 heads of 32, float32: 40 and 52.  Matrix cores
+// are busy for a fifth (boards) to a half (by queries), in float32 three fifths of that: a wave's
+// products, its exponentials and its reads of LDS follow one another, and two waves a SIMD, for which
+// the registers are just enough, cover a part of that.  By keys the workgroups of a causal sequence are few and of all lengths; the rows
+// that they read do not bound them (half the traffic, by an order of the workgroups in which the
+// memory's parts share them, took as long).
+//
 // ds is rounded to the elements' type for its products, times scale, without which float16 would
 // overflow earlier.  Its sum over a row is 0 but for what the rounding of out took from delta, which
 // the first launch so finds and the second has again; dq, for which that comes too late, has ds to
@@ -316,20 +326,23 @@ constexpr int kComputeUnits = 256;
 
 // Sums of 128 columns are a workgroup's each, of the keys or of the values (scores are formed in
 // both: five products in place of four): with both a wave has no room for a second one on its SIMD,
-// whose products run while the first forms its probabilities.
-template <int kDim>
-constexpr bool sums_apart() {
-  return kDim > 64;
+// whose products run while the first forms its probabilities.  (All three gradients of 8 x 8 heads
+// of 1024 keys, bf16: 182 us, 268 together; of 64 columns 118 apart, 91 together.)  In float32 a
+// wave is alone on its SIMD in either case, and they are apart only where the workgroups are fewer
+// than the compute units: 8 x 8 heads 1460 us, 1116 together; 8 x 2 key heads 1402 and 1683.
+template <class T, int kDim>
+bool sums_apart(int64_t blocks) {
+  return kDim > 64 && (sizeof(T) == 2 || blocks < kComputeUnits);
 }
 
-template <class T, int kDim, bool kDirect>
+template <class T, int kDim, bool kDirect, bool kApart>
 __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_kv_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
   __shared__ __attribute__((aligned(1024))) char queries0[L::kBytes], queries1[L::kBytes];
   __shared__ __attribute__((aligned(1024))) char grads0[L::kBytes], grads1[L::kBytes];
   __shared__ __attribute__((aligned(16))) RowStats stats0, stats1;
   const int64_t block = block_index();
-  if constexpr (!sums_apart<kDim>())
+  if constexpr (!kApart)
     grad_kv<T, kDim, kDirect, true, true>(args, block, queries0, queries1, grads0, grads1, stats0,
                                           stats1);
   else if (block % 2 == 0)
@@ -397,11 +410,27 @@ int omq_attention_grad(const omq_attention_args* a, const void* grad_out, const 
       const int64_t far_out = (kTileKeys + 1) * (int64_t)a->q_heads * a->dim;
       args.even = Even::kRowsAStep % args.group == 0 &&
                   Even::possible(a->dim, far > far_out ? far : far_out);
-      const int64_t blocks = args.slots * a->k_heads * (sums_apart<dim.value>() ? 2 : 1);
+      using T = decltype(t);
+      int64_t blocks = args.slots * a->k_heads;
+      const bool apart = sums_apart<T, dim.value>(blocks);
+      blocks *= apart ? 2 : 1;
+      // (all gradients of causal sequences of 4096, bf16: two with 16 heads over 4 of 128 784 us, in
+      // one order 829; one with 16 over 8 of 128 428 and 450; neighbours paired 817 and 444)
       args.paired = a->causal && blocks > kComputeUnits && blocks <= 2 * kComputeUnits;
       const dim3 grid = grid_of(blocks, kWaves * kWave);
-      attention_grad_kv_kernel<decltype(t), dim.value, direct.value>
-          <<<grid, kWaves * kWave, 0, st>>>(args);
+      const auto go = [&](auto split) {
+        attention_grad_kv_kernel<T, dim.value, direct.value, split.value>
+            <<<grid, kWaves * kWave, 0, st>>>(args);
+      };
+      if constexpr (dim.value <= 64) {
+        go(std::false_type{});
+      } else if constexpr (sizeof(T) == 2) {
+        go(std::true_type{});
+      } else if (apart) {
+        go(std::true_type{});
+      } else {
+        go(std::false_type{});
+      }
     });
   }
   return net_status(name);

@@ -17,14 +17,14 @@ Those that training uses (all but add_rms_norm_fp8) are differentiable; their gr
 functions of their own (``token_embedding_grad``, ``add_rms_norm_grad``,
 ``clipped_policy_loss_with_grad``, ``head_norm_rotary_grad``, ``attention_grad``,
 ``token_logprobs_with_grad``; dropout is its own gradient) for a program that runs its backward
-pass by hand.  Every gradient is a function of
-its inputs alone, bit for bit: sums run in a fixed order.  There are no second derivatives and no
-forward-mode ones, and none of the other functions: those raise.
+pass by hand.  Every gradient is a function of its inputs alone, bit for bit: sums run in a fixed
+order.  There are no second derivatives and no forward-mode ones, and none of the other functions:
+those raise.
 
 Elements are float32, bfloat16 or float16.  Sums and statistics are kept in float32, and a result
-is rounded once (attention also rounds what its matrix products take).  Tensors of rows (the last dimension) may be slices of wider ones as long as the
-rows' elements are adjacent and the rows equally far apart; other arguments, and dropout's x, must
-be contiguous.
+is rounded once (attention also rounds what its matrix products take).  Tensors of rows (the last
+dimension) may be slices of wider ones as long as the rows' elements are adjacent and the rows
+equally far apart; other arguments, and dropout's x, must be contiguous.
 There is no CPU implementation: tensors must be on a HIP device, and a missing library raises.
 """
 from __future__ import annotations
@@ -399,7 +399,7 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                    k_starts: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None):
     """(grad_q, grad_k, grad_v) of attention from its arguments, the gradient of out, and out and
     lse of attention_with_lse.  The gradients of the scores are rounded to the elements' type
-    before they multiply k and q."""
+    before they multiply q (for k they have twice its bits)."""
     scale, k_starts = _attention_args(q, scale, q_starts, k_starts)
     return _ATTENTION_GRAD(grad_out, q, k, v, out, lse, scale, causal, q_starts, k_starts,
                            k_lengths)
