@@ -140,6 +140,8 @@ class TokenPolicy(nn.Module):
             self.value = nn.Linear(dim, 1)
         self.steps = 0
         self.to(device)
+        if heads:  # (now, and not within a graph that may be captured later)
+            self.rotation.of(self.table, False)
 
     # ---- training --------------------------------------------------------------------------
     def tokens(self, features: torch.Tensor) -> torch.Tensor:

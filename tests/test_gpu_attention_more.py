@@ -183,3 +183,48 @@ def test_heads_that_start_anywhere(device, dtype):
     a = step(q, k, v, go)
     b = step(*(t.contiguous() for t in (q, k, v, go)))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_gradients_of_any_layout_under_autograd(device):
+    """An expanded gradient and a transposed one are those of their contiguous copies; k and v shared
+    by all sequences get the sum of theirs."""
+    g = gen(41)
+    q = randn(g, 3, 50, 4, 32, dtype=torch.float32).to(device).requires_grad_()
+    k, v = (randn(g, 1, 60, 2, 32, dtype=torch.float32).to(device).requires_grad_()
+            for _ in range(2))
+    w = randn(g, 3, 4, 32, 50, dtype=torch.float32).to(device)
+
+    def run(loss):
+        out = net_ops.attention(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1))
+        return torch.autograd.grad(loss(out), (q, k, v))
+
+    def by_hand(grad):
+        ke, ve = (t.detach().expand(3, -1, -1, -1) for t in (k, v))
+        out, lse = net_ops.attention_with_lse(q.detach(), ke, ve)
+        gq, gk, gv = net_ops.attention_grad(grad.contiguous(), q.detach(), ke, ve, out, lse)
+        return gq, gk.sum(0, keepdim=True), gv.sum(0, keepdim=True)
+
+    for loss, grad in ((lambda o: o.sum(), torch.ones_like(q)),
+                       (lambda o: (o.permute(0, 2, 3, 1) * w).sum(), w.permute(0, 3, 1, 2))):
+        assert all(torch.equal(a, b) for a, b in zip(run(loss), by_hand(grad)))
+
+
+def test_nothing_to_attend_to(device):
+    """Sequences of no queries, of no keys, a batch of none, and rows of no sequence."""
+    for dtype in DTYPES:
+        q = torch.ones(2, 3, 2, 16, dtype=dtype, device=device, requires_grad=True)
+        none = torch.empty(2, 0, 2, 16, dtype=dtype, device=device, requires_grad=True)
+        out, lse = net_ops.attention_with_lse(q, none, none)
+        assert not bool(out.any()) and bool((lse == -math.inf).all())
+        gq, gk, gv = net_ops.attention_grad(torch.ones_like(out), q, none, none, out, lse)
+        assert not bool(gq.any()) and gk.shape == none.shape
+        out = net_ops.attention(none, q, q)
+        assert out.shape == none.shape
+        gk = torch.autograd.grad(out.sum(), q)[0]
+        assert not bool(gk.any())
+        starts = torch.zeros(1, dtype=torch.int32, device=device)
+        rows = torch.ones(5, 2, 16, dtype=dtype, device=device)
+        out, lse = net_ops.attention_with_lse(rows, rows, rows, q_starts=starts)
+        assert not bool(out.any()) and bool((lse == -math.inf).all())
+        assert not any(bool(t.any()) for t in net_ops.attention_grad(rows, rows, rows, rows, out, lse,
+                                                                      q_starts=starts))
