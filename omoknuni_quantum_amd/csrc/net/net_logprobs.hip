@@ -189,8 +189,9 @@ struct RowSlope {
 };
 
 __device__ inline RowSlope slope_of(const RowEnd& o, float base, float a, float b) {
-  // (about a base of -inf, that of a part without weight, y and e are those of base 0)
-  const float d = y_between(base_of(base), o.base);
+  // (a part without weight has only e = 0 and NaN: no 2^d, which may be infinite, 0 times which is NaN)
+  if (base == -kInf) return {o.inv_s, 0.0f, 0.0f};
+  const float d = y_between(base, o.base);
   const float scale = __builtin_amdgcn_exp2f(d);
   if (scale == 0.0f) return {scale * o.inv_s, 0.0f, 0.0f};  // (d may be -inf)
   return {scale * o.inv_s, fmaf(b, d * kLn2 - o.log_s + o.entropy, a), b * kLn2};
