@@ -347,9 +347,13 @@ __device__ inline void put_gradient(T* grad, const F8& y, const F8& e, const Row
   F8 g = {};
   if (some) {
     g = gradient(y, e, r);
-    if (r.inv != r.inv) {  // (NaN reaches the legal logits alone)
+    // (a slope above 2^26 may be infinite times y, and 0 times that is NaN; NaN of a row reaches the
+    // legal logits alone)
+    const bool number = r.inv == r.inv;
+    if (!(number && fabsf(r.slope) <= 0x1p26f && fabsf(r.shift) <= 0x1p126f)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = e[j] == 0.0f && y[j] == -0x1p100f ? 0.0f : g[j];
+      for (int j = 0; j < 8; ++j)
+        g[j] = e[j] == 0.0f && (number || y[j] == -0x1p100f) ? 0.0f : g[j];
     }
     if ((uint32_t)(token - col) < 8u) {
       const float gt = gradient_of_token(o, z_token, wl, we);

@@ -1,5 +1,5 @@
-"""More of the log-probabilities on the GPU: rows whose legal tokens lie in one wave's part.  Bounds
-as in test_gpu_logprobs.py."""
+"""More of the log-probabilities on the GPU: rows whose legal tokens lie in one wave's part, and
+entropy weights of any size.  Bounds as in test_gpu_logprobs.py."""
 import math
 
 import pytest
@@ -48,3 +48,29 @@ def test_legal_tokens_of_one_wave(device, dtype, vocab, at, level):
     for grad in gradients(device, z, tokens, legal, a, b):
         within(grad, want, e_grad.nan_to_num(0.0))
         assert not bool(grad.cpu()[0][~legal[0]].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [40, 600, 3000, 8192, 16384, 20_000])
+@pytest.mark.parametrize("weight", [1e8, 1e9, -3e9, 1e20, 1e30])
+def test_large_entropy_weights(device, dtype, vocab, weight):
+    """0 at tokens that are not legal, or of probability 0 (a third are -1e30, a third are not
+    legal)."""
+    g = gen(vocab)
+    z = randn(g, 4, vocab)
+    z[:, ::3] = -1e30
+    legal = torch.ones(4, vocab, dtype=torch.bool)
+    legal[:, 1::3] = False
+    z[:, 1::3] = math.nan
+    z = z.to(dtype)
+    tokens = torch.tensor([2, 5, -1, 3])
+    a, b = randn(g, 4), torch.full((4,), weight)
+    want = net_ref.token_logprobs(z, tokens, legal, 0, a, b)[4]
+    e_grad = bounds(z.nan_to_num(0.0), legal, tokens, a, b)[2]
+    for grad in gradients(device, z, tokens, legal, a, b):
+        # (where p is 0 the bound's allowance for p grows with the logit; the gradient is 0)
+        grad = grad.cpu()
+        assert not bool(grad[:, ::3][tokens[:, None].expand(4, vocab)[:, ::3] !=
+                                     torch.arange(vocab)[::3]].any())
+        assert not bool(grad[:, 1::3].any())
+        within(grad[:, 2::3], want[:, 2::3], e_grad[:, 2::3])
