@@ -261,7 +261,9 @@ int omq_attention_forward(const omq_attention_args* a, void* out, float* lse, vo
 /* Bytes of workspace of omq_attention_grad; negative for what it refuses. */
 int64_t omq_attention_grad_workspace(const omq_attention_args* a);
 
-/* Gradients of sum(grad_out * out) from the forward pass's out and lse.
+/* Gradients of sum(grad_out * out) from the forward pass's out and lse.  Those may be of more keys
+ * than the call's (a part of a row's keys, whose parts were joined by their lse): then they are the
+ * part's share.
  *   grad_out, out, grad_q  as out above
  *   grad_k, grad_v         [rows of k (all of them), k_heads, dim], contiguous; 0 for rows of no
  *                          sequence and behind a sequence's keys */

@@ -28,6 +28,10 @@
 namespace omq_net {
 namespace {
 
+// How far from 1 the sum of a whole row's probabilities may be: lse's rounding takes it 2^-25 |lse| away
+// and its sum's less; the share of hidden keys that passes for rounding is below out's own (2^-9, 2^-12).
+constexpr float kWhole = 0x1p-12f;
+
 template <class T, int kDim, bool kDirect>
 __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_q_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
@@ -84,16 +88,31 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
 
   F16 dq[kDim / 32] = {};
   uint32_t found = 0;
-  float rest = 0.0f;  // sum of ds: scale times what out's rounding took from delta
+  // sums of ds and p: scale times what out's rounding took from delta, where the probabilities are a
+  // whole row's
+  float rest = 0.0f, mass = 0.0f;
+  const auto lost = [&] {
+    const float r = rest + other_half(rest), m = mass + other_half(mass);
+    return __builtin_fabsf(m - 1.0f) <= kWhole ? r / a.scale : 0.0f;
+  };
   typename L::Lane own;
   // the two products of 32 keys, and ds in place of s
   const auto slopes = [&](int k0, int b, F16& s, const F16& dp, float shift, bool cuts)
       __attribute__((always_inline)) {
+    if (cuts) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (k0 + 32 * b + result_row(r) >= x.limit) s[r] = -kInf32;
+    }
+    float here_mass = 0.0f;  // (each step of a long sum would round at its size)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float p = __builtin_amdgcn_exp2f(fmaf(s[r], args.score_scale, -base));
+      here_mass += p;
       s[r] = p * fmaf(dp[r], a.scale, -shift);
+      if (r % 4 == 3) asm volatile("" : "+v"(here_mass));
     }
+    mass += here_mass;
     if (cuts) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -113,8 +132,8 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
       two_products<T, kDim>(s, keys, 32 * (i % 2), qf, dp, values, 32 * (i % 2), gf, own);
       slopes(0, i, s, dp, delta * a.scale, 32 * i + 32 > x.least);
     }
-    rest += other_half(rest);
-    delta += rest / a.scale, rest = 0.0f;
+    delta += lost();
+    rest = mass = 0.0f;
   }
   const float shift = delta * a.scale;
   const auto step = [&](int k0, const char* keys, const char* values, char* next_keys,
@@ -140,10 +159,10 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
     step(k0, keys0, values0, keys1, values1);
     if (k0 + kTileKeys < x.block_most) step(k0 + kTileKeys, keys1, values1, keys0, values0);
   }
-  rest += other_half(rest);
+  delta += lost();
   const bool hidden = __any(found != 0) && lane < 32;  // (a lane finds for other lanes' rows)
   if (!x.there) return;
-  if (lane < 32) args.delta[out_row] = delta + rest / a.scale;
+  if (lane < 32) args.delta[out_row] = delta;
   T* grad = static_cast<T*>(args.grad_q) + out_row * a.dim;
   store_column<T, kDim, kDirect>(grad, dq, 1.0f, a.dim);
   if (__builtin_expect(hidden, 0))

@@ -399,7 +399,10 @@ def attention_grad(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                    k_starts: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None):
     """(grad_q, grad_k, grad_v) of attention from its arguments, the gradient of out, and out and
     lse of attention_with_lse.  The gradients of the scores are rounded to the elements' type
-    before they multiply q (for k they have twice its bits)."""
+    before they multiply q (for k they have twice its bits).
+
+    Where a row's keys come in parts (each with an out and lse of its own, joined by the lse), a call
+    for one part with the joined out and lse gives its share: grad_q of the parts add up."""
     scale, k_starts = _attention_args(q, scale, q_starts, k_starts)
     return _ATTENTION_GRAD(grad_out, q, k, v, out, lse, scale, causal, q_starts, k_starts,
                            k_lengths)
