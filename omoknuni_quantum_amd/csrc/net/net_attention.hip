@@ -20,8 +20,11 @@ namespace {
 
 // Probabilities are formed about a maximum that follows the running one only where that has grown
 // by more than a factor of 2^8: the sums' rescaling, a product for each of a row's columns, is
-// left out for most tiles, and a probability is at most 2^8 (float16 holds 2^15).
+// left out for most tiles, and a probability is at most 2^8.  Float16 holds 2^15 and loses bits below
+// 2^-14: its probabilities are taken times 2^7, and so are their sums l and o.
 constexpr float kLag = 8.0f;
+template <class T>
+constexpr float kUp = std::is_same_v<T, f16> ? 7.0f : 0.0f;  // log2
 
 // A row's output so far: sums about the maximum m; l over this half's keys.
 template <int kDim>
@@ -31,8 +34,10 @@ struct Softmax {
   uint32_t found = 0;
 };
 
+template <class T>
 __device__ inline float lse_of(float m, float l, float scale) {
-  return l == 0.0f ? -kInf32 : fmaf(m, scale, __builtin_amdgcn_logf(l) * 0.6931471805599453f);
+  constexpr float kDown = std::is_same_v<T, f16> ? 0x1p-7f : 1.0f;  // 2^-kUp
+  return l == 0.0f ? -kInf32 : fmaf(m, scale, __builtin_amdgcn_logf(l * kDown) * 0.6931471805599453f);
 }
 
 // Attends to one or two blocks of 32 keys from k0, of which the row sees those below `limit`; cuts:
@@ -71,7 +76,7 @@ __device__ __attribute__((always_inline)) inline void attend(
 #pragma unroll
     for (int d = 0; d < kDim / 32; ++d) x.o[d] *= keep;
   }
-  const float base = x.m == -kInf32 ? 0.0f : x.m * scale;
+  const float base = (x.m == -kInf32 ? 0.0f : x.m * scale) - kUp<T>;
   float l = 0.0f;  // (a sum of its own: each step of a long one would round at its size)
   const auto form = [&](int b, int r) __attribute__((always_inline)) {
     s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale, -base));
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   if (__builtin_expect(hidden, 0))
     add_hidden<T, false>(out, a.dim, x.least / kTileKeys * kTileKeys, x.limit,
                          [=](int j) { return v_rows + j * a.v_row_stride; });
-  if (args.lse && lane < 32) args.lse[out_row] = lse_of(sum.m, l, a.scale);
+  if (args.lse && lane < 32) args.lse[out_row] = lse_of<T>(sum.m, l, a.scale);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(kWave) void attention_few_kernel(AttentionArgs args
     T* out = static_cast<T*>(args.out) + out_row * a.dim;
     store_column<T, kDim, kDirect>(out, sum.o, l == 0.0f ? 0.0f : 1.0f / l, a.dim);
     if (hidden) add_hidden<T, false>(out, a.dim, from, to, value);
-    if (args.lse && lane < 32) args.lse[out_row] = lse_of(sum.m, l, a.scale);
+    if (args.lse && lane < 32) args.lse[out_row] = lse_of<T>(sum.m, l, a.scale);
     return;
   }
   const int64_t part = split * args.out_rows + out_row;
@@ -296,7 +301,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs args)
   for (int i = 0; i < 2; ++i)
     if (lane + 64 * i < dim)
       static_cast<T*>(args.out)[row * dim + lane + 64 * i] = (T)x[i];
-  if (args.lse && lane == 0) args.lse[row] = lse_of(m, l, args.a.scale);
+  if (args.lse && lane == 0) args.lse[row] = lse_of<T>(m, l, args.a.scale);
 }
 
 // Whether a call takes the kernel for few rows, and with how many parts (all us, bf16 unless said).
