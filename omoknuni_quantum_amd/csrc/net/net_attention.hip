@@ -355,12 +355,11 @@ int check_attention(const char* name, const omq_attention_args* a) {
   const int64_t n = a->q_starts ? 1 : a->sequences;
   const int64_t most = OMQ_NET_MAX_COUNT - 4095;  // (a tile past the last is counted in 32 bits)
   if (a->dim > OMQ_NET_MAX_HEAD_DIM || a->sequences > most || a->q_len > most || a->k_len > most ||
-      a->q_len * a->q_heads > most || a->k_len * a->q_heads > most ||
-      (n > 0 && (a->q_len * a->q_heads > most / n || a->k_len * a->q_heads > most / n)))
+      a->q_len * a->q_heads > most || (n > 0 && a->q_len * a->q_heads > most / n))
     return net_fail(OMQ_NET_E_LIMIT,
-                    "%s: sequences %lld of %lld queries and %lld keys, %d heads (rows of heads at "
-                    "most %d), dim %d (at most %d)",
-                    name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len,
+                    "%s: sequences %lld of %lld queries and %lld keys (at most %d), %d heads (rows of "
+                    "heads of queries at most %d), dim %d (at most %d)",
+                    name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len, (int)most,
                     a->q_heads, (int)most, a->dim, OMQ_NET_MAX_HEAD_DIM);
   if (!(a->scale > 0.0f && a->scale < kInf32))
     return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be finite and above 0", name, a->scale);
