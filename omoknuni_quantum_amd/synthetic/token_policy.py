@@ -101,8 +101,12 @@ class RotaryTable:
         """(positions, frequencies, sections) of a batch, or of packed tokens 3 * cell + content."""
         device = tokens.device
         if device not in self.held:
-            cell = torch.arange(self.board**2, dtype=torch.int32, device=device)
-            self.held[device] = (self._places(cell),
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the rotation's table is not on {device} yet, and a graph that is "
+                                   "captured would not fill it: run the network there once before")
+            # (from the host: the copies have ended when they return, whichever stream comes next)
+            cell = torch.arange(self.board**2, dtype=torch.int32)
+            self.held[device] = (self._places(cell).to(device),
                                  net_ops.rotary_frequencies(self.sections, 100.0, device))
         positions, frequencies = self.held[device]
         return self._places(tokens // 3) if packed else positions, frequencies, self.sections
