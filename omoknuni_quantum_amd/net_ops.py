@@ -292,6 +292,10 @@ class _HeadNormRotary(torch.autograd.Function):
         return gq, gk, None, None, gqw, gkw, None, None, None
 
 
+def _sections(frequencies, sections):
+    return tuple(int(n) for n in ((frequencies.numel(),) if sections is None else sections))
+
+
 def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
                      frequencies: torch.Tensor, q_weight: torch.Tensor | None = None,
                      k_weight: torch.Tensor | None = None, eps: float = 1e-6, sections=None,
@@ -312,7 +316,7 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     q and k may be slices of one product's output: a head's elements must be adjacent and the
     tokens equally far apart.  At most 256 columns and 4 axes.  Differentiable in q, k and the
     weights."""
-    sections = (frequencies.shape[0],) if sections is None else tuple(int(n) for n in sections)
+    sections = _sections(frequencies, sections)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
                                     (q_weight is not None and q_weight.requires_grad) or
                                     (k_weight is not None and k_weight.requires_grad)):
@@ -328,7 +332,7 @@ def head_norm_rotary_grad(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.T
                           interleaved: bool = False):
     """(grad_q, grad_k, grad_q_weight, grad_k_weight) of head_norm_rotary from its arguments and
     the gradients of its two results (contiguous).  The last two are None without weights."""
-    sections = (frequencies.shape[0],) if sections is None else tuple(int(n) for n in sections)
+    sections = _sections(frequencies, sections)
     gq, gk, gqw, gkw = _ROTARY_GRAD(grad_q, grad_k, q, k, positions, frequencies, q_weight,
                                     k_weight, eps, sections, interleaved)
     return (gq, gk, gqw, gkw) if q_weight is not None else (gq, gk, None, None)
@@ -353,8 +357,9 @@ class _Attention(torch.autograd.Function):
 
 
 def _attention_args(q, scale, q_starts, k_starts):
-    return (q.shape[-1] ** -0.5 if scale is None else float(scale),
-            q_starts if k_starts is None else k_starts)
+    if scale is None:  # (a q without columns is refused with the other shapes)
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    return float(scale), q_starts if k_starts is None else k_starts
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
