@@ -248,7 +248,7 @@ typedef struct omq_attention_args {
   int64_t v_seq_stride, v_row_stride, v_head_stride;
   const int32_t *q_starts, *k_starts, *k_lengths;
   int32_t q_heads, k_heads, dim, dtype, causal;
-  float scale; /* finite, above 0 */
+  float scale; /* above 0, at most 2^127 */
 } omq_attention_args;
 
 /* Bytes of workspace of omq_attention_forward; negative for what it refuses. */

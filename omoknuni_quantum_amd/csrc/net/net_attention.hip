@@ -361,8 +361,8 @@ int check_attention(const char* name, const omq_attention_args* a) {
                     "heads of queries at most %d), dim %d (at most %d)",
                     name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len, (int)most,
                     a->q_heads, (int)most, a->dim, OMQ_NET_MAX_HEAD_DIM);
-  if (!(a->scale > 0.0f && a->scale < kInf32))
-    return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be finite and above 0", name, a->scale);
+  if (!(a->scale > 0.0f && a->scale <= 0x1p127f))  // (its product with log2 e is finite)
+    return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be above 0 and at most 2^127", name, a->scale);
   if (!a->q_starts != !a->k_starts)
     return net_fail(OMQ_NET_E_ARG, "%s: starts of queries and keys, or of neither", name);
   if (a->q_seq_stride < 0 || a->q_row_stride < 0 || a->q_head_stride < 0 || a->k_seq_stride < 0 ||

@@ -25,7 +25,6 @@
 
 #include <algorithm>
 #include <array>
-#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -625,8 +624,8 @@ omq_attention_args attention_args(const char* name, const at::Tensor& q, const a
   if (kl) a.k_lengths = index_row(name, "k_lengths", *kl, a.sequences);
   a.q_row_stride = q.stride(-3), a.k_row_stride = k.stride(-3), a.v_row_stride = v.stride(-3);
   a.q_head_stride = q.stride(-2), a.k_head_stride = k.stride(-2), a.v_head_stride = v.stride(-2);
-  TORCH_CHECK(scale > 0.0 && std::isfinite((float)scale) && (float)scale > 0.0f, "omq_net::", name,
-              ": scale ", scale, " must be finite and above 0");
+  TORCH_CHECK((float)scale > 0.0f && (float)scale <= 0x1p127f, "omq_net::", name, ": scale ", scale,
+              " must be finite and above 0 (at most 2^127)");
   a.scale = (float)scale;
   a.causal = causal;
   if (!dev.is_meta()) a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
