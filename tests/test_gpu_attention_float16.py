@@ -30,4 +30,5 @@ def test_many_keys_of_small_probability(device, keys, queries, above):
     limit = want * (off + U[torch.float16]) + 2.0**-25
     assert float((out.double() - want).abs().max()) <= limit
     exact = above + math.log1p(others)
-    assert float((lse.double() - exact).abs().max()) <= (keys / 32 + 40 + 4 * above) * u + 4 * u * exact
+    limit = (keys / 32 + 40 + 4 * above + 4 * exact) * u
+    assert float((lse.double() - exact).abs().max()) <= limit

@@ -1,5 +1,6 @@
-"""More of the attention's gradients on the GPU: parts of the keys with the whole row's out and lse
-and float16 gradients of any size.  Bounds as in test_gpu_attention.py."""
+"""More of the attention's gradients on the GPU: parts of the keys with the whole row's out and lse,
+float16 gradients of any size, and the launches by keys of many workgroups.  Bounds as in
+test_gpu_attention.py."""
 import pytest
 import torch
 
@@ -99,3 +100,55 @@ def test_float16_keys_that_bring_more_and_more(device, lq, lk, causal):
     for name, t in zip(("q", "k", "v"), got):
         within(t[0], want[name], bound[name])
     assert not bool(got[0][0, ::3].any())
+
+
+# ---- many workgroups by keys --------------------------------------------------------------------
+def whole(device, dtype, causal, seqs, dim, packed):
+    scale = dim**-0.5
+    if packed:
+        args = [torch.cat(t).to(device) for t in zip(*seqs)]
+        starts = [torch.tensor([0] + [len(s[i]) for s in seqs]).cumsum(0).int().to(device)
+                  for i in (0, 1)]
+        kw = dict(causal=causal, q_starts=starts[0], k_starts=starts[1])
+    else:
+        args, kw = [torch.stack(t).to(device) for t in zip(*seqs)], dict(causal=causal)
+    q, k, v, go = args
+    out, lse = net_ops.attention_with_lse(q, k, v, **kw)
+    got = [t.cpu() for t in (out, lse, *net_ops.attention_grad(go, q, k, v, out, lse, **kw))]
+    at = [0, 0]
+    for i, s in enumerate(seqs):
+        want, bound = dense(*s[:3], scale, causal, s[3])
+        for name, t in zip(("out", "lse", "q", "k", "v"), got):
+            side = name in ("k", "v")
+            mine = t[at[side]:at[side] + len(s[side])] if packed else t[i]
+            within(mine, want[name], bound[name])
+        at = [at[0] + len(s[0]), at[1] + len(s[1])]
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [(torch.bfloat16, 128, 4), (torch.float16, 128, 4),
+                                             (torch.bfloat16, 100, 4), (torch.float16, 64, 8),
+                                             (torch.float32, 64, 8)])
+@pytest.mark.parametrize("sequences,length", [(5, 800), (5, 900), (3, 1600)])
+def test_causal_workgroups_that_share_a_unit(device, dtype, dim, heads, sequences, length):
+    """More workgroups than compute units and fewer than twice as many, an even and an odd number of
+    tiles (of 128 keys): every key has its gradients."""
+    g = gen(length + dim)
+    seqs = [inputs(g, length, length, heads, heads, dim, dtype) for _ in range(sequences)]
+    whole(device, dtype, True, seqs, dim, False)
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [(torch.bfloat16, 128, 4), (torch.float16, 64, 8)])
+@pytest.mark.parametrize("lengths", [(700, 1, 300, 0, 1299, 900), (2000, 3, 1000, 640, 5)])
+def test_packed_causal_workgroups_that_share_a_unit(device, dtype, dim, heads, lengths):
+    g = gen(sum(lengths) + dim)
+    seqs = [inputs(g, n, n + 7 * (n % 2), heads, heads, dim, dtype) for n in lengths]
+    whole(device, dtype, True, seqs, dim, True)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [100, 128])
+def test_float32_keys_and_values_together(device, causal, dim):
+    """Sums of 128 columns in one workgroup, where those fill the chip."""
+    g = gen(dim)
+    seqs = [inputs(g, 70, 520, 4, 4, dim, torch.float32) for _ in range(16)]
+    whole(device, torch.float32, causal, seqs, dim, False)
