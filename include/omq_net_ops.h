@@ -238,8 +238,9 @@ int omq_head_norm_rotary_grad(const omq_rotary* r, const void* grad_q_out, const
  *   lse     float32 [rows of q, q_heads], contiguous
  * Products are formed from the elements' type and summed in float32; p is rounded to the elements'
  * type before it multiplies v, as are the gradients of the scores before they multiply q (for k they
- * have twice its bits).  Rows of heads of queries (q_len times q_heads, of all sequences) and
- * k_len are at most OMQ_NET_MAX_COUNT - 4095 each. */
+ * have twice its bits); float16 takes both times powers of two, so that small ones
+ * keep their bits.  Rows of heads of queries (q_len times q_heads, of all sequences) and k_len are
+ * at most OMQ_NET_MAX_COUNT - 4095 each. */
 typedef struct omq_attention_args {
   int64_t sequences, q_len, k_len;
   const void *q, *k, *v;

@@ -371,7 +371,8 @@ __device__ __attribute__((always_inline)) inline void here() {
 // one's reads under way with the first one's products.
 template <class T, int kDim>
 __device__ __attribute__((always_inline)) inline void two_products(
-    F16& s, const char* tile, int row0, const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
+    F16& s, const char* tile, int row0,
+    const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
     F16& s2, const char* tile2, int row2,
     const typename Operand<T>::Frag (&f2)[kDim / Operand<T>::kChunk],
     const typename Tile<T, kDim>::Lane& lane) {
@@ -393,7 +394,8 @@ __device__ __attribute__((always_inline)) inline void two_products(
 
 template <class T, int kDim>
 __device__ __attribute__((always_inline)) inline void one_product(
-    F16& s, const char* tile, int row0, const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
+    F16& s, const char* tile, int row0,
+    const typename Operand<T>::Frag (&f)[kDim / Operand<T>::kChunk],
     const typename Tile<T, kDim>::Lane& lane) {
   using L = Tile<T, kDim>;
   typename L::Frag a[L::kChunks];
@@ -406,7 +408,7 @@ __device__ __attribute__((always_inline)) inline void one_product(
 }
 
 // acc += (columns of the tile's 32 rows from row0) x w, a group of the columns' operands at a time;
-// the first group is read by `columns_ahead`, before w is formed.
+// the first group is read (Columns::read) before w is formed.
 template <class T, int kDim>
 struct Columns {
   using L = Tile<T, kDim>;
@@ -523,8 +525,8 @@ inline bool chunks_aligned(int dtype, int64_t dim, std::initializer_list<const v
   return ok;
 }
 
-// Keys and values for the loads straight into LDS; others pass through registers.  8 x 8 heads of 1024
-// keys of 64 columns, bf16: 28 us straight, 52 with rows 2 bytes off (of 128: 45 and 92).
+// Keys and values for the loads straight into LDS; others pass through registers.  8 x 8 heads of
+// 1024 keys of 64 columns, bf16: 28 us straight, 52 with rows 2 bytes off (of 128: 45 and 92).
 inline bool direct_tiles(const omq_attention_args& a) {
   return chunks_aligned(a.dtype, a.dim, {a.k, a.v},
                         {a.k_seq_stride, a.k_row_stride, a.k_head_stride, a.v_seq_stride,

@@ -9,10 +9,10 @@
 // type at most, as the output's own rounding; m and l are float32.
 //
 // Bound by a wave's products, its exponentials and its reads of LDS, which overlap only in part:
-// eight causal texts of up to 8192 with 32 heads over 8 of 128, bf16: 1100 us, 950 TFLOP/s (a large
-// product of matrices: 1336), matrix cores 46 % busy.  256 boards of 49 to 361 cells with 8 heads of
-// 64, float16: 73 us, of 128-row tiles that are half full; 32 boards of 225 cells: 12.6 us; 64 of
-// 225 cells with 4 heads of 32, float32: 28.
+// eight causal texts of up to 8192 with 32 heads over 8 of 128, bf16: 1090 to 1140 us over several
+// cards, 920 to 960 TFLOP/s (a large product of matrices: 1336), matrix cores 45 % busy.  256 boards
+// of 49 to 361 cells with 8 heads of 64, float16: 75 us, of 128-row tiles that are half full; 32
+// boards of 225 cells: 12.7 us; 64 of 225 cells with 4 heads of 32, float32: 28.
 #include "net_attention.h"
 
 namespace omq_net {
@@ -104,7 +104,8 @@ __device__ __attribute__((always_inline)) inline void attend(
 }
 
 template <class T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_kernel(AttentionArgs args) {
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void
+attention_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
   __shared__ __attribute__((aligned(1024))) char keys0[L::kBytes], keys1[L::kBytes];
   __shared__ __attribute__((aligned(1024))) char values0[L::kBytes], values1[L::kBytes];
@@ -357,10 +358,10 @@ int check_attention(const char* name, const omq_attention_args* a) {
   if (a->dim > OMQ_NET_MAX_HEAD_DIM || a->sequences > most || a->q_len > most || a->k_len > most ||
       a->q_len * a->q_heads > most || (n > 0 && a->q_len * a->q_heads > most / n))
     return net_fail(OMQ_NET_E_LIMIT,
-                    "%s: sequences %lld of %lld queries and %lld keys (at most %d), %d heads (rows of "
-                    "heads of queries at most %d), dim %d (at most %d)",
-                    name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len, (int)most,
-                    a->q_heads, (int)most, a->dim, OMQ_NET_MAX_HEAD_DIM);
+                    "%s: sequences %lld of %lld queries and %lld keys (at most %d), %d heads (rows "
+                    "of heads of queries at most %d), dim %d (at most %d)",
+                    name, (long long)a->sequences, (long long)a->q_len, (long long)a->k_len,
+                    (int)most, a->q_heads, (int)most, a->dim, OMQ_NET_MAX_HEAD_DIM);
   if (!(a->scale > 0.0f && a->scale <= 0x1p127f))  // (its product with log2 e is finite)
     return net_fail(OMQ_NET_E_ARG, "%s: scale %g must be above 0 and at most 2^127", name, a->scale);
   if (!a->q_starts != !a->k_starts)

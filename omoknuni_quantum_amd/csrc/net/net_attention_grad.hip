@@ -3,18 +3,20 @@
 //   delta_i = g_i . out_i;   ds_ij = p_ij (g_i . v_j - delta_i) scale
 //   dq_i = sum_j ds_ij k_j;  dk_j = sum_i ds_ij q_i;  dv_j = sum_i p_ij g_i
 // Two launches, each with its sums in registers: by queries (dq, and delta for the other) and by
-// keys (dk and dv).  Scores are formed in both, seven products in place of five, and no sum is
-// split over workgroups, which would take atomics or float32 copies of dq; every result is the
-// same bits at every call.  Rows of queries that share a key head are rows of one sum.
+// keys (dk and dv).  Scores are formed in both, and no sum is split over workgroups, which would
+// take atomics or float32 copies of dq; every result is the same bits at every call.  For five
+// products of the formulas that is seven; in 16 bits dq takes one more (below), and where the sums
+// by keys are apart (sums_apart) the scores one more: eight up to 64 columns, nine above.  Rows of
+// queries that share a key head are rows of one sum.
 //
-// Two causal sequences of 4096 with 16 heads over 4 of 128, bf16: 290 us by queries, 575 by keys
-// (950 and 600 TFLOP/s of what they multiply); 256 boards of 49 to 361 cells with 8 heads over 4 of
-// 64, float16: 107 and 144 us; 64 of 225 cells with 4 heads of 32, float32: 40 and 52.  Matrix cores
-// are busy for a fifth (boards) to a half (by queries), in float32 three fifths of that: a wave's
-// products, its exponentials and its reads of LDS follow one another, and two waves a SIMD, for which
-// the registers are just enough, cover a part of that.  By keys the workgroups of a causal sequence are few and of all lengths; the rows
-// that they read do not bound them (half the traffic, by an order of the workgroups in which the
-// memory's parts share them, took as long).
+// Two causal sequences of 4096 with 16 heads over 4 of 128, bf16: 285 us by queries, 515 by keys
+// (960 and 670 TFLOP/s of what they multiply); 256 boards of 49 to 361 cells with 8 heads over 4 of
+// 64, float16: 116 and 143 us; 64 of 225 cells with 4 heads of 32, float32: 40 and 52.  Matrix cores
+// are busy for a fifth of the time (boards) to a half (by queries), in float32 for three fifths: a
+// wave's products, its exponentials and its reads of LDS follow one another, and two waves a SIMD,
+// for which the registers are just enough, cover a part of that.  By keys the workgroups of a causal
+// sequence are few and of all lengths; the rows that they read do not bound them (half the traffic,
+// by an order of the workgroups in which the memory's parts share them, took as long).
 //
 // ds is rounded to the elements' type for its products, times scale, without which float16 would
 // overflow earlier.  Its sum over a row is 0 but for what the rounding of out took from delta, which
@@ -28,16 +30,18 @@
 namespace omq_net {
 namespace {
 
-// How far from 1 the sum of a whole row's probabilities may be: lse's rounding takes it 2^-25 |lse| away
-// and its sum's less; the share of hidden keys that passes for rounding is below out's own (2^-9, 2^-12).
+// How far from 1 the sum of a whole row's probabilities may be: lse's rounding takes it 2^-25 |lse|
+// away and its sum's less; the share of hidden keys that passes for rounding is below out's own
+// (2^-9, 2^-12).
 constexpr float kWhole = 0x1p-12f;
 
-// float16 holds 2^-14 to 2^16 in full.  A slope is a probability, 1 / keys or so, times a gradient of
-// out, which a mean over a batch makes small: its float16 products take it times a power of two, a
-// column's own (a query's of dq, a key's of dk), that puts the column's largest slope so far at 2^9 to
-// 2^15; the sums so far are brought along where it changes.  (Without, dq and dk of 225 keys are off by
-// 1e-2 of their size where grad_out is of 1e-4; it takes 3 % of packed boards' training, 323 -> 334 us.)
-template <class T, int kDim>
+// float16 holds 2^-14 to 2^16 in full.  A slope is a probability, 1 / keys or so, times a gradient
+// of out, which a mean over a batch makes small: its float16 products take it times a power of two,
+// a column's own (a query's of dq, a key's of dk), that puts the column's largest slope so far at 2^9
+// to 2^15; the sums so far are brought along where it changes.  (Without, dq and dk of 225 keys are
+// off by 1e-2 of their size where grad_out is of 1e-4; it takes 3 % of packed boards' training, 323
+// -> 334 us.)
+template <class T>
 struct Lift {
   static constexpr bool kOn = std::is_same_v<T, f16>;
   float up, down;  // the power of two (over that of the probabilities), and what undoes both
@@ -64,7 +68,8 @@ template <class T>
 constexpr float kProbabilityUp = std::is_same_v<T, f16> ? 12.0f : 0.0f;
 
 template <class T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_q_kernel(AttentionArgs args) {
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void
+attention_grad_q_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
   __shared__ __attribute__((aligned(1024))) char keys0[L::kBytes], keys1[L::kBytes];
   __shared__ __attribute__((aligned(1024))) char values0[L::kBytes], values1[L::kBytes];
@@ -122,7 +127,7 @@ __global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void at
   // sums of ds and p: scale times what out's rounding took from delta, where the probabilities are a
   // whole row's
   float rest = 0.0f, mass = 0.0f;
-  Lift<T, kDim> lift{1.0f, 1.0f};
+  Lift<T> lift{1.0f, 1.0f};
   float scale = a.scale;  // times lift.up, as are all slopes
   const auto lost = [&] {
     const float r = rest + other_half(rest), m = mass + other_half(mass);
@@ -308,8 +313,8 @@ __device__ __attribute__((always_inline)) inline void grad_kv(const AttentionArg
     load_row<T, kDim, kDirect>(vf, static_cast<const T*>(a.v) + q.v_at + key * a.v_row_stride +
                                        kv * a.v_head_stride, a.dim);
   F16 dk[kDim / 32] = {}, dv[kDim / 32] = {};
-  constexpr float kUp = Lift<T, kDim>::kOn ? 0x1p12f : 1.0f;  // 2^kProbabilityUp, of p here
-  Lift<T, kDim> lift{1.0f / kUp, 1.0f};
+  constexpr float kUp = Lift<T>::kOn ? 0x1p12f : 1.0f;  // 2^kProbabilityUp, of p here
+  Lift<T> lift{1.0f / kUp, 1.0f};
   uint32_t found_q = 0, found_g = 0;
   typename L::Lane own;
   const auto step = [&](int64_t next, const char* queries, const char* grads,
@@ -412,7 +417,8 @@ bool sums_apart(int64_t blocks) {
 }
 
 template <class T, int kDim, bool kDirect, bool kApart>
-__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void attention_grad_kv_kernel(AttentionArgs args) {
+__global__ __launch_bounds__(kWaves* kWave, (waves_per_simd<T, kDim>())) void
+attention_grad_kv_kernel(AttentionArgs args) {
   using L = Tile<T, kDim>;
   __shared__ __attribute__((aligned(1024))) char queries0[L::kBytes], queries1[L::kBytes];
   __shared__ __attribute__((aligned(1024))) char grads0[L::kBytes], grads1[L::kBytes];

@@ -15,10 +15,13 @@
 // logits again; the candidates (a logit and an index in 64 bits, no two alike) are ranked by
 // counting.  Where more candidates tie than the list holds, they are found one after another.
 //
-// Bound by memory: a row of up to 16384 tokens is held in registers (8192 rows of 4672, bf16, mask and
-// gradient: 39 us, 4.9 TB/s, instructions as busy as memory); a longer one is read by a workgroup,
-// its alternatives from the few threads that hold them, and a second time for the gradient (2048
-// rows of 131072, bf16: 100 us, 5.3 TB/s, and 10 for 8 alternatives).
+// Bound by memory and, with a gradient, as much by instructions: a row of up to 16384 tokens is held
+// in registers (8192 rows of 4672, bf16, mask and gradient: 43 us, 4.4 TB/s, 40 where the inputs
+// repeat); a longer one is read by a workgroup, its alternatives from the few threads that hold them,
+// and a second time for the gradient (2048 rows of 131072, bf16: 102 us, 5.3 TB/s, and 13 for 8
+// alternatives; 301 with the gradient).  Under autograd the forward pass leaves a row's statistics,
+// and the gradient is a launch that reads the logits again: 29 + 39 us of the former rows, 102 + 191
+// of the latter.
 #include <type_traits>
 
 #include "net_logits.h"
@@ -189,7 +192,7 @@ struct RowSlope {
 };
 
 __device__ inline RowSlope slope_of(const RowEnd& o, float base, float a, float b) {
-  // (a part without weight has only e = 0 and NaN: no 2^d, which may be infinite, 0 times which is NaN)
+  // (a part without weight has only e = 0 and NaN; 2^d of it may be infinite, and 0 times that NaN)
   if (base == -kInf) return {o.inv_s, 0.0f, 0.0f};
   const float d = y_between(base, o.base);
   const float scale = __builtin_amdgcn_exp2f(d);
@@ -260,8 +263,9 @@ __device__ inline float largest_but(float v, int top) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), __builtin_ctzll(at)));
 }
 
-// mine: the thread's largest logit.  each(f): f(logit, index) for the thread's logits; some(reaches, f):
-// the same for those of the threads for which `reaches` is true, by whichever threads.
+// mine: the thread's largest logit.  each(f): f(logit, index) for the thread's logits;
+// some(reaches, f): the same for those of the threads for which `reaches` is true, by whichever
+// threads.
 template <int kThreads, class Each, class Some>
 __device__ inline void best_of_row(const LogprobArgs& a, int64_t row, const RowEnd& o, float mine,
                                    TopSpace<kThreads>& sp, Each&& each, Some&& some) {
@@ -566,8 +570,8 @@ void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     using T = decltype(t);
     const int64_t v = a.r.vocab;
     // as few threads a row as hold it in two or three blocks each: what a row costs beside its loads
-    // goes by its waves (8192 rows of 4672, bf16, with gradient: 38 us by 256 threads, 51 by 512;
-    // 65536 of 362: 41 by 64, 78 by 128; 4096 of 10000: 39 by 512, 48 by 1024)
+    // goes by its waves (8192 rows of 4672, bf16, with gradient: 44 us by 256 threads, 56 by 512;
+    // 65536 of 362: 42 by 64, 76 by 128; 4096 of 10000: 46 by 512, 52 by 1024)
     if (v <= 512) return launch_rows<T, 64, 1, kGrad>(a, st);
     if (v <= 1024) return launch_rows<T, 64, 2, kGrad>(a, st);
     if (v <= 2048) return launch_rows<T, 128, 2, kGrad>(a, st);
@@ -578,8 +582,8 @@ void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     if (v <= 16384) return launch_rows<T, 1024, 2, kGrad>(a, st);
     // workgroups of 256 threads where there is one for each compute unit twice: a row's end (its
     // sums' join, its alternatives) takes as long in all, and the other rows' loads go on (131072
-    // tokens, bf16, 8 alternatives: 2048 rows 112 us, 154 with 1024 threads; 512 rows 37 and 39; 256
-    // rows 32 and 21)
+    // tokens, bf16, 8 alternatives: 2048 rows 117 us, 157 with 1024 threads; 512 rows 41 and 41; 256
+    // rows 33 and 21)
     const auto go = [&](auto threads) {
       constexpr int kThreads = threads.value;
       const dim3 grid = grid_of(a.r.rows, kThreads);

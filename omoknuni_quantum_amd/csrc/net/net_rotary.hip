@@ -11,8 +11,8 @@
 // some tokens: it forms the sines and cosines of the tokens' pairs once, in LDS, for all of them (an
 // angle costs about as many instructions as a lane's norm).  The next heads' loads are under way
 // while one's are formed.  With inputs out of the caches 115200 tokens with 4 + 4 heads of 32,
-// float32, take 55 us on the chip (4.3 TB/s), the gradient of 16384 tokens with 32 + 8 heads of
-// 128, bf16, 101 us (5.0 TB/s): memory, and its latency where rows are short.
+// float32, take 62 us (3.8 TB/s; 56 where they repeat), the gradient of 16384 tokens with 32 + 8
+// heads of 128, bf16, 106 us (4.8 TB/s): memory, and its latency where rows are short.
 #include <type_traits>
 
 #include "net_common.h"
@@ -348,8 +348,8 @@ RotaryArgs layout_of(const omq_rotary& r, bool grad) {
     s.tile = (int)(tile < 1 ? 1 : tile);
     s.tiles = ceil_div(r.tokens, s.tile);
     s.magic = s.heads > 1 ? (uint32_t)((0x100000000ull + s.heads - 1) / s.heads) : 0;
-    // (of the gradient: enough for the chip, few enough for their sums: 16384 tokens as above 80 us,
-    // of 512 groups 87, of 2048 85, of as many as tiles 93)
+    // (of the gradient: enough for the chip, few enough for their sums: 16384 tokens as above 106 us,
+    // of 512 groups 109, of 2048 111, of as many as tiles 117)
     s.groups = grad && r.q_weight && s.tiles > kGradGroups ? kGradGroups : s.tiles;
   }
   return a;

@@ -469,8 +469,9 @@ omq_rotary rotary_args(const char* name, const at::Tensor& q, const at::Tensor& 
   TORCH_CHECK(q.dim() >= 2 && k.dim() == q.dim() &&
                   q.sizes().slice(0, q.dim() - 2) == k.sizes().slice(0, k.dim() - 2) &&
                   q.size(-1) == k.size(-1) && q.size(-1) >= 1 && q.size(-2) >= 1 && k.size(-2) >= 1,
-              "omq_net::", name, ": q and k must be [..., heads, dim] of the same tokens and dim, not ",
-              q.sizes(), " and ", k.sizes());
+              "omq_net::", name,
+              ": q and k must be [..., heads, dim] of the same tokens and dim, not ", q.sizes(),
+              " and ", k.sizes());
   TORCH_CHECK(q.scalar_type() == k.scalar_type(), "omq_net::", name, ": q and k must be of one type");
   r.dtype = type_of(name, "q", q);
   r.dim = (int)std::min<int64_t>(q.size(-1), INT32_MAX);
@@ -595,15 +596,16 @@ omq_attention_args attention_args(const char* name, const at::Tensor& q, const a
   TORCH_CHECK(!qs == !ks, "omq_net::", name, ": starts of queries and keys, or of neither");
   TORCH_CHECK(k.dim() == q.dim() && k.sizes() == v.sizes() && k.size(-1) == q.size(-1) &&
                   (q.dim() == 3 || k.size(0) == q.size(0)),
-              "omq_net::", name, ": k and v must have q's sequences and dim, not ", k.sizes(), " and ",
-              v.sizes(), " with ", q.sizes());
+              "omq_net::", name, ": k and v must have q's sequences and dim, not ", k.sizes(),
+              " and ", v.sizes(), " with ", q.sizes());
   TORCH_CHECK(q.size(-1) >= 1 && q.size(-2) >= 1 && k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0,
               "omq_net::", name, ": heads of queries (", q.size(-2),
               ") must be a multiple of those of keys (", k.size(-2), ")");
   a.dtype = type_of(name, "q", q);
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "omq_net::",
               name, ": q, k and v must be of one type");
-  for (const auto& [arg, t] : {std::pair<const char*, const at::Tensor*>{"q", &q}, {"k", &k}, {"v", &v}})
+  using Named = std::pair<const char*, const at::Tensor*>;
+  for (const auto& [arg, t] : {Named{"q", &q}, Named{"k", &k}, Named{"v", &v}})
     TORCH_CHECK(t->size(-1) == 1 || t->stride(-1) == 1 || t->numel() == 0, "omq_net::", name,
                 ": the elements of a head of ", arg, " must be adjacent (use .contiguous())");
   a.q_len = q.size(-3);

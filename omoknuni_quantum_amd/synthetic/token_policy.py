@@ -6,7 +6,8 @@ other's), looked up in one table; two kinds of layer alternate on the residual, 
 the cells and one over the channels, each behind a root-mean-square norm of the residual sum; the
 policy is one logit per cell, the value a mean over the cells.  With `heads` the cells attend to
 one another in place of the product: queries and keys normed and rotated by row and column.  Such
-a network takes boards of different sizes, packed one after another (``forward(tokens, starts)``).
+a network's ``forward(tokens, starts)`` takes boards of different sizes, packed one after another;
+``train_step`` and the evaluator take boards of one size.
 
 * ``evaluator()`` has ``evaluate_batch(features)`` (the protocol of ``MCTS``): the norms before the
   channel products give them their input in 8 bits with a scale for every row, and so are those
@@ -281,7 +282,6 @@ class Evaluator:
         occupied = (features[:, 0] + features[:, 1]).flatten(1) > 0
         policies = torch.softmax(logits.masked_fill_(occupied, -math.inf), 1)
         return policies.masked_fill_(occupied, 0.0), values  # (NaN where all are)
-
 
     @torch.no_grad()
     def best_moves(self, features: torch.Tensor, top: int = 5):
