@@ -9,8 +9,8 @@
 // type at most, as the output's own rounding; m and l are float32.
 //
 // Bound by a wave's products, its exponentials and its reads of LDS, which overlap only in part:
-// eight causal texts of up to 8192 with 32 heads over 8 of 128, bf16: 1090 to 1140 us over several
-// cards, 920 to 960 TFLOP/s (a large product of matrices: 1336), matrix cores 45 % busy.  256 boards
+// eight causal texts of up to 8192 with 32 heads over 8 of 128, bf16: 1090 to 1216 us over several
+// cards, 860 to 960 TFLOP/s (a large product of matrices: 1336), matrix cores 45 % busy.  256 boards
 // of 49 to 361 cells with 8 heads of 64, float16: 75 us, of 128-row tiles that are half full; 32
 // boards of 225 cells: 12.7 us; 64 of 225 cells with 4 heads of 32, float32: 28.
 #include "net_attention.h"
